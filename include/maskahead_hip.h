@@ -339,6 +339,76 @@ int ma_rebuild_packed(const ma_prefix *old_store, int B, int H, int D, const ma_
                       const int64_t *stage, int64_t stage_stride, int st, int64_t *remap, int64_t remap_stride,
                       int32_t *phys, int64_t phys_stride, int live, int32_t *status, void *stream);
 
+/* ---------------------------------------------------------------- pages of 4-bit K/V
+ * A cache shared by a batch of requests whose lengths lie on the device.  No counterpart in
+ * the reference (its PackedKVCache holds one scalar length for all batch rows,
+ * cache.py:94-96); codes, scales and zeros are those of its quantizers (reference.py:58-90,
+ * 182-213).  A page holds page_tokens tokens of every KV head; request b's token p lies in
+ * page table[b][p / page_tokens].  Whole groups of 32 tokens are packed in records of 40 D
+ * bytes (layout: csrc/ma_pages.h); the newest lengths[b] % 32 tokens are 16-bit rows 0.. of
+ * the request's tail.  A page id outside [0, num_pages) and lengths past the table's width
+ * are read as if the tokens were not there.
+ *   pool    [num_pages, H, page_tokens/32, 40 D] u8, a (page, head)'s records contiguous;
+ *           s_pool = bytes between pages and between heads, 16-byte aligned like pool
+ *   k_tail, v_tail  [B, H, 32, D] in dtype (bf16 or f16), sharing the strides s_tail (b, h, t)
+ *   table   [B, width] i32, row stride s_table;  lengths [B] i32
+ *   mask    [B, H, mask_tokens] u8 (strides s_mask; 0 = dead, as are positions past
+ *           mask_tokens) for ma_paged_attention, or NULL */
+typedef struct ma_pages {
+    void *pool;
+    void *k_tail;
+    void *v_tail;
+    const int32_t *table;
+    const int32_t *lengths;
+    const uint8_t *mask;
+    int64_t s_pool[2];
+    int64_t s_tail[3];
+    int64_t s_table;
+    int64_t s_mask[2];
+    int32_t num_pages, width, page_tokens, mask_tokens;
+    int32_t dtype, reserved;
+} ma_pages;
+
+/* Page plan of one step: request b goes from lengths[b] to ends[b] = max(0, lengths[b] +
+ * new_lens[b]) tokens (new_lens negative: gives tokens back, all of them with any value of
+ * at most -lengths[b]).  ring [num_pages] i32 holds the free pages' ids, first in first out;
+ * state [4] i32 = (place of the oldest, free pages, 0, status).  Growing requests take pages
+ * in request order, oldest first; then the pages given back enter the ring, in request and
+ * page order, free from the next plan on.  table entries that appear are written, those that
+ * go become -1; slots [B, T] i64 = page id * page_tokens + offset of new token i, -1 for i >=
+ * new_lens[b].  lengths is not written: the caller takes ends when the tokens are stored.
+ * A plan that cannot be met changes nothing (slots -1, ends = lengths) and adds to status:
+ * 1 the ring runs out, 2 a request outgrows its table row, 4 new_lens[b] > T, 8 a negative
+ * length.  status is never cleared here.  One launch; plans of one ring are ordered by the
+ * caller (one stream). */
+int ma_page_plan(const int32_t *lengths, const int32_t *new_lens, int B, int T, int page_tokens, int32_t *table,
+                 int64_t s_table, int width, int32_t *ring, int num_pages, int32_t *state, int64_t *slots,
+                 int32_t *ends, void *stream);
+/* Append of new_lens[b] (0 .. T) tokens k, v [B, H, T, D] behind request b's lengths[b]
+ * tokens: every group of 32 that [tail | new] completes is quantized with ma_quantize_keys'
+ * and ma_quantize_values' arithmetic into the record that slots (ma_page_plan's) names, and
+ * the rest becomes the tail.  Requests without new tokens, and those whose slots are -1, are
+ * left as they are.  k, v share p->dtype.  One launch. */
+int ma_page_append(const ma_pages *p, ma_tensor4 k, ma_tensor4 v, int B, int H, int T, int D,
+                   const int32_t *new_lens, const int64_t *slots, void *stream);
+/* Tokens starts[b] .. starts[b] + n of every request (starts NULL: from 0) as k_out, v_out
+ * [B, H, n, D] in bf16, f16 or f32 (f32(code) * f32(scale) + f32(zero), rounded once), zero
+ * from lengths[b] on. */
+int ma_page_dequant(const ma_pages *p, int B, int H, int D, const int32_t *starts, int n, ma_tensor4 k_out,
+                    ma_tensor4 v_out, void *stream);
+/* Attention of a block of T queries of every request over [its stored tokens | the block's
+ * own keys]: splitk_attention (splitk.py:493-579) with one length per request.  kc, vc
+ * [B, H, T, D] (ptr NULL: none).  new_lens [B] (NULL: T for all) counts the block's real
+ * positions: rows t >= new_lens[b] of out stay as they are, keys j >= new_lens[b] are not
+ * seen.  causal_block > 0: key j is seen by query t only if (lengths[b] + j) / causal_block <=
+ * (lengths[b] + t) / causal_block.  A row that sees nothing is zero.  q, kc, vc, out share
+ * p->dtype.  workspace: ma_paged_workspace_bytes() bytes, 256-byte aligned; its contents are
+ * not read before they are written. */
+int64_t ma_paged_workspace_bytes(int B, int H, int Hq, int T, int D);
+int ma_paged_attention(ma_tensor4 q, int B, int Hq, int T, int D, const ma_pages *p, int H, ma_tensor4 kc,
+                       ma_tensor4 vc, const int32_t *new_lens, int causal_block, float scale, ma_tensor4 out,
+                       void *workspace, int64_t workspace_bytes, void *stream);
+
 #ifdef __cplusplus
 }
 #endif

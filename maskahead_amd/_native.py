@@ -46,12 +46,24 @@ class MaTensor4(ctypes.Structure):
                 ("s", ctypes.c_int64 * 3)]
 
 
+class MaPages(ctypes.Structure):
+    _fields_ = [
+        ("pool", ctypes.c_void_p), ("k_tail", ctypes.c_void_p), ("v_tail", ctypes.c_void_p),
+        ("table", ctypes.c_void_p), ("lengths", ctypes.c_void_p), ("mask", ctypes.c_void_p),
+        ("s_pool", ctypes.c_int64 * 2), ("s_tail", ctypes.c_int64 * 3), ("s_table", ctypes.c_int64),
+        ("s_mask", ctypes.c_int64 * 2), ("num_pages", ctypes.c_int32), ("width", ctypes.c_int32),
+        ("page_tokens", ctypes.c_int32), ("mask_tokens", ctypes.c_int32), ("dtype", ctypes.c_int32),
+        ("reserved", ctypes.c_int32),
+    ]
+
+
 _P = ctypes.c_void_p
 _I = ctypes.c_int
 _I64 = ctypes.c_int64
 _F = ctypes.c_float
 _PREF = ctypes.POINTER(MaPrefix)
 _T4 = MaTensor4
+_PAGES = ctypes.POINTER(MaPages)
 _I64P = ctypes.POINTER(ctypes.c_int64)
 
 # name -> (restype, argtypes); must match include/maskahead_hip.h
@@ -97,6 +109,11 @@ SIGNATURES = {
     "ma_rebuild_plan": (_I, [_P, _I64, _P, _I, _I64, _I, _I, _I, _I, _I, _I, _P, _I64, _P, _I64, _P, _I64, _P, _P]),
     "ma_rebuild_packed": (_I, [_PREF, _I, _I, _I, _PREF, _P, _I64, _I, _P, _I64, _I, _P, _I64, _I, _P, _I64, _I,
                                _P, _I64, _P, _I64, _I, _P, _P]),
+    "ma_page_plan": (_I, [_P, _P, _I, _I, _I, _P, _I64, _I, _P, _I, _P, _P, _P, _P]),
+    "ma_page_append": (_I, [_PAGES, _T4, _T4, _I, _I, _I, _I, _P, _P, _P]),
+    "ma_page_dequant": (_I, [_PAGES, _I, _I, _I, _P, _I, _T4, _T4, _P]),
+    "ma_paged_workspace_bytes": (_I64, [_I, _I, _I, _I, _I]),
+    "ma_paged_attention": (_I, [_T4, _I, _I, _I, _I, _PAGES, _I, _T4, _T4, _P, _I, _F, _T4, _P, _I64, _P]),
 }
 
 _lib = None

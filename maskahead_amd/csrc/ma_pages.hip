@@ -1,0 +1,568 @@
+// Pages of 4-bit K/V: the plan (block tables, slot maps, free ring) from request lengths, the
+// append that quantizes into pages, and the read-back at 16 or 32 bits.  The store's layout
+// is in ma_pages.h.
+#include "ma_pages.h"
+#include "ma_quant.h"
+
+using namespace ma;
+
+namespace {
+
+// ------------------------------------------------------------------ plan
+// pages(x) = ceil(x / P).  Request b grows by max(0, pages(end) - pages(len)) pages, whose ids
+// are the ring's entries from head + (growth of the requests before it) on, and gives back
+// max(0, pages(len) - pages(end)), which go behind the ring's newest entry.  Reads (the count
+// oldest entries) and writes (the places behind them) of the ring never meet, so one launch
+// needs no order between its workgroups: each scans all B requests' growth itself (8 B a
+// request, from L2 after the first) and writes the slots of its own PLAN_SLOTS (request,
+// token) pairs.  The ring's state is written by the workgroup that arrives last, when every
+// other has read it.
+constexpr int PLAN_THREADS = 256;
+constexpr int PLAN_SLOTS = 2048;
+constexpr int PLAN_SCAN = 4 * PLAN_THREADS;   // requests per scan step
+
+enum { PLAN_NO_PAGES = 1, PLAN_WIDTH = 2, PLAN_TOKENS = 4, PLAN_LENGTH = 8 };
+
+struct PlanArgs {
+    const int32_t *lengths, *new_lens;
+    int32_t *table, *ring, *state, *ends;
+    int64_t *slots;
+    int64_t s_table, nflat;   // nflat = B * max(T, 1)
+    int B, T, page, width, num_pages;
+};
+
+__device__ __forceinline__ int64_t wave_scan_i64(int64_t x, int lane) {
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) {
+        const int64_t y = __shfl_up(x, o);
+        if (lane >= o) x += y;
+    }
+    return x;
+}
+
+__global__ __launch_bounds__(PLAN_THREADS) void page_plan_kernel(PlanArgs a) {
+    __shared__ int grow_off[PLAN_SLOTS], back_off[PLAN_SLOTS];   // of this workgroup's requests
+    __shared__ int64_t wsum[2][PLAN_THREADS / 64];
+    __shared__ int bad_s;
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    const int Tm = max(a.T, 1);
+    const int64_t f0 = (int64_t)blockIdx.x * PLAN_SLOTS;
+    const int nf = (int)min((int64_t)PLAN_SLOTS, a.nflat - f0);
+    const int b0 = (int)(f0 / Tm), b1 = (int)((f0 + nf - 1) / Tm);
+    const int r0 = (int)(f0 - (int64_t)b0 * Tm);                  // token of the first pair
+    const int head = a.state[0], count = a.state[1];
+    if (tid == 0) bad_s = 0;
+    __syncthreads();
+    int64_t gsum = 0, bsum = 0;   // of the requests before this scan step
+    int bad = 0;
+    for (int base = 0; base < a.B; base += PLAN_SCAN) {
+        int64_t g[4], k[4], gt = 0, kt = 0;
+        const int first = base + 4 * tid;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const int b = first + i;
+            g[i] = gt;
+            k[i] = kt;
+            if (b < a.B) {
+                const int64_t len = a.lengths[b], n = a.new_lens[b];
+                const int64_t end = max(len + n, (int64_t)0);
+                const int64_t p0 = (len + a.page - 1) / a.page, p1 = (end + a.page - 1) / a.page;
+                if (len < 0) bad |= PLAN_LENGTH;
+                if (n > a.T) bad |= PLAN_TOKENS;
+                if (max(p0, p1) > a.width) bad |= PLAN_WIDTH;
+                gt += max(p1 - p0, (int64_t)0);
+                kt += max(p0 - p1, (int64_t)0);
+            }
+        }
+        const int64_t gi = wave_scan_i64(gt, lane), ki = wave_scan_i64(kt, lane);
+        __syncthreads();   // wsum of the step before is read
+        if (lane == 63) {
+            wsum[0][wave] = gi;
+            wsum[1][wave] = ki;
+        }
+        __syncthreads();
+        int64_t go = gsum + gi - gt, ko = bsum + ki - kt;
+#pragma unroll
+        for (int w = 0; w < PLAN_THREADS / 64; ++w) {
+            if (w < wave) {
+                go += wsum[0][w];
+                ko += wsum[1][w];
+            }
+            gsum += wsum[0][w];
+            bsum += wsum[1][w];
+        }
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const int b = first + i;
+            if (b >= b0 && b <= b1 && b < a.B) {   // (beyond num_pages only where the plan is refused)
+                grow_off[b - b0] = (int)min(go + g[i], (int64_t)a.num_pages);
+                back_off[b - b0] = (int)min(ko + k[i], (int64_t)a.num_pages);
+            }
+        }
+    }
+    if (bad) atomicOr(&bad_s, bad);
+    __syncthreads();
+    bad = bad_s | (gsum > count ? PLAN_NO_PAGES : 0);
+    // head and count are the caller's: a ring outside its own bounds is never indexed
+    if (head < 0 || count < 0 || head >= a.num_pages || count > a.num_pages || bsum > a.num_pages - count)
+        bad |= PLAN_NO_PAGES;
+    for (int f = tid; f < nf; f += PLAN_THREADS) {
+        const unsigned flat = (unsigned)f + (unsigned)r0;
+        const int bl = (int)(flat / (unsigned)Tm), b = b0 + bl;
+        const int i = (int)(flat - (unsigned)bl * (unsigned)Tm);
+        const int len = a.lengths[b], n = a.new_lens[b];
+        if (i == 0) a.ends[b] = bad ? len : (int)max((int64_t)len + n, (int64_t)0);
+        if (i >= a.T) continue;
+        int64_t slot = -1;
+        if (!bad && i < n) {
+            const int pos = len + i;
+            const int pi = pos / a.page, off = pos - pi * a.page;
+            const int p0 = (int)(((int64_t)len + a.page - 1) / a.page);
+            int32_t *row = a.table + (int64_t)b * a.s_table;
+            int id;
+            if (pi >= p0) {
+                int at = head + grow_off[bl] + (pi - p0);      // < 2 num_pages
+                if (at >= a.num_pages) at -= a.num_pages;
+                id = a.ring[at];
+                if (off == 0) row[pi] = id;                    // every new page begins with a new token
+            } else {
+                id = row[pi];
+            }
+            slot = (int64_t)id * a.page + off;
+        }
+        a.slots[(int64_t)b * a.T + i] = slot;
+    }
+    // pages that go back: a wave per request that gives some, of the requests whose first pair
+    // is this workgroup's
+    if (!bad && bsum > 0) {
+        const int lo = r0 ? 1 : 0, nb = b1 - b0 + 1;
+        for (int s = lo + wave * 64; s < nb; s += PLAN_THREADS) {
+            int p0 = 0, p1 = 0;
+            if (s + lane < nb) {
+                const int64_t len = a.lengths[b0 + s + lane], n = a.new_lens[b0 + s + lane];
+                p0 = (int)((len + a.page - 1) / a.page);
+                p1 = (int)((max(len + n, (int64_t)0) + a.page - 1) / a.page);
+            }
+            uint64_t todo = __ballot(p0 > p1);
+            while (todo) {
+                const int l = __ffsll((unsigned long long)todo) - 1;
+                todo &= todo - 1;
+                const int q0 = __shfl(p0, l), q1 = __shfl(p1, l);
+                int32_t *row = a.table + (int64_t)(b0 + s + l) * a.s_table;
+                for (int j = lane; j < q0 - q1; j += 64) {
+                    int64_t at = (int64_t)head + count + back_off[s + l] + j;   // < 3 num_pages
+                    at %= a.num_pages;
+                    a.ring[at] = row[q1 + j];
+                    row[q1 + j] = -1;
+                }
+            }
+        }
+    }
+    __syncthreads();   // the workgroup's reads of the state are done
+    if (tid == 0 && atomicAdd(&a.state[2], 1) == (int)gridDim.x - 1) {
+        if (!bad) {
+            a.state[0] = (int)((head + gsum) % a.num_pages);
+            a.state[1] = (int)(count - gsum + bsum);
+        }
+        a.state[2] = 0;
+        if (bad) a.state[3] |= bad;
+    }
+}
+
+// ------------------------------------------------------------------ append
+// One workgroup = one group of 32 tokens of one (request, KV head): the window of request b
+// is [its tail | its new tokens], group u the window's tokens 32 u ...  Rows go to LDS at 16
+// bits; a thread quantizes one key channel (32 tokens) or one value group (32 channels of a
+// token), codes as bytes in LDS, and the words are put together in the operands' order, 16
+// bytes a thread.  The workgroup of group 0 is the only reader of the old tail, so it also
+// writes the new one, behind its barrier.
+struct AppendArgs {
+    PagesDev p;
+    const uint16_t *k, *v;
+    int64_t s_kb, s_kh, s_kt, s_vb, s_vh, s_vt;
+    const int32_t *new_lens;
+    const int64_t *slots;
+    int T;
+};
+
+// 8 codes (bytes, elements 0..3 in a, 4..7 in b) as one word, nibbles 0 2 4 6 1 3 5 7
+__device__ __forceinline__ uint32_t pack_word(uint32_t a, uint32_t b) {
+    return (a & 0xfu) | ((a >> 12) & 0xf0u) | ((b << 8) & 0xf00u) | ((b >> 4) & 0xf000u) | ((a << 8) & 0xf0000u) |
+           ((a >> 4) & 0xf00000u) | ((b << 16) & 0xf000000u) | ((b << 4) & 0xf0000000u);
+}
+
+template <int D, int DT>
+__global__ __launch_bounds__(256) void page_append_kernel(AppendArgs a) {
+    constexpr int XS = D + 8;           // row stride of the 16-bit window, elements
+    constexpr int VS = PG_GROUP + 8;    // row stride of the value codes (channel-major), bytes
+    __shared__ __attribute__((aligned(16))) uint16_t X[2][PG_GROUP * XS];
+    __shared__ __attribute__((aligned(16))) uint8_t kc[PG_GROUP * D];
+    __shared__ __attribute__((aligned(16))) uint8_t vc[D * VS];
+    const int tid = threadIdx.x, u = blockIdx.x, h = blockIdx.y, b = blockIdx.z;
+    const int n = min(a.new_lens[b], a.T);
+    if (n <= 0 || a.slots[(int64_t)b * a.T] < 0) return;
+    const int len = pg_length(a.p, b), r = len & (PG_GROUP - 1);
+    const int whole = (r + n) / PG_GROUP;
+    if (u >= max(whole, 1)) return;
+    const uint16_t *kn = a.k + (int64_t)b * a.s_kb + (int64_t)h * a.s_kh;
+    const uint16_t *vn = a.v + (int64_t)b * a.s_vb + (int64_t)h * a.s_vh;
+    uint16_t *kt = a.p.kt + (int64_t)b * a.p.s_tb + (int64_t)h * a.p.s_th;
+    uint16_t *vt = a.p.vt + (int64_t)b * a.p.s_tb + (int64_t)h * a.p.s_th;
+    constexpr int CH = D / 8;           // 16-byte chunks of a row
+    if (u < whole) {
+#pragma unroll
+        for (int x = tid; x < 2 * PG_GROUP * CH; x += 256) {
+            const int kv = x / (PG_GROUP * CH), row = x / CH % PG_GROUP, c = x % CH;
+            const int j = u * PG_GROUP + row - r;    // new token, or below 0 a row of the tail
+            const uint16_t *src = kv ? (j < 0 ? vt + (int64_t)row * a.p.s_tt : vn + (int64_t)j * a.s_vt)
+                                     : (j < 0 ? kt + (int64_t)row * a.p.s_tt : kn + (int64_t)j * a.s_kt);
+            *(uint4 *)&X[kv][row * XS + 8 * c] = pg_load16(src + 8 * c);
+        }
+        __syncthreads();
+        // the group's record: its last token is a new one, and a group lies in one page
+        const int64_t slot = a.slots[(int64_t)b * a.T + (u + 1) * PG_GROUP - r - 1];
+        const int64_t page = slot >= 0 ? slot / a.p.page_tokens : -1;
+        uint8_t *rec = nullptr;
+        if (page >= 0 && page < a.p.num_pages)
+            rec = a.p.pool + page * a.p.s_page + (int64_t)h * a.p.s_head +
+                  (slot - page * a.p.page_tokens) / PG_GROUP * (int64_t)(40 * D);
+        auto ld = [](uint16_t x) { return DT == MA_BF16 ? ma_bf16_to_f32(x) : ma_f16_to_f32(x); };
+        if (tid < D) {
+            float x[PG_GROUP], lo = INFINITY, hi = -INFINITY;
+#pragma unroll
+            for (int t = 0; t < PG_GROUP; ++t) {
+                x[t] = ld(X[0][t * XS + tid]);
+                lo = fminf(lo, x[t]);
+                hi = fmaxf(hi, x[t]);
+            }
+            const QuantGroup q = quant_params(lo, hi, DT);
+#pragma unroll
+            for (int t = 0; t < PG_GROUP; ++t) kc[t * D + tid] = (uint8_t)quant_code(x[t], q, DT);
+            if (rec) {
+                *(_Float16 *)(rec + 32 * D + 2 * tid) = (_Float16)q.step;
+                *(_Float16 *)(rec + 34 * D + 2 * tid) = (_Float16)q.lo;
+            }
+        } else if (tid >= 128 && tid < 128 + D) {
+            const int t = tid & 31, cg = (tid - 128) >> 5;
+            float x[32], lo = INFINITY, hi = -INFINITY;
+#pragma unroll
+            for (int c = 0; c < 32; ++c) {
+                x[c] = ld(X[1][t * XS + 32 * cg + c]);
+                lo = fminf(lo, x[c]);
+                hi = fmaxf(hi, x[c]);
+            }
+            const QuantGroup q = quant_params(lo, hi, DT);
+#pragma unroll
+            for (int c = 0; c < 32; ++c) vc[(32 * cg + c) * VS + t] = (uint8_t)quant_code(x[c], q, DT);
+            if (rec) {
+                *(_Float16 *)(rec + 36 * D + 2 * (32 * cg + t)) = (_Float16)q.step;
+                *(_Float16 *)(rec + 38 * D + 2 * (32 * cg + t)) = (_Float16)q.lo;
+            }
+        }
+        __syncthreads();
+        if (rec) {
+            if (tid < 128) {            // (mt, h, m): D / 32 words
+                const int m = tid & 15, hh = (tid >> 4) & 3, mt = tid >> 6;
+                const uint8_t *src = &kc[(8 * (m >> 2) + 4 * mt + (m & 3)) * D + (D / 4) * hh];
+                uint32_t w[D / 32];
+#pragma unroll
+                for (int cb = 0; cb < D / 32; ++cb) {
+                    const uint2 c = *(const uint2 *)(src + 8 * cb);
+                    w[cb] = pack_word(c.x, c.y);
+                }
+                if constexpr (D == 128) *(uint4 *)(rec + 16 * tid) = uint4{w[0], w[1], w[2], w[3]};
+                else *(uint2 *)(rec + 8 * tid) = uint2{w[0], w[1]};
+            } else if (tid < 128 + D) { // (half, h, m): 4 words
+                const int x = tid - 128, m = x & 15, hh = (x >> 4) & 3, half = x >> 6;
+                uint32_t w[4];
+#pragma unroll
+                for (int c = 0; c < 4; ++c) {
+                    const uint2 s = *(const uint2 *)&vc[((D / 16) * m + 4 * half + c) * VS + 8 * hh];
+                    w[c] = pack_word(s.x, s.y);
+                }
+                *(uint4 *)(rec + 16 * D + 16 * x) = uint4{w[0], w[1], w[2], w[3]};
+            }
+        }
+    }
+    if (u != 0) return;
+    // the tail: new tokens behind the last whole group (in front of them, where none was
+    // completed, the tail's own rows stay)
+    const int first = whole ? 0 : r, j0 = whole ? whole * PG_GROUP - r : 0, cnt = n - j0;
+    for (int x = tid; x < 2 * cnt * CH; x += 256) {
+        const int kv = x / (cnt * CH), row = x / CH % cnt, c = x % CH;
+        const uint16_t *src = kv ? vn + (int64_t)(j0 + row) * a.s_vt : kn + (int64_t)(j0 + row) * a.s_kt;
+        uint16_t *dst = (kv ? vt : kt) + (int64_t)(first + row) * a.p.s_tt;
+        pg_store16(dst + 8 * c, pg_load16(src + 8 * c));
+    }
+}
+
+// ------------------------------------------------------------------ read-back
+// One wave = one group of 32 tokens of one (request, KV head), K by code words of 8 channels
+// (a lane keeps one octet of channels, so its parameters, for every token), V by lanes of
+// D / 16 channels x 8 tokens; every store instruction writes whole rows.
+struct DequantArgs {
+    PagesDev p;
+    const int32_t *starts;
+    void *ko, *vo;
+    int64_t s_kb, s_kh, s_kt, s_vb, s_vh, s_vt;
+    int n, groups;
+};
+
+// elements 2k, 2k+1 of a code word
+__device__ __forceinline__ void unpack_word(uint32_t w, uint32_t (&c)[8]) {
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+        c[2 * k] = (w >> (4 * k)) & 15u;
+        c[2 * k + 1] = (w >> (16 + 4 * k)) & 15u;
+    }
+}
+
+template <int OT>
+__device__ __forceinline__ uint32_t pack2(float a, float b) {
+    if constexpr (OT == MA_BF16) return ma_pack_bf16x2(a, b);
+    const f16x2_t v = {(_Float16)a, (_Float16)b};
+    return __builtin_bit_cast(uint32_t, v);
+}
+
+// N (4 or 8) values at element offset off
+template <int OT, int N>
+__device__ __forceinline__ void store_n(void *base, int64_t off, const float *x) {
+    if constexpr (OT == MA_F32) {
+#pragma unroll
+        for (int i = 0; i < N; i += 4)
+            pg_store16((float *)base + off + i, uint4{__float_as_uint(x[i]), __float_as_uint(x[i + 1]),
+                                                      __float_as_uint(x[i + 2]), __float_as_uint(x[i + 3])});
+    } else if constexpr (N == 8) {
+        pg_store16((uint16_t *)base + off, uint4{pack2<OT>(x[0], x[1]), pack2<OT>(x[2], x[3]), pack2<OT>(x[4], x[5]),
+                                                 pack2<OT>(x[6], x[7])});
+    } else {
+        pg_store8((uint16_t *)base + off, uint2{pack2<OT>(x[0], x[1]), pack2<OT>(x[2], x[3])});
+    }
+}
+
+__device__ __forceinline__ float half_of(uint32_t w, int hi) { return ma_f16_to_f32((uint16_t)(hi ? w >> 16 : w)); }
+
+template <int D, int OT>
+__global__ __launch_bounds__(256) void page_dequant_kernel(DequantArgs a, int dtype) {
+    constexpr int NO = D / 8, TPI = 64 / NO;   // octets of a row, tokens a wave takes at once
+    constexpr int NC = D / 16;
+    const int lane = threadIdx.x & 63;
+    const int gx = blockIdx.x * 4 + (threadIdx.x >> 6), h = blockIdx.y, b = blockIdx.z;
+    if (gx >= a.groups) return;
+    const int start = a.starts ? max(a.starts[b], 0) : 0;
+    const int len = pg_length(a.p, b);
+    const int64_t grp = start / PG_GROUP + (int64_t)gx;
+    const int64_t t0 = grp * PG_GROUP - start;                 // output row of the group's token 0
+    if (t0 >= a.n) return;
+    const int live = (int)min(max((int64_t)len - grp * PG_GROUP, (int64_t)0), (int64_t)PG_GROUP);   // its tokens
+    const int64_t kb = (int64_t)b * a.s_kb + (int64_t)h * a.s_kh, vb = (int64_t)b * a.s_vb + (int64_t)h * a.s_vh;
+    const int oct = lane % NO, tk = lane / NO;
+    if (live < PG_GROUP) {   // the tail, and what lies behind it
+        const int64_t tb = (int64_t)b * a.p.s_tb + (int64_t)h * a.p.s_th;
+        for (int t = tk; t < PG_GROUP; t += TPI) {
+            const int64_t row = t0 + t;
+            if (row < 0 || row >= a.n) continue;
+            float k[8] = {}, v[8] = {};
+            if (t < live) {
+                const uint4 kw = pg_load16(a.p.kt + tb + t * a.p.s_tt + 8 * oct);
+                const uint4 vw = pg_load16(a.p.vt + tb + t * a.p.s_tt + 8 * oct);
+                const uint32_t kx[4] = {kw.x, kw.y, kw.z, kw.w}, vx[4] = {vw.x, vw.y, vw.z, vw.w};
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                    const uint16_t ke = (uint16_t)(kx[i / 2] >> (16 * (i & 1)));
+                    const uint16_t ve = (uint16_t)(vx[i / 2] >> (16 * (i & 1)));
+                    k[i] = dtype == MA_BF16 ? ma_bf16_to_f32(ke) : ma_f16_to_f32(ke);
+                    v[i] = dtype == MA_BF16 ? ma_bf16_to_f32(ve) : ma_f16_to_f32(ve);
+                }
+            }
+            store_n<OT, 8>(a.ko, kb + row * a.s_kt + 8 * oct, k);
+            store_n<OT, 8>(a.vo, vb + row * a.s_vt + 8 * oct, v);
+        }
+        return;
+    }
+    const int per = a.p.page_tokens / PG_GROUP;
+    const int64_t pg = grp / per;
+    const uint8_t *rec = pg_record(a.p, a.p.table[(int64_t)b * a.p.s_table + pg], (int)(grp - pg * per), h, 40 * D);
+    {
+        const int hh = oct / (D / 32), cb = oct % (D / 32);
+        uint4 s4{}, z4{};
+        if (rec) {
+            s4 = *(const uint4 *)(rec + 32 * D + 16 * oct);
+            z4 = *(const uint4 *)(rec + 34 * D + 16 * oct);
+        }
+        const uint32_t sw[4] = {s4.x, s4.y, s4.z, s4.w}, zw[4] = {z4.x, z4.y, z4.z, z4.w};
+        uint32_t w[PG_GROUP / TPI];
+#pragma unroll
+        for (int i = 0; i < PG_GROUP / TPI; ++i) {
+            const int t = tk + i * TPI, mt = (t >> 2) & 1, m = 4 * (t >> 3) + (t & 3);
+            w[i] = rec ? *(const uint32_t *)(rec + 4 * (((mt * 4 + hh) * 16 + m) * (D / 32) + cb)) : 0u;
+        }
+#pragma unroll
+        for (int i = 0; i < PG_GROUP / TPI; ++i) {
+            const int64_t row = t0 + tk + i * TPI;
+            uint32_t c[8];
+            unpack_word(w[i], c);
+            float x[8];
+#pragma unroll
+            for (int e = 0; e < 8; ++e) x[e] = ma_dq(c[e], half_of(sw[e / 2], e & 1), half_of(zw[e / 2], e & 1));
+            if (row >= 0 && row < a.n) store_n<OT, 8>(a.ko, kb + row * a.s_kt + 8 * oct, x);
+        }
+    }
+    {
+        const int m = lane & 15, hh = lane >> 4;
+        uint4 s4{}, z4{};
+        uint32_t w[NC];
+#pragma unroll
+        for (int i = 0; i < NC; ++i) w[i] = 0u;
+        if (rec) {
+            const int cg = NC * m / 32;
+            s4 = *(const uint4 *)(rec + 36 * D + 2 * (32 * cg + 8 * hh));
+            z4 = *(const uint4 *)(rec + 38 * D + 2 * (32 * cg + 8 * hh));
+#pragma unroll
+            for (int half = 0; half < D / 64; ++half) {
+                const uint4 c = *(const uint4 *)(rec + 16 * D + 16 * (half * 64 + lane));
+                w[4 * half] = c.x;
+                w[4 * half + 1] = c.y;
+                w[4 * half + 2] = c.z;
+                w[4 * half + 3] = c.w;
+            }
+        }
+        const uint32_t sw[4] = {s4.x, s4.y, s4.z, s4.w}, zw[4] = {z4.x, z4.y, z4.z, z4.w};
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            const int64_t row = t0 + 8 * hh + i;
+            const float s = half_of(sw[i / 2], i & 1), z = half_of(zw[i / 2], i & 1);
+            float x[NC];
+#pragma unroll
+            for (int c = 0; c < NC; ++c) x[c] = ma_dq((w[c] >> ((i & 1) * 16 + (i / 2) * 4)) & 15u, s, z);
+            if (row >= 0 && row < a.n) store_n<OT, NC>(a.vo, vb + row * a.s_vt + NC * m, x);
+        }
+    }
+}
+
+bool no_data(const ma_tensor4 &t) { return t.ptr == nullptr; }
+
+}  // namespace
+
+int ma::pg_check(const ma_pages *p, int B, int H, int D, const char *who) {
+    if (!p || B <= 0 || H <= 0) {
+        ma_set_error("%s: bad geometry (B=%d H=%d)", who, B, H);
+        return MA_EINVAL;
+    }
+    if (D != 64 && D != 128) {
+        ma_set_error("%s: head_dim %d is not built (64, 128)", who, D);
+        return MA_EUNSUPPORTED;
+    }
+    if (p->dtype != MA_BF16 && p->dtype != MA_F16) {
+        ma_set_error("%s: tails must be bf16 or f16", who);
+        return MA_EUNSUPPORTED;
+    }
+    if (!p->pool || !p->k_tail || !p->v_tail || !p->table || !p->lengths) {
+        ma_set_error("%s: NULL page store", who);
+        return MA_EINVAL;
+    }
+    if (p->num_pages <= 0 || p->width <= 0 || p->page_tokens <= 0 || p->page_tokens % PG_GROUP ||
+        (p->mask && p->mask_tokens < 0)) {
+        ma_set_error("%s: bad page store (num_pages=%d width=%d page_tokens=%d, a multiple of 32)", who, p->num_pages,
+                     p->width, p->page_tokens);
+        return MA_EINVAL;
+    }
+    if (((uintptr_t)p->pool | (uintptr_t)p->s_pool[0] | (uintptr_t)p->s_pool[1]) % 16) {
+        ma_set_error("%s: pool and its strides must be 16-byte aligned", who);
+        return MA_EINVAL;
+    }
+    if ((int64_t)p->width * p->page_tokens > INT32_MAX) {
+        ma_set_error("%s: a request of more than 2^31 - 1 tokens is not built", who);
+        return MA_EUNSUPPORTED;
+    }
+    return MA_OK;
+}
+
+extern "C" int ma_page_plan(const int32_t *lengths, const int32_t *new_lens, int B, int T, int page_tokens,
+                            int32_t *table, int64_t s_table, int width, int32_t *ring, int num_pages, int32_t *state,
+                            int64_t *slots, int32_t *ends, void *stream) {
+    const char *who = "ma_page_plan";
+    if (B <= 0 || T < 0 || page_tokens <= 0 || page_tokens % PG_GROUP || width <= 0 || num_pages <= 0) {
+        ma_set_error("%s: bad arguments (B=%d T=%d page_tokens=%d, a multiple of 32, width=%d num_pages=%d)", who, B, T,
+                     page_tokens, width, num_pages);
+        return MA_EINVAL;
+    }
+    if (!lengths || !new_lens || !table || !ring || !state || !ends || (T > 0 && !slots)) {
+        ma_set_error("%s: NULL argument", who);
+        return MA_EINVAL;
+    }
+    const int64_t nflat = (int64_t)B * (T > 0 ? T : 1), wgs = (nflat + PLAN_SLOTS - 1) / PLAN_SLOTS;
+    if ((int64_t)width * page_tokens > INT32_MAX || wgs > INT32_MAX || num_pages > INT32_MAX / 4) {
+        ma_set_error("%s: more than 2^31 - 1 tokens of a request, 2^29 pages or 2^42 slots are not built", who);
+        return MA_EUNSUPPORTED;
+    }
+    PlanArgs a{lengths, new_lens, table, ring, state, ends, slots, s_table, nflat, B, T, page_tokens, width, num_pages};
+    page_plan_kernel<<<dim3((unsigned)wgs), PLAN_THREADS, 0, (hipStream_t)stream>>>(a);
+    return ma_check_launch(who);
+}
+
+extern "C" int ma_page_append(const ma_pages *p, ma_tensor4 k, ma_tensor4 v, int B, int H, int T, int D,
+                              const int32_t *new_lens, const int64_t *slots, void *stream) {
+    const char *who = "ma_page_append";
+    if (int rc = pg_check(p, B, H, D, who)) return rc;
+    if (T <= 0 || no_data(k) || no_data(v) || !new_lens || !slots) {
+        ma_set_error("%s: bad arguments (T=%d, or a NULL tensor)", who, T);
+        return MA_EINVAL;
+    }
+    if (k.dtype != p->dtype || v.dtype != p->dtype) {
+        ma_set_error("%s: new tokens and tails must share one dtype", who);
+        return MA_EINVAL;
+    }
+    const int64_t units = ((int64_t)T + PG_GROUP - 1) / PG_GROUP;
+    if (B > 65535 || H > 65535) {
+        ma_set_error("%s: more than 65535 requests or heads are not built", who);
+        return MA_EUNSUPPORTED;
+    }
+    AppendArgs a{pages_dev(p), (const uint16_t *)k.ptr, (const uint16_t *)v.ptr, k.s[0], k.s[1], k.s[2], v.s[0],
+                 v.s[1], v.s[2], new_lens, slots, T};
+    // (31 + T) / 32 groups can become whole, one workgroup at least writes the tail
+    const dim3 grid((unsigned)units, H, B);
+    hipStream_t st = (hipStream_t)stream;
+    if (D == 128 && p->dtype == MA_BF16) page_append_kernel<128, MA_BF16><<<grid, 256, 0, st>>>(a);
+    else if (D == 128) page_append_kernel<128, MA_F16><<<grid, 256, 0, st>>>(a);
+    else if (p->dtype == MA_BF16) page_append_kernel<64, MA_BF16><<<grid, 256, 0, st>>>(a);
+    else page_append_kernel<64, MA_F16><<<grid, 256, 0, st>>>(a);
+    return ma_check_launch(who);
+}
+
+extern "C" int ma_page_dequant(const ma_pages *p, int B, int H, int D, const int32_t *starts, int n, ma_tensor4 k_out,
+                               ma_tensor4 v_out, void *stream) {
+    const char *who = "ma_page_dequant";
+    if (int rc = pg_check(p, B, H, D, who)) return rc;
+    if (n < 0 || (n > 0 && (no_data(k_out) || no_data(v_out)))) {
+        ma_set_error("%s: bad arguments (n=%d, or a NULL output)", who, n);
+        return MA_EINVAL;
+    }
+    if (k_out.dtype != v_out.dtype || k_out.dtype < MA_F32 || k_out.dtype > MA_BF16) {
+        ma_set_error("%s: outputs must share one dtype of bf16, f16, f32", who);
+        return MA_EINVAL;
+    }
+    if (B > 65535 || H > 65535) {
+        ma_set_error("%s: more than 65535 requests or heads are not built", who);
+        return MA_EUNSUPPORTED;
+    }
+    if (n == 0) return MA_OK;
+    // a range that begins inside a group touches one more
+    const int groups = (int)(((int64_t)n + PG_GROUP - 1) / PG_GROUP) + (starts ? 1 : 0);
+    DequantArgs a{pages_dev(p), starts, k_out.ptr, v_out.ptr, k_out.s[0], k_out.s[1], k_out.s[2], v_out.s[0],
+                  v_out.s[1], v_out.s[2], n, groups};
+    const dim3 grid((unsigned)((groups + 3) / 4), H, B);
+    hipStream_t st = (hipStream_t)stream;
+#define MA_DQ(d, o) page_dequant_kernel<d, o><<<grid, 256, 0, st>>>(a, p->dtype)
+    if (D == 128) {
+        if (k_out.dtype == MA_BF16) MA_DQ(128, MA_BF16);
+        else if (k_out.dtype == MA_F16) MA_DQ(128, MA_F16);
+        else MA_DQ(128, MA_F32);
+    } else {
+        if (k_out.dtype == MA_BF16) MA_DQ(64, MA_BF16);
+        else if (k_out.dtype == MA_F16) MA_DQ(64, MA_F16);
+        else MA_DQ(64, MA_F32);
+    }
+#undef MA_DQ
+    return ma_check_launch(who);
+}
