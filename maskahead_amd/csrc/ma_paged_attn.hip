@@ -63,15 +63,38 @@ __device__ __forceinline__ Items items_of(const AttnArgs &a, int b) {
     return r;
 }
 
+// ... of a request that the whole wave looks at
+__device__ __forceinline__ Items items_at(const AttnArgs &a, int b) {
+    Items r = items_of(a, b);
+    r.n = uniform(r.n);
+    r.len = uniform(r.len);
+    r.ng = uniform(r.ng);
+    r.rem = uniform(r.rem);
+    r.items = uniform(r.items);
+    return r;
+}
+
+// The lane's number, as a value that nothing is known of: what is computed from it stays where
+// it is used, where the compiler would otherwise keep every address of the rare paths in
+// registers across the main loop (it spilled 170 of them).
+__device__ __forceinline__ int hidden(int lane) {
+    asm volatile("" : "+v"(lane));
+    return lane;
+}
+
+// (x & mask) | bits in one instruction (its constants lie in registers)
+__device__ __forceinline__ uint32_t and_or(uint32_t x, uint32_t mask, uint32_t bits) {
+    uint32_t r;
+    asm("v_and_or_b32 %0, %1, %2, %3" : "=v"(r) : "v"(x), "s"(mask), "v"(bits));
+    return r;
+}
 // pairs of codes as f16 (exact), the k-th pair of a code word
 __device__ __forceinline__ f16x2_t code_pair(uint32_t w, int k) {
     const uint32_t x = k & 2 ? w >> 8 : w;
-    if (k & 1) {
-        const uint32_t y = (x & 0x00f000f0u) | 0x54005400u;   // 64 + code
-        return __builtin_bit_cast(f16x2_t, y) - (f16x2_t){(_Float16)64.0f, (_Float16)64.0f};
-    }
-    const uint32_t y = (x & 0x000f000fu) | 0x64006400u;       // 1024 + code
-    return __builtin_bit_cast(f16x2_t, y) - (f16x2_t){(_Float16)1024.0f, (_Float16)1024.0f};
+    if (k & 1)     // 64 + code
+        return __builtin_bit_cast(f16x2_t, and_or(x, 0x00f000f0u, 0x54005400u)) - (f16x2_t){(_Float16)64.0f, (_Float16)64.0f};
+    return __builtin_bit_cast(f16x2_t, and_or(x, 0x000f000fu, 0x64006400u)) -      // 1024 + code
+           (f16x2_t){(_Float16)1024.0f, (_Float16)1024.0f};
 }
 
 // the 8 values of a code word; s, z: their parameters, pair by pair
@@ -107,14 +130,18 @@ __device__ __forceinline__ float sum_rows(float v) {
 
 // one record's words of a wave
 template <int D>
-struct Raw {
-    uint4 ks[D / 32], kz[D / 32], vs, vz, v[D / 64];
+struct RawK {
+    uint4 s[D / 32], z[D / 32];
     uint32_t k[2][D / 32];
+};
+template <int D>
+struct RawV {
+    uint4 s, z, v[D / 64];
 };
 
 template <int D>
-__device__ __forceinline__ void load_k(Raw<D> &w, const uint8_t *rec, int lane) {
-    const int h = lane >> 4;
+__device__ __forceinline__ void load_k(RawK<D> &w, const uint8_t *rec, int lane_) {
+    const uint32_t lane = (uint32_t)hidden(lane_), h = lane >> 4;   // scalar base + 32-bit lane offsets
 #pragma unroll
     for (int mt = 0; mt < 2; ++mt) {
         if constexpr (D == 128) {
@@ -127,40 +154,196 @@ __device__ __forceinline__ void load_k(Raw<D> &w, const uint8_t *rec, int lane) 
     }
 #pragma unroll
     for (int cb = 0; cb < D / 32; ++cb) {
-        w.ks[cb] = *(const uint4 *)(rec + 32 * D + 2 * (D / 4) * h + 16 * cb);
-        w.kz[cb] = *(const uint4 *)(rec + 34 * D + 2 * (D / 4) * h + 16 * cb);
+        w.s[cb] = *(const uint4 *)(rec + 32 * D + ((D / 2) * h + 16 * cb));
+        w.z[cb] = *(const uint4 *)(rec + 34 * D + ((D / 2) * h + 16 * cb));
     }
 }
 template <int D>
-__device__ __forceinline__ void load_v(Raw<D> &w, const uint8_t *rec, int lane) {
-    const int h = lane >> 4, m = lane & 15, cg = (D / 16) * m / 32;
+__device__ __forceinline__ void load_v(RawV<D> &w, const uint8_t *rec, int lane_) {
+    const uint32_t lane = (uint32_t)hidden(lane_), h = lane >> 4, m = lane & 15u, cg = (D / 16) * m / 32;
 #pragma unroll
-    for (int half = 0; half < D / 64; ++half) w.v[half] = *(const uint4 *)(rec + 16 * D + 16 * (64 * half + lane));
-    w.vs = *(const uint4 *)(rec + 36 * D + 2 * (32 * cg + 8 * h));
-    w.vz = *(const uint4 *)(rec + 38 * D + 2 * (32 * cg + 8 * h));
+    for (int half = 0; half < D / 64; ++half) w.v[half] = *(const uint4 *)(rec + (16 * D + 1024 * half) + 16 * lane);
+    w.s = *(const uint4 *)(rec + 36 * D + 2 * (32 * cg + 8 * h));
+    w.z = *(const uint4 *)(rec + 38 * D + 2 * (32 * cg + 8 * h));
+}
+// the same registers for a wave that unpacks one or the other
+template <int D>
+__device__ __forceinline__ void v_into(RawK<D> &w, const RawV<D> &v) {
+#pragma unroll
+    for (int mt = 0; mt < 2; ++mt)
+#pragma unroll
+        for (int x = 0; x < D / 32; ++x) {
+            const int ct = mt * (D / 32) + x;
+            const uint4 y = v.v[ct / 4];
+            w.k[mt][x] = (ct & 3) == 0 ? y.x : (ct & 3) == 1 ? y.y : (ct & 3) == 2 ? y.z : y.w;
+        }
+    w.s[0] = v.s;
+    w.z[0] = v.z;
+}
+template <int D>
+__device__ __forceinline__ RawV<D> v_from(const RawK<D> &w) {
+    RawV<D> v;
+#pragma unroll
+    for (int x = 0; x < D / 64; ++x) {
+        const uint32_t *y = &w.k[0][0] + 4 * x;
+        v.v[x] = uint4{y[0], y[1], y[2], y[3]};
+    }
+    v.s = w.s[0];
+    v.z = w.z[0];
+    return v;
+}
+template <int D>
+__device__ __forceinline__ uint32_t v_word(const RawV<D> &w, int ct) {
+    const uint4 x = w.v[ct / 4];
+    return (ct & 3) == 0 ? x.x : (ct & 3) == 1 ? x.y : (ct & 3) == 2 ? x.z : x.w;
+}
+
+__device__ __forceinline__ uint32_t halves_of(uint32_t bits) {   // bit 0 -> low half, bit 1 -> high half
+    return (bits & 1u ? 0xffffu : 0u) | (bits & 2u ? 0xffff0000u : 0u);
+}
+// a dead token's value is 0 whatever its parameters say; live: bit i = token i of the lane's 8
+template <int D>
+__device__ __forceinline__ void clear_dead(RawV<D> &w, uint32_t live) {
+    const uint32_t h0 = halves_of(live), h1 = halves_of(live >> 2), h2 = halves_of(live >> 4), h3 = halves_of(live >> 6);
+    w.s = uint4{w.s.x & h0, w.s.y & h1, w.s.z & h2, w.s.w & h3};
+    w.z = uint4{w.z.x & h0, w.z.y & h1, w.z.z & h2, w.z.w & h3};
+}
+
+// the nonzero bytes of x, as 4 bits
+__device__ __forceinline__ uint32_t byte_bits(uint32_t x) {
+    x |= x >> 4;
+    x |= x >> 2;
+    x |= x >> 1;
+    return ((x & 0x01010101u) * 0x10204080u) >> 28;
+}
+// the seen ones of a lane's 8 tokens from position pos on, of a request with a mask
+__device__ __forceinline__ uint32_t mask_bits(const PagesDev &p, int b, int h, int pos) {
+    const uint8_t *m = p.mask + (int64_t)b * p.s_mb + (int64_t)h * p.s_mh;
+    const int n = p.mask_tokens;
+    if (n >= 8) {     // 8 bytes that the mask has, moved to where they belong
+        const int at = min(pos, n - 8), out = min(pos - at, 8);
+        const pg_b8 v = *(const pg_b8 *)(m + (uint32_t)at);
+        return (byte_bits(v.x) | byte_bits(v.y) << 4) >> out;
+    }
+    uint32_t bits = 0;
+    for (int i = 0; i < 8; ++i)
+        if (pos + i < n && m[pos + i]) bits |= 1u << i;
+    return bits;
+}
+
+// ---- rows of 16-bit K and V (the tail, or 32 keys of the block) as operands
+struct Rows {
+    const uint16_t *k, *v;
+    int64_t sk, sv;
+    int j0, cnt;      // first row, rows there are
+    bool tail;
+};
+// item x behind the packed groups of (b, h); cnt 0: nothing there
+__device__ __forceinline__ Rows rows_of(const AttnArgs &a, const Items &it, int b, int h, int x) {
+    Rows r;
+    r.tail = it.rem && x == 0;
+    if (r.tail) {
+        r.k = a.p.kt + (int64_t)b * a.p.s_tb + (int64_t)h * a.p.s_th;
+        r.v = a.p.vt + (int64_t)b * a.p.s_tb + (int64_t)h * a.p.s_th;
+        r.sk = r.sv = a.p.s_tt;
+        r.j0 = 0;
+        r.cnt = it.rem;
+    } else {
+        r.k = (const uint16_t *)a.kc.ptr + (int64_t)b * a.kc.s[0] + (int64_t)h * a.kc.s[1];
+        r.v = (const uint16_t *)a.vc.ptr + (int64_t)b * a.vc.s[0] + (int64_t)h * a.vc.s[1];
+        r.sk = a.kc.s[2];
+        r.sv = a.vc.s[2];
+        r.j0 = (x - (it.rem ? 1 : 0)) * PG_GROUP;
+        r.cnt = a.kc.ptr ? it.n : 0;
+    }
+    return r;
+}
+// the seen ones of lane quarter hh's 8 rows
+template <bool MASK>
+__device__ __forceinline__ uint32_t rows_live(const AttnArgs &a, const Items &it, const Rows &r, int b, int h, int hh) {
+    uint32_t seen = 255u >> min(max(r.j0 + 8 * hh + 8 - r.cnt, 0), 8);
+    if (MASK && r.tail) seen &= mask_bits(a.p, b, h, it.ng * PG_GROUP + 8 * hh);
+    return seen;
+}
+// (rows behind the last are read from the last one, so that no load waits for a branch; their
+// scores are masked)
+template <int D>
+__device__ __forceinline__ void rows_k(const Rows &r, int lane, int mt, uint4 *k) {
+    const int n16 = lane & 15, hh = lane >> 4;
+    const int j = min(r.j0 + 8 * (n16 >> 2) + 4 * mt + (n16 & 3), r.cnt - 1);
+    const uint16_t *src = r.k + (int64_t)j * r.sk + (D / 4) * hh;
+#pragma unroll
+    for (int cb = 0; cb < D / 32; ++cb) k[cb] = pg_load16(src + 8 * cb);
+}
+// V: 8 tokens x D/16 channels of a lane as they lie (0 where not seen), and one channel of
+// them as an operand
+template <int D>
+__device__ __forceinline__ void rows_v(const Rows &r, int lane, uint32_t seen, uint32_t (&vw)[8][D / 32]) {
+    constexpr int NC = D / 16;
+    const int n16 = lane & 15, hh = lane >> 4;
+#pragma unroll
+    for (int y = 0; y < 8; ++y) {
+        const int j = min(r.j0 + 8 * hh + y, r.cnt - 1);
+        const uint16_t *src = r.v + (int64_t)j * r.sv + NC * n16;
+        const uint32_t ok = (seen >> y) & 1u ? 0xffffffffu : 0u;
+        if constexpr (NC == 8) {
+            const uint4 x = pg_load16(src);
+            vw[y][0] = x.x & ok; vw[y][1] = x.y & ok; vw[y][2] = x.z & ok; vw[y][3] = x.w & ok;
+        } else {
+            const uint2 x = pg_load8(src);
+            vw[y][0] = x.x & ok; vw[y][1] = x.y & ok;
+        }
+    }
+}
+template <int D>
+__device__ __forceinline__ uint4 rows_channel(const uint32_t (&vw)[8][D / 32], int ct) {
+    uint32_t x[4];
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+        const uint32_t lo = vw[2 * k][ct / 2], hi = vw[2 * k + 1][ct / 2];
+        x[k] = ct & 1 ? (lo >> 16) | (hi & 0xffff0000u) : (lo & 0xffffu) | (hi << 16);
+    }
+    return uint4{x[0], x[1], x[2], x[3]};
+}
+// of row's (head group, block position) pair, the tokens of the block's item that it sees
+__device__ __forceinline__ uint32_t causal_live(const AttnArgs &a, const Items &it, const Rows &r, int row, int hh,
+                                                uint32_t live) {
+    if (r.tail || a.causal <= 0) return live;
+    const int tq = row % a.T;
+    const int64_t lim = ((int64_t)it.len + tq) / a.causal * a.causal + a.causal - it.len;    // keys j < lim
+    const int64_t over = r.j0 + 8 * hh + 8 - lim;
+    return live & (255u >> (over < 0 ? 0 : over > 8 ? 8 : (int)over));
 }
 
 // a row tile's running softmax and output: lane (n = lane & 15, h = lane >> 4) holds row n,
-// channels (D/16)(4 h + r) + ct in acc[ct][r]; m and l of row n, l over the lane's own tokens
+// channels (D/16)(4 h + r) + ct in acc[ct][r]; the row's reference maximum m and, in every
+// component of l, its sum of probabilities (a product with ones: the sum of what is multiplied)
 template <int D>
 struct Tile {
-    f32x4_t acc[D / 16];
-    float m, l;
+    f32x4_t acc[D / 16], l;
+    float m;
 };
+template <int D>
+__device__ __forceinline__ void clear(Tile<D> &t) {
+#pragma unroll
+    for (int ct = 0; ct < D / 16; ++ct) t.acc[ct] = f32x4_t{};
+    t.l = f32x4_t{};
+    t.m = NO_MAX;
+}
 
-// scores s (x sl2 -> exponents of 2) of a lane's 8 tokens -> probabilities; live: bit i =
-// token i is seen.  Raises the row's maximum where needed.
+// scores s (x c -> exponents of 2) of a lane's 8 tokens -> probabilities; live: bit i = token
+// i is seen.  Raises the row's maximum where needed.
 template <int D>
 __device__ __forceinline__ void softmax8(Tile<D> &t, const f32x4_t &s0, const f32x4_t &s1, float c, bool masked,
                                          uint32_t live, float (&p)[8]) {
     float x[8];
-    float mx = -INFINITY;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-        x[i] = __builtin_fmaf(i < 4 ? s0[i & 3] : s1[i & 3], c, -t.m);
-        if (masked) x[i] = (live >> i) & 1u ? x[i] : -INFINITY;
-        mx = fmaxf(mx, x[i]);
+    for (int i = 0; i < 8; ++i) x[i] = __builtin_fmaf(i < 4 ? s0[i & 3] : s1[i & 3], c, -t.m);
+    if (masked) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) x[i] = (live >> i) & 1u ? x[i] : -INFINITY;
     }
+    const float mx = fmaxf(fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])), fmaxf(fmaxf(x[4], x[5]), fmaxf(x[6], x[7])));
     if (__any(mx > LAZY)) {
         float top = -INFINITY;
 #pragma unroll
@@ -178,51 +361,87 @@ __device__ __forceinline__ void softmax8(Tile<D> &t, const f32x4_t &s0, const f3
         t.l *= f;
         t.m = m;
     }
-    float sum = 0.f;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-        p[i] = __builtin_amdgcn_exp2f(x[i]);
-        sum += p[i];
+    for (int i = 0; i < 8; ++i) p[i] = __builtin_amdgcn_exp2f(x[i]);
+}
+
+__device__ __forceinline__ f16x8_t as_f16(const float (&p)[8]) {
+    f16x8_t r;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) r[i] = (_Float16)p[i];
+    return r;
+}
+__device__ __forceinline__ f16x8_t ones_f16() {
+    f16x8_t r;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) r[i] = (_Float16)1.0f;
+    return r;
+}
+
+// 16-bit rows as they are: f16 like the packed ones, bf16 in bf16 products with each
+// probability as a sum of two bf16
+template <bool BF16>
+struct Probs {
+    f16x8_t p;
+};
+template <>
+struct Probs<true> {
+    b16x8_t hi, lo;
+};
+template <int CB, bool BF16>
+__device__ __forceinline__ f32x4_t rows_scores(const uint4 *k, const uint4 *q) {
+    f32x4_t s{};
+#pragma unroll
+    for (int cb = 0; cb < CB; ++cb) {
+        if constexpr (BF16) s = mfma16(__builtin_bit_cast(b16x8_t, k[cb]), __builtin_bit_cast(b16x8_t, q[cb]), s);
+        else s = mfma16(__builtin_bit_cast(f16x8_t, k[cb]), __builtin_bit_cast(f16x8_t, q[cb]), s);
     }
-    t.l += sum;
+    return s;
 }
-
-__device__ __forceinline__ uint32_t halves_of(uint32_t bits) {   // bit 0 -> low half, bit 1 -> high half
-    return (bits & 1u ? 0xffffu : 0u) | (bits & 2u ? 0xffff0000u : 0u);
-}
-
-// the seen ones of a lane's 8 tokens from position pos on
-__device__ __forceinline__ uint32_t mask_bits(const PagesDev &p, int b, int h, int64_t pos) {
-    const uint8_t *m = p.mask + (int64_t)b * p.s_mb + (int64_t)h * p.s_mh + pos;
-    uint32_t bits = 0;
-    if (pos + 8 <= p.mask_tokens) {
-        const pg_b8 v = *(const pg_b8 *)m;
+template <int D, bool BF16>
+__device__ __forceinline__ Probs<BF16> rows_probs(Tile<D> &t, const f32x4_t &s0, const f32x4_t &s1, float c, uint32_t live) {
+    Probs<BF16> r;
+    float p[8];
+    softmax8(t, s0, s1, c, true, live, p);
+    if constexpr (BF16) {
+        b16x8_t one;
 #pragma unroll
-        for (int i = 0; i < 8; ++i) bits |= ((i < 4 ? v.x : v.y) >> (8 * (i & 3)) & 255u) ? 1u << i : 0u;
+        for (int y = 0; y < 8; ++y) {
+            r.hi[y] = (__bf16)p[y];
+            r.lo[y] = (__bf16)(p[y] - (float)r.hi[y]);
+            one[y] = (__bf16)1.0f;
+        }
+        t.l = mfma16(one, r.lo, mfma16(one, r.hi, t.l));
     } else {
-        for (int i = 0; i < 8; ++i)
-            if (pos + i < p.mask_tokens && m[i]) bits |= 1u << i;
+        r.p = as_f16(p);
+        t.l = mfma16(ones_f16(), r.p, t.l);
     }
-    return bits;
+    return r;
+}
+__device__ __forceinline__ f32x4_t rows_values(uint4 v, const Probs<true> &p, f32x4_t acc) {
+    const b16x8_t x = __builtin_bit_cast(b16x8_t, v);
+    return mfma16(x, p.lo, mfma16(x, p.hi, acc));
+}
+__device__ __forceinline__ f32x4_t rows_values(uint4 v, const Probs<false> &p, f32x4_t acc) {
+    return mfma16(__builtin_bit_cast(f16x8_t, v), p.p, acc);
 }
 
-// Q of one row tile as B operands: lane (n, h) = row n, channels (D/4) h + 8 cb + (0..7)
+// ---- Q of one row tile as B operands: lane (n, h) = row n, channels (D/4) h + 8 cb + (0..7);
+// rows behind the request's new tokens are zero
 template <int D>
-__device__ __forceinline__ const uint16_t *q_row(const AttnArgs &a, int b, int h, int row, int n, bool &ok) {
-    const int g = row / a.T, t = row - g * a.T;
-    ok = row < a.R && t < n;
-    return (const uint16_t *)a.q.ptr + (int64_t)b * a.q.s[0] + (int64_t)(h * a.G + g) * a.q.s[1] +
-           (int64_t)t * a.q.s[2];
-}
-template <int D>
-__device__ __forceinline__ void load_q_raw(const AttnArgs &a, int b, int h, int row, int n, int hh, uint4 *q) {
-    bool ok;
-    const uint16_t *src = q_row<D>(a, b, h, row, n, ok);
+__device__ __forceinline__ void load_q(const AttnArgs &a, int b, int h, int row, int n, int hh, uint4 *q) {
+    const int rc = min(row, a.R - 1), g = rc / a.T, t = rc - g * a.T;
+    const uint32_t ok = row < a.R && t < n ? 0xffffffffu : 0u;
+    const uint16_t *src = (const uint16_t *)a.q.ptr + (int64_t)b * a.q.s[0] + (int64_t)(h * a.G + g) * a.q.s[1] +
+                          (int64_t)t * a.q.s[2] + (D / 4) * hh;
 #pragma unroll
-    for (int cb = 0; cb < D / 32; ++cb) q[cb] = ok ? pg_load16(src + (D / 4) * hh + 8 * cb) : uint4{0, 0, 0, 0};
+    for (int cb = 0; cb < D / 32; ++cb) {
+        const uint4 x = pg_load16(src + 8 * cb);
+        q[cb] = uint4{x.x & ok, x.y & ok, x.z & ok, x.w & ok};
+    }
 }
 // bf16 queries as f16: scaled by a power of two that puts the row's largest in [1, 2), so that
-// no query overflows f16 and what underflows is below 2^-24 of it; the factor goes into c
+// no query overflows f16 and what underflows is below 2^-24 of it; returns the factor back
 template <int D>
 __device__ __forceinline__ float q_as_f16(uint4 *q) {
     float mx = 0.f;
@@ -250,25 +469,25 @@ __device__ __forceinline__ float q_as_f16(uint4 *q) {
     return up;
 }
 
-template <int D, int NT>
-struct Shared {
-    static constexpr int OS = D + 4;                 // row stride of a wave's output rows, f32
-    float o[WAVES][16 * OS];
-    float m[WAVES][16], l[WAVES][16];
-    uint4 q[NT > 2 ? NT * (D / 32) * 64 : 1];        // Q operands of many row tiles
-    float qc[NT > 2 ? NT * 16 : 1];
-    int64_t wsum[WAVES];
-    int64_t found_pre;
-    int found_b;
+// ---- the line of items
+struct Stretch {
+    int64_t w, s, e, chunk;   // this workgroup's place and its items [s, e); items of a stretch
+    int64_t pre;              // items (x HR) of the requests before b
+    int b;                    // the request in which s lies
+};
+struct ScanShared {
+    int64_t wsum[16], pre;
+    int b;
 };
 
-// items of all requests; the request in which the line's position s (of HR lines of every
-// request's items, in a row) lies and the items before it
-template <class S>
-__device__ __forceinline__ int64_t scan_items(const AttnArgs &a, S &sh, int64_t &total_out, int64_t HR, int min_items,
-                                              int64_t &chunk) {
+// Items of all requests, by a scan of the lengths in every workgroup (8 B a request, from L2);
+// the line holds HR items of each, stretches are of a multiple of `unit` items
+template <int THREADS>
+__device__ __forceinline__ Stretch find_stretch(const AttnArgs &a, ScanShared &sh, int unit) {
+    constexpr int NW = THREADS / 64;
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-    const int per = (a.B + 255) / 256, first = tid * per;
+    const int64_t HR = (int64_t)a.H * a.RG;
+    const int per = (a.B + THREADS - 1) / THREADS, first = tid * per;
     int64_t sum = 0;
     for (int i = 0; i < per; ++i)
         if (first + i < a.B) sum += items_of(a, first + i).items;
@@ -282,20 +501,20 @@ __device__ __forceinline__ int64_t scan_items(const AttnArgs &a, S &sh, int64_t 
     __syncthreads();
     int64_t before = inc - sum, total = 0;
 #pragma unroll
-    for (int w = 0; w < WAVES; ++w) {
+    for (int w = 0; w < NW; ++w) {
         if (w < wave) before += sh.wsum[w];
         total += sh.wsum[w];
     }
     total = uniform(total) * HR;
-    const int64_t most = (total + min_items - 1) / min_items;
-    const int64_t weff = most < a.W ? most : (int64_t)a.W;
-    chunk = weff > 0 ? (total + weff - 1) / weff : 1;
+    Stretch r;
     // stretches of one XCD's workgroups lie next to one another: row groups share its L2
-    const int w8 = a.W / 8;
-    const int64_t w = (int64_t)(blockIdx.x % 8) * w8 + blockIdx.x / 8;
-    const int64_t s = w * chunk;
-    if (s < total) {
-        const int64_t want = s / HR;
+    r.w = (int64_t)(blockIdx.x % 8) * (a.W / 8) + blockIdx.x / 8;
+    const int64_t each = (total + a.W - 1) / a.W;
+    r.chunk = max((each + unit - 1) / unit, (int64_t)1) * unit;
+    r.s = r.w * r.chunk;
+    r.e = min(r.s + r.chunk, total);
+    if (r.s < total) {
+        const int64_t want = r.s / HR;
         if (want >= before && want < before + sum) {
             int64_t pre = before;
             int b = first;
@@ -304,259 +523,201 @@ __device__ __forceinline__ int64_t scan_items(const AttnArgs &a, S &sh, int64_t 
                 if (want < pre + n) break;
                 pre += n;
             }
-            sh.found_b = b;
-            sh.found_pre = pre;
+            sh.b = b;
+            sh.pre = pre;
         }
     }
     __syncthreads();
-    total_out = total;
-    return w;
+    r.b = uniform(sh.b);
+    r.pre = uniform(sh.pre);
+    return r;
 }
 
-template <int D, int NT, bool BF16>
-__global__ __launch_bounds__(256, NT == 1 ? 2 : 1) void paged_attn_kernel(AttnArgs a, int min_items) {
-    constexpr int CB = D / 32, NC = D / 16;
-    constexpr bool QLDS = NT > 2;
-    __shared__ Shared<D, NT> sh;
-    const int tid = threadIdx.x, lane = tid & 63, wave = uniform(tid >> 6), n16 = lane & 15, hh = lane >> 4;
-    const int HR = a.H * a.RG;
-    int64_t total, chunk;
-    const int64_t w = scan_items(a, sh, total, HR, min_items, chunk);
-    const int64_t s = w * chunk;
-    int4 desc{-1, 0, 0, 0};
-    const int64_t e = min(s + chunk, total);
-    int b = uniform(sh.found_b);
-    int64_t pre = uniform(sh.found_pre), pos = s;
-    Items it = pos < e ? items_of(a, b) : Items{};
-    while (pos < e) {
-        const int64_t rel = pos - HR * pre;
-        const int hr = (int)(rel / it.items), i0 = (int)(rel - (int64_t)hr * it.items);
-        const int i1 = (int)min((int64_t)it.items, i0 + (e - pos));
-        const int h = hr / a.RG, rg = hr - h * a.RG;
-        const int row0 = rg * NT * 16;
+// the part of a segment that lies in a stretch
+struct Part {
+    int h, rg, hr, i0, i1;
+    bool whole;
+    int64_t slot;     // of its partial, where it is not whole: the first or the last of the stretch
+};
+__device__ __forceinline__ Part part_of(const AttnArgs &a, const Stretch &st, const Items &it, int64_t pos) {
+    Part p;
+    const int64_t rel = pos - (int64_t)a.H * a.RG * st.pre;
+    p.hr = (int)(rel / it.items);
+    p.i0 = (int)(rel - (int64_t)p.hr * it.items);
+    p.i1 = (int)min((int64_t)it.items, p.i0 + (st.e - pos));
+    p.h = p.hr / a.RG;
+    p.rg = p.hr - p.h * a.RG;
+    p.whole = p.i0 == 0 && p.i1 == it.items;
+    p.slot = 2 * st.w + (pos > st.s ? 1 : 0);
+    return p;
+}
+// what the merge needs of a cut segment, left by its first stretch: (request, (head, row
+// group), first slot, stretches)
+__device__ __forceinline__ int4 cut_desc(const Stretch &st, const Items &it, const Part &p, int64_t pos) {
+    return int4{st.b, p.hr, (int)p.slot, (int)((pos + it.items - 1) / st.chunk - st.w + 1)};
+}
+__device__ __forceinline__ void next_part(const AttnArgs &a, Stretch &st, Items &it, const Part &p, int64_t &pos) {
+    pos += p.i1 - p.i0;
+    if (p.i1 == it.items && p.hr == a.H * a.RG - 1 && pos < st.e) {
+        st.pre += it.items;
+        do it = items_at(a, ++st.b);
+        while (it.items == 0);
+    }
+}
 
-        // ---- Q
-        uint4 q[QLDS ? 1 : NT][CB];
+// the record of group i of (b, h); absent ones are read from the pool's first record, dead
+template <int D>
+__device__ __forceinline__ const uint8_t *record_of(const AttnArgs &a, const int32_t *trow, int i, int h, bool &dead) {
+    const int per = a.p.page_tokens / PG_GROUP, pg = i / per;
+    const uint8_t *r = pg_record(a.p, uniform(trow[pg]), i - pg * per, h, 40 * D);
+    dead = r == nullptr;
+    return dead ? a.p.pool : r;
+}
+
+template <bool BF16>
+__device__ __forceinline__ uint32_t pack_out(float x, float y) {
+    if constexpr (BF16) return ma_pack_bf16x2(x, y);
+    const f16x2_t z = {(_Float16)x, (_Float16)y};
+    return __builtin_bit_cast(uint32_t, z);
+}
+// NC channels of a row, to its place in out
+template <int NC, bool BF16>
+__device__ __forceinline__ void store_out(const AttnArgs &a, int b, int h, int row, int ch, const float *o) {
+    const int g = row / a.T, t = row - g * a.T;
+    uint16_t *dst = (uint16_t *)a.out.ptr + (int64_t)b * a.out.s[0] + (int64_t)(h * a.G + g) * a.out.s[1] +
+                    (int64_t)t * a.out.s[2] + ch;
+    uint32_t y[NC / 2];
+#pragma unroll
+    for (int k = 0; k < NC / 2; ++k) y[k] = pack_out<BF16>(o[2 * k], o[2 * k + 1]);
+    if constexpr (NC == 8) pg_store16(dst, uint4{y[0], y[1], y[2], y[3]});
+    else pg_store8(dst, uint2{y[0], y[1]});
+}
+
+// ------------------------------------------------------------------ few rows
+// NT row tiles of 16; the four waves of a workgroup take a segment's items in turn and are
+// joined in LDS at its end.
+template <int D, int NT>
+struct FewShared {
+    static constexpr int OS = D + 4;                 // row stride of a wave's output rows, f32
+    float o[WAVES][16 * OS];
+    float m[WAVES][16], l[WAVES][16];
+    ScanShared scan;
+};
+
+template <int D, int NT, bool BF16, bool MASK>
+__global__ __launch_bounds__(256, NT == 1 ? 3 : 2) void paged_few_kernel(AttnArgs a) {
+    constexpr int CB = D / 32, NC = D / 16;
+    __shared__ FewShared<D, NT> sh;
+    const int tid = threadIdx.x, lane = tid & 63, wave = uniform(tid >> 6), n16 = lane & 15, hh = lane >> 4;
+    Stretch st = find_stretch<256>(a, sh.scan, WAVES);
+    int4 desc{-1, 0, 0, 0};
+    int64_t pos = st.s;
+    Items it = pos < st.e ? items_at(a, st.b) : Items{};
+    while (pos < st.e) {
+        const Part pt = part_of(a, st, it, pos);
+        const int b = st.b, h = pt.h, row0 = pt.rg * NT * 16;
+        uint4 q[NT][CB];
         float c[NT];
-        if constexpr (QLDS) {
-            __syncthreads();   // the segment before is done with sh.q
-            for (int nt = wave; nt < NT; nt += WAVES) {
-                uint4 t[CB];
-                load_q_raw<D>(a, b, h, row0 + nt * 16 + n16, it.n, hh, t);
-                const float up = BF16 ? q_as_f16<D>(t) : 1.f;
-#pragma unroll
-                for (int cb = 0; cb < CB; ++cb) sh.q[(nt * CB + cb) * 64 + lane] = t[cb];
-                if (hh == 0) sh.qc[nt * 16 + n16] = up * a.sl2;
-            }
-            __syncthreads();
-#pragma unroll
-            for (int nt = 0; nt < NT; ++nt) c[nt] = sh.qc[nt * 16 + n16];
-        } else {
-#pragma unroll
-            for (int nt = 0; nt < NT; ++nt) {
-                load_q_raw<D>(a, b, h, row0 + nt * 16 + n16, it.n, hh, q[nt]);
-                c[nt] = (BF16 ? q_as_f16<D>(q[nt]) : 1.f) * a.sl2;
-            }
-        }
         Tile<D> t[NT];
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
-#pragma unroll
-            for (int ct = 0; ct < NC; ++ct) t[nt].acc[ct] = f32x4_t{};
-            t[nt].m = NO_MAX;
-            t[nt].l = 0.f;
+            load_q<D>(a, b, h, row0 + nt * 16 + (hidden(lane) & 15), it.n, hh, q[nt]);
+            c[nt] = (BF16 ? q_as_f16<D>(q[nt]) : 1.f) * a.sl2;
+            clear(t[nt]);
         }
-
-        // ---- packed groups: this wave's items i0 + wave, + 4, ...
-        const int per = a.p.page_tokens / PG_GROUP;
         const int32_t *trow = a.p.table + (int64_t)b * a.p.s_table;
-        auto record = [&](int i) -> const uint8_t * {
-            const int pg = i / per;
-            return pg_record(a.p, trow[pg], i - pg * per, h, 40 * D);
-        };
-        const int last = min(i1, it.ng);
-        Raw<D> w4;
-        int i = i0 + wave;
-        const uint8_t *rec = nullptr;
+        const int last = min(pt.i1, it.ng);
+        int i = pt.i0 + wave;
+        RawK<D> rk;
+        RawV<D> rv;
+        bool dead = false;
         if (i < last) {
-            rec = record(i);
-            if (rec) {
-                load_k(w4, rec, lane);
-                load_v(w4, rec, lane);
-            }
+            const uint8_t *rec = record_of<D>(a, trow, i, h, dead);
+            load_k(rk, rec, lane);
+            load_v(rv, rec, lane);
         }
         for (; i < last; i += WAVES) {
-            const uint8_t *next = i + WAVES < last ? record(i + WAVES) : nullptr;
-            const bool dead = rec == nullptr;
-            f16x8_t kf[2][CB], vf[NC];
-            if (!dead) {
+            // (the last round loads its own record again: no branch around the loads)
+            bool dead_next;
+            const uint8_t *next = record_of<D>(a, trow, i + WAVES < last ? i + WAVES : i, h, dead_next);
+            f32x4_t s0[NT], s1[NT];
 #pragma unroll
-                for (int mt = 0; mt < 2; ++mt)
+            for (int nt = 0; nt < NT; ++nt) s0[nt] = s1[nt] = f32x4_t{};
 #pragma unroll
-                    for (int cb = 0; cb < CB; ++cb) kf[mt][cb] = word_values(w4.k[mt][cb], w4.ks[cb], w4.kz[cb]);
-            }
-            if (next) load_k(w4, next, lane);
-            bool masked = false;
-            uint32_t live = 255u;
-            if (!dead) {
-                if (a.p.mask) {
-                    masked = true;
-                    live = mask_bits(a.p, b, h, (int64_t)i * PG_GROUP + 8 * hh);
-                    // a dead token's value is 0 whatever its parameters say
-                    const uint32_t h0 = halves_of(live), h1 = halves_of(live >> 2), h2 = halves_of(live >> 4),
-                                   h3 = halves_of(live >> 6);
-                    w4.vs = uint4{w4.vs.x & h0, w4.vs.y & h1, w4.vs.z & h2, w4.vs.w & h3};
-                    w4.vz = uint4{w4.vz.x & h0, w4.vz.y & h1, w4.vz.z & h2, w4.vz.w & h3};
-                }
+            for (int cb = 0; cb < CB; ++cb) {
+                const f16x8_t k0 = word_values(rk.k[0][cb], rk.s[cb], rk.z[cb]);
+                const f16x8_t k1 = word_values(rk.k[1][cb], rk.s[cb], rk.z[cb]);
 #pragma unroll
-                for (int ct = 0; ct < NC; ++ct) {
-                    const uint4 x = w4.v[ct / 4];
-                    const uint32_t word = (ct & 3) == 0 ? x.x : (ct & 3) == 1 ? x.y : (ct & 3) == 2 ? x.z : x.w;
-                    vf[ct] = word_values(word, w4.vs, w4.vz);
+                for (int nt = 0; nt < NT; ++nt) {
+                    const f16x8_t qf = __builtin_bit_cast(f16x8_t, q[nt][cb]);
+                    s0[nt] = mfma16(k0, qf, s0[nt]);
+                    s1[nt] = mfma16(k1, qf, s1[nt]);
                 }
             }
-            if (next) load_v(w4, next, lane);
-            rec = next;
-            if (dead) continue;
+            load_k(rk, next, lane);
+            const bool masked = MASK || dead;
+            uint32_t live = dead ? 0u : 255u;
+            if (masked) {
+                if (MASK) live &= mask_bits(a.p, b, h, i * PG_GROUP + 8 * (hidden(lane) >> 4));
+                clear_dead(rv, live);
+            }
+            f16x8_t pf[NT];
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt) {
-                f32x4_t s0{}, s1{};
-#pragma unroll
-                for (int cb = 0; cb < CB; ++cb) {
-                    const uint4 qw = QLDS ? sh.q[(nt * CB + cb) * 64 + lane] : q[QLDS ? 0 : nt][cb];
-                    const f16x8_t qf = __builtin_bit_cast(f16x8_t, qw);
-                    s0 = mfma16(kf[0][cb], qf, s0);
-                    s1 = mfma16(kf[1][cb], qf, s1);
-                }
                 float p[8];
-                softmax8(t[nt], s0, s1, c[nt], masked, live, p);
-                f16x8_t pf;
-#pragma unroll
-                for (int x = 0; x < 8; ++x) pf[x] = (_Float16)p[x];
-#pragma unroll
-                for (int ct = 0; ct < NC; ++ct) t[nt].acc[ct] = mfma16(vf[ct], pf, t[nt].acc[ct]);
+                softmax8(t[nt], s0[nt], s1[nt], c[nt], masked, live, p);
+                pf[nt] = as_f16(p);
+                t[nt].l = mfma16(ones_f16(), pf[nt], t[nt].l);
             }
-        }
-
-        // ---- the tail and the block's own keys
-        for (; i < i1; i += WAVES) {
-            const int x = i - it.ng;
-            const bool tail = it.rem && x == 0;
-            const int j0 = tail ? 0 : (x - (it.rem ? 1 : 0)) * PG_GROUP;      // first row
-            const int cnt = tail ? it.rem : it.n;                              // rows there are
-            if (!tail && !a.kc.ptr) continue;                                  // (a request with nothing to see)
-            const uint16_t *kb, *vb;
-            int64_t sk, sv;
-            if (tail) {
-                kb = a.p.kt + (int64_t)b * a.p.s_tb + (int64_t)h * a.p.s_th;
-                vb = a.p.vt + (int64_t)b * a.p.s_tb + (int64_t)h * a.p.s_th;
-                sk = sv = a.p.s_tt;
-            } else {
-                kb = (const uint16_t *)a.kc.ptr + (int64_t)b * a.kc.s[0] + (int64_t)h * a.kc.s[1];
-                vb = (const uint16_t *)a.vc.ptr + (int64_t)b * a.vc.s[0] + (int64_t)h * a.vc.s[1];
-                sk = a.kc.s[2];
-                sv = a.vc.s[2];
-            }
-            uint32_t seen = 0;
-#pragma unroll
-            for (int y = 0; y < 8; ++y) seen |= j0 + 8 * hh + y < cnt ? 1u << y : 0u;
-            if (tail && a.p.mask) seen &= mask_bits(a.p, b, h, (int64_t)it.ng * PG_GROUP + 8 * hh);
-            uint4 kw[2][CB];
-#pragma unroll
-            for (int mt = 0; mt < 2; ++mt) {
-                const int j = j0 + 8 * (n16 >> 2) + 4 * mt + (n16 & 3);
-#pragma unroll
-                for (int cb = 0; cb < CB; ++cb)
-                    kw[mt][cb] = j < cnt ? pg_load16(kb + (int64_t)j * sk + (D / 4) * hh + 8 * cb) : uint4{0, 0, 0, 0};
-            }
-            // V: 8 tokens x NC channels of a lane, turned so that a register pair holds tokens
-            uint32_t vw[8][NC / 2];
-#pragma unroll
-            for (int y = 0; y < 8; ++y) {
-                const bool ok = (seen >> y) & 1u;
-                const uint16_t *src = vb + (int64_t)(j0 + 8 * hh + y) * sv + NC * n16;
-                if constexpr (NC == 8) {
-                    const uint4 r = ok ? pg_load16(src) : uint4{0, 0, 0, 0};
-                    vw[y][0] = r.x; vw[y][1] = r.y; vw[y][2] = r.z; vw[y][3] = r.w;
-                } else {
-                    const uint2 r = ok ? pg_load8(src) : uint2{0, 0};
-                    vw[y][0] = r.x; vw[y][1] = r.y;
-                }
-            }
-            uint4 vt[NC];
 #pragma unroll
             for (int ct = 0; ct < NC; ++ct) {
-                uint32_t r[4];
+                const f16x8_t vf = word_values(v_word(rv, ct), rv.s, rv.z);
 #pragma unroll
-                for (int k = 0; k < 4; ++k) {
-                    const uint32_t lo = vw[2 * k][ct / 2], hi = vw[2 * k + 1][ct / 2];
-                    r[k] = ct & 1 ? (lo >> 16) | (hi & 0xffff0000u) : (lo & 0xffffu) | (hi << 16);
-                }
-                vt[ct] = uint4{r[0], r[1], r[2], r[3]};
+                for (int nt = 0; nt < NT; ++nt) t[nt].acc[ct] = mfma16(vf, pf[nt], t[nt].acc[ct]);
             }
+            load_v(rv, next, lane);
+            dead = dead_next;
+        }
+        // the tail and the block's own keys
+        for (; i < pt.i1; i += WAVES) {
+            const Rows r = rows_of(a, it, b, h, i - it.ng);
+            if (r.cnt == 0) continue;
+            const int l = hidden(lane), lh = l >> 4;
+            const uint32_t seen = rows_live<MASK>(a, it, r, b, h, lh);
+            f32x4_t s[2][NT];
 #pragma unroll
-            for (int nt = 0; nt < NT; ++nt) {
-                const int row = row0 + nt * 16 + n16;
-                uint4 qw[CB];
-                load_q_raw<D>(a, b, h, row, it.n, hh, qw);
-                uint32_t live = seen;
-                if (!tail && a.causal > 0) {
-                    const int tq = row % a.T;
-                    const int64_t lim = ((int64_t)it.len + tq) / a.causal * a.causal + a.causal - it.len;
-                    uint32_t ok = 0;
+            for (int mt = 0; mt < 2; ++mt) {
+                uint4 k[CB];
+                rows_k<D>(r, l, mt, k);
 #pragma unroll
-                    for (int y = 0; y < 8; ++y) ok |= j0 + 8 * hh + y < lim ? 1u << y : 0u;
-                    live &= ok;
+                for (int nt = 0; nt < NT; ++nt) {
+                    uint4 qr[CB];
+                    load_q<D>(a, b, h, row0 + nt * 16 + (l & 15), it.n, lh, qr);
+                    s[mt][nt] = rows_scores<CB, BF16>(k, qr);
                 }
-                f32x4_t s0{}, s1{};
-                float p[8];
-                if constexpr (BF16) {
+            }
+            Probs<BF16> p[NT];
 #pragma unroll
-                    for (int cb = 0; cb < CB; ++cb) {
-                        const b16x8_t qf = __builtin_bit_cast(b16x8_t, qw[cb]);
-                        s0 = mfma16(__builtin_bit_cast(b16x8_t, kw[0][cb]), qf, s0);
-                        s1 = mfma16(__builtin_bit_cast(b16x8_t, kw[1][cb]), qf, s1);
-                    }
-                    softmax8(t[nt], s0, s1, a.sl2, true, live, p);
-                    b16x8_t hi, lo;
+            for (int nt = 0; nt < NT; ++nt)
+                p[nt] = rows_probs<D, BF16>(t[nt], s[0][nt], s[1][nt], a.sl2,
+                                            causal_live(a, it, r, row0 + nt * 16 + (l & 15), lh, seen));
+            __builtin_amdgcn_sched_barrier(0);   // the values' loads stay behind the scores' registers
+            uint32_t vw[8][NC / 2];
+            rows_v<D>(r, l, seen, vw);
 #pragma unroll
-                    for (int y = 0; y < 8; ++y) {
-                        hi[y] = (__bf16)p[y];
-                        lo[y] = (__bf16)(p[y] - (float)hi[y]);
-                    }
+            for (int ct = 0; ct < NC; ++ct) {
+                const uint4 v = rows_channel<D>(vw, ct);
 #pragma unroll
-                    for (int ct = 0; ct < NC; ++ct) {
-                        const b16x8_t vf = __builtin_bit_cast(b16x8_t, vt[ct]);
-                        t[nt].acc[ct] = mfma16(vf, lo, mfma16(vf, hi, t[nt].acc[ct]));
-                    }
-                } else {
-#pragma unroll
-                    for (int cb = 0; cb < CB; ++cb) {
-                        const f16x8_t qf = __builtin_bit_cast(f16x8_t, qw[cb]);
-                        s0 = mfma16(__builtin_bit_cast(f16x8_t, kw[0][cb]), qf, s0);
-                        s1 = mfma16(__builtin_bit_cast(f16x8_t, kw[1][cb]), qf, s1);
-                    }
-                    softmax8(t[nt], s0, s1, a.sl2, true, live, p);
-                    f16x8_t pf;
-#pragma unroll
-                    for (int y = 0; y < 8; ++y) pf[y] = (_Float16)p[y];
-#pragma unroll
-                    for (int ct = 0; ct < NC; ++ct)
-                        t[nt].acc[ct] = mfma16(__builtin_bit_cast(f16x8_t, vt[ct]), pf, t[nt].acc[ct]);
-                }
+                for (int nt = 0; nt < NT; ++nt) t[nt].acc[ct] = rows_values(v, p[nt], t[nt].acc[ct]);
             }
         }
-
-        // ---- the waves' parts joined; whole segments written out, cut ones left as a partial
-        const bool whole = i0 == 0 && i1 == it.items;
-        const int64_t slot = 2 * w + (pos > s ? 1 : 0);   // cut: the first or the last of the stretch
+        // the waves' parts joined; whole segments written out, cut ones left as a partial
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
-            const float l = sum_rows(t[nt].l);
             __syncthreads();
             if (hh == 0) {
                 sh.m[wave][n16] = t[nt].m;
-                sh.l[wave][n16] = l;
+                sh.l[wave][n16] = t[nt].l[0];
             }
 #pragma unroll
             for (int r = 0; r < 4; ++r)
@@ -564,10 +725,10 @@ __global__ __launch_bounds__(256, NT == 1 ? 2 : 1) void paged_attn_kernel(AttnAr
                 for (int ct = 0; ct < NC; ct += 4) {
                     const f32x4_t v = {t[nt].acc[ct][r], t[nt].acc[ct + 1][r], t[nt].acc[ct + 2][r],
                                        t[nt].acc[ct + 3][r]};
-                    *(f32x4_t *)&sh.o[wave][n16 * Shared<D, NT>::OS + NC * (4 * hh + r) + ct] = v;
+                    *(f32x4_t *)&sh.o[wave][n16 * FewShared<D, NT>::OS + NC * (4 * hh + r) + ct] = v;
                 }
             __syncthreads();
-            const int r = tid >> 4, x = tid & 15;      // row, channels NC x + (0 .. NC - 1)
+            const int r = hidden(tid) >> 4, x = tid & 15;      // row, channels NC x + (0 .. NC - 1)
             const int row = row0 + nt * 16 + r;
             if (row < a.R) {
                 float m = sh.m[0][r];
@@ -582,32 +743,18 @@ __global__ __launch_bounds__(256, NT == 1 ? 2 : 1) void paged_attn_kernel(AttnAr
                     lt += sh.l[v][r] * f;
 #pragma unroll
                     for (int k = 0; k < NC; k += 4) {
-                        const f32x4_t y = *(const f32x4_t *)&sh.o[v][r * Shared<D, NT>::OS + NC * x + k];
+                        const f32x4_t y = *(const f32x4_t *)&sh.o[v][r * FewShared<D, NT>::OS + NC * x + k];
 #pragma unroll
                         for (int z = 0; z < 4; ++z) o[k + z] += y[z] * f;
                     }
                 }
-                if (whole) {
-                    const int g = row / a.T, tq = row - g * a.T;
-                    if (tq < it.n) {
-                        const float inv = lt == 0.f ? 0.f : 1.f / lt;
-                        uint16_t *dst = (uint16_t *)a.out.ptr + (int64_t)b * a.out.s[0] +
-                                        (int64_t)(h * a.G + g) * a.out.s[1] + (int64_t)tq * a.out.s[2] + NC * x;
-                        uint32_t y[NC / 2];
+                if (pt.whole) {
+                    const float inv = lt == 0.f ? 0.f : 1.f / lt;
 #pragma unroll
-                        for (int k = 0; k < NC / 2; ++k) {
-                            if constexpr (BF16) {
-                                y[k] = ma_pack_bf16x2(o[2 * k] * inv, o[2 * k + 1] * inv);
-                            } else {
-                                const f16x2_t z = {(_Float16)(o[2 * k] * inv), (_Float16)(o[2 * k + 1] * inv)};
-                                y[k] = __builtin_bit_cast(uint32_t, z);
-                            }
-                        }
-                        if constexpr (NC == 8) pg_store16(dst, uint4{y[0], y[1], y[2], y[3]});
-                        else pg_store8(dst, uint2{y[0], y[1]});
-                    }
+                    for (int k = 0; k < NC; ++k) o[k] *= inv;
+                    if (row % a.T < it.n) store_out<NC, BF16>(a, b, h, row, NC * x, o);
                 } else {
-                    const int64_t at = slot * (NT * 16) + nt * 16 + r;
+                    const int64_t at = pt.slot * (NT * 16) + nt * 16 + r;
                     if (x == 0) {
                         a.wm[at] = m;
                         a.wl[at] = lt;
@@ -618,43 +765,293 @@ __global__ __launch_bounds__(256, NT == 1 ? 2 : 1) void paged_attn_kernel(AttnAr
                 }
             }
         }
-        // the first stretch of a cut segment names it to the merge: (request, (head, row group),
-        // first slot, stretches)
-        if (!whole && i0 == 0) {
-            const int64_t seg_end = pos + it.items;
-            desc = int4{b, hr, (int)slot, (int)((seg_end - 1) / chunk - w + 1)};
-        }
-        pos += i1 - i0;
-        if (i1 == it.items && hr == HR - 1 && pos < e) {
-            pre += it.items;
-            do it = items_of(a, ++b);
-            while (it.items == 0);
-        }
+        if (!pt.whole && pt.i0 == 0) desc = cut_desc(st, it, pt, pos);
+        next_part(a, st, it, pt, pos);
     }
-    if (tid == 0) a.desc[w] = desc;
+    if (tid == 0) a.desc[st.w] = desc;
 }
 
-// Partials of a cut segment, joined: its first partial lies in slot desc.z, the stretch after
-// workgroup w's in slot 2 (w + 1), and so on.  A workgroup takes 4 rows; 4 groups of 16 threads
-// a row take every fourth partial and are joined in LDS, in a fixed order.
-template <int D, int NT, bool BF16>
-__global__ __launch_bounds__(256) void page_merge_kernel(AttnArgs a) {
-    constexpr int NC = D / 16;
-    __shared__ float sm[4][4], sl[4][4];
-    __shared__ float so[4][4][D];
+// ------------------------------------------------------------------ many rows
+// 8 waves over 2 RW row tiles of 16: wave w takes row tiles 2 (w % RW) and + 1 and, of a step's
+// 4 items, those of w / RW modulo 8 / RW.  A step's K and V become operands in LDS once for all
+// rows: wave w unpacks the keys (w even) or values (w odd) of item w / 2 of the next step into
+// the other buffer while it computes, one barrier a step.  An item's 16 operands lie as the
+// lanes read them (1 KB each, no bank conflicts).
+constexpr int MWAVES = 8, STEP = 4;
+
+template <int D>
+struct ManyShared {
+    static constexpr int OPS = 2 * (D / 32) + D / 16;     // operands of an item: K [2][D/32], V [D/16]
+    uint4 op[2][STEP][OPS][64];
+    uint32_t live[2][STEP];                               // bit j: the item's token j is seen
+    ScanShared scan;
+};
+
+template <int D, int RW, bool BF16, bool MASK>
+__global__ __launch_bounds__(512, 2) void paged_many_kernel(AttnArgs a) {
+    constexpr int CB = D / 32, NC = D / 16, TW = MWAVES / RW;
+    extern __shared__ __attribute__((aligned(16))) char lds[];
+    ManyShared<D> &sh = *(ManyShared<D> *)lds;
+    const int tid = threadIdx.x, lane = tid & 63, wave = uniform(tid >> 6), hh = lane >> 4;
+    const int rw = wave % RW, tw = wave / RW;
+    const int si = wave >> 1;              // the item of a step that this wave unpacks
+    const bool sv = wave & 1;              // its values (else its keys)
+    Stretch st = find_stretch<512>(a, sh.scan, STEP);
+    int4 desc{-1, 0, 0, 0};
+    int64_t pos = st.s;
+    Items it = pos < st.e ? items_at(a, st.b) : Items{};
+    while (pos < st.e) {
+        const Part pt = part_of(a, st, it, pos);
+        const int b = st.b, h = pt.h, row0 = pt.rg * (2 * RW * 16) + rw * 32;
+        const bool busy = row0 < a.R;      // this wave has rows
+        uint4 q[2][CB];
+        float c[2];
+        Tile<D> t[2];
+#pragma unroll
+        for (int nt = 0; nt < 2; ++nt) {
+            load_q<D>(a, b, h, row0 + nt * 16 + (hidden(lane) & 15), it.n, hh, q[nt]);
+            c[nt] = (BF16 ? q_as_f16<D>(q[nt]) : 1.f) * a.sl2;
+            clear(t[nt]);
+        }
+        const int32_t *trow = a.p.table + (int64_t)b * a.p.s_table;
+        // the seen tokens of an item, from its values' wave
+        auto note_live = [&](int x, uint32_t live) {
+            uint32_t all = 0;
+#pragma unroll
+            for (int y = 0; y < 4; ++y) all |= (uint32_t)__builtin_amdgcn_readlane((int)live, 16 * y) << (8 * y);
+            if (lane == 0) sh.live[x & 1][si] = all;
+        };
+
+        // ---- packed groups
+        const int last = min(pt.i1, it.ng), steps = max(last - pt.i0 + STEP - 1, 0) / STEP;
+        RawK<D> raw;
+        bool dead = false;
+        // the words of step x's item of this wave (behind the last one: of the last, again)
+        auto fetch = [&](int x) {
+            const uint8_t *rec = record_of<D>(a, trow, min(pt.i0 + x * STEP + si, last - 1), h, dead);
+            if (sv) {
+                RawV<D> v;
+                load_v(v, rec, lane);
+                v_into(raw, v);
+            } else {
+                load_k(raw, rec, lane);
+            }
+        };
+        // ... as operands in buffer x & 1
+        auto unpack = [&](int x) {
+            uint4(*op)[64] = sh.op[x & 1][si];
+            if (!sv) {
+#pragma unroll
+                for (int mt = 0; mt < 2; ++mt)
+#pragma unroll
+                    for (int cb = 0; cb < CB; ++cb)
+                        op[mt * CB + cb][lane] = __builtin_bit_cast(uint4, word_values(raw.k[mt][cb], raw.s[cb], raw.z[cb]));
+            } else {
+                uint32_t live = dead ? 0u : 255u;
+                RawV<D> rv = v_from(raw);
+                if (MASK) live &= mask_bits(a.p, b, h, (pt.i0 + x * STEP + si) * PG_GROUP + 8 * (hidden(lane) >> 4));
+                if (MASK || dead) clear_dead(rv, live);
+#pragma unroll
+                for (int ct = 0; ct < NC; ++ct)
+                    op[2 * CB + ct][lane] = __builtin_bit_cast(uint4, word_values(v_word(rv, ct), rv.s, rv.z));
+                note_live(x, live);
+            }
+        };
+        if (steps > 0) fetch(0);
+        for (int x = -1; x < steps; ++x) {
+            if (x + 1 < steps) {
+                unpack(x + 1);
+                if (x + 2 < steps) fetch(x + 2);
+            }
+            const int g1 = busy && x >= 0 ? min(last - pt.i0 - x * STEP, STEP) : 0;
+            for (int g = tw; g < g1; g += TW) {
+                const uint4(*op)[64] = sh.op[x & 1][g];
+                const uint32_t all = (uint32_t)uniform((int)sh.live[x & 1][g]);
+                const uint32_t live = all >> (8 * hh) & 255u;
+                f32x4_t s0[2] = {}, s1[2] = {};
+#pragma unroll
+                for (int cb = 0; cb < CB; ++cb) {
+                    const f16x8_t k0 = __builtin_bit_cast(f16x8_t, op[cb][lane]);
+                    const f16x8_t k1 = __builtin_bit_cast(f16x8_t, op[CB + cb][lane]);
+#pragma unroll
+                    for (int nt = 0; nt < 2; ++nt) {
+                        const f16x8_t qf = __builtin_bit_cast(f16x8_t, q[nt][cb]);
+                        s0[nt] = mfma16(k0, qf, s0[nt]);
+                        s1[nt] = mfma16(k1, qf, s1[nt]);
+                    }
+                }
+                f16x8_t pf[2];
+#pragma unroll
+                for (int nt = 0; nt < 2; ++nt) {
+                    float p[8];
+                    softmax8(t[nt], s0[nt], s1[nt], c[nt], all != 0xffffffffu, live, p);
+                    pf[nt] = as_f16(p);
+                    t[nt].l = mfma16(ones_f16(), pf[nt], t[nt].l);
+                }
+#pragma unroll
+                for (int ct = 0; ct < NC; ++ct) {
+                    const f16x8_t vf = __builtin_bit_cast(f16x8_t, op[2 * CB + ct][lane]);
+#pragma unroll
+                    for (int nt = 0; nt < 2; ++nt) t[nt].acc[ct] = mfma16(vf, pf[nt], t[nt].acc[ct]);
+                }
+            }
+            __syncthreads();
+        }
+
+        // ---- the tail and the block's own keys, four items at a time
+        for (int i = max(pt.i0, it.ng); i < pt.i1; i += STEP) {
+            if (i + si < pt.i1) {
+                const Rows r = rows_of(a, it, b, h, i + si - it.ng);
+                const int l = hidden(lane);
+                uint4(*op)[64] = sh.op[0][si];
+                if (r.cnt > 0 && !sv) {
+#pragma unroll
+                    for (int mt = 0; mt < 2; ++mt) {
+                        uint4 k[CB];
+                        rows_k<D>(r, l, mt, k);
+#pragma unroll
+                        for (int cb = 0; cb < CB; ++cb) op[mt * CB + cb][lane] = k[cb];
+                    }
+                } else if (r.cnt > 0) {
+                    const uint32_t live = rows_live<MASK>(a, it, r, b, h, l >> 4);
+                    uint32_t vw[8][NC / 2];
+                    rows_v<D>(r, l, live, vw);
+#pragma unroll
+                    for (int ct = 0; ct < NC; ++ct) op[2 * CB + ct][lane] = rows_channel<D>(vw, ct);
+                    note_live(0, live);
+                }
+            }
+            __syncthreads();
+            const int g1 = busy ? min(pt.i1 - i, STEP) : 0;
+            for (int g = tw; g < g1; g += TW) {
+                const Rows r = rows_of(a, it, b, h, i + g - it.ng);
+                if (r.cnt == 0) continue;
+                const uint4(*op)[64] = sh.op[0][g];
+                const int l = hidden(lane), lh = l >> 4;
+                const uint32_t live = (uint32_t)uniform((int)sh.live[0][g]) >> (8 * lh) & 255u;
+                Probs<BF16> p[2];
+#pragma unroll
+                for (int nt = 0; nt < 2; ++nt) {
+                    const int row = row0 + nt * 16 + (l & 15);
+                    uint4 qr[CB], k[CB];
+                    load_q<D>(a, b, h, row, it.n, lh, qr);
+                    f32x4_t s[2];
+#pragma unroll
+                    for (int mt = 0; mt < 2; ++mt) {
+#pragma unroll
+                        for (int cb = 0; cb < CB; ++cb) k[cb] = op[mt * CB + cb][l];
+                        s[mt] = rows_scores<CB, BF16>(k, qr);
+                    }
+                    p[nt] = rows_probs<D, BF16>(t[nt], s[0], s[1], a.sl2, causal_live(a, it, r, row, lh, live));
+                }
+#pragma unroll
+                for (int ct = 0; ct < NC; ++ct) {
+                    const uint4 v = op[2 * CB + ct][l];
+#pragma unroll
+                    for (int nt = 0; nt < 2; ++nt) t[nt].acc[ct] = rows_values(v, p[nt], t[nt].acc[ct]);
+                }
+            }
+            __syncthreads();
+        }
+        // waves that share rows joined (lane by lane, through the operands' space), then each row
+        // tile written out or left as a partial
+        if constexpr (TW > 1) {
+            constexpr int NV = NC * 4 + 2;
+            float *lw = (float *)sh.op;
+#pragma unroll
+            for (int nt = 0; nt < 2; ++nt) {
+                if (tw > 0) {
+                    float *dst = lw + (wave * NV) * 64 + lane;
+#pragma unroll
+                    for (int ct = 0; ct < NC; ++ct)
+#pragma unroll
+                        for (int r = 0; r < 4; ++r) dst[(ct * 4 + r) * 64] = t[nt].acc[ct][r];
+                    dst[NC * 4 * 64] = t[nt].l[0];
+                    dst[(NC * 4 + 1) * 64] = t[nt].m;
+                }
+                __syncthreads();
+                if (tw == 0) {
+                    float m = t[nt].m;
+#pragma unroll
+                    for (int v = 1; v < TW; ++v) m = fmaxf(m, lw[((v * RW + rw) * NV + NC * 4 + 1) * 64 + lane]);
+                    const float f0 = __builtin_amdgcn_exp2f(t[nt].m - m);
+                    t[nt].l[0] *= f0;
+#pragma unroll
+                    for (int ct = 0; ct < NC; ++ct) t[nt].acc[ct] *= f0;
+#pragma unroll
+                    for (int v = 1; v < TW; ++v) {
+                        const float *src = lw + ((v * RW + rw) * NV) * 64 + lane;
+                        const float f = __builtin_amdgcn_exp2f(src[(NC * 4 + 1) * 64] - m);
+                        t[nt].l[0] += src[NC * 4 * 64] * f;
+#pragma unroll
+                        for (int ct = 0; ct < NC; ++ct)
+#pragma unroll
+                            for (int r = 0; r < 4; ++r) t[nt].acc[ct][r] += src[(ct * 4 + r) * 64] * f;
+                    }
+                    t[nt].m = m;
+                }
+                __syncthreads();
+            }
+        }
+        if (tw == 0 && busy) {
+#pragma unroll
+            for (int nt = 0; nt < 2; ++nt) {
+                const int row = row0 + nt * 16 + (hidden(lane) & 15);
+                if (row >= a.R) continue;
+                const float l = t[nt].l[0];
+                if (pt.whole) {
+                    if (row % a.T >= it.n) continue;
+                    const float inv = l == 0.f ? 0.f : 1.f / l;
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) {
+                        float o[NC];
+#pragma unroll
+                        for (int ct = 0; ct < NC; ++ct) o[ct] = t[nt].acc[ct][r] * inv;
+                        store_out<NC, BF16>(a, b, h, row, NC * (4 * hh + r), o);
+                    }
+                } else {
+                    const int64_t at = pt.slot * (2 * RW * 16) + rw * 32 + nt * 16 + (row & 15);
+                    if (hh == 0) {
+                        a.wm[at] = t[nt].m;
+                        a.wl[at] = l;
+                    }
+#pragma unroll
+                    for (int r = 0; r < 4; ++r)
+#pragma unroll
+                        for (int ct = 0; ct < NC; ct += 4)
+                            *(f32x4_t *)&a.wo[at * D + NC * (4 * hh + r) + ct] =
+                                f32x4_t{t[nt].acc[ct][r], t[nt].acc[ct + 1][r], t[nt].acc[ct + 2][r], t[nt].acc[ct + 3][r]};
+                }
+            }
+        }
+        if (!pt.whole && pt.i0 == 0) desc = cut_desc(st, it, pt, pos);
+        next_part(a, st, it, pt, pos);
+    }
+    if (tid == 0) a.desc[st.w] = desc;
+}
+
+// ------------------------------------------------------------------ merge
+// Partials of a cut segment, joined: its first lies in slot desc.z, the stretch after workgroup
+// w's in slot 2 (w + 1), and so on.  16 threads a row; GR groups of them take every GR-th
+// partial and are joined in LDS, in a fixed order.
+template <int D, int GR, bool BF16>
+__global__ __launch_bounds__(256) void paged_merge_kernel(AttnArgs a, int rows) {
+    constexpr int NC = D / 16, RPW = 16 / GR;
+    __shared__ float sm[RPW][GR], sl[RPW][GR];
+    __shared__ float so[RPW][GR][D];
     const int w = blockIdx.x;
     const int4 d = a.desc[w];
     if (d.x < 0) return;
-    const int r = threadIdx.x >> 6, grp = (threadIdx.x >> 4) & 3, x = threadIdx.x & 15;
+    const int r = threadIdx.x / (16 * GR), grp = (threadIdx.x >> 4) % GR, x = threadIdx.x & 15;
     const int h = d.y / a.RG, rg = d.y - h * a.RG;
-    const int rt = blockIdx.y * 4 + r, row = rg * NT * 16 + rt;
+    const int rt = blockIdx.y * RPW + r, row = rg * rows + rt;
     const int n = a.new_lens ? min(max(a.new_lens[d.x], 0), a.T) : a.T;
     float m = NO_MAX, l = 0.f, o[NC];
 #pragma unroll
     for (int k = 0; k < NC; ++k) o[k] = 0.f;
     if (row < a.R) {
-        for (int k = grp; k < d.w; k += 4) {
-            const int64_t at = (k ? 2 * (int64_t)(w + k) : (int64_t)d.z) * (NT * 16) + rt;
+        for (int k = grp; k < d.w; k += GR) {
+            const int64_t at = (k ? 2 * (int64_t)(w + k) : (int64_t)d.z) * rows + rt;
             const float pm = a.wm[at], pl = a.wl[at];
             const float nm = fmaxf(m, pm);
             const float f = __builtin_amdgcn_exp2f(m - nm), g = __builtin_amdgcn_exp2f(pm - nm);
@@ -668,61 +1065,60 @@ __global__ __launch_bounds__(256) void page_merge_kernel(AttnArgs a) {
             }
         }
     }
-    if (x == 0) {
-        sm[r][grp] = m;
-        sl[r][grp] = l;
+    if constexpr (GR > 1) {
+        if (x == 0) {
+            sm[r][grp] = m;
+            sl[r][grp] = l;
+        }
+#pragma unroll
+        for (int y = 0; y < NC; ++y) so[r][grp][NC * x + y] = o[y];
+        __syncthreads();
+        if (grp != 0) return;
+        m = sm[r][0];
+#pragma unroll
+        for (int v = 1; v < GR; ++v) m = fmaxf(m, sm[r][v]);
+        l = 0.f;
+#pragma unroll
+        for (int k = 0; k < NC; ++k) o[k] = 0.f;
+#pragma unroll
+        for (int v = 0; v < GR; ++v) {
+            const float f = __builtin_amdgcn_exp2f(sm[r][v] - m);
+            l += sl[r][v] * f;
+#pragma unroll
+            for (int k = 0; k < NC; ++k) o[k] += so[r][v][NC * x + k] * f;
+        }
     }
-#pragma unroll
-    for (int y = 0; y < NC; ++y) so[r][grp][NC * x + y] = o[y];
-    __syncthreads();
-    if (grp != 0 || row >= a.R) return;
-    const int g = row / a.T, t = row - g * a.T;
-    if (t >= n) return;
-    m = fmaxf(fmaxf(sm[r][0], sm[r][1]), fmaxf(sm[r][2], sm[r][3]));
-    l = 0.f;
-#pragma unroll
-    for (int k = 0; k < NC; ++k) o[k] = 0.f;
-#pragma unroll
-    for (int v = 0; v < 4; ++v) {
-        const float f = __builtin_amdgcn_exp2f(sm[r][v] - m);
-        l += sl[r][v] * f;
-#pragma unroll
-        for (int k = 0; k < NC; ++k) o[k] += so[r][v][NC * x + k] * f;
-    }
+    if (row >= a.R || row % a.T >= n) return;
     const float inv = l == 0.f ? 0.f : 1.f / l;
-    uint16_t *dst = (uint16_t *)a.out.ptr + (int64_t)d.x * a.out.s[0] + (int64_t)(h * a.G + g) * a.out.s[1] +
-                    (int64_t)t * a.out.s[2] + NC * x;
 #pragma unroll
-    for (int k = 0; k < NC; ++k) {
-        if constexpr (BF16) dst[k] = ma_f32_to_bf16(o[k] * inv);
-        else dst[k] = __builtin_bit_cast(uint16_t, (_Float16)(o[k] * inv));
-    }
+    for (int k = 0; k < NC; ++k) o[k] *= inv;
+    store_out<NC, BF16>(a, d.x, h, row, NC * x, o);
 }
 
 // ------------------------------------------------------------------ host
 struct Shape {
-    int NT, RG, W;
+    int nt, rw, rows, RG, W;   // nt > 0: few rows, nt tiles; else many rows, rw waves of 2 tiles; rows of a slot
 };
 
-// Row tiles of 16 a wave holds, and row groups.  An item costs a wave about 100 (unpacking K
-// and V) + 65 a row tile (both products and the softmax), so more tiles a wave are better until
-// registers end; of the built numbers the cheapest split of ceil(R / 16) tiles is taken.
+// Up to 32 rows go to the waves of the few-rows kernel (1 or 2 tiles each); more rows to the
+// many-rows kernel in row groups of at most 16 tiles, the groups as even as its built 4, 8 and
+// 16 tiles allow.
 Shape shape_of(int R) {
-    const int tiles = (R + 15) / 16;
-    const int built[] = {1, 2, 4, 7};
-    Shape best{1, tiles, 0};
-    int64_t cost = INT64_MAX;
-    for (int nt : built) {
-        const int rg = (tiles + nt - 1) / nt;
-        const int64_t c = (int64_t)rg * (100 + 65 * nt);
-        if (c < cost) {
-            cost = c;
-            best = Shape{nt, rg, 0};
-        }
+    const int tiles = (R + 15) / 16, cus = ma_num_cus() / 8 * 8;
+    Shape s{};
+    if (tiles <= 2) {
+        s.nt = tiles;
+        s.rows = tiles * 16;
+        s.RG = 1;
+        s.W = cus * (tiles == 1 ? 3 : 2);    // as many workgroups as are resident at once
+        return s;
     }
-    // as many workgroups as are resident at once
-    best.W = ma_num_cus() / 8 * 8 * (best.NT == 1 ? 2 : 1);
-    return best;
+    const int groups = (tiles + 15) / 16, per = (tiles + groups - 1) / groups;
+    s.rw = per <= 4 ? 2 : per <= 8 ? 4 : 8;
+    s.rows = s.rw * 32;
+    s.RG = (R + s.rows - 1) / s.rows;
+    s.W = cus;
+    return s;
 }
 
 int64_t align256(int64_t x) { return (x + 255) / 256 * 256; }
@@ -731,7 +1127,7 @@ struct Layout {
     int64_t wl, wo, desc, bytes;   // wm at 0
 };
 Layout layout_of(const Shape &s, int D) {
-    const int64_t rows = 2LL * s.W * s.NT * 16;
+    const int64_t rows = 2LL * s.W * s.rows;
     Layout l;
     l.wl = align256(rows * 4);
     l.wo = l.wl + align256(rows * 4);
@@ -740,18 +1136,38 @@ Layout layout_of(const Shape &s, int D) {
     return l;
 }
 
-template <int D, int NT, bool BF16>
-int launch(const AttnArgs &a, hipStream_t st) {
-    paged_attn_kernel<D, NT, BF16><<<a.W, 256, 0, st>>>(a, WAVES);
-    page_merge_kernel<D, NT, BF16><<<dim3(a.W, NT * 4), 256, 0, st>>>(a);
-    return ma_check_launch("ma_paged_attention");
+template <int D, int RW, bool BF16, bool MASK>
+int launch_many(const AttnArgs &a, hipStream_t st) {
+    constexpr int LDS = (int)sizeof(ManyShared<D>);
+    static_assert(LDS <= 160 * 1024, "two steps of operands in one CU's LDS");
+    if (LDS > 64 * 1024) {
+        const hipError_t e = hipFuncSetAttribute((const void *)paged_many_kernel<D, RW, BF16, MASK>,
+                                                 hipFuncAttributeMaxDynamicSharedMemorySize, LDS);
+        if (e != hipSuccess) {
+            ma_set_error("ma_paged_attention: %d bytes of LDS refused: %s", LDS, hipGetErrorString(e));
+            return MA_EHIP;
+        }
+    }
+    paged_many_kernel<D, RW, BF16, MASK><<<a.W, 512, LDS, st>>>(a);
+    return MA_OK;
 }
+
+template <int D, bool BF16, bool MASK>
+int launch_attn(const AttnArgs &a, const Shape &s, hipStream_t st) {
+    if (s.nt == 1) paged_few_kernel<D, 1, BF16, MASK><<<a.W, 256, 0, st>>>(a);
+    else if (s.nt == 2) paged_few_kernel<D, 2, BF16, MASK><<<a.W, 256, 0, st>>>(a);
+    else if (s.rw == 2) return launch_many<D, 2, BF16, MASK>(a, st);
+    else if (s.rw == 4) return launch_many<D, 4, BF16, MASK>(a, st);
+    else return launch_many<D, 8, BF16, MASK>(a, st);
+    return MA_OK;
+}
+
 template <int D, bool BF16>
-int launch_nt(const AttnArgs &a, int nt, hipStream_t st) {
-    if (nt == 1) return launch<D, 1, BF16>(a, st);
-    if (nt == 2) return launch<D, 2, BF16>(a, st);
-    if (nt == 4) return launch<D, 4, BF16>(a, st);
-    return launch<D, 7, BF16>(a, st);
+int launch(const AttnArgs &a, const Shape &s, hipStream_t st) {
+    if (int rc = a.p.mask ? launch_attn<D, BF16, true>(a, s, st) : launch_attn<D, BF16, false>(a, s, st)) return rc;
+    if (s.nt) paged_merge_kernel<D, 4, BF16><<<dim3(a.W, s.rows / 4), 256, 0, st>>>(a, s.rows);
+    else paged_merge_kernel<D, 1, BF16><<<dim3(a.W, s.rows / 16), 256, 0, st>>>(a, s.rows);
+    return ma_check_launch("ma_paged_attention");
 }
 
 }  // namespace
@@ -805,6 +1221,6 @@ extern "C" int ma_paged_attention(ma_tensor4 q, int B, int Hq, int T, int D, con
     a.wo = (float *)(ws + l.wo);
     a.desc = (int4 *)(ws + l.desc);
     hipStream_t st = (hipStream_t)stream;
-    if (D == 128) return p->dtype == MA_BF16 ? launch_nt<128, true>(a, s.NT, st) : launch_nt<128, false>(a, s.NT, st);
-    return p->dtype == MA_BF16 ? launch_nt<64, true>(a, s.NT, st) : launch_nt<64, false>(a, s.NT, st);
+    if (D == 128) return p->dtype == MA_BF16 ? launch<128, true>(a, s, st) : launch<128, false>(a, s, st);
+    return p->dtype == MA_BF16 ? launch<64, true>(a, s, st) : launch<64, false>(a, s, st);
 }
