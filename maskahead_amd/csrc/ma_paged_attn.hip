@@ -39,7 +39,7 @@ struct AttnArgs {
     int B, H, G, T, R, RG, causal, W;
     float sl2;                // scale * log2(e)
     float *wm, *wl, *wo;      // partials of slots [2 W]: per row maximum and sum, unnormalised rows
-    int4 *desc;               // [W]: the segment whose first stretch is this workgroup's (see merge)
+    int4 *desc;               // [B, H, RG]: what note_segment says of every segment
 };
 
 // values that every lane holds alike, as scalars
@@ -52,26 +52,23 @@ struct Items {
     int n, len, ng, rem, items;   // the request's new tokens, stored tokens, whole groups, tail, items
 };
 
-__device__ __forceinline__ Items items_of(const AttnArgs &a, int b) {
+__device__ __forceinline__ Items items_from(const AttnArgs &a, int n, int len) {
     Items r;
-    r.n = a.new_lens ? min(max(a.new_lens[b], 0), a.T) : a.T;
-    r.len = pg_length(a.p, b);
-    r.ng = r.len / PG_GROUP;
-    r.rem = r.len % PG_GROUP;
-    const int cur = a.kc.ptr ? (r.n + PG_GROUP - 1) / PG_GROUP : 0;
-    r.items = r.n ? max(r.ng + (r.rem ? 1 : 0) + cur, 1) : 0;
+    r.n = n;
+    r.len = len;
+    r.ng = len / PG_GROUP;
+    r.rem = len % PG_GROUP;
+    const int cur = a.kc.ptr ? (n + PG_GROUP - 1) / PG_GROUP : 0;
+    r.items = n ? max(r.ng + (r.rem ? 1 : 0) + cur, 1) : 0;
     return r;
 }
-
+__device__ __forceinline__ Items items_of(const AttnArgs &a, int b) {
+    return items_from(a, a.new_lens ? min(max(a.new_lens[b], 0), a.T) : a.T, pg_length(a.p, b));
+}
 // ... of a request that the whole wave looks at
 __device__ __forceinline__ Items items_at(const AttnArgs &a, int b) {
-    Items r = items_of(a, b);
-    r.n = uniform(r.n);
-    r.len = uniform(r.len);
-    r.ng = uniform(r.ng);
-    r.rem = uniform(r.rem);
-    r.items = uniform(r.items);
-    return r;
+    const Items r = items_of(a, b);
+    return items_from(a, uniform(r.n), uniform(r.len));
 }
 
 // The lane's number, as a value that nothing is known of: what is computed from it stays where
@@ -166,19 +163,34 @@ __device__ __forceinline__ void load_v(RawV<D> &w, const uint8_t *rec, int lane_
     w.s = *(const uint4 *)(rec + 36 * D + 2 * (32 * cg + 8 * h));
     w.z = *(const uint4 *)(rec + 38 * D + 2 * (32 * cg + 8 * h));
 }
-// the same registers for a wave that unpacks one or the other
+// the values' words in the keys' registers, for a wave that unpacks one or the other: the same
+// loads at other places, so that neither is copied (poff: place of a lane's parameters)
 template <int D>
-__device__ __forceinline__ void v_into(RawK<D> &w, const RawV<D> &v) {
+__device__ __forceinline__ void load_either(RawK<D> &w, const uint8_t *rec, int lane, bool v, int poff_) {
+    const uint32_t off = (uint32_t)hidden(lane) * (D == 128 ? 16 : 8), poff = (uint32_t)hidden(poff_);
+    const uint8_t *codes = rec + (v ? 16 * D : 0), *par = rec + (v ? 36 * D : 32 * D);
+    if constexpr (D == 128) {
 #pragma unroll
-    for (int mt = 0; mt < 2; ++mt)
-#pragma unroll
-        for (int x = 0; x < D / 32; ++x) {
-            const int ct = mt * (D / 32) + x;
-            const uint4 y = v.v[ct / 4];
-            w.k[mt][x] = (ct & 3) == 0 ? y.x : (ct & 3) == 1 ? y.y : (ct & 3) == 2 ? y.z : y.w;
+        for (int mt = 0; mt < 2; ++mt) {
+            const uint4 c = *(const uint4 *)(codes + 1024 * mt + off);
+            w.k[mt][0] = c.x; w.k[mt][1] = c.y; w.k[mt][2] = c.z; w.k[mt][3] = c.w;
         }
-    w.s[0] = v.s;
-    w.z[0] = v.z;
+    } else {   // (values: 16 bytes of a lane, as two words and two words)
+#pragma unroll
+        for (int mt = 0; mt < 2; ++mt) {
+            const uint2 c = *(const uint2 *)(codes + (v ? 8 * mt : 512 * mt) + (v ? 2 * off : off));
+            w.k[mt][0] = c.x; w.k[mt][1] = c.y;
+        }
+    }
+    w.s[0] = *(const uint4 *)(par + poff);
+    w.z[0] = *(const uint4 *)(par + 2 * D + poff);
+    if (!v) {
+#pragma unroll
+        for (int cb = 1; cb < D / 32; ++cb) {
+            w.s[cb] = *(const uint4 *)(par + 16 * cb + poff);
+            w.z[cb] = *(const uint4 *)(par + (2 * D + 16 * cb) + poff);
+        }
+    }
 }
 template <int D>
 __device__ __forceinline__ RawV<D> v_from(const RawK<D> &w) {
@@ -331,8 +343,18 @@ __device__ __forceinline__ void clear(Tile<D> &t) {
     t.m = NO_MAX;
 }
 
-// scores s (x c -> exponents of 2) of a lane's 8 tokens -> probabilities; live: bit i = token
-// i is seen.  Raises the row's maximum where needed.
+// max of three without the quieting that fmaxf puts before each of its arguments
+__device__ __forceinline__ float max3(float x, float y, float z) {
+    float r;
+    asm("v_max3_f32 %0, %1, %2, %3" : "=v"(r) : "v"(x), "v"(y), "v"(z));
+    return r;
+}
+__device__ __forceinline__ float max8(const float (&x)[8]) {
+    return max3(max3(x[0], x[1], x[2]), max3(x[3], x[4], x[5]), max3(x[6], x[7], x[7]));
+}
+
+// scores s (x c -> exponents of 2) of a lane's 8 tokens -> probabilities; live (where masked):
+// bit i = token i is seen.  Raises the row's maximum where needed.
 template <int D>
 __device__ __forceinline__ void softmax8(Tile<D> &t, const f32x4_t &s0, const f32x4_t &s1, float c, bool masked,
                                          uint32_t live, float (&p)[8]) {
@@ -340,19 +362,15 @@ __device__ __forceinline__ void softmax8(Tile<D> &t, const f32x4_t &s0, const f3
 #pragma unroll
     for (int i = 0; i < 8; ++i) x[i] = __builtin_fmaf(i < 4 ? s0[i & 3] : s1[i & 3], c, -t.m);
     if (masked) {
+        const uint32_t l = (uint32_t)hidden((int)live);   // (its bits are looked at in here only)
 #pragma unroll
-        for (int i = 0; i < 8; ++i) x[i] = (live >> i) & 1u ? x[i] : -INFINITY;
+        for (int i = 0; i < 8; ++i) x[i] = (l >> i) & 1u ? x[i] : -INFINITY;
     }
-    const float mx = fmaxf(fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])), fmaxf(fmaxf(x[4], x[5]), fmaxf(x[6], x[7])));
-    if (__any(mx > LAZY)) {
-        float top = -INFINITY;
+    if (__any(max8(x) > LAZY)) {
+        // (what is dead stays at -inf, whatever its score)
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            x[i] = (i < 4 ? s0[i & 3] : s1[i & 3]) * c;
-            if (masked) x[i] = (live >> i) & 1u ? x[i] : -INFINITY;
-            top = fmaxf(top, x[i]);
-        }
-        const float m = fmaxf(t.m, max_rows(top));
+        for (int i = 0; i < 8; ++i) x[i] = x[i] == -INFINITY ? -INFINITY : (i < 4 ? s0[i & 3] : s1[i & 3]) * c;
+        const float m = fmaxf(t.m, max_rows(max8(x)));
         const float f = __builtin_amdgcn_exp2f(t.m - m);
 #pragma unroll
         for (int i = 0; i < 8; ++i) x[i] -= m;
@@ -474,10 +492,11 @@ struct Stretch {
     int64_t w, s, e, chunk;   // this workgroup's place and its items [s, e); items of a stretch
     int64_t pre;              // items (x HR) of the requests before b
     int b;                    // the request in which s lies
+    Items it;                 // ... and what it has
 };
 struct ScanShared {
     int64_t wsum[16], pre;
-    int b;
+    int b, n, len;
 };
 
 // Items of all requests, by a scan of the lengths in every workgroup (8 B a request, from L2);
@@ -489,8 +508,13 @@ __device__ __forceinline__ Stretch find_stretch(const AttnArgs &a, ScanShared &s
     const int64_t HR = (int64_t)a.H * a.RG;
     const int per = (a.B + THREADS - 1) / THREADS, first = tid * per;
     int64_t sum = 0;
+    Items own{};   // of this thread's first request
     for (int i = 0; i < per; ++i)
-        if (first + i < a.B) sum += items_of(a, first + i).items;
+        if (first + i < a.B) {
+            const Items it = items_of(a, first + i);
+            if (i == 0) own = it;
+            sum += it.items;
+        }
     int64_t inc = sum;
 #pragma unroll
     for (int o = 1; o < 64; o <<= 1) {
@@ -518,18 +542,20 @@ __device__ __forceinline__ Stretch find_stretch(const AttnArgs &a, ScanShared &s
         if (want >= before && want < before + sum) {
             int64_t pre = before;
             int b = first;
-            for (;; ++b) {
-                const int n = items_of(a, b).items;
-                if (want < pre + n) break;
-                pre += n;
+            while (want >= pre + own.items) {
+                pre += own.items;
+                own = items_of(a, ++b);
             }
             sh.b = b;
             sh.pre = pre;
+            sh.n = own.n;
+            sh.len = own.len;
         }
     }
     __syncthreads();
     r.b = uniform(sh.b);
     r.pre = uniform(sh.pre);
+    r.it = items_from(a, uniform(sh.n), uniform(sh.len));
     return r;
 }
 
@@ -539,7 +565,8 @@ struct Part {
     bool whole;
     int64_t slot;     // of its partial, where it is not whole: the first or the last of the stretch
 };
-__device__ __forceinline__ Part part_of(const AttnArgs &a, const Stretch &st, const Items &it, int64_t pos) {
+__device__ __forceinline__ Part part_of(const AttnArgs &a, const Stretch &st, int64_t pos) {
+    const Items &it = st.it;
     Part p;
     const int64_t rel = pos - (int64_t)a.H * a.RG * st.pre;
     p.hr = (int)(rel / it.items);
@@ -551,17 +578,19 @@ __device__ __forceinline__ Part part_of(const AttnArgs &a, const Stretch &st, co
     p.slot = 2 * st.w + (pos > st.s ? 1 : 0);
     return p;
 }
-// what the merge needs of a cut segment, left by its first stretch: (request, (head, row
-// group), first slot, stretches)
-__device__ __forceinline__ int4 cut_desc(const Stretch &st, const Items &it, const Part &p, int64_t pos) {
-    return int4{st.b, p.hr, (int)p.slot, (int)((pos + it.items - 1) / st.chunk - st.w + 1)};
+// The segment's first stretch says what the merge needs of it: (first slot, stretches, first
+// workgroup), or no stretches where it is whole.
+__device__ __forceinline__ void note_segment(const AttnArgs &a, const Stretch &st, const Part &p, int64_t pos) {
+    if (p.i0 != 0 || threadIdx.x != 0) return;
+    const int n = p.whole ? 0 : (int)((pos + st.it.items - 1) / st.chunk - st.w + 1);
+    a.desc[(int64_t)st.b * a.H * a.RG + p.hr] = int4{(int)p.slot, n, (int)st.w, 0};
 }
-__device__ __forceinline__ void next_part(const AttnArgs &a, Stretch &st, Items &it, const Part &p, int64_t &pos) {
+__device__ __forceinline__ void next_part(const AttnArgs &a, Stretch &st, const Part &p, int64_t &pos) {
     pos += p.i1 - p.i0;
-    if (p.i1 == it.items && p.hr == a.H * a.RG - 1 && pos < st.e) {
-        st.pre += it.items;
-        do it = items_at(a, ++st.b);
-        while (it.items == 0);
+    if (p.i1 == st.it.items && p.hr == a.H * a.RG - 1 && pos < st.e) {
+        st.pre += st.it.items;
+        do st.it = items_at(a, ++st.b);
+        while (st.it.items == 0);
     }
 }
 
@@ -610,11 +639,10 @@ __global__ __launch_bounds__(256, NT == 1 ? 3 : 2) void paged_few_kernel(AttnArg
     __shared__ FewShared<D, NT> sh;
     const int tid = threadIdx.x, lane = tid & 63, wave = uniform(tid >> 6), n16 = lane & 15, hh = lane >> 4;
     Stretch st = find_stretch<256>(a, sh.scan, WAVES);
-    int4 desc{-1, 0, 0, 0};
     int64_t pos = st.s;
-    Items it = pos < st.e ? items_at(a, st.b) : Items{};
     while (pos < st.e) {
-        const Part pt = part_of(a, st, it, pos);
+        const Items it = st.it;
+        const Part pt = part_of(a, st, pos);
         const int b = st.b, h = pt.h, row0 = pt.rg * NT * 16;
         uint4 q[NT][CB];
         float c[NT];
@@ -765,10 +793,9 @@ __global__ __launch_bounds__(256, NT == 1 ? 3 : 2) void paged_few_kernel(AttnArg
                 }
             }
         }
-        if (!pt.whole && pt.i0 == 0) desc = cut_desc(st, it, pt, pos);
-        next_part(a, st, it, pt, pos);
+        note_segment(a, st, pt, pos);
+        next_part(a, st, pt, pos);
     }
-    if (tid == 0) a.desc[st.w] = desc;
 }
 
 // ------------------------------------------------------------------ many rows
@@ -797,11 +824,10 @@ __global__ __launch_bounds__(512, 2) void paged_many_kernel(AttnArgs a) {
     const int si = wave >> 1;              // the item of a step that this wave unpacks
     const bool sv = wave & 1;              // its values (else its keys)
     Stretch st = find_stretch<512>(a, sh.scan, STEP);
-    int4 desc{-1, 0, 0, 0};
     int64_t pos = st.s;
-    Items it = pos < st.e ? items_at(a, st.b) : Items{};
     while (pos < st.e) {
-        const Part pt = part_of(a, st, it, pos);
+        const Items it = st.it;
+        const Part pt = part_of(a, st, pos);
         const int b = st.b, h = pt.h, row0 = pt.rg * (2 * RW * 16) + rw * 32;
         const bool busy = row0 < a.R;      // this wave has rows
         uint4 q[2][CB];
@@ -824,18 +850,13 @@ __global__ __launch_bounds__(512, 2) void paged_many_kernel(AttnArgs a) {
 
         // ---- packed groups
         const int last = min(pt.i1, it.ng), steps = max(last - pt.i0 + STEP - 1, 0) / STEP;
+        const int poff = sv ? 2 * (32 * (NC * (lane & 15) / 32) + 8 * hh) : (D / 2) * hh;
         RawK<D> raw;
         bool dead = false;
         // the words of step x's item of this wave (behind the last one: of the last, again)
         auto fetch = [&](int x) {
             const uint8_t *rec = record_of<D>(a, trow, min(pt.i0 + x * STEP + si, last - 1), h, dead);
-            if (sv) {
-                RawV<D> v;
-                load_v(v, rec, lane);
-                v_into(raw, v);
-            } else {
-                load_k(raw, rec, lane);
-            }
+            load_either(raw, rec, lane, sv, poff);
         };
         // ... as operands in buffer x & 1
         auto unpack = [&](int x) {
@@ -864,6 +885,12 @@ __global__ __launch_bounds__(512, 2) void paged_many_kernel(AttnArgs a) {
                 if (x + 2 < steps) fetch(x + 2);
             }
             const int g1 = busy && x >= 0 ? min(last - pt.i0 - x * STEP, STEP) : 0;
+            // the keys' operands of an item come while the one before is multiplied by its values
+            f16x8_t kf[2 * CB];
+            if (tw < g1) {
+#pragma unroll
+                for (int y = 0; y < 2 * CB; ++y) kf[y] = __builtin_bit_cast(f16x8_t, sh.op[x & 1][tw][y][lane]);
+            }
             for (int g = tw; g < g1; g += TW) {
                 const uint4(*op)[64] = sh.op[x & 1][g];
                 const uint32_t all = (uint32_t)uniform((int)sh.live[x & 1][g]);
@@ -871,15 +898,17 @@ __global__ __launch_bounds__(512, 2) void paged_many_kernel(AttnArgs a) {
                 f32x4_t s0[2] = {}, s1[2] = {};
 #pragma unroll
                 for (int cb = 0; cb < CB; ++cb) {
-                    const f16x8_t k0 = __builtin_bit_cast(f16x8_t, op[cb][lane]);
-                    const f16x8_t k1 = __builtin_bit_cast(f16x8_t, op[CB + cb][lane]);
 #pragma unroll
                     for (int nt = 0; nt < 2; ++nt) {
                         const f16x8_t qf = __builtin_bit_cast(f16x8_t, q[nt][cb]);
-                        s0[nt] = mfma16(k0, qf, s0[nt]);
-                        s1[nt] = mfma16(k1, qf, s1[nt]);
+                        s0[nt] = mfma16(kf[cb], qf, s0[nt]);
+                        s1[nt] = mfma16(kf[CB + cb], qf, s1[nt]);
                     }
                 }
+                // the values' operands come while the scores become probabilities
+                f16x8_t vf[NC];
+#pragma unroll
+                for (int ct = 0; ct < NC; ++ct) vf[ct] = __builtin_bit_cast(f16x8_t, op[2 * CB + ct][lane]);
                 f16x8_t pf[2];
 #pragma unroll
                 for (int nt = 0; nt < 2; ++nt) {
@@ -888,12 +917,13 @@ __global__ __launch_bounds__(512, 2) void paged_many_kernel(AttnArgs a) {
                     pf[nt] = as_f16(p);
                     t[nt].l = mfma16(ones_f16(), pf[nt], t[nt].l);
                 }
+                const uint4(*next)[64] = sh.op[x & 1][min(g + TW, STEP - 1)];
 #pragma unroll
-                for (int ct = 0; ct < NC; ++ct) {
-                    const f16x8_t vf = __builtin_bit_cast(f16x8_t, op[2 * CB + ct][lane]);
+                for (int y = 0; y < 2 * CB; ++y) kf[y] = __builtin_bit_cast(f16x8_t, next[y][lane]);
 #pragma unroll
-                    for (int nt = 0; nt < 2; ++nt) t[nt].acc[ct] = mfma16(vf, pf[nt], t[nt].acc[ct]);
-                }
+                for (int ct = 0; ct < NC; ++ct)
+#pragma unroll
+                    for (int nt = 0; nt < 2; ++nt) t[nt].acc[ct] = mfma16(vf[ct], pf[nt], t[nt].acc[ct]);
             }
             __syncthreads();
         }
@@ -1024,34 +1054,34 @@ __global__ __launch_bounds__(512, 2) void paged_many_kernel(AttnArgs a) {
                 }
             }
         }
-        if (!pt.whole && pt.i0 == 0) desc = cut_desc(st, it, pt, pos);
-        next_part(a, st, it, pt, pos);
+        note_segment(a, st, pt, pos);
+        next_part(a, st, pt, pos);
     }
-    if (tid == 0) a.desc[st.w] = desc;
 }
 
 // ------------------------------------------------------------------ merge
-// Partials of a cut segment, joined: its first lies in slot desc.z, the stretch after workgroup
-// w's in slot 2 (w + 1), and so on.  16 threads a row; GR groups of them take every GR-th
+// Partials of a cut segment, joined: the first lies in desc.x, the stretch after workgroup w's
+// in slot 2 (w + 1), and so on.  16 threads a row; four groups of them take every fourth
 // partial and are joined in LDS, in a fixed order.
-template <int D, int GR, bool BF16>
+template <int D, bool BF16>
 __global__ __launch_bounds__(256) void paged_merge_kernel(AttnArgs a, int rows) {
-    constexpr int NC = D / 16, RPW = 16 / GR;
+    constexpr int NC = D / 16, GR = 4, RPW = 16 / GR;
     __shared__ float sm[RPW][GR], sl[RPW][GR];
     __shared__ float so[RPW][GR][D];
-    const int w = blockIdx.x;
-    const int4 d = a.desc[w];
-    if (d.x < 0) return;
-    const int r = threadIdx.x / (16 * GR), grp = (threadIdx.x >> 4) % GR, x = threadIdx.x & 15;
-    const int h = d.y / a.RG, rg = d.y - h * a.RG;
+    const int b = blockIdx.x / (a.H * a.RG), hr = blockIdx.x - b * (a.H * a.RG);
+    const int n = a.new_lens ? min(max(a.new_lens[b], 0), a.T) : a.T;
+    if (n == 0) return;                     // (nobody wrote its segments)
+    const int4 d = a.desc[blockIdx.x];
+    if (d.y == 0) return;
+    const int w = d.z, r = threadIdx.x / (16 * GR), grp = (threadIdx.x >> 4) % GR, x = threadIdx.x & 15;
+    const int h = hr / a.RG, rg = hr - h * a.RG;
     const int rt = blockIdx.y * RPW + r, row = rg * rows + rt;
-    const int n = a.new_lens ? min(max(a.new_lens[d.x], 0), a.T) : a.T;
     float m = NO_MAX, l = 0.f, o[NC];
 #pragma unroll
     for (int k = 0; k < NC; ++k) o[k] = 0.f;
     if (row < a.R) {
-        for (int k = grp; k < d.w; k += GR) {
-            const int64_t at = (k ? 2 * (int64_t)(w + k) : (int64_t)d.z) * rows + rt;
+        for (int k = grp; k < d.y; k += GR) {
+            const int64_t at = (k ? 2 * (int64_t)(w + k) : (int64_t)d.x) * rows + rt;
             const float pm = a.wm[at], pl = a.wl[at];
             const float nm = fmaxf(m, pm);
             const float f = __builtin_amdgcn_exp2f(m - nm), g = __builtin_amdgcn_exp2f(pm - nm);
@@ -1065,34 +1095,32 @@ __global__ __launch_bounds__(256) void paged_merge_kernel(AttnArgs a, int rows) 
             }
         }
     }
-    if constexpr (GR > 1) {
-        if (x == 0) {
-            sm[r][grp] = m;
-            sl[r][grp] = l;
-        }
+    if (x == 0) {
+        sm[r][grp] = m;
+        sl[r][grp] = l;
+    }
 #pragma unroll
-        for (int y = 0; y < NC; ++y) so[r][grp][NC * x + y] = o[y];
-        __syncthreads();
-        if (grp != 0) return;
-        m = sm[r][0];
+    for (int y = 0; y < NC; ++y) so[r][grp][NC * x + y] = o[y];
+    __syncthreads();
+    if (grp != 0) return;
+    m = sm[r][0];
 #pragma unroll
-        for (int v = 1; v < GR; ++v) m = fmaxf(m, sm[r][v]);
-        l = 0.f;
+    for (int v = 1; v < GR; ++v) m = fmaxf(m, sm[r][v]);
+    l = 0.f;
 #pragma unroll
-        for (int k = 0; k < NC; ++k) o[k] = 0.f;
+    for (int k = 0; k < NC; ++k) o[k] = 0.f;
 #pragma unroll
-        for (int v = 0; v < GR; ++v) {
-            const float f = __builtin_amdgcn_exp2f(sm[r][v] - m);
-            l += sl[r][v] * f;
+    for (int v = 0; v < GR; ++v) {
+        const float f = __builtin_amdgcn_exp2f(sm[r][v] - m);
+        l += sl[r][v] * f;
 #pragma unroll
-            for (int k = 0; k < NC; ++k) o[k] += so[r][v][NC * x + k] * f;
-        }
+        for (int k = 0; k < NC; ++k) o[k] += so[r][v][NC * x + k] * f;
     }
     if (row >= a.R || row % a.T >= n) return;
     const float inv = l == 0.f ? 0.f : 1.f / l;
 #pragma unroll
     for (int k = 0; k < NC; ++k) o[k] *= inv;
-    store_out<NC, BF16>(a, d.x, h, row, NC * x, o);
+    store_out<NC, BF16>(a, b, h, row, NC * x, o);
 }
 
 // ------------------------------------------------------------------ host
@@ -1126,13 +1154,13 @@ int64_t align256(int64_t x) { return (x + 255) / 256 * 256; }
 struct Layout {
     int64_t wl, wo, desc, bytes;   // wm at 0
 };
-Layout layout_of(const Shape &s, int D) {
+Layout layout_of(const Shape &s, int64_t segments, int D) {
     const int64_t rows = 2LL * s.W * s.rows;
     Layout l;
     l.wl = align256(rows * 4);
     l.wo = l.wl + align256(rows * 4);
     l.desc = l.wo + align256(rows * D * 4);
-    l.bytes = l.desc + align256((int64_t)s.W * sizeof(int4));
+    l.bytes = l.desc + align256(segments * sizeof(int4));
     return l;
 }
 
@@ -1165,8 +1193,8 @@ int launch_attn(const AttnArgs &a, const Shape &s, hipStream_t st) {
 template <int D, bool BF16>
 int launch(const AttnArgs &a, const Shape &s, hipStream_t st) {
     if (int rc = a.p.mask ? launch_attn<D, BF16, true>(a, s, st) : launch_attn<D, BF16, false>(a, s, st)) return rc;
-    if (s.nt) paged_merge_kernel<D, 4, BF16><<<dim3(a.W, s.rows / 4), 256, 0, st>>>(a, s.rows);
-    else paged_merge_kernel<D, 1, BF16><<<dim3(a.W, s.rows / 16), 256, 0, st>>>(a, s.rows);
+    // (a row group of few rows has fewer than its slots hold)
+    paged_merge_kernel<D, BF16><<<dim3(a.B * a.H * a.RG, (min(s.rows, a.R) + 3) / 4), 256, 0, st>>>(a, s.rows);
     return ma_check_launch("ma_paged_attention");
 }
 
@@ -1175,7 +1203,8 @@ int launch(const AttnArgs &a, const Shape &s, hipStream_t st) {
 extern "C" int64_t ma_paged_workspace_bytes(int B, int H, int Hq, int T, int D) {
     if (B <= 0 || H <= 0 || Hq <= 0 || Hq % H || T <= 0 || (D != 64 && D != 128)) return -1;
     if ((int64_t)(Hq / H) * T > INT32_MAX / 16) return -1;
-    return layout_of(shape_of(Hq / H * T), D).bytes;
+    const Shape s = shape_of(Hq / H * T);
+    return (int64_t)B * H * s.RG > INT32_MAX ? -1 : layout_of(s, (int64_t)B * H * s.RG, D).bytes;
 }
 
 extern "C" int ma_paged_attention(ma_tensor4 q, int B, int Hq, int T, int D, const ma_pages *p, int H, ma_tensor4 kc,
@@ -1198,7 +1227,7 @@ extern "C" int ma_paged_attention(ma_tensor4 q, int B, int Hq, int T, int D, con
         return MA_EWORKSPACE;
     }
     const Shape s = shape_of(Hq / H * T);
-    const Layout l = layout_of(s, D);
+    const Layout l = layout_of(s, (int64_t)B * H * s.RG, D);
     char *ws = (char *)workspace;
     AttnArgs a{};
     a.q = q;
