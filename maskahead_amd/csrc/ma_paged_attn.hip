@@ -125,6 +125,21 @@ __device__ __forceinline__ float sum_rows(float v) {
     return ma_sum_xor32(__uint_as_float(r[0]) + __uint_as_float(r[1]));
 }
 
+// A record, and 16 (8) bytes of it at a scalar base and a lane's 32-bit offset.  The address
+// space is in the type: as a plain pointer put together from lanes' halves it would be read by
+// flat loads, whose results come in no order.
+typedef const __attribute__((address_space(1))) uint8_t *rec_t;
+typedef __attribute__((ext_vector_type(4))) uint32_t w4_t;
+typedef __attribute__((ext_vector_type(2))) uint32_t w2_t;
+__device__ __forceinline__ uint4 rec16(rec_t base, uint32_t off) {
+    const w4_t v = *(const __attribute__((address_space(1))) w4_t *)(base + off);
+    return uint4{v[0], v[1], v[2], v[3]};
+}
+__device__ __forceinline__ uint2 rec8(rec_t base, uint32_t off) {
+    const w2_t v = *(const __attribute__((address_space(1))) w2_t *)(base + off);
+    return uint2{v[0], v[1]};
+}
+
 // one record's words of a wave
 template <int D>
 struct RawK {
@@ -137,58 +152,59 @@ struct RawV {
 };
 
 template <int D>
-__device__ __forceinline__ void load_k(RawK<D> &w, const uint8_t *rec, int lane_) {
-    const uint32_t lane = (uint32_t)hidden(lane_), h = lane >> 4;   // scalar base + 32-bit lane offsets
+__device__ __forceinline__ void load_k(RawK<D> &w, rec_t rec, int lane_) {
+    const uint32_t lane = (uint32_t)hidden(lane_), par = (D / 2) * (lane >> 4);
 #pragma unroll
     for (int mt = 0; mt < 2; ++mt) {
         if constexpr (D == 128) {
-            const uint4 c = *(const uint4 *)(rec + mt * 1024 + lane * 16);
+            const uint4 c = rec16(rec + 1024 * mt, 16 * lane);
             w.k[mt][0] = c.x; w.k[mt][1] = c.y; w.k[mt][2] = c.z; w.k[mt][3] = c.w;
         } else {
-            const uint2 c = *(const uint2 *)(rec + mt * 512 + lane * 8);
+            const uint2 c = rec8(rec + 512 * mt, 8 * lane);
             w.k[mt][0] = c.x; w.k[mt][1] = c.y;
         }
     }
 #pragma unroll
     for (int cb = 0; cb < D / 32; ++cb) {
-        w.s[cb] = *(const uint4 *)(rec + 32 * D + ((D / 2) * h + 16 * cb));
-        w.z[cb] = *(const uint4 *)(rec + 34 * D + ((D / 2) * h + 16 * cb));
+        w.s[cb] = rec16(rec + 32 * D + 16 * cb, par);
+        w.z[cb] = rec16(rec + 34 * D + 16 * cb, par);
     }
 }
 template <int D>
-__device__ __forceinline__ void load_v(RawV<D> &w, const uint8_t *rec, int lane_) {
-    const uint32_t lane = (uint32_t)hidden(lane_), h = lane >> 4, m = lane & 15u, cg = (D / 16) * m / 32;
+__device__ __forceinline__ void load_v(RawV<D> &w, rec_t rec, int lane_) {
+    const uint32_t lane = (uint32_t)hidden(lane_);
+    const uint32_t par = 2 * (32 * ((D / 16) * (lane & 15u) / 32) + 8 * (lane >> 4));
 #pragma unroll
-    for (int half = 0; half < D / 64; ++half) w.v[half] = *(const uint4 *)(rec + (16 * D + 1024 * half) + 16 * lane);
-    w.s = *(const uint4 *)(rec + 36 * D + 2 * (32 * cg + 8 * h));
-    w.z = *(const uint4 *)(rec + 38 * D + 2 * (32 * cg + 8 * h));
+    for (int half = 0; half < D / 64; ++half) w.v[half] = rec16(rec + 16 * D + 1024 * half, 16 * lane);
+    w.s = rec16(rec + 36 * D, par);
+    w.z = rec16(rec + 38 * D, par);
 }
 // the values' words in the keys' registers, for a wave that unpacks one or the other: the same
 // loads at other places, so that neither is copied (poff: place of a lane's parameters)
 template <int D>
-__device__ __forceinline__ void load_either(RawK<D> &w, const uint8_t *rec, int lane, bool v, int poff_) {
+__device__ __forceinline__ void load_either(RawK<D> &w, rec_t rec, int lane, bool v, int poff_) {
     const uint32_t off = (uint32_t)hidden(lane) * (D == 128 ? 16 : 8), poff = (uint32_t)hidden(poff_);
-    const uint8_t *codes = rec + (v ? 16 * D : 0), *par = rec + (v ? 36 * D : 32 * D);
+    const rec_t codes = rec + (v ? 16 * D : 0), par = rec + (v ? 36 * D : 32 * D);
     if constexpr (D == 128) {
 #pragma unroll
         for (int mt = 0; mt < 2; ++mt) {
-            const uint4 c = *(const uint4 *)(codes + 1024 * mt + off);
+            const uint4 c = rec16(codes + 1024 * mt, off);
             w.k[mt][0] = c.x; w.k[mt][1] = c.y; w.k[mt][2] = c.z; w.k[mt][3] = c.w;
         }
     } else {   // (values: 16 bytes of a lane, as two words and two words)
 #pragma unroll
         for (int mt = 0; mt < 2; ++mt) {
-            const uint2 c = *(const uint2 *)(codes + (v ? 8 * mt : 512 * mt) + (v ? 2 * off : off));
+            const uint2 c = rec8(codes + (v ? 8 * mt : 512 * mt), v ? 2 * off : off);
             w.k[mt][0] = c.x; w.k[mt][1] = c.y;
         }
     }
-    w.s[0] = *(const uint4 *)(par + poff);
-    w.z[0] = *(const uint4 *)(par + 2 * D + poff);
+    w.s[0] = rec16(par, poff);
+    w.z[0] = rec16(par + 2 * D, poff);
     if (!v) {
 #pragma unroll
         for (int cb = 1; cb < D / 32; ++cb) {
-            w.s[cb] = *(const uint4 *)(par + 16 * cb + poff);
-            w.z[cb] = *(const uint4 *)(par + (2 * D + 16 * cb) + poff);
+            w.s[cb] = rec16(par + 16 * cb, poff);
+            w.z[cb] = rec16(par + (2 * D + 16 * cb), poff);
         }
     }
 }
@@ -594,13 +610,27 @@ __device__ __forceinline__ void next_part(const AttnArgs &a, Stretch &st, const 
     }
 }
 
-// the record of group i of (b, h); absent ones are read from the pool's first record, dead
+// The records of a wave's next 64 packed items, one a lane: items first, first + 4, ... below
+// last of one (request, head).  Looked up at once, so that no item waits for its table entry
+// (a load in the loop also waits for every load before it).  Records are 16-byte aligned: bit 0
+// says that the table names no page, and the address is then the pool's first record.
+struct Records {
+    uint32_t lo, hi;
+};
 template <int D>
-__device__ __forceinline__ const uint8_t *record_of(const AttnArgs &a, const int32_t *trow, int i, int h, bool &dead) {
-    const int per = a.p.page_tokens / PG_GROUP, pg = i / per;
-    const uint8_t *r = pg_record(a.p, uniform(trow[pg]), i - pg * per, h, 40 * D);
-    dead = r == nullptr;
-    return dead ? a.p.pool : r;
+__device__ __forceinline__ Records find_records(const AttnArgs &a, int b, int h, int first, int last, int lane) {
+    const int per = a.p.page_tokens / PG_GROUP, i = first + 4 * lane, pg = i / per;
+    uint64_t r = (uint64_t)a.p.pool | 1u;
+    if (i < last) {
+        const uint8_t *rec = pg_record(a.p, a.p.table[(int64_t)b * a.p.s_table + pg], i - pg * per, h, 40 * D);
+        if (rec) r = (uint64_t)rec;
+    }
+    return Records{(uint32_t)r, (uint32_t)(r >> 32)};
+}
+__device__ __forceinline__ rec_t record_at(const Records &r, int k, bool &dead) {
+    const uint32_t lo = (uint32_t)__builtin_amdgcn_readlane((int)r.lo, k), hi = (uint32_t)__builtin_amdgcn_readlane((int)r.hi, k);
+    dead = lo & 1u;
+    return (rec_t)((uint64_t)hi << 32 | (lo & ~1u));
 }
 
 template <bool BF16>
@@ -653,21 +683,25 @@ __global__ __launch_bounds__(256, NT == 1 ? 3 : 2) void paged_few_kernel(AttnArg
             c[nt] = (BF16 ? q_as_f16<D>(q[nt]) : 1.f) * a.sl2;
             clear(t[nt]);
         }
-        const int32_t *trow = a.p.table + (int64_t)b * a.p.s_table;
         const int last = min(pt.i1, it.ng);
-        int i = pt.i0 + wave;
+        int i = pt.i0 + wave, k = 0;
+        Records recs = find_records<D>(a, b, h, i, last, lane);
         RawK<D> rk;
         RawV<D> rv;
         bool dead = false;
         if (i < last) {
-            const uint8_t *rec = record_of<D>(a, trow, i, h, dead);
+            const rec_t rec = record_at(recs, 0, dead);
             load_k(rk, rec, lane);
             load_v(rv, rec, lane);
         }
         for (; i < last; i += WAVES) {
-            // (the last round loads its own record again: no branch around the loads)
+            if (++k == 64) {
+                recs = find_records<D>(a, b, h, i + WAVES, last, lane);
+                k = 0;
+            }
+            // (behind the last one the pool's first record is loaded: no branch around the loads)
             bool dead_next;
-            const uint8_t *next = record_of<D>(a, trow, i + WAVES < last ? i + WAVES : i, h, dead_next);
+            const rec_t next = record_at(recs, k, dead_next);
             f32x4_t s0[NT], s1[NT];
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt) s0[nt] = s1[nt] = f32x4_t{};
@@ -839,7 +873,6 @@ __global__ __launch_bounds__(512, 2) void paged_many_kernel(AttnArgs a) {
             c[nt] = (BF16 ? q_as_f16<D>(q[nt]) : 1.f) * a.sl2;
             clear(t[nt]);
         }
-        const int32_t *trow = a.p.table + (int64_t)b * a.p.s_table;
         // the seen tokens of an item, from its values' wave
         auto note_live = [&](int x, uint32_t live) {
             uint32_t all = 0;
@@ -853,9 +886,11 @@ __global__ __launch_bounds__(512, 2) void paged_many_kernel(AttnArgs a) {
         const int poff = sv ? 2 * (32 * (NC * (lane & 15) / 32) + 8 * hh) : (D / 2) * hh;
         RawK<D> raw;
         bool dead = false;
-        // the words of step x's item of this wave (behind the last one: of the last, again)
+        Records recs;
+        // the words of step x's item of this wave (behind the last one: of the pool's first record)
         auto fetch = [&](int x) {
-            const uint8_t *rec = record_of<D>(a, trow, min(pt.i0 + x * STEP + si, last - 1), h, dead);
+            if (x % 64 == 0) recs = find_records<D>(a, b, h, pt.i0 + x * STEP + si, last, lane);
+            const rec_t rec = record_at(recs, x % 64, dead);
             load_either(raw, rec, lane, sv, poff);
         };
         // ... as operands in buffer x & 1
