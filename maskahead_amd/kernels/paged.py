@@ -30,19 +30,38 @@ def record_bytes(head_dim: int) -> int:
     return 40 * int(head_dim)
 
 
-def _i32(t: torch.Tensor, name: str, shape: tuple, device: torch.device | None = None) -> torch.Tensor:
+def _i32(t: torch.Tensor, name: str, shape: tuple, index: int) -> None:
+    """A contiguous int32 tensor of this shape on GPU `index` (checked together; what is wrong
+    is looked for only when something is)."""
+    if t.is_cuda and t.dtype is torch.int32 and t.shape == shape and t.is_contiguous() and t.get_device() == index:
+        return
     N.require_gpu(t, name)
     if t.dtype != torch.int32 or tuple(t.shape) != shape or not t.is_contiguous():
         raise ValueError(f"{name} must be a contiguous int32 tensor of shape {shape}, got {t.dtype} {tuple(t.shape)}")
-    if device is not None and t.device != device:
-        raise ValueError(f"{name} is on {t.device}, expected {device}")
-    return t
+    raise ValueError(f"{name} is on {t.device}, expected cuda:{index}")
 
 
-def _same_device(device: torch.device, **tensors) -> None:
+def _check_table(t: torch.Tensor, b: int) -> None:
+    if t.ndim != 2 or t.dtype is not torch.int32 or t.shape[0] != b or (t.shape[1] > 1 and t.stride(1) != 1):
+        raise ValueError(f"block_table must be an int32 [{b}, width] tensor with contiguous rows")
+
+
+def _same_device(index: int, **tensors) -> None:
     for name, t in tensors.items():
-        if t is not None and t.device != device:
-            raise ValueError(f"{name} is on {t.device}, expected {device}")
+        if t is not None and t.get_device() != index:
+            raise ValueError(f"{name} is on {t.device}, expected cuda:{index}")
+
+
+def _call(index: int, name: str, *args) -> None:
+    """Entry point `name` on GPU `index`'s current stream, which is its last argument."""
+    fn = getattr(N.load(), name)
+    if torch._C._cuda_getDevice() == index:
+        rc = fn(*args, torch._C._cuda_getCurrentRawStream(index))
+    else:
+        with torch.cuda.device(index):
+            rc = fn(*args, torch._C._cuda_getCurrentRawStream(index))
+    if rc:
+        N.check(rc, name)
 
 
 class PagedPrefix:
@@ -59,7 +78,7 @@ class PagedPrefix:
     tokens were not there.  Strides and addresses are taken when the descriptor is made."""
 
     __slots__ = ("pool", "k_tail", "v_tail", "block_table", "lengths", "mask", "batch", "heads", "head_dim",
-                 "page_tokens", "dtype", "device", "_nat")
+                 "page_tokens", "dtype", "device", "index", "_nat")
 
     def __init__(self, pool: torch.Tensor, k_tail: torch.Tensor, v_tail: torch.Tensor, block_table: torch.Tensor,
                  lengths: torch.Tensor, mask: torch.Tensor | None = None):
@@ -78,19 +97,18 @@ class PagedPrefix:
         if k_tail.dtype not in (torch.bfloat16, torch.float16):
             raise N.KernelUnavailableError(f"tails of {k_tail.dtype} are not built (bf16, f16)")
         b = k_tail.shape[0]
-        if block_table.ndim != 2 or block_table.dtype != torch.int32 or block_table.shape[0] != b or \
-                (block_table.shape[1] > 1 and block_table.stride(1) != 1):
-            raise ValueError(f"block_table must be an int32 [{b}, width] tensor with contiguous rows")
+        _check_table(block_table, b)
         if mask is not None and (mask.ndim != 3 or mask.dtype != torch.uint8 or tuple(mask.shape[:2]) != (b, hkv) or
                                  (mask.shape[2] > 1 and mask.stride(2) != 1)):
             raise ValueError(f"mask must be a uint8 [{b}, {hkv}, tokens] tensor with contiguous tokens")
         N.require_gpu(pool, "pool")
-        _i32(lengths, "lengths", (b,))
-        _same_device(pool.device, k_tail=k_tail, v_tail=v_tail, block_table=block_table, lengths=lengths, mask=mask)
+        index = pool.get_device()
+        _i32(lengths, "lengths", (b,), index)
+        _same_device(index, k_tail=k_tail, v_tail=v_tail, block_table=block_table, lengths=lengths, mask=mask)
         self.pool, self.k_tail, self.v_tail = pool, k_tail, v_tail
         self.block_table, self.lengths, self.mask = block_table, lengths, mask
         self.batch, self.heads, self.head_dim, self.page_tokens = b, hkv, d, per * GROUP
-        self.dtype, self.device = k_tail.dtype, pool.device
+        self.dtype, self.device, self.index = k_tail.dtype, pool.device, index
         p = N.MaPages()
         p.pool, p.k_tail, p.v_tail = pool.data_ptr(), k_tail.data_ptr(), v_tail.data_ptr()
         p.table, p.lengths = block_table.data_ptr(), lengths.data_ptr()
@@ -107,19 +125,6 @@ class PagedPrefix:
 
     def native(self) -> N.MaPages:
         return self._nat
-
-
-def _on(device: torch.device):
-    """The device's context where it is not the current one (kernels go to its streams)."""
-    return torch.cuda.device(device)
-
-
-def _call(device: torch.device, name: str, *args) -> None:
-    if device.index == torch.cuda.current_device():
-        N.call(name, *args)
-        return
-    with _on(device):
-        N.call(name, *args)
 
 
 def plan_pages(lengths: torch.Tensor, new_lens: torch.Tensor, block_table: torch.Tensor, free_ring: torch.Tensor,
@@ -139,33 +144,34 @@ def plan_pages(lengths: torch.Tensor, new_lens: torch.Tensor, block_table: torch
     adds to the status, which stays until the caller clears it: 1 the pages run out, 2 a
     request outgrows its table row, 4 new_lens[b] > tokens, 8 a negative length
     (``check_plan`` reads it and raises)."""
-    b = lengths.shape[0]
-    _i32(lengths, "lengths", (b,))
-    dev = lengths.device
-    _i32(new_lens, "new_lens", (b,), dev)
-    if block_table.ndim != 2 or block_table.dtype != torch.int32 or block_table.shape[0] != b or \
-            (block_table.shape[1] > 1 and block_table.stride(1) != 1):
-        raise ValueError(f"block_table must be an int32 [{b}, width] tensor with contiguous rows")
-    _i32(free_ring, "free_ring", (free_ring.numel(),), dev)
-    _i32(ring_state, "ring_state", (4,), dev)
+    if lengths.ndim != 1:
+        raise ValueError(f"lengths must be [B], got {tuple(lengths.shape)}")
+    N.require_gpu(lengths, "lengths")
+    shape, index = lengths.shape, lengths.get_device()
+    b = shape[0]
+    _i32(lengths, "lengths", shape, index)
+    _i32(new_lens, "new_lens", shape, index)
+    _check_table(block_table, b)
+    _i32(free_ring, "free_ring", (free_ring.numel(),), index)
+    _i32(ring_state, "ring_state", (4,), index)
     tokens = int(tokens)
     if tokens < 0:
         raise ValueError("tokens must not be negative")
     if slots is None:
-        slots = torch.empty((b, tokens), device=dev, dtype=torch.int64)
-    elif slots.dtype != torch.int64 or tuple(slots.shape) != (b, tokens) or not slots.is_contiguous():
+        slots = torch.empty((b, tokens), device=lengths.device, dtype=torch.int64)
+    elif slots.dtype is not torch.int64 or slots.shape != (b, tokens) or not slots.is_contiguous():
         raise ValueError(f"slots must be a contiguous int64 [{b}, {tokens}] tensor")
     if ends is None:
-        ends = torch.empty((b,), device=dev, dtype=torch.int32)
+        ends = torch.empty_like(lengths)
     else:
-        _i32(ends, "ends", (b,), dev)
-    _same_device(dev, block_table=block_table, slots=slots)
+        _i32(ends, "ends", shape, index)
+    if block_table.get_device() != index or slots.get_device() != index:
+        _same_device(index, block_table=block_table, slots=slots)
     if b == 0:
         return slots, ends
-    _call(dev, "ma_page_plan", lengths.data_ptr(), new_lens.data_ptr(), b, tokens, int(page_tokens),
-          block_table.data_ptr(), block_table.stride(0), block_table.shape[1], free_ring.data_ptr(),
-          free_ring.numel(), ring_state.data_ptr(), slots.data_ptr() if tokens else None, ends.data_ptr(),
-          N.stream_of(lengths))
+    _call(index, "ma_page_plan", lengths.data_ptr(), new_lens.data_ptr(), b, tokens, int(page_tokens),
+          block_table.data_ptr(), block_table.stride(0), block_table.shape[1], free_ring.data_ptr(), free_ring.numel(),
+          ring_state.data_ptr(), slots.data_ptr() if tokens else None, ends.data_ptr())
     return slots, ends
 
 
@@ -182,16 +188,18 @@ def check_plan(ring_state: torch.Tensor) -> None:
         raise RuntimeError("page plan refused: " + ", ".join(text for bit, text in _PLAN_ERRORS if status & bit))
 
 
-def _check_block(name: str, t: torch.Tensor, prefix: PagedPrefix, heads: int | None = None) -> None:
-    if t.ndim != 4 or t.shape[0] != prefix.batch or t.shape[3] != prefix.head_dim or \
-            (heads is not None and t.shape[1] != heads):
+def _check_block(name: str, t: torch.Tensor, prefix: PagedPrefix, heads: int | None = None) -> torch.Size:
+    """[B, heads, T, D] of the prefix's batch, head_dim, dtype and device; returns the shape."""
+    s = t.shape
+    if len(s) != 4 or s[0] != prefix.batch or s[3] != prefix.head_dim or (heads is not None and s[1] != heads):
         raise ValueError(f"{name} must be [{prefix.batch}, {'H' if heads is None else heads}, T, {prefix.head_dim}], "
-                         f"got {tuple(t.shape)}")
-    N.require_gpu(t, name)
-    if t.device != prefix.device:
+                         f"got {tuple(s)}")
+    if t.get_device() != prefix.index:
+        N.require_gpu(t, name)
         raise ValueError(f"{name} is on {t.device}, expected {prefix.device}")
-    if t.dtype != prefix.dtype:
+    if t.dtype is not prefix.dtype:
         raise ValueError(f"{name} is {t.dtype}, the prefix {prefix.dtype}")
+    return s
 
 
 def append_pages(prefix: PagedPrefix, key: torch.Tensor, value: torch.Tensor, new_lens: torch.Tensor,
@@ -201,19 +209,19 @@ def append_pages(prefix: PagedPrefix, key: torch.Tensor, value: torch.Tensor, ne
     page that ``slots`` (``plan_pages``) names, the rest stays in the tail at 16 bits.
     prefix.lengths is not written: it is to become plan_pages' ends when every layer has been
     appended to.  Requests without new tokens, or whose slots are -1, are left as they are."""
-    _check_block("key", key, prefix, prefix.heads)
-    _check_block("value", value, prefix, prefix.heads)
-    b, h, t, d = key.shape
-    if value.shape != key.shape:
+    shape = _check_block("key", key, prefix, prefix.heads)
+    if _check_block("value", value, prefix, prefix.heads) != shape:
         raise ValueError("key and value shapes differ")
-    _i32(new_lens, "new_lens", (b,), prefix.device)
-    if slots.dtype != torch.int64 or tuple(slots.shape) != (b, t) or not slots.is_contiguous():
+    b, h, t, d = shape
+    _i32(new_lens, "new_lens", (b,), prefix.index)
+    if slots.dtype is not torch.int64 or slots.shape != (b, t) or not slots.is_contiguous():
         raise ValueError(f"slots must be a contiguous int64 [{b}, {t}] tensor")
-    _same_device(prefix.device, slots=slots)
+    if slots.get_device() != prefix.index:
+        raise ValueError(f"slots is on {slots.device}, expected {prefix.device}")
     if b == 0 or t == 0:
         return
-    _call(prefix.device, "ma_page_append", prefix.native(), N.t4(key), N.t4(value), b, h, t, d, new_lens.data_ptr(),
-          slots.data_ptr(), N.stream_of(key))
+    _call(prefix.index, "ma_page_append", prefix._nat, N.t4(key), N.t4(value), b, h, t, d, new_lens.data_ptr(),
+          slots.data_ptr())
 
 
 def dequantize_pages(prefix: PagedPrefix, tokens: int, *, starts: torch.Tensor | None = None,
@@ -231,14 +239,14 @@ def dequantize_pages(prefix: PagedPrefix, tokens: int, *, starts: torch.Tensor |
     if out_value is None:
         out_value = torch.empty(shape, device=prefix.device, dtype=dtype)
     for name, t in (("out_key", out_key), ("out_value", out_value)):
-        if tuple(t.shape) != shape or t.dtype != dtype or t.device != prefix.device:
+        if t.shape != shape or t.dtype is not dtype or t.get_device() != prefix.index:
             raise ValueError(f"{name} must be {dtype} {shape} on {prefix.device}")
     if starts is not None:
-        _i32(starts, "starts", (prefix.batch,), prefix.device)
+        _i32(starts, "starts", (prefix.batch,), prefix.index)
     if prefix.batch == 0 or tokens == 0:
         return out_key, out_value
-    _call(prefix.device, "ma_page_dequant", prefix.native(), prefix.batch, prefix.heads, prefix.head_dim,
-          N.ptr(starts), tokens, N.t4(out_key), N.t4(out_value), N.stream_of(out_key))
+    _call(prefix.index, "ma_page_dequant", prefix._nat, prefix.batch, prefix.heads, prefix.head_dim, N.ptr(starts),
+          tokens, N.t4(out_key), N.t4(out_value))
     return out_key, out_value
 
 
@@ -255,37 +263,34 @@ def paged_attention(query: torch.Tensor, prefix: PagedPrefix, current_key: torch
     t only if (lengths[b] + j) // causal_block <= (lengths[b] + t) // causal_block.  A row that
     sees nothing is zero.  ``out`` [B, Hq, T, D] (not overlapping the inputs) receives the
     result; without it a new tensor does, whose rows t >= new_lens[b] are undefined."""
-    _check_block("query", query, prefix)
-    b, hq, t, d = query.shape
-    if hq == 0 or hq % prefix.heads:
+    shape = _check_block("query", query, prefix)
+    b, hq, t, d = shape
+    h = prefix.heads
+    if hq == 0 or hq % h:
         raise ValueError("Hq must be a positive multiple of Hkv")
     if (current_key is None) != (current_value is None):
         raise ValueError("current_key and current_value go together")
     if current_key is not None:
-        _check_block("current_key", current_key, prefix, prefix.heads)
-        _check_block("current_value", current_value, prefix, prefix.heads)
-        if current_key.shape[2] != t or current_value.shape[2] != t:
+        if _check_block("current_key", current_key, prefix, h)[2] != t or \
+                _check_block("current_value", current_value, prefix, h)[2] != t:
             raise ValueError(f"the block's keys and values must hold {t} positions like its queries")
     if new_lens is not None:
-        _i32(new_lens, "new_lens", (b,), prefix.device)
+        _i32(new_lens, "new_lens", (b,), prefix.index)
     if causal_block < 0:
         raise ValueError("causal_block must not be negative")
     if out is None:
-        out = torch.empty((b, hq, t, d), device=query.device, dtype=query.dtype)
-    else:
-        _check_block("out", out, prefix, hq)
-        if out.shape[2] != t:
-            raise ValueError(f"out must be {tuple(query.shape)}")
+        out = torch.empty(shape, device=query.device, dtype=query.dtype)
+    elif _check_block("out", out, prefix, hq) != shape:
+        raise ValueError(f"out must be {tuple(shape)}")
     if b == 0 or t == 0:
         return out
     scale = float(scaling) if scaling is not None else d ** -0.5
-    need = N.size_query("ma_paged_workspace_bytes", b, prefix.heads, hq, t, d)
+    need = N.size_query("ma_paged_workspace_bytes", b, h, hq, t, d)
     if need < 0:
-        raise N.KernelUnavailableError(f"head_dim {d} with {hq // prefix.heads * t} rows per KV head is not built")
+        raise N.KernelUnavailableError(f"{hq // h * t} rows for each of {b * h} KV heads are not built")
     ws = torch.empty((need,), device=query.device, dtype=torch.uint8)
-    _call(prefix.device, "ma_paged_attention", N.t4(query), b, hq, t, d, prefix.native(), prefix.heads,
-          N.t4(current_key), N.t4(current_value), N.ptr(new_lens), int(causal_block), scale, N.t4(out),
-          ws.data_ptr(), need, N.stream_of(query))
+    _call(prefix.index, "ma_paged_attention", N.t4(query), b, hq, t, d, prefix._nat, h, N.t4(current_key),
+          N.t4(current_value), N.ptr(new_lens), int(causal_block), scale, N.t4(out), ws.data_ptr(), need)
     return out
 
 
