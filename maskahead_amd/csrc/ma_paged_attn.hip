@@ -531,12 +531,7 @@ __device__ __forceinline__ Stretch find_stretch(const AttnArgs &a, ScanShared &s
             if (i == 0) own = it;
             sum += it.items;
         }
-    int64_t inc = sum;
-#pragma unroll
-    for (int o = 1; o < 64; o <<= 1) {
-        const int64_t y = __shfl_up(inc, o);
-        if (lane >= o) inc += y;
-    }
+    const int64_t inc = pg_wave_scan(sum, lane);
     if (lane == 63) sh.wsum[wave] = inc;
     __syncthreads();
     int64_t before = inc - sum, total = 0;
@@ -549,12 +544,12 @@ __device__ __forceinline__ Stretch find_stretch(const AttnArgs &a, ScanShared &s
     Stretch r;
     // stretches of one XCD's workgroups lie next to one another: row groups share its L2
     r.w = (int64_t)(blockIdx.x % 8) * (a.W / 8) + blockIdx.x / 8;
-    const int64_t each = (total + a.W - 1) / a.W;
+    const int64_t each = pg_div(total + a.W - 1, a.W);
     r.chunk = max((each + unit - 1) / unit, (int64_t)1) * unit;
     r.s = r.w * r.chunk;
     r.e = min(r.s + r.chunk, total);
     if (r.s < total) {
-        const int64_t want = r.s / HR;
+        const int64_t want = pg_div(r.s, HR);
         if (want >= before && want < before + sum) {
             int64_t pre = before;
             int b = first;
@@ -585,7 +580,7 @@ __device__ __forceinline__ Part part_of(const AttnArgs &a, const Stretch &st, in
     const Items &it = st.it;
     Part p;
     const int64_t rel = pos - (int64_t)a.H * a.RG * st.pre;
-    p.hr = (int)(rel / it.items);
+    p.hr = (int)pg_div(rel, it.items);
     p.i0 = (int)(rel - (int64_t)p.hr * it.items);
     p.i1 = (int)min((int64_t)it.items, p.i0 + (st.e - pos));
     p.h = p.hr / a.RG;
@@ -598,7 +593,7 @@ __device__ __forceinline__ Part part_of(const AttnArgs &a, const Stretch &st, in
 // workgroup), or no stretches where it is whole.
 __device__ __forceinline__ void note_segment(const AttnArgs &a, const Stretch &st, const Part &p, int64_t pos) {
     if (p.i0 != 0 || threadIdx.x != 0) return;
-    const int n = p.whole ? 0 : (int)((pos + st.it.items - 1) / st.chunk - st.w + 1);
+    const int n = p.whole ? 0 : (int)(pg_div(pos + st.it.items - 1, st.chunk) - st.w + 1);
     a.desc[(int64_t)st.b * a.H * a.RG + p.hr] = int4{(int)p.slot, n, (int)st.w, 0};
 }
 __device__ __forceinline__ void next_part(const AttnArgs &a, Stretch &st, const Part &p, int64_t &pos) {
@@ -677,12 +672,10 @@ __global__ __launch_bounds__(256, NT == 1 ? 3 : 2) void paged_few_kernel(AttnArg
         uint4 q[NT][CB];
         float c[NT];
         Tile<D> t[NT];
+        // (the queries' loads and the table's are under way together, the first record's behind
+        // them while the queries are scaled)
 #pragma unroll
-        for (int nt = 0; nt < NT; ++nt) {
-            load_q<D>(a, b, h, row0 + nt * 16 + (hidden(lane) & 15), it.n, hh, q[nt]);
-            c[nt] = (BF16 ? q_as_f16<D>(q[nt]) : 1.f) * a.sl2;
-            clear(t[nt]);
-        }
+        for (int nt = 0; nt < NT; ++nt) load_q<D>(a, b, h, row0 + nt * 16 + (hidden(lane) & 15), it.n, hh, q[nt]);
         const int last = min(pt.i1, it.ng);
         int i = pt.i0 + wave, k = 0;
         Records recs = find_records<D>(a, b, h, i, last, lane);
@@ -693,6 +686,11 @@ __global__ __launch_bounds__(256, NT == 1 ? 3 : 2) void paged_few_kernel(AttnArg
             const rec_t rec = record_at(recs, 0, dead);
             load_k(rk, rec, lane);
             load_v(rv, rec, lane);
+        }
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) {
+            c[nt] = (BF16 ? q_as_f16<D>(q[nt]) : 1.f) * a.sl2;
+            clear(t[nt]);
         }
         for (; i < last; i += WAVES) {
             if (++k == 64) {
@@ -763,7 +761,8 @@ __global__ __launch_bounds__(256, NT == 1 ? 3 : 2) void paged_few_kernel(AttnArg
             for (int nt = 0; nt < NT; ++nt)
                 p[nt] = rows_probs<D, BF16>(t[nt], s[0][nt], s[1][nt], a.sl2,
                                             causal_live(a, it, r, row0 + nt * 16 + (l & 15), lh, seen));
-            __builtin_amdgcn_sched_barrier(0);   // the values' loads stay behind the scores' registers
+            // (the values' loads stay behind the scores' registers: ahead of them the main loop spilled)
+            __builtin_amdgcn_sched_barrier(0);
             uint32_t vw[8][NC / 2];
             rows_v<D>(r, l, seen, vw);
 #pragma unroll
@@ -868,11 +867,7 @@ __global__ __launch_bounds__(512, 2) void paged_many_kernel(AttnArgs a) {
         float c[2];
         Tile<D> t[2];
 #pragma unroll
-        for (int nt = 0; nt < 2; ++nt) {
-            load_q<D>(a, b, h, row0 + nt * 16 + (hidden(lane) & 15), it.n, hh, q[nt]);
-            c[nt] = (BF16 ? q_as_f16<D>(q[nt]) : 1.f) * a.sl2;
-            clear(t[nt]);
-        }
+        for (int nt = 0; nt < 2; ++nt) load_q<D>(a, b, h, row0 + nt * 16 + (hidden(lane) & 15), it.n, hh, q[nt]);
         // the seen tokens of an item, from its values' wave
         auto note_live = [&](int x, uint32_t live) {
             uint32_t all = 0;
@@ -914,6 +909,11 @@ __global__ __launch_bounds__(512, 2) void paged_many_kernel(AttnArgs a) {
             }
         };
         if (steps > 0) fetch(0);
+#pragma unroll
+        for (int nt = 0; nt < 2; ++nt) {
+            c[nt] = (BF16 ? q_as_f16<D>(q[nt]) : 1.f) * a.sl2;
+            clear(t[nt]);
+        }
         for (int x = -1; x < steps; ++x) {
             if (x + 1 < steps) {
                 unpack(x + 1);
@@ -1105,9 +1105,8 @@ __global__ __launch_bounds__(256) void paged_merge_kernel(AttnArgs a, int rows) 
     __shared__ float so[RPW][GR][D];
     const int b = blockIdx.x / (a.H * a.RG), hr = blockIdx.x - b * (a.H * a.RG);
     const int n = a.new_lens ? min(max(a.new_lens[b], 0), a.T) : a.T;
-    if (n == 0) return;                     // (nobody wrote its segments)
     const int4 d = a.desc[blockIdx.x];
-    if (d.y == 0) return;
+    if ((n == 0) | (d.y == 0)) return;      // (n 0: nobody wrote its segments)
     const int w = d.z, r = threadIdx.x / (16 * GR), grp = (threadIdx.x >> 4) % GR, x = threadIdx.x & 15;
     const int h = hr / a.RG, rg = hr - h * a.RG;
     const int rt = blockIdx.y * RPW + r, row = rg * rows + rt;

@@ -89,6 +89,23 @@ __device__ __forceinline__ const uint8_t *pg_record(const PagesDev &p, int page_
     return p.pool + (int64_t)page_id * p.s_page + (int64_t)h * p.s_head + (int64_t)gi * rec;
 }
 
+// inclusive prefix sum over the wave of values >= 0: by lane moves where 32 bits hold every sum
+__device__ __forceinline__ int64_t pg_wave_scan(int64_t x, int lane) {
+    if (!__any(x >= (int64_t)1 << 25)) return (int64_t)ma_wave_prefix_u32((uint32_t)x);
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) {
+        const int64_t y = __shfl_up(x, o);
+        if (lane >= o) x += y;
+    }
+    return x;
+}
+
+// x / y of whole numbers >= 0 that the whole wave holds; in 32 bits where they fit
+__device__ __forceinline__ int64_t pg_div(int64_t x, int64_t y) {
+    if (((x | y) >> 32) == 0) return (int64_t)((uint32_t)x / (uint32_t)y);
+    return x / y;
+}
+
 // host: the checks every entry point over a store makes
 int pg_check(const ma_pages *p, int B, int H, int D, const char *who);
 

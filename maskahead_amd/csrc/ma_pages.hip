@@ -31,13 +31,18 @@ struct PlanArgs {
     int B, T, page, width, num_pages;
 };
 
-__device__ __forceinline__ int64_t wave_scan_i64(int64_t x, int lane) {
-#pragma unroll
-    for (int o = 1; o < 64; o <<= 1) {
-        const int64_t y = __shfl_up(x, o);
-        if (lane >= o) x += y;
-    }
-    return x;
+// a request's step: tokens after it, pages before and after it (`most` + 1 where there are more
+// than `most`); all in 32 bits, len + n < 2^32
+struct Step {
+    uint32_t end, p0, p1;
+};
+__device__ __forceinline__ Step step_of(int len, int n, uint32_t page, uint32_t most) {
+    Step s;
+    const int64_t end = max((int64_t)len + n, (int64_t)0);
+    s.end = (uint32_t)end;
+    s.p0 = ((uint32_t)max(len, 0) + page - 1) / page;
+    s.p1 = end > INT32_MAX ? most + 1 : (s.end + page - 1) / page;
+    return s;
 }
 
 __global__ __launch_bounds__(PLAN_THREADS) void page_plan_kernel(PlanArgs a) {
@@ -64,17 +69,16 @@ __global__ __launch_bounds__(PLAN_THREADS) void page_plan_kernel(PlanArgs a) {
             g[i] = gt;
             k[i] = kt;
             if (b < a.B) {
-                const int64_t len = a.lengths[b], n = a.new_lens[b];
-                const int64_t end = max(len + n, (int64_t)0);
-                const int64_t p0 = (len + a.page - 1) / a.page, p1 = (end + a.page - 1) / a.page;
+                const int len = a.lengths[b], n = a.new_lens[b];
+                const Step st = step_of(len, n, a.page, a.width);
                 if (len < 0) bad |= PLAN_LENGTH;
                 if (n > a.T) bad |= PLAN_TOKENS;
-                if (max(p0, p1) > a.width) bad |= PLAN_WIDTH;
-                gt += max(p1 - p0, (int64_t)0);
-                kt += max(p0 - p1, (int64_t)0);
+                if (max(st.p0, st.p1) > (uint32_t)a.width) bad |= PLAN_WIDTH;
+                gt += st.p1 > st.p0 ? st.p1 - st.p0 : 0;
+                kt += st.p0 > st.p1 ? st.p0 - st.p1 : 0;
             }
         }
-        const int64_t gi = wave_scan_i64(gt, lane), ki = wave_scan_i64(kt, lane);
+        const int64_t gi = pg_wave_scan(gt, lane), ki = pg_wave_scan(kt, lane);
         __syncthreads();   // wsum of the step before is read
         if (lane == 63) {
             wsum[0][wave] = gi;
@@ -106,31 +110,49 @@ __global__ __launch_bounds__(PLAN_THREADS) void page_plan_kernel(PlanArgs a) {
     // head and count are the caller's: a ring outside its own bounds is never indexed
     if (head < 0 || count < 0 || head >= a.num_pages || count > a.num_pages || bsum > a.num_pages - count)
         bad |= PLAN_NO_PAGES;
-    for (int f = tid; f < nf; f += PLAN_THREADS) {
+    // a thread's pairs: first every page id is read, then everything is written (a write to the
+    // table would hold back the next pair's reads)
+    constexpr int PER = PLAN_SLOTS / PLAN_THREADS;
+    int id[PER], off[PER], end[PER];
+    int32_t *fresh[PER];      // where a page that appears is noted
+#pragma unroll
+    for (int y = 0; y < PER; ++y) {
+        const int f = tid + y * PLAN_THREADS;
+        id[y] = -1;
+        off[y] = 0;
+        fresh[y] = nullptr;
+        end[y] = 0;
+        if (f >= nf) continue;
         const unsigned flat = (unsigned)f + (unsigned)r0;
         const int bl = (int)(flat / (unsigned)Tm), b = b0 + bl;
         const int i = (int)(flat - (unsigned)bl * (unsigned)Tm);
         const int len = a.lengths[b], n = a.new_lens[b];
-        if (i == 0) a.ends[b] = bad ? len : (int)max((int64_t)len + n, (int64_t)0);
-        if (i >= a.T) continue;
-        int64_t slot = -1;
-        if (!bad && i < n) {
-            const int pos = len + i;
-            const int pi = pos / a.page, off = pos - pi * a.page;
-            const int p0 = (int)(((int64_t)len + a.page - 1) / a.page);
-            int32_t *row = a.table + (int64_t)b * a.s_table;
-            int id;
-            if (pi >= p0) {
-                int at = head + grow_off[bl] + (pi - p0);      // < 2 num_pages
-                if (at >= a.num_pages) at -= a.num_pages;
-                id = a.ring[at];
-                if (off == 0) row[pi] = id;                    // every new page begins with a new token
-            } else {
-                id = row[pi];
-            }
-            slot = (int64_t)id * a.page + off;
+        end[y] = bad ? len : (int)max((int64_t)len + n, (int64_t)0);
+        if (bad || i >= n) continue;
+        const uint32_t pos = (uint32_t)(len + i), pi = pos / (uint32_t)a.page;
+        const uint32_t p0 = ((uint32_t)len + a.page - 1) / (uint32_t)a.page;
+        off[y] = (int)(pos - pi * a.page);
+        int32_t *row = a.table + (int64_t)b * a.s_table + pi;
+        const int32_t *src = row;
+        if (pi >= p0) {
+            int at = head + grow_off[bl] + (int)(pi - p0);      // < 2 num_pages
+            if (at >= a.num_pages) at -= a.num_pages;
+            src = a.ring + at;
+            if (off[y] == 0) fresh[y] = row;                   // every new page begins with a new token
         }
-        a.slots[(int64_t)b * a.T + i] = slot;
+        id[y] = *src;
+    }
+#pragma unroll
+    for (int y = 0; y < PER; ++y) {
+        const int f = tid + y * PLAN_THREADS;
+        if (f >= nf) continue;
+        const unsigned flat = (unsigned)f + (unsigned)r0;
+        const int bl = (int)(flat / (unsigned)Tm), b = b0 + bl;
+        const int i = (int)(flat - (unsigned)bl * (unsigned)Tm);
+        if (i == 0) a.ends[b] = end[y];
+        // (an id below 0 is no page, with or without an offset)
+        if (i < a.T) a.slots[(int64_t)b * a.T + i] = id[y] < 0 ? -1 : (int64_t)id[y] * a.page + off[y];
+        if (fresh[y]) *fresh[y] = id[y];
     }
     // pages that go back: a wave per request that gives some, of the requests whose first pair
     // is this workgroup's
@@ -139,9 +161,9 @@ __global__ __launch_bounds__(PLAN_THREADS) void page_plan_kernel(PlanArgs a) {
         for (int s = lo + wave * 64; s < nb; s += PLAN_THREADS) {
             int p0 = 0, p1 = 0;
             if (s + lane < nb) {
-                const int64_t len = a.lengths[b0 + s + lane], n = a.new_lens[b0 + s + lane];
-                p0 = (int)((len + a.page - 1) / a.page);
-                p1 = (int)((max(len + n, (int64_t)0) + a.page - 1) / a.page);
+                const Step st = step_of(a.lengths[b0 + s + lane], a.new_lens[b0 + s + lane], a.page, a.width);
+                p0 = (int)st.p0;
+                p1 = (int)st.p1;
             }
             uint64_t todo = __ballot(p0 > p1);
             while (todo) {
@@ -199,9 +221,10 @@ __global__ __launch_bounds__(256) void page_append_kernel(AppendArgs a) {
     __shared__ __attribute__((aligned(16))) uint8_t kc[PG_GROUP * D];
     __shared__ __attribute__((aligned(16))) uint8_t vc[D * VS];
     const int tid = threadIdx.x, u = blockIdx.x, h = blockIdx.y, b = blockIdx.z;
-    const int n = min(a.new_lens[b], a.T);
-    if (n <= 0 || a.slots[(int64_t)b * a.T] < 0) return;
-    const int len = pg_length(a.p, b), r = len & (PG_GROUP - 1);
+    // (looked at together, so that their loads are under way together)
+    const int n = min(a.new_lens[b], a.T), len = pg_length(a.p, b), r = len & (PG_GROUP - 1);
+    const int64_t slot0 = a.slots[(int64_t)b * a.T];
+    if ((n <= 0) | (slot0 < 0)) return;
     const int whole = (r + n) / PG_GROUP;
     if (u >= max(whole, 1)) return;
     const uint16_t *kn = a.k + (int64_t)b * a.s_kb + (int64_t)h * a.s_kh;
