@@ -110,49 +110,43 @@ __global__ __launch_bounds__(PLAN_THREADS) void page_plan_kernel(PlanArgs a) {
     // head and count are the caller's: a ring outside its own bounds is never indexed
     if (head < 0 || count < 0 || head >= a.num_pages || count > a.num_pages || bsum > a.num_pages - count)
         bad |= PLAN_NO_PAGES;
-    // a thread's pairs: first every page id is read, then everything is written (a write to the
-    // table would hold back the next pair's reads)
+    // A thread's pairs, in three rounds without branches -- lengths, page ids, writes -- so that
+    // each round's loads are under way together (pairs behind the last are the last one again,
+    // pairs without a page read the ring's first entry).
     constexpr int PER = PLAN_SLOTS / PLAN_THREADS;
-    int id[PER], off[PER], end[PER];
-    int32_t *fresh[PER];      // where a page that appears is noted
+    int bl[PER], tok[PER], len[PER], n[PER], id[PER];
 #pragma unroll
     for (int y = 0; y < PER; ++y) {
-        const int f = tid + y * PLAN_THREADS;
-        id[y] = -1;
-        off[y] = 0;
-        fresh[y] = nullptr;
-        end[y] = 0;
-        if (f >= nf) continue;
-        const unsigned flat = (unsigned)f + (unsigned)r0;
-        const int bl = (int)(flat / (unsigned)Tm), b = b0 + bl;
-        const int i = (int)(flat - (unsigned)bl * (unsigned)Tm);
-        const int len = a.lengths[b], n = a.new_lens[b];
-        end[y] = bad ? len : (int)max((int64_t)len + n, (int64_t)0);
-        if (bad || i >= n) continue;
-        const uint32_t pos = (uint32_t)(len + i), pi = pos / (uint32_t)a.page;
-        const uint32_t p0 = ((uint32_t)len + a.page - 1) / (uint32_t)a.page;
-        off[y] = (int)(pos - pi * a.page);
-        int32_t *row = a.table + (int64_t)b * a.s_table + pi;
-        const int32_t *src = row;
-        if (pi >= p0) {
-            int at = head + grow_off[bl] + (int)(pi - p0);      // < 2 num_pages
-            if (at >= a.num_pages) at -= a.num_pages;
-            src = a.ring + at;
-            if (off[y] == 0) fresh[y] = row;                   // every new page begins with a new token
-        }
-        id[y] = *src;
+        const unsigned flat = (unsigned)min(tid + y * PLAN_THREADS, nf - 1) + (unsigned)r0;
+        bl[y] = (int)(flat / (unsigned)Tm);
+        tok[y] = (int)(flat - (unsigned)bl[y] * (unsigned)Tm);
+        len[y] = a.lengths[b0 + bl[y]];
+        n[y] = a.new_lens[b0 + bl[y]];
+    }
+    auto fresh = [&](int y, uint32_t pi) {    // a page that appears (its first token is a new one)
+        return pi >= ((uint32_t)len[y] + a.page - 1) / (uint32_t)a.page;
+    };
+#pragma unroll
+    for (int y = 0; y < PER; ++y) {
+        const bool has = !bad && tok[y] < n[y];
+        const uint32_t pi = (uint32_t)(len[y] + tok[y]) / (uint32_t)a.page;
+        const uint32_t p0 = ((uint32_t)len[y] + a.page - 1) / (uint32_t)a.page;
+        int at = head + grow_off[bl[y]] + (int)(pi - p0);       // (fresh pages: < 2 num_pages)
+        if (at >= a.num_pages) at -= a.num_pages;
+        const int32_t *old = a.table + (int64_t)(b0 + bl[y]) * a.s_table + pi;
+        const int32_t *src = pi >= p0 ? a.ring + at : old;
+        id[y] = *(has ? src : a.ring);
     }
 #pragma unroll
     for (int y = 0; y < PER; ++y) {
-        const int f = tid + y * PLAN_THREADS;
-        if (f >= nf) continue;
-        const unsigned flat = (unsigned)f + (unsigned)r0;
-        const int bl = (int)(flat / (unsigned)Tm), b = b0 + bl;
-        const int i = (int)(flat - (unsigned)bl * (unsigned)Tm);
-        if (i == 0) a.ends[b] = end[y];
+        if (tid + y * PLAN_THREADS >= nf) continue;
+        const int b = b0 + bl[y];
+        const uint32_t pos = (uint32_t)(len[y] + tok[y]), pi = pos / (uint32_t)a.page, off = pos - pi * a.page;
+        const bool has = !bad && tok[y] < n[y];
+        if (tok[y] == 0) a.ends[b] = bad ? len[y] : (int)max((int64_t)len[y] + n[y], (int64_t)0);
         // (an id below 0 is no page, with or without an offset)
-        if (i < a.T) a.slots[(int64_t)b * a.T + i] = id[y] < 0 ? -1 : (int64_t)id[y] * a.page + off[y];
-        if (fresh[y]) *fresh[y] = id[y];
+        if (tok[y] < a.T) a.slots[(int64_t)b * a.T + tok[y]] = has && id[y] >= 0 ? (int64_t)id[y] * a.page + off : -1;
+        if (has && off == 0 && fresh(y, pi)) a.table[(int64_t)b * a.s_table + pi] = id[y];
     }
     // pages that go back: a wave per request that gives some, of the requests whose first pair
     // is this workgroup's
@@ -192,12 +186,17 @@ __global__ __launch_bounds__(PLAN_THREADS) void page_plan_kernel(PlanArgs a) {
 }
 
 // ------------------------------------------------------------------ append
-// One workgroup = one group of 32 tokens of one (request, KV head): the window of request b
-// is [its tail | its new tokens], group u the window's tokens 32 u ...  Rows go to LDS at 16
-// bits; a thread quantizes one key channel (32 tokens) or one value group (32 channels of a
-// token), codes as bytes in LDS, and the words are put together in the operands' order, 16
-// bytes a thread.  The workgroup of group 0 is the only reader of the old tail, so it also
-// writes the new one, behind its barrier.
+// One wave = the keys or the values of one group of 32 tokens of one (request, KV head): the
+// window of request b is [its tail | its new tokens], group u the window's tokens 32 u ...
+// Nothing goes through LDS: the lanes of a values wave hold the 8 tokens x D/16 channels whose
+// words they store (1 KB a store instruction), those of a keys wave 4 channels of 16 (D 64: 8)
+// tokens, whose minimum and maximum need one (two) lane moves, and two lanes make a word.  The
+// waves of group 0 are the only readers of the old tail, so they also write the new one.
+//
+// bound: 4 D bytes read and 1.25 D written a token and head.  A quotient rounded to a bf16 code
+// needs no division: with 8-bit significands a / step is never nearer than 2^-17 (relative) to
+// where bf16 rounds the other way, and a * rcp(step) is within 2^-22 of it; a / 15 likewise
+// (2^-13).  f16 quotients come as near as 2^-23 and are divided.
 struct AppendArgs {
     PagesDev p;
     const uint16_t *k, *v;
@@ -207,115 +206,240 @@ struct AppendArgs {
     int T;
 };
 
-// 8 codes (bytes, elements 0..3 in a, 4..7 in b) as one word, nibbles 0 2 4 6 1 3 5 7
-__device__ __forceinline__ uint32_t pack_word(uint32_t a, uint32_t b) {
-    return (a & 0xfu) | ((a >> 12) & 0xf0u) | ((b << 8) & 0xf00u) | ((b >> 4) & 0xf000u) | ((a << 8) & 0xf0000u) |
-           ((a >> 4) & 0xf00000u) | ((b << 16) & 0xf000000u) | ((b << 4) & 0xf0000000u);
+template <int DT>
+__device__ __forceinline__ void unpack2(uint32_t w, float &a, float &b) {
+    if constexpr (DT == MA_BF16) {
+        a = __uint_as_float(w << 16);
+        b = __uint_as_float(w & 0xffff0000u);
+    } else {
+        a = ma_f16_to_f32((uint16_t)w);
+        b = ma_f16_to_f32((uint16_t)(w >> 16));
+    }
+}
+// two values rounded to DT, as f32
+template <int DT>
+__device__ __forceinline__ void round2(float &a, float &b) {
+    if constexpr (DT == MA_BF16) unpack2<DT>(ma_pack_bf16x2(a, b), a, b);
+    else a = ma_round_f16(a), b = ma_round_f16(b);
+}
+template <int DT>
+__device__ __forceinline__ QuantGroup group_params(float lo, float hi) {
+    if constexpr (DT != MA_BF16) return quant_params(lo, hi, DT);
+    float step = ma_round_bf16(ma_round_bf16(hi - lo) * (1.0f / 15.0f));
+    step = ma_round_bf16(fmaxf(step, 1e-8f));
+    return {lo, step, __builtin_amdgcn_rcpf(step)};
+}
+// minimum / maximum of three, without the quieting that fminf / fmaxf put before each argument
+__device__ __forceinline__ float min3(float x, float y, float z) {
+    float r;
+    asm("v_min3_f32 %0, %1, %2, %3" : "=v"(r) : "v"(x), "v"(y), "v"(z));
+    return r;
+}
+__device__ __forceinline__ float max3(float x, float y, float z) {
+    float r;
+    asm("v_max3_f32 %0, %1, %2, %3" : "=v"(r) : "v"(x), "v"(y), "v"(z));
+    return r;
+}
+// The quotients whose nearest whole numbers (half to even) are the codes of two values; NaN's
+// code is 0, as quant_code's.  A bf16 quotient is at most 15 (1 + 2^-8); f16's, with a step that
+// f16 holds in few bits, may be more.
+template <int DT>
+__device__ __forceinline__ void codes2(float &a, float &b, const QuantGroup &qa, const QuantGroup &qb) {
+    a -= qa.lo;
+    b -= qb.lo;
+    round2<DT>(a, b);
+    if constexpr (DT == MA_BF16) {
+        a *= qa.inv;
+        b *= qb.inv;
+    } else {
+        a = quant_div(a, qa, DT);
+        b = quant_div(b, qb, DT);
+    }
+    round2<DT>(a, b);
+    if constexpr (DT != MA_BF16) {
+        a = __builtin_amdgcn_fmed3f(a, 0.0f, 15.0f);
+        b = __builtin_amdgcn_fmed3f(b, 0.0f, 15.0f);
+    }
+}
+// x rounded half to even into one byte of w (v_cvt_pk_u8_f32; NaN: 0)
+__device__ __forceinline__ uint32_t put_byte(float x, uint32_t byte, uint32_t w) {
+    return __builtin_amdgcn_cvt_pk_u8_f32(x, byte, w);
+}
+__device__ __forceinline__ uint32_t f16x2_bits(float a, float b) {
+    const f16x2_t v = {(_Float16)a, (_Float16)b};
+    return __builtin_bit_cast(uint32_t, v);
 }
 
 template <int D, int DT>
 __global__ __launch_bounds__(256) void page_append_kernel(AppendArgs a) {
-    constexpr int XS = D + 8;           // row stride of the 16-bit window, elements
-    constexpr int VS = PG_GROUP + 8;    // row stride of the value codes (channel-major), bytes
-    __shared__ __attribute__((aligned(16))) uint16_t X[2][PG_GROUP * XS];
-    __shared__ __attribute__((aligned(16))) uint8_t kc[PG_GROUP * D];
-    __shared__ __attribute__((aligned(16))) uint8_t vc[D * VS];
-    const int tid = threadIdx.x, u = blockIdx.x, h = blockIdx.y, b = blockIdx.z;
+    constexpr int NC = D / 16, CL = D / 4, SL = 64 / CL, TPL = PG_GROUP / SL;   // CL lanes a row, SL slices of the tokens
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int u = blockIdx.x * 2 + (wave >> 1), h = blockIdx.y, b = blockIdx.z;
+    const bool val = wave & 1;
     // (looked at together, so that their loads are under way together)
     const int n = min(a.new_lens[b], a.T), len = pg_length(a.p, b), r = len & (PG_GROUP - 1);
     const int64_t slot0 = a.slots[(int64_t)b * a.T];
     if ((n <= 0) | (slot0 < 0)) return;
     const int whole = (r + n) / PG_GROUP;
     if (u >= max(whole, 1)) return;
-    const uint16_t *kn = a.k + (int64_t)b * a.s_kb + (int64_t)h * a.s_kh;
-    const uint16_t *vn = a.v + (int64_t)b * a.s_vb + (int64_t)h * a.s_vh;
-    uint16_t *kt = a.p.kt + (int64_t)b * a.p.s_tb + (int64_t)h * a.p.s_th;
-    uint16_t *vt = a.p.vt + (int64_t)b * a.p.s_tb + (int64_t)h * a.p.s_th;
-    constexpr int CH = D / 8;           // 16-byte chunks of a row
+    const uint16_t *fresh = val ? a.v + (int64_t)b * a.s_vb + (int64_t)h * a.s_vh
+                                : a.k + (int64_t)b * a.s_kb + (int64_t)h * a.s_kh;
+    const int64_t st = val ? a.s_vt : a.s_kt;
+    uint16_t *tail = (val ? a.p.vt : a.p.kt) + (int64_t)b * a.p.s_tb + (int64_t)h * a.p.s_th;
     if (u < whole) {
+        const int j0 = u * PG_GROUP - r;    // the new token that is the group's token 0 (below 0: a row of the tail)
+        // rows first, first + 1, ... of the group at a lane's channel ch: read(i, pointer to row first + i)
+        auto rows = [&](int first, int count, int ch, auto read) {
+            if (j0 >= 0) {      // new tokens alone: one pointer a lane, moved on by a scalar
+                const uint16_t *p = fresh + (int64_t)(j0 + first) * st + ch;
 #pragma unroll
-        for (int x = tid; x < 2 * PG_GROUP * CH; x += 256) {
-            const int kv = x / (PG_GROUP * CH), row = x / CH % PG_GROUP, c = x % CH;
-            const int j = u * PG_GROUP + row - r;    // new token, or below 0 a row of the tail
-            const uint16_t *src = kv ? (j < 0 ? vt + (int64_t)row * a.p.s_tt : vn + (int64_t)j * a.s_vt)
-                                     : (j < 0 ? kt + (int64_t)row * a.p.s_tt : kn + (int64_t)j * a.s_kt);
-            *(uint4 *)&X[kv][row * XS + 8 * c] = pg_load16(src + 8 * c);
-        }
-        __syncthreads();
+                for (int i = 0; i < count; ++i, p += st) read(i, p);
+            } else {
+#pragma unroll
+                for (int i = 0; i < count; ++i) {
+                    const int t = first + i;
+                    read(i, (j0 + t < 0 ? tail + (int64_t)t * a.p.s_tt : fresh + (int64_t)(j0 + t) * st) + ch);
+                }
+            }
+        };
         // the group's record: its last token is a new one, and a group lies in one page
-        const int64_t slot = a.slots[(int64_t)b * a.T + (u + 1) * PG_GROUP - r - 1];
+        const int64_t slot = a.slots[(int64_t)b * a.T + j0 + PG_GROUP - 1];
         const int64_t page = slot >= 0 ? slot / a.p.page_tokens : -1;
         uint8_t *rec = nullptr;
         if (page >= 0 && page < a.p.num_pages)
             rec = a.p.pool + page * a.p.s_page + (int64_t)h * a.p.s_head +
                   (slot - page * a.p.page_tokens) / PG_GROUP * (int64_t)(40 * D);
-        auto ld = [](uint16_t x) { return DT == MA_BF16 ? ma_bf16_to_f32(x) : ma_f16_to_f32(x); };
-        if (tid < D) {
-            float x[PG_GROUP], lo = INFINITY, hi = -INFINITY;
+        if (!val) {
+            const int c4 = lane % CL, sl = lane / CL, odd = c4 & 1;
+            uint2 x[TPL];
+            rows(sl * TPL, TPL, 4 * c4, [&](int i, const uint16_t *src) { x[i] = pg_load8(src); });
+            float lo[4], hi[4];
 #pragma unroll
-            for (int t = 0; t < PG_GROUP; ++t) {
-                x[t] = ld(X[0][t * XS + tid]);
-                lo = fminf(lo, x[t]);
-                hi = fmaxf(hi, x[t]);
-            }
-            const QuantGroup q = quant_params(lo, hi, DT);
+            for (int c = 0; c < 4; ++c) lo[c] = INFINITY, hi[c] = -INFINITY;
 #pragma unroll
-            for (int t = 0; t < PG_GROUP; ++t) kc[t * D + tid] = (uint8_t)quant_code(x[t], q, DT);
-            if (rec) {
-                *(_Float16 *)(rec + 32 * D + 2 * tid) = (_Float16)q.step;
-                *(_Float16 *)(rec + 34 * D + 2 * tid) = (_Float16)q.lo;
-            }
-        } else if (tid >= 128 && tid < 128 + D) {
-            const int t = tid & 31, cg = (tid - 128) >> 5;
-            float x[32], lo = INFINITY, hi = -INFINITY;
+            for (int i = 0; i < TPL; i += 2) {
+                float v[2][4];
 #pragma unroll
-            for (int c = 0; c < 32; ++c) {
-                x[c] = ld(X[1][t * XS + 32 * cg + c]);
-                lo = fminf(lo, x[c]);
-                hi = fmaxf(hi, x[c]);
-            }
-            const QuantGroup q = quant_params(lo, hi, DT);
-#pragma unroll
-            for (int c = 0; c < 32; ++c) vc[(32 * cg + c) * VS + t] = (uint8_t)quant_code(x[c], q, DT);
-            if (rec) {
-                *(_Float16 *)(rec + 36 * D + 2 * (32 * cg + t)) = (_Float16)q.step;
-                *(_Float16 *)(rec + 38 * D + 2 * (32 * cg + t)) = (_Float16)q.lo;
-            }
-        }
-        __syncthreads();
-        if (rec) {
-            if (tid < 128) {            // (mt, h, m): D / 32 words
-                const int m = tid & 15, hh = (tid >> 4) & 3, mt = tid >> 6;
-                const uint8_t *src = &kc[(8 * (m >> 2) + 4 * mt + (m & 3)) * D + (D / 4) * hh];
-                uint32_t w[D / 32];
-#pragma unroll
-                for (int cb = 0; cb < D / 32; ++cb) {
-                    const uint2 c = *(const uint2 *)(src + 8 * cb);
-                    w[cb] = pack_word(c.x, c.y);
+                for (int e = 0; e < 2; ++e) {
+                    unpack2<DT>(x[i + e].x, v[e][0], v[e][1]);
+                    unpack2<DT>(x[i + e].y, v[e][2], v[e][3]);
                 }
-                if constexpr (D == 128) *(uint4 *)(rec + 16 * tid) = uint4{w[0], w[1], w[2], w[3]};
-                else *(uint2 *)(rec + 8 * tid) = uint2{w[0], w[1]};
-            } else if (tid < 128 + D) { // (half, h, m): 4 words
-                const int x = tid - 128, m = x & 15, hh = (x >> 4) & 3, half = x >> 6;
-                uint32_t w[4];
 #pragma unroll
                 for (int c = 0; c < 4; ++c) {
-                    const uint2 s = *(const uint2 *)&vc[((D / 16) * m + 4 * half + c) * VS + 8 * hh];
-                    w[c] = pack_word(s.x, s.y);
+                    lo[c] = min3(lo[c], v[0][c], v[1][c]);
+                    hi[c] = max3(hi[c], v[0][c], v[1][c]);
                 }
-                *(uint4 *)(rec + 16 * D + 16 * x) = uint4{w[0], w[1], w[2], w[3]};
             }
+            QuantGroup q[4];
+#pragma unroll
+            for (int c = 0; c < 4; ++c) {
+                lo[c] = -ma_max_xor32(-lo[c]);
+                hi[c] = ma_max_xor32(hi[c]);
+                if constexpr (SL == 4) {
+                    lo[c] = fminf(lo[c], __shfl_xor(lo[c], 16));
+                    hi[c] = fmaxf(hi[c], __shfl_xor(hi[c], 16));
+                }
+                q[c] = group_params<DT>(lo[c], hi[c]);
+            }
+            if (!rec) goto tail_rows;
+            if (sl == 0) {
+                *(uint2 *)(rec + 32 * D + 8 * c4) = uint2{f16x2_bits(q[0].step, q[1].step), f16x2_bits(q[2].step, q[3].step)};
+                *(uint2 *)(rec + 34 * D + 8 * c4) = uint2{f16x2_bits(q[0].lo, q[1].lo), f16x2_bits(q[2].lo, q[3].lo)};
+            }
+            // a lane's bytes of a token's word: elements 0..3 (even lanes) or 4..7 of the octet
+            const int o = c4 >> 1, hh = o / (D / 32), cb = o % (D / 32);
+#pragma unroll
+            for (int i = 0; i < TPL; i += 2) {
+                uint32_t w[2];
+#pragma unroll
+                for (int e = 0; e < 2; ++e) {
+                    float v[4];
+                    unpack2<DT>(x[i + e].x, v[0], v[1]);
+                    unpack2<DT>(x[i + e].y, v[2], v[3]);
+                    codes2<DT>(v[0], v[1], q[0], q[1]);
+                    codes2<DT>(v[2], v[3], q[2], q[3]);
+                    const uint32_t lo4 = put_byte(v[1], 2 + odd, put_byte(v[0], odd, 0));
+                    const uint32_t hi4 = put_byte(v[3], 2 + odd, put_byte(v[2], odd, 0));
+                    const uint32_t mine = lo4 | hi4 << 4;
+                    w[e] = mine | ma_dpp<0xB1>(mine);      // with the other lane's, lane ^ 1
+                }
+                // even lanes store the word of token i, odd lanes that of token i + 1
+                const int t = sl * TPL + i, mt = (t >> 2) & 1, m = 4 * (t >> 3) + (t & 3) + odd;
+                *(uint32_t *)(rec + ((mt * 4 + hh) * 16 + m) * (D / 8) + 4 * cb) = odd ? w[1] : w[0];
+            }
+        } else {
+            const int m = lane & 15, hh = lane >> 4;
+            uint32_t x[8][NC / 2];
+            rows(8 * hh, 8, NC * m, [&](int i, const uint16_t *src) {
+                if constexpr (NC == 8) {
+                    const uint4 y = pg_load16(src);
+                    x[i][0] = y.x; x[i][1] = y.y; x[i][2] = y.z; x[i][3] = y.w;
+                } else {
+                    const uint2 y = pg_load8(src);
+                    x[i][0] = y.x; x[i][1] = y.y;
+                }
+            });
+            QuantGroup q[8];
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                float lo = INFINITY, hi = -INFINITY;
+#pragma unroll
+                for (int c = 0; c < NC / 2; ++c) {
+                    float v0, v1;
+                    unpack2<DT>(x[i][c], v0, v1);
+                    lo = min3(lo, v0, v1);
+                    hi = max3(hi, v0, v1);
+                }
+                lo = fminf(lo, ma_quad<0xB1>(lo));
+                hi = fmaxf(hi, ma_quad<0xB1>(hi));
+                lo = fminf(lo, ma_quad<0x4E>(lo));
+                hi = fmaxf(hi, ma_quad<0x4E>(hi));
+                if constexpr (NC == 4) {                   // 8 lanes a channel group
+                    lo = fminf(lo, ma_quad<0x141>(lo));
+                    hi = fmaxf(hi, ma_quad<0x141>(hi));
+                }
+                q[i] = group_params<DT>(lo, hi);
+            }
+            if (!rec) goto tail_rows;
+            if (m % (32 / NC) == 0) {
+                uint8_t *par = rec + 36 * D + 2 * (32 * (NC * m / 32) + 8 * hh);
+                *(uint4 *)par = uint4{f16x2_bits(q[0].step, q[1].step), f16x2_bits(q[2].step, q[3].step),
+                                      f16x2_bits(q[4].step, q[5].step), f16x2_bits(q[6].step, q[7].step)};
+                *(uint4 *)(par + 2 * D) = uint4{f16x2_bits(q[0].lo, q[1].lo), f16x2_bits(q[2].lo, q[3].lo),
+                                                f16x2_bits(q[4].lo, q[5].lo), f16x2_bits(q[6].lo, q[7].lo)};
+            }
+            uint32_t w[NC];
+#pragma unroll
+            for (int c = 0; c < NC / 2; ++c) {
+                // tokens 0 4 1 5 in the low nibbles of the bytes, 2 6 3 7 in the high ones
+                uint32_t lo0 = 0, lo1 = 0, hi0 = 0, hi1 = 0;
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                    float v0, v1;
+                    unpack2<DT>(x[i][c], v0, v1);
+                    codes2<DT>(v0, v1, q[i], q[i]);
+                    const uint32_t byte = (i >> 2) + 2 * (i & 1);
+                    if (i & 2) hi0 = put_byte(v0, byte, hi0), hi1 = put_byte(v1, byte, hi1);
+                    else lo0 = put_byte(v0, byte, lo0), lo1 = put_byte(v1, byte, lo1);
+                }
+                w[2 * c] = lo0 | hi0 << 4;
+                w[2 * c + 1] = lo1 | hi1 << 4;
+            }
+#pragma unroll
+            for (int half = 0; half < D / 64; ++half)
+                *(uint4 *)(rec + 16 * D + 1024 * half + 16 * lane) = uint4{w[4 * half], w[4 * half + 1], w[4 * half + 2],
+                                                                           w[4 * half + 3]};
         }
     }
+tail_rows:
     if (u != 0) return;
     // the tail: new tokens behind the last whole group (in front of them, where none was
-    // completed, the tail's own rows stay)
+    // completed, the tail's own rows stay); its old rows were read above, by this wave alone
     const int first = whole ? 0 : r, j0 = whole ? whole * PG_GROUP - r : 0, cnt = n - j0;
-    for (int x = tid; x < 2 * cnt * CH; x += 256) {
-        const int kv = x / (cnt * CH), row = x / CH % cnt, c = x % CH;
-        const uint16_t *src = kv ? vn + (int64_t)(j0 + row) * a.s_vt : kn + (int64_t)(j0 + row) * a.s_kt;
-        uint16_t *dst = (kv ? vt : kt) + (int64_t)(first + row) * a.p.s_tt;
-        pg_store16(dst + 8 * c, pg_load16(src + 8 * c));
+    constexpr int CH = D / 8;           // 16-byte chunks of a row
+    for (int x = lane; x < cnt * CH; x += 64) {
+        const int rw = x / CH, c = x % CH;
+        pg_store16(tail + (int64_t)(first + rw) * a.p.s_tt + 8 * c, pg_load16(fresh + (int64_t)(j0 + rw) * st + 8 * c));
     }
 }
 
@@ -543,8 +667,8 @@ extern "C" int ma_page_append(const ma_pages *p, ma_tensor4 k, ma_tensor4 v, int
     }
     AppendArgs a{pages_dev(p), (const uint16_t *)k.ptr, (const uint16_t *)v.ptr, k.s[0], k.s[1], k.s[2], v.s[0],
                  v.s[1], v.s[2], new_lens, slots, T};
-    // (31 + T) / 32 groups can become whole, one workgroup at least writes the tail
-    const dim3 grid((unsigned)units, H, B);
+    // (31 + T) / 32 groups can become whole, one at least writes the tail; two groups a workgroup
+    const dim3 grid((unsigned)((units + 1) / 2), H, B);
     hipStream_t st = (hipStream_t)stream;
     if (D == 128 && p->dtype == MA_BF16) page_append_kernel<128, MA_BF16><<<grid, 256, 0, st>>>(a);
     else if (D == 128) page_append_kernel<128, MA_F16><<<grid, 256, 0, st>>>(a);
