@@ -36,7 +36,9 @@ struct AttnArgs {
     ma_tensor4 q, kc, vc, out;
     PagesDev p;
     const int32_t *new_lens;
-    int B, H, G, T, R, RG, causal, W;
+    int B, H, G, T, R, RG, HR, causal, W;   // HR = H * RG
+    int max_len;              // tokens that a table row can name
+    int start;                // items that a segment's start is worth (see Items)
     float sl2;                // scale * log2(e)
     float *wm, *wl, *wo;      // partials of slots [2 W]: per row maximum and sum, unnormalised rows
     int4 *desc;               // [B, H, RG]: what note_segment says of every segment
@@ -44,14 +46,14 @@ struct AttnArgs {
 
 // values that every lane holds alike, as scalars
 __device__ __forceinline__ int uniform(int x) { return __builtin_amdgcn_readfirstlane(x); }
-__device__ __forceinline__ int64_t uniform(int64_t x) {
-    return (int64_t)(uint32_t)uniform((int)(uint32_t)x) | ((int64_t)uniform((int)(x >> 32)) << 32);
-}
 
+// What a request has: new tokens, stored tokens, whole groups, tail, and the items of one of its
+// segments.  The first `start` items of a segment are no work: they stand for its start and end
+// (queries, table, first loads; joining, writing), so that stretches of equal length are of
+// equal time.  A request without new tokens has none.
 struct Items {
-    int n, len, ng, rem, items;   // the request's new tokens, stored tokens, whole groups, tail, items
+    int n, len, ng, rem, items;
 };
-
 __device__ __forceinline__ Items items_from(const AttnArgs &a, int n, int len) {
     Items r;
     r.n = n;
@@ -59,11 +61,11 @@ __device__ __forceinline__ Items items_from(const AttnArgs &a, int n, int len) {
     r.ng = len / PG_GROUP;
     r.rem = len % PG_GROUP;
     const int cur = a.kc.ptr ? (n + PG_GROUP - 1) / PG_GROUP : 0;
-    r.items = n ? max(r.ng + (r.rem ? 1 : 0) + cur, 1) : 0;
+    r.items = n ? a.start + r.ng + (r.rem ? 1 : 0) + cur : 0;
     return r;
 }
 __device__ __forceinline__ Items items_of(const AttnArgs &a, int b) {
-    return items_from(a, a.new_lens ? min(max(a.new_lens[b], 0), a.T) : a.T, pg_length(a.p, b));
+    return items_from(a, a.new_lens ? min(max(a.new_lens[b], 0), a.T) : a.T, min(max(a.p.lengths[b], 0), a.max_len));
 }
 // ... of a request that the whole wave looks at
 __device__ __forceinline__ Items items_at(const AttnArgs &a, int b) {
@@ -503,27 +505,47 @@ __device__ __forceinline__ float q_as_f16(uint4 *q) {
     return up;
 }
 
-// ---- the line of items
+// ---- the line of items (the host sees to it that its length fits 31 bits)
 struct Stretch {
-    int64_t w, s, e, chunk;   // this workgroup's place and its items [s, e); items of a stretch
-    int64_t pre;              // items (x HR) of the requests before b
-    int b;                    // the request in which s lies
-    Items it;                 // ... and what it has
+    int w, s, e, chunk;   // this workgroup's place and its items [s, e); items of a stretch
+    int pre;              // items (x HR) of the requests before b
+    int b;                // the request in which s lies
+    Items it;             // ... and what it has
 };
 struct ScanShared {
-    int64_t wsum[16], pre;
-    int b, n, len;
+    int wsum[16], b, pre, n, len;
 };
-
-// Items of all requests, by a scan of the lengths in every workgroup (8 B a request, from L2);
-// the line holds HR items of each, stretches are of a multiple of `unit` items
+// this workgroup's stretch of a line of `total` items; stretches are a multiple of `unit`
+__device__ __forceinline__ void cut_line(const AttnArgs &a, Stretch &r, int total, int unit) {
+    // stretches of one XCD's workgroups lie next to one another: row groups share its L2
+    r.w = (int)(blockIdx.x % 8) * (a.W / 8) + (int)(blockIdx.x / 8);
+    const int each = (int)((unsigned)(total + a.W - 1) / (unsigned)a.W);
+    r.chunk = max((each + unit - 1) / unit, 1) * unit;
+    r.s = r.w * r.chunk;
+    r.e = min(r.s + r.chunk, total);
+}
+// Items of all requests, by a scan of the lengths in every workgroup (8 B a request, from L2): of
+// up to 64 requests in every wave, without a barrier
 template <int THREADS>
 __device__ __forceinline__ Stretch find_stretch(const AttnArgs &a, ScanShared &sh, int unit) {
     constexpr int NW = THREADS / 64;
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-    const int64_t HR = (int64_t)a.H * a.RG;
+    Stretch r;
+    if (a.B <= 64) {
+        const Items own = lane < a.B ? items_of(a, lane) : Items{};
+        const int inc = (int)ma_wave_prefix_u32((uint32_t)own.items);
+        cut_line(a, r, __builtin_amdgcn_readlane(inc, 63) * a.HR, unit);
+        const int want = (int)((unsigned)r.s / (unsigned)a.HR);
+        // (behind the line's end no lane is found, and nothing is looked at)
+        const uint64_t here = __ballot(want >= inc - own.items && want < inc);
+        const int l = here ? __ffsll((unsigned long long)here) - 1 : 0;
+        r.b = l;
+        r.pre = __builtin_amdgcn_readlane(inc - own.items, l);
+        r.it = items_from(a, __builtin_amdgcn_readlane(own.n, l), __builtin_amdgcn_readlane(own.len, l));
+        return r;
+    }
     const int per = (a.B + THREADS - 1) / THREADS, first = tid * per;
-    int64_t sum = 0;
+    int sum = 0;
     Items own{};   // of this thread's first request
     for (int i = 0; i < per; ++i)
         if (first + i < a.B) {
@@ -531,37 +553,27 @@ __device__ __forceinline__ Stretch find_stretch(const AttnArgs &a, ScanShared &s
             if (i == 0) own = it;
             sum += it.items;
         }
-    const int64_t inc = pg_wave_scan(sum, lane);
+    const int inc = (int)ma_wave_prefix_u32((uint32_t)sum);
     if (lane == 63) sh.wsum[wave] = inc;
     __syncthreads();
-    int64_t before = inc - sum, total = 0;
+    int before = inc - sum, total = 0;
 #pragma unroll
     for (int w = 0; w < NW; ++w) {
         if (w < wave) before += sh.wsum[w];
         total += sh.wsum[w];
     }
-    total = uniform(total) * HR;
-    Stretch r;
-    // stretches of one XCD's workgroups lie next to one another: row groups share its L2
-    r.w = (int64_t)(blockIdx.x % 8) * (a.W / 8) + blockIdx.x / 8;
-    const int64_t each = pg_div(total + a.W - 1, a.W);
-    r.chunk = max((each + unit - 1) / unit, (int64_t)1) * unit;
-    r.s = r.w * r.chunk;
-    r.e = min(r.s + r.chunk, total);
-    if (r.s < total) {
-        const int64_t want = pg_div(r.s, HR);
-        if (want >= before && want < before + sum) {
-            int64_t pre = before;
-            int b = first;
-            while (want >= pre + own.items) {
-                pre += own.items;
-                own = items_of(a, ++b);
-            }
-            sh.b = b;
-            sh.pre = pre;
-            sh.n = own.n;
-            sh.len = own.len;
+    cut_line(a, r, uniform(total) * a.HR, unit);
+    const int want = (int)((unsigned)r.s / (unsigned)a.HR);
+    if (want >= before && want < before + sum) {
+        int pre = before, b = first;
+        while (want >= pre + own.items) {
+            pre += own.items;
+            own = items_of(a, ++b);
         }
+        sh.b = b;
+        sh.pre = pre;
+        sh.n = own.n;
+        sh.len = own.len;
     }
     __syncthreads();
     r.b = uniform(sh.b);
@@ -572,37 +584,39 @@ __device__ __forceinline__ Stretch find_stretch(const AttnArgs &a, ScanShared &s
 
 // the part of a segment that lies in a stretch
 struct Part {
-    int h, rg, hr, i0, i1;
-    bool whole;
-    int64_t slot;     // of its partial, where it is not whole: the first or the last of the stretch
+    int h, rg, hr, i0, i1;   // its items of work [i0, i1)
+    int next;                // where the stretch goes on
+    bool first, whole;       // the segment begins here; all of it lies here
+    int slot;                // of its partial, where it is not whole: the first or the last of the stretch
 };
-__device__ __forceinline__ Part part_of(const AttnArgs &a, const Stretch &st, int64_t pos) {
-    const Items &it = st.it;
+__device__ __forceinline__ Part part_of(const AttnArgs &a, const Stretch &st, int pos) {
     Part p;
-    const int64_t rel = pos - (int64_t)a.H * a.RG * st.pre;
-    p.hr = (int)pg_div(rel, it.items);
-    p.i0 = (int)(rel - (int64_t)p.hr * it.items);
-    p.i1 = (int)min((int64_t)it.items, p.i0 + (st.e - pos));
-    p.h = p.hr / a.RG;
+    const int rel = pos - a.HR * st.pre;
+    p.hr = (int)((unsigned)rel / (unsigned)st.it.items);
+    const int i0 = rel - p.hr * st.it.items, i1 = min(st.it.items, i0 + (st.e - pos));
+    p.h = a.RG == 1 ? p.hr : (int)((unsigned)p.hr / (unsigned)a.RG);
     p.rg = p.hr - p.h * a.RG;
-    p.whole = p.i0 == 0 && p.i1 == it.items;
+    p.next = pos + i1 - i0;
+    p.first = i0 == 0;
+    p.whole = i0 == 0 && i1 == st.it.items;
+    p.i0 = max(i0 - a.start, 0);
+    p.i1 = max(i1 - a.start, 0);
     p.slot = 2 * st.w + (pos > st.s ? 1 : 0);
     return p;
 }
 // The segment's first stretch says what the merge needs of it: (first slot, stretches, first
 // workgroup), or no stretches where it is whole.
-__device__ __forceinline__ void note_segment(const AttnArgs &a, const Stretch &st, const Part &p, int64_t pos) {
-    if (p.i0 != 0 || threadIdx.x != 0) return;
-    const int n = p.whole ? 0 : (int)(pg_div(pos + st.it.items - 1, st.chunk) - st.w + 1);
-    a.desc[(int64_t)st.b * a.H * a.RG + p.hr] = int4{(int)p.slot, n, (int)st.w, 0};
+__device__ __forceinline__ void note_segment(const AttnArgs &a, const Stretch &st, const Part &p, int pos) {
+    if (!p.first || threadIdx.x != 0) return;
+    const int n = p.whole ? 0 : (int)((unsigned)(pos + st.it.items - 1) / (unsigned)st.chunk) - st.w + 1;
+    a.desc[(int64_t)st.b * a.HR + p.hr] = int4{p.slot, n, st.w, 0};
 }
-__device__ __forceinline__ void next_part(const AttnArgs &a, Stretch &st, const Part &p, int64_t &pos) {
-    pos += p.i1 - p.i0;
-    if (p.i1 == st.it.items && p.hr == a.H * a.RG - 1 && pos < st.e) {
-        st.pre += st.it.items;
-        do st.it = items_at(a, ++st.b);
-        while (st.it.items == 0);
-    }
+__device__ __forceinline__ void next_part(const AttnArgs &a, Stretch &st, const Part &p, int &pos) {
+    pos = p.next;
+    if (pos >= st.e || pos - a.HR * st.pre < a.HR * st.it.items) return;
+    st.pre += st.it.items;
+    do st.it = items_at(a, ++st.b);
+    while (st.it.items == 0);
 }
 
 // The records of a wave's next 64 packed items, one a lane: items first, first + 4, ... below
@@ -664,7 +678,7 @@ __global__ __launch_bounds__(256, NT == 1 ? 3 : 2) void paged_few_kernel(AttnArg
     __shared__ FewShared<D, NT> sh;
     const int tid = threadIdx.x, lane = tid & 63, wave = uniform(tid >> 6), n16 = lane & 15, hh = lane >> 4;
     Stretch st = find_stretch<256>(a, sh.scan, WAVES);
-    int64_t pos = st.s;
+    int pos = st.s;
     while (pos < st.e) {
         const Items it = st.it;
         const Part pt = part_of(a, st, pos);
@@ -815,7 +829,7 @@ __global__ __launch_bounds__(256, NT == 1 ? 3 : 2) void paged_few_kernel(AttnArg
                     for (int k = 0; k < NC; ++k) o[k] *= inv;
                     if (row % a.T < it.n) store_out<NC, BF16>(a, b, h, row, NC * x, o);
                 } else {
-                    const int64_t at = pt.slot * (NT * 16) + nt * 16 + r;
+                    const int64_t at = (int64_t)pt.slot * (NT * 16) + nt * 16 + r;
                     if (x == 0) {
                         a.wm[at] = m;
                         a.wl[at] = lt;
@@ -857,7 +871,7 @@ __global__ __launch_bounds__(512, 2) void paged_many_kernel(AttnArgs a) {
     const int si = wave >> 1;              // the item of a step that this wave unpacks
     const bool sv = wave & 1;              // its values (else its keys)
     Stretch st = find_stretch<512>(a, sh.scan, STEP);
-    int64_t pos = st.s;
+    int pos = st.s;
     while (pos < st.e) {
         const Items it = st.it;
         const Part pt = part_of(a, st, pos);
@@ -1075,7 +1089,7 @@ __global__ __launch_bounds__(512, 2) void paged_many_kernel(AttnArgs a) {
                         store_out<NC, BF16>(a, b, h, row, NC * (4 * hh + r), o);
                     }
                 } else {
-                    const int64_t at = pt.slot * (2 * RW * 16) + rw * 32 + nt * 16 + (row & 15);
+                    const int64_t at = (int64_t)pt.slot * (2 * RW * 16) + rw * 32 + nt * 16 + (row & 15);
                     if (hh == 0) {
                         a.wm[at] = t[nt].m;
                         a.wl[at] = l;
@@ -1103,7 +1117,7 @@ __global__ __launch_bounds__(256) void paged_merge_kernel(AttnArgs a, int rows) 
     constexpr int NC = D / 16, GR = 4, RPW = 16 / GR;
     __shared__ float sm[RPW][GR], sl[RPW][GR];
     __shared__ float so[RPW][GR][D];
-    const int b = blockIdx.x / (a.H * a.RG), hr = blockIdx.x - b * (a.H * a.RG);
+    const int b = blockIdx.x / a.HR, hr = blockIdx.x - b * a.HR;
     const int n = a.new_lens ? min(max(a.new_lens[b], 0), a.T) : a.T;
     const int4 d = a.desc[blockIdx.x];
     if ((n == 0) | (d.y == 0)) return;      // (n 0: nobody wrote its segments)
@@ -1159,8 +1173,10 @@ __global__ __launch_bounds__(256) void paged_merge_kernel(AttnArgs a, int rows) 
 
 // ------------------------------------------------------------------ host
 struct Shape {
-    int nt, rw, rows, RG, W;   // nt > 0: few rows, nt tiles; else many rows, rw waves of 2 tiles; rows of a slot
+    int nt, rw, rows, RG, W, start;   // nt > 0: few rows, nt tiles; else many rows, rw waves of 2 tiles; rows of a slot
 };
+
+constexpr int FEW_START = 16, MANY_START = 8;   // items that a segment's start is worth
 
 // Up to 32 rows go to the waves of the few-rows kernel (1 or 2 tiles each); more rows to the
 // many-rows kernel in row groups of at most 16 tiles, the groups as even as its built 4, 8 and
@@ -1173,6 +1189,7 @@ Shape shape_of(int R) {
         s.rows = tiles * 16;
         s.RG = 1;
         s.W = cus * (tiles == 1 ? 3 : 2);    // as many workgroups as are resident at once
+        s.start = FEW_START;
         return s;
     }
     const int groups = (tiles + 15) / 16, per = (tiles + groups - 1) / groups;
@@ -1180,6 +1197,7 @@ Shape shape_of(int R) {
     s.rows = s.rw * 32;
     s.RG = (R + s.rows - 1) / s.rows;
     s.W = cus;
+    s.start = MANY_START;
     return s;
 }
 
@@ -1261,6 +1279,13 @@ extern "C" int ma_paged_attention(ma_tensor4 q, int B, int Hq, int T, int D, con
         return MA_EWORKSPACE;
     }
     const Shape s = shape_of(Hq / H * T);
+    // the line: every request as long as its table row, with room for what the stretches round up
+    const int64_t most = s.start + (int64_t)p->width * p->page_tokens / PG_GROUP + 1 + (T + PG_GROUP - 1) / PG_GROUP;
+    if (most * B * H * s.RG + 64LL * s.W > INT32_MAX) {
+        ma_set_error("%s: %d requests of up to %lld tokens and %d row groups of each head are not built (2^31 items)", who,
+                     B, (long long)p->width * p->page_tokens, s.RG);
+        return MA_EUNSUPPORTED;
+    }
     const Layout l = layout_of(s, (int64_t)B * H * s.RG, D);
     char *ws = (char *)workspace;
     AttnArgs a{};
@@ -1276,6 +1301,9 @@ extern "C" int ma_paged_attention(ma_tensor4 q, int B, int Hq, int T, int D, con
     a.T = T;
     a.R = a.G * T;
     a.RG = s.RG;
+    a.HR = H * s.RG;
+    a.max_len = p->width * p->page_tokens;
+    a.start = s.start;
     a.causal = causal_block;
     a.W = s.W;
     a.sl2 = scale * MA_LOG2E;

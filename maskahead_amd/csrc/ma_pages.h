@@ -100,12 +100,6 @@ __device__ __forceinline__ int64_t pg_wave_scan(int64_t x, int lane) {
     return x;
 }
 
-// x / y of whole numbers >= 0 that the whole wave holds; in 32 bits where they fit
-__device__ __forceinline__ int64_t pg_div(int64_t x, int64_t y) {
-    if (((x | y) >> 32) == 0) return (int64_t)((uint32_t)x / (uint32_t)y);
-    return x / y;
-}
-
 // host: the checks every entry point over a store makes
 int pg_check(const ma_pages *p, int B, int H, int D, const char *who);
 
