@@ -39,6 +39,7 @@ struct AttnArgs {
     int B, H, G, T, R, RG, HR, causal, W;   // HR = H * RG
     int max_len;              // tokens that a table row can name
     int start;                // items that a segment's start is worth (see Items)
+    int dense;                // log2 of the items that one of 16-bit rows is worth
     float sl2;                // scale * log2(e)
     float *wm, *wl, *wo;      // partials of slots [2 W]: per row maximum and sum, unnormalised rows
     int4 *desc;               // [B, H, RG]: what note_segment says of every segment
@@ -61,7 +62,7 @@ __device__ __forceinline__ Items items_from(const AttnArgs &a, int n, int len) {
     r.ng = len / PG_GROUP;
     r.rem = len % PG_GROUP;
     const int cur = a.kc.ptr ? (n + PG_GROUP - 1) / PG_GROUP : 0;
-    r.items = n ? a.start + r.ng + (r.rem ? 1 : 0) + cur : 0;
+    r.items = n ? a.start + r.ng + (((r.rem ? 1 : 0) + cur) << a.dense) : 0;
     return r;
 }
 __device__ __forceinline__ Items items_of(const AttnArgs &a, int b) {
@@ -335,14 +336,16 @@ __device__ __forceinline__ uint4 rows_channel(const uint32_t (&vw)[8][D / 32], i
     }
     return uint4{x[0], x[1], x[2], x[3]};
 }
-// of row's (head group, block position) pair, the tokens of the block's item that it sees
-__device__ __forceinline__ uint32_t causal_live(const AttnArgs &a, const Items &it, const Rows &r, int row, int hh,
-                                                uint32_t live) {
-    if (r.tail || a.causal <= 0) return live;
-    const int tq = row % a.T;
-    const int64_t lim = ((int64_t)it.len + tq) / a.causal * a.causal + a.causal - it.len;    // keys j < lim
-    const int64_t over = r.j0 + 8 * hh + 8 - lim;
-    return live & (255u >> (over < 0 ? 0 : over > 8 ? 8 : (int)over));
+// how many of the block's keys its position t sees: to the end of its causal block, counted from
+// the request's first token (len + t has 32 bits, its sum with a block has not)
+__device__ __forceinline__ int keys_seen(const AttnArgs &a, const Items &it, int t) {
+    if (a.causal <= 0) return it.n;
+    const unsigned in = ((unsigned)it.len + (unsigned)t) % (unsigned)a.causal;    // its place in the block
+    return (int)min((unsigned)it.n, (unsigned)t + ((unsigned)a.causal - in));
+}
+// the tokens of an item behind the packed groups that a row sees which sees `keys` of the block's
+__device__ __forceinline__ uint32_t causal_live(const Rows &r, int keys, int hh, uint32_t live) {
+    return r.tail ? live : live & (255u >> min(max(r.j0 + 8 * hh + 8 - keys, 0), 8));
 }
 
 // a row tile's running softmax and output: lane (n = lane & 15, h = lane >> 4) holds row n,
@@ -599,8 +602,12 @@ __device__ __forceinline__ Part part_of(const AttnArgs &a, const Stretch &st, in
     p.next = pos + i1 - i0;
     p.first = i0 == 0;
     p.whole = i0 == 0 && i1 == st.it.items;
-    p.i0 = max(i0 - a.start, 0);
-    p.i1 = max(i1 - a.start, 0);
+    auto work = [&](int i) {     // items of work before place i (one of 16-bit rows lies where it begins)
+        const int u = max(i - a.start, 0), over = u - st.it.ng;
+        return over <= 0 ? u : st.it.ng + ((over + (1 << a.dense) - 1) >> a.dense);
+    };
+    p.i0 = work(i0);
+    p.i1 = work(i1);
     p.slot = 2 * st.w + (pos > st.s ? 1 : 0);
     return p;
 }
@@ -774,7 +781,7 @@ __global__ __launch_bounds__(256, NT == 1 ? 3 : 2) void paged_few_kernel(AttnArg
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt)
                 p[nt] = rows_probs<D, BF16>(t[nt], s[0][nt], s[1][nt], a.sl2,
-                                            causal_live(a, it, r, row0 + nt * 16 + (l & 15), lh, seen));
+                                            causal_live(r, keys_seen(a, it, (row0 + nt * 16 + (l & 15)) % a.T), lh, seen));
             // (the values' loads stay behind the scores' registers: ahead of them the main loop spilled)
             __builtin_amdgcn_sched_barrier(0);
             uint32_t vw[8][NC / 2];
@@ -977,57 +984,67 @@ __global__ __launch_bounds__(512, 2) void paged_many_kernel(AttnArgs a) {
             __syncthreads();
         }
 
-        // ---- the tail and the block's own keys, four items at a time
-        for (int i = max(pt.i0, it.ng); i < pt.i1; i += STEP) {
-            if (i + si < pt.i1) {
-                const Rows r = rows_of(a, it, b, h, i + si - it.ng);
-                const int l = hidden(lane);
-                uint4(*op)[64] = sh.op[0][si];
-                if (r.cnt > 0 && !sv) {
+        // ---- the tail and the block's own keys, four items a step too; what no row of the group
+        // sees is left out, what none of the wave's sees too
+        const int r1 = min((pt.rg + 1) * (2 * RW * 16), a.R) - 1, t1 = pt.rg * (2 * RW * 16) / a.T == r1 / a.T ? r1 % a.T : a.T - 1;
+        const int d0 = max(pt.i0, it.ng);
+        const int d1 = min(pt.i1, it.ng + (it.rem ? 1 : 0) + (a.kc.ptr ? (keys_seen(a, it, t1) + PG_GROUP - 1) / PG_GROUP : 0));
+        if (d0 < d1) {
+            const int l = hidden(lane), lh = l >> 4;
+            int keys[2];
+#pragma unroll
+            for (int nt = 0; nt < 2; ++nt) {
+                const int row = row0 + nt * 16 + (l & 15);
+                keys[nt] = keys_seen(a, it, row % a.T);
+                if (BF16) load_q<D>(a, b, h, row, it.n, lh, q[nt]);    // (as they are, not as f16)
+            }
+            for (int i = d0, x = 0; i < d1; i += STEP, ++x) {
+                if (i + si < d1) {
+                    const Rows r = rows_of(a, it, b, h, i + si - it.ng);
+                    uint4(*op)[64] = sh.op[x & 1][si];
+                    if (!sv) {
+                        uint4 k[2][CB];
+#pragma unroll
+                        for (int mt = 0; mt < 2; ++mt) rows_k<D>(r, l, mt, k[mt]);
+#pragma unroll
+                        for (int y = 0; y < 2 * CB; ++y) op[y][l] = k[y / CB][y % CB];
+                    } else {
+                        const uint32_t live = rows_live<MASK>(a, it, r, b, h, lh);
+                        uint32_t w[8][NC / 2];
+                        rows_v<D>(r, l, live, w);
+#pragma unroll
+                        for (int ct = 0; ct < NC; ++ct) op[2 * CB + ct][l] = rows_channel<D>(w, ct);
+                        note_live(x, live);
+                    }
+                }
+                __syncthreads();
+                const int g1 = busy ? min(d1 - i, STEP) : 0;
+                for (int g = tw; g < g1; g += TW) {
+                    const Rows r = rows_of(a, it, b, h, i + g - it.ng);
+                    const uint4(*op)[64] = sh.op[x & 1][g];
+                    const uint32_t all = (uint32_t)uniform((int)sh.live[x & 1][g]) >> (8 * lh) & 255u;
+                    const uint32_t see[2] = {causal_live(r, keys[0], lh, all), causal_live(r, keys[1], lh, all)};
+                    if (!__any(see[0] | see[1])) continue;
+                    f32x4_t s[2][2];
 #pragma unroll
                     for (int mt = 0; mt < 2; ++mt) {
                         uint4 k[CB];
-                        rows_k<D>(r, l, mt, k);
-#pragma unroll
-                        for (int cb = 0; cb < CB; ++cb) op[mt * CB + cb][lane] = k[cb];
-                    }
-                } else if (r.cnt > 0) {
-                    const uint32_t live = rows_live<MASK>(a, it, r, b, h, l >> 4);
-                    uint32_t vw[8][NC / 2];
-                    rows_v<D>(r, l, live, vw);
-#pragma unroll
-                    for (int ct = 0; ct < NC; ++ct) op[2 * CB + ct][lane] = rows_channel<D>(vw, ct);
-                    note_live(0, live);
-                }
-            }
-            __syncthreads();
-            const int g1 = busy ? min(pt.i1 - i, STEP) : 0;
-            for (int g = tw; g < g1; g += TW) {
-                const Rows r = rows_of(a, it, b, h, i + g - it.ng);
-                if (r.cnt == 0) continue;
-                const uint4(*op)[64] = sh.op[0][g];
-                const int l = hidden(lane), lh = l >> 4;
-                const uint32_t live = (uint32_t)uniform((int)sh.live[0][g]) >> (8 * lh) & 255u;
-                Probs<BF16> p[2];
-#pragma unroll
-                for (int nt = 0; nt < 2; ++nt) {
-                    const int row = row0 + nt * 16 + (l & 15);
-                    uint4 qr[CB], k[CB];
-                    load_q<D>(a, b, h, row, it.n, lh, qr);
-                    f32x4_t s[2];
-#pragma unroll
-                    for (int mt = 0; mt < 2; ++mt) {
 #pragma unroll
                         for (int cb = 0; cb < CB; ++cb) k[cb] = op[mt * CB + cb][l];
-                        s[mt] = rows_scores<CB, BF16>(k, qr);
+#pragma unroll
+                        for (int nt = 0; nt < 2; ++nt) s[nt][mt] = rows_scores<CB, BF16>(k, q[nt]);
                     }
-                    p[nt] = rows_probs<D, BF16>(t[nt], s[0], s[1], a.sl2, causal_live(a, it, r, row, lh, live));
-                }
+                    Probs<BF16> p[2];
 #pragma unroll
-                for (int ct = 0; ct < NC; ++ct) {
-                    const uint4 v = op[2 * CB + ct][l];
+                    for (int nt = 0; nt < 2; ++nt)
+                        p[nt] = rows_probs<D, BF16>(t[nt], s[nt][0], s[nt][1], a.sl2, see[nt]);
+                    __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-                    for (int nt = 0; nt < 2; ++nt) t[nt].acc[ct] = rows_values(v, p[nt], t[nt].acc[ct]);
+                    for (int ct = 0; ct < NC; ++ct) {
+                        const uint4 v = op[2 * CB + ct][l];
+#pragma unroll
+                        for (int nt = 0; nt < 2; ++nt) t[nt].acc[ct] = rows_values(v, p[nt], t[nt].acc[ct]);
+                    }
                 }
             }
             __syncthreads();
@@ -1128,19 +1145,29 @@ __global__ __launch_bounds__(256) void paged_merge_kernel(AttnArgs a, int rows) 
 #pragma unroll
     for (int k = 0; k < NC; ++k) o[k] = 0.f;
     if (row < a.R) {
-        for (int k = grp; k < d.y; k += GR) {
-            const int64_t at = (k ? 2 * (int64_t)(w + k) : (int64_t)d.x) * rows + rt;
-            const float pm = a.wm[at], pl = a.wl[at];
-            const float nm = fmaxf(m, pm);
-            const float f = __builtin_amdgcn_exp2f(m - nm), g = __builtin_amdgcn_exp2f(pm - nm);
-            m = nm;
-            l = l * f + pl * g;
+        // two partials a turn, their loads under way together (behind the last one it is loaded again)
+        for (int k0 = grp; k0 < d.y; k0 += 2 * GR) {
+            float pm[2], pl[2];
+            f32x4_t v[2][NC / 4];
 #pragma unroll
-            for (int y = 0; y < NC; y += 4) {
-                const f32x4_t v = *(const f32x4_t *)&a.wo[at * D + NC * x + y];
+            for (int z = 0; z < 2; ++z) {
+                const int k = min(k0 + z * GR, d.y - 1);
+                const int64_t at = (k ? 2 * (int64_t)(w + k) : (int64_t)d.x) * rows + rt;
+                pm[z] = a.wm[at];
+                pl[z] = a.wl[at];
 #pragma unroll
-                for (int z = 0; z < 4; ++z) o[y + z] = o[y + z] * f + v[z] * g;
+                for (int y = 0; y < NC / 4; ++y) v[z][y] = *(const f32x4_t *)&a.wo[at * D + NC * x + 4 * y];
             }
+            const bool two = k0 + GR < d.y;
+            const float nm = fmaxf(m, two ? fmaxf(pm[0], pm[1]) : pm[0]);
+            const float f = __builtin_amdgcn_exp2f(m - nm), g0 = __builtin_amdgcn_exp2f(pm[0] - nm);
+            const float g1 = two ? __builtin_amdgcn_exp2f(pm[1] - nm) : 0.f;
+            m = nm;
+            l = l * f + pl[0] * g0 + pl[1] * g1;
+            // (selected, not left out: a branch took the loads with it)
+#pragma unroll
+            for (int y = 0; y < NC; ++y)
+                o[y] = o[y] * f + v[0][y / 4][y % 4] * g0 + (two ? v[1][y / 4][y % 4] : 0.f) * g1;
         }
     }
     if (x == 0) {
@@ -1173,10 +1200,11 @@ __global__ __launch_bounds__(256) void paged_merge_kernel(AttnArgs a, int rows) 
 
 // ------------------------------------------------------------------ host
 struct Shape {
-    int nt, rw, rows, RG, W, start;   // nt > 0: few rows, nt tiles; else many rows, rw waves of 2 tiles; rows of a slot
+    int nt, rw, rows, RG, W, start, dense;   // nt > 0: few rows, nt tiles; else many rows, rw waves of 2 tiles; rows of a slot
 };
 
 constexpr int FEW_START = 16, MANY_START = 8;   // items that a segment's start is worth
+constexpr int MANY_DENSE = 1;
 
 // Up to 32 rows go to the waves of the few-rows kernel (1 or 2 tiles each); more rows to the
 // many-rows kernel in row groups of at most 16 tiles, the groups as even as its built 4, 8 and
@@ -1190,6 +1218,7 @@ Shape shape_of(int R) {
         s.RG = 1;
         s.W = cus * (tiles == 1 ? 3 : 2);    // as many workgroups as are resident at once
         s.start = FEW_START;
+        s.dense = 0;
         return s;
     }
     const int groups = (tiles + 15) / 16, per = (tiles + groups - 1) / groups;
@@ -1198,6 +1227,7 @@ Shape shape_of(int R) {
     s.RG = (R + s.rows - 1) / s.rows;
     s.W = cus;
     s.start = MANY_START;
+    s.dense = MANY_DENSE;
     return s;
 }
 
@@ -1280,7 +1310,8 @@ extern "C" int ma_paged_attention(ma_tensor4 q, int B, int Hq, int T, int D, con
     }
     const Shape s = shape_of(Hq / H * T);
     // the line: every request as long as its table row, with room for what the stretches round up
-    const int64_t most = s.start + (int64_t)p->width * p->page_tokens / PG_GROUP + 1 + (T + PG_GROUP - 1) / PG_GROUP;
+    const int64_t most = s.start + (int64_t)p->width * p->page_tokens / PG_GROUP +
+                         ((1 + (T + PG_GROUP - 1) / PG_GROUP) << s.dense);
     if (most * B * H * s.RG + 64LL * s.W > INT32_MAX) {
         ma_set_error("%s: %d requests of up to %lld tokens and %d row groups of each head are not built (2^31 items)", who,
                      B, (long long)p->width * p->page_tokens, s.RG);
@@ -1304,6 +1335,7 @@ extern "C" int ma_paged_attention(ma_tensor4 q, int B, int Hq, int T, int D, con
     a.HR = H * s.RG;
     a.max_len = p->width * p->page_tokens;
     a.start = s.start;
+    a.dense = s.dense;
     a.causal = causal_block;
     a.W = s.W;
     a.sl2 = scale * MA_LOG2E;
