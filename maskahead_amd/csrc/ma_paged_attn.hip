@@ -467,10 +467,11 @@ __device__ __forceinline__ f32x4_t rows_values(uint4 v, const Probs<false> &p, f
 
 // ---- Q of one row tile as B operands: lane (n, h) = row n, channels (D/4) h + 8 cb + (0..7);
 // rows behind the request's new tokens are zero
-template <int D>
+// (WORDS: as they lie there, where such rows are left out later)
+template <int D, bool WORDS = false>
 __device__ __forceinline__ void load_q(const AttnArgs &a, int b, int h, int row, int n, int hh, uint4 *q) {
     const int rc = min(row, a.R - 1), g = rc / a.T, t = rc - g * a.T;
-    const uint32_t ok = row < a.R && t < n ? 0xffffffffu : 0u;
+    const uint32_t ok = WORDS || (row < a.R && t < n) ? 0xffffffffu : 0u;
     const uint16_t *src = (const uint16_t *)a.q.ptr + (int64_t)b * a.q.s[0] + (int64_t)(h * a.G + g) * a.q.s[1] +
                           (int64_t)t * a.q.s[2] + (D / 4) * hh;
 #pragma unroll
@@ -860,6 +861,13 @@ __global__ __launch_bounds__(256, NT == 1 ? 3 : 2) void paged_few_kernel(AttnArg
 // lanes read them (1 KB each, no bank conflicts).
 constexpr int MWAVES = 8, STEP = 4;
 
+// place of row rt's channels (D/16) x + (0 .. 3) in a partial: as the tile's wave holds them,
+// [tile][channels mod 4][4 channels] of 64 lanes' 16 bytes
+template <int D>
+__device__ __forceinline__ int partial_at(int rt, int x) {
+    return ((rt >> 4) * (D / 16) + (x & 3) * (D / 64)) * 256 + ((x >> 2) * 16 + (rt & 15)) * 4;
+}
+
 template <int D>
 struct ManyShared {
     static constexpr int OPS = 2 * (D / 32) + D / 16;     // operands of an item: K [2][D/32], V [D/16]
@@ -995,8 +1003,9 @@ __global__ __launch_bounds__(512, 2) void paged_many_kernel(AttnArgs a) {
 #pragma unroll
             for (int nt = 0; nt < 2; ++nt) {
                 const int row = row0 + nt * 16 + (l & 15);
+                // (as they are, not as f16; a row that is none is left out when results are stored)
+                if (BF16) load_q<D, true>(a, b, h, row, it.n, lh, q[nt]);
                 keys[nt] = keys_seen(a, it, row % a.T);
-                if (BF16) load_q<D>(a, b, h, row, it.n, lh, q[nt]);    // (as they are, not as f16)
             }
             for (int i = d0, x = 0; i < d1; i += STEP, ++x) {
                 if (i + si < d1) {
@@ -1106,16 +1115,18 @@ __global__ __launch_bounds__(512, 2) void paged_many_kernel(AttnArgs a) {
                         store_out<NC, BF16>(a, b, h, row, NC * (4 * hh + r), o);
                     }
                 } else {
-                    const int64_t at = (int64_t)pt.slot * (2 * RW * 16) + rw * 32 + nt * 16 + (row & 15);
+                    const int64_t slot = (int64_t)pt.slot * (2 * RW * 16);
+                    const int rt = rw * 32 + nt * 16 + (hidden(lane) & 15);
                     if (hh == 0) {
-                        a.wm[at] = t[nt].m;
-                        a.wl[at] = l;
+                        a.wm[slot + rt] = t[nt].m;
+                        a.wl[slot + rt] = l;
                     }
+                    float *dst = a.wo + slot * D + partial_at<D>(rt, 4 * hh);
 #pragma unroll
                     for (int r = 0; r < 4; ++r)
 #pragma unroll
                         for (int ct = 0; ct < NC; ct += 4)
-                            *(f32x4_t *)&a.wo[at * D + NC * (4 * hh + r) + ct] =
+                            *(f32x4_t *)&dst[(r * (NC / 4) + ct / 4) * 256] =
                                 f32x4_t{t[nt].acc[ct][r], t[nt].acc[ct + 1][r], t[nt].acc[ct + 2][r], t[nt].acc[ct + 3][r]};
                 }
             }
@@ -1127,20 +1138,25 @@ __global__ __launch_bounds__(512, 2) void paged_many_kernel(AttnArgs a) {
 
 // ------------------------------------------------------------------ merge
 // Partials of a cut segment, joined: the first lies in desc.x, the stretch after workgroup w's
-// in slot 2 (w + 1), and so on.  16 threads a row; four groups of them take every fourth
-// partial and are joined in LDS, in a fixed order.
-template <int D, bool BF16>
+// in slot 2 (w + 1), and so on.  A workgroup joins 64 pairs of a row and D/16 channels; its four
+// waves take every fourth partial and are joined in LDS, in a fixed order.  Partials of few rows
+// lie row by row (4 rows of 16 pairs), those of many as their waves hold them (TILES: 16 rows of
+// a tile's 4 pairs, 256 contiguous bytes a load).
+template <int D, bool BF16, bool TILES>
 __global__ __launch_bounds__(256) void paged_merge_kernel(AttnArgs a, int rows) {
-    constexpr int NC = D / 16, GR = 4, RPW = 16 / GR;
-    __shared__ float sm[RPW][GR], sl[RPW][GR];
-    __shared__ float so[RPW][GR][D];
+    constexpr int NC = D / 16, GR = 4;
+    __shared__ float sm[GR][64], sl[GR][64];
+    __shared__ f32x4_t so[GR][NC / 4][64];
     const int b = blockIdx.x / a.HR, hr = blockIdx.x - b * a.HR;
     const int n = a.new_lens ? min(max(a.new_lens[b], 0), a.T) : a.T;
     const int4 d = a.desc[blockIdx.x];
     if ((n == 0) | (d.y == 0)) return;      // (n 0: nobody wrote its segments)
-    const int w = d.z, r = threadIdx.x / (16 * GR), grp = (threadIdx.x >> 4) % GR, x = threadIdx.x & 15;
-    const int h = hr / a.RG, rg = hr - h * a.RG;
-    const int rt = blockIdx.y * RPW + r, row = rg * rows + rt;
+    const int grp = threadIdx.x >> 6, u = threadIdx.x & 63;
+    const int x = TILES ? 4 * (blockIdx.y & 3) + (u >> 4) : u & 15;
+    const int rt = TILES ? 16 * (blockIdx.y >> 2) + (u & 15) : 4 * blockIdx.y + (u >> 4);
+    const int h = hr / a.RG, rg = hr - h * a.RG, row = rg * rows + rt;
+    const int off = TILES ? partial_at<D>(rt, x) : rt * D + NC * x;      // ... of its first 4 channels
+    constexpr int next = TILES ? 256 : 4;                                // from 4 channels to the next 4
     float m = NO_MAX, l = 0.f, o[NC];
 #pragma unroll
     for (int k = 0; k < NC; ++k) o[k] = 0.f;
@@ -1152,11 +1168,11 @@ __global__ __launch_bounds__(256) void paged_merge_kernel(AttnArgs a, int rows) 
 #pragma unroll
             for (int z = 0; z < 2; ++z) {
                 const int k = min(k0 + z * GR, d.y - 1);
-                const int64_t at = (k ? 2 * (int64_t)(w + k) : (int64_t)d.x) * rows + rt;
-                pm[z] = a.wm[at];
-                pl[z] = a.wl[at];
+                const int64_t at = (k ? 2 * (int64_t)(d.z + k) : (int64_t)d.x) * rows;
+                pm[z] = a.wm[at + rt];
+                pl[z] = a.wl[at + rt];
 #pragma unroll
-                for (int y = 0; y < NC / 4; ++y) v[z][y] = *(const f32x4_t *)&a.wo[at * D + NC * x + 4 * y];
+                for (int y = 0; y < NC / 4; ++y) v[z][y] = *(const f32x4_t *)&a.wo[at * D + off + next * y];
             }
             const bool two = k0 + GR < d.y;
             const float nm = fmaxf(m, two ? fmaxf(pm[0], pm[1]) : pm[0]);
@@ -1170,26 +1186,24 @@ __global__ __launch_bounds__(256) void paged_merge_kernel(AttnArgs a, int rows) 
                 o[y] = o[y] * f + v[0][y / 4][y % 4] * g0 + (two ? v[1][y / 4][y % 4] : 0.f) * g1;
         }
     }
-    if (x == 0) {
-        sm[r][grp] = m;
-        sl[r][grp] = l;
-    }
+    sm[grp][u] = m;
+    sl[grp][u] = l;
 #pragma unroll
-    for (int y = 0; y < NC; ++y) so[r][grp][NC * x + y] = o[y];
+    for (int y = 0; y < NC / 4; ++y) so[grp][y][u] = f32x4_t{o[4 * y], o[4 * y + 1], o[4 * y + 2], o[4 * y + 3]};
     __syncthreads();
     if (grp != 0) return;
-    m = sm[r][0];
+    m = sm[0][u];
 #pragma unroll
-    for (int v = 1; v < GR; ++v) m = fmaxf(m, sm[r][v]);
+    for (int v = 1; v < GR; ++v) m = fmaxf(m, sm[v][u]);
     l = 0.f;
 #pragma unroll
     for (int k = 0; k < NC; ++k) o[k] = 0.f;
 #pragma unroll
     for (int v = 0; v < GR; ++v) {
-        const float f = __builtin_amdgcn_exp2f(sm[r][v] - m);
-        l += sl[r][v] * f;
+        const float f = __builtin_amdgcn_exp2f(sm[v][u] - m);
+        l += sl[v][u] * f;
 #pragma unroll
-        for (int k = 0; k < NC; ++k) o[k] += so[r][v][NC * x + k] * f;
+        for (int k = 0; k < NC; ++k) o[k] += so[v][k / 4][u][k % 4] * f;
     }
     if (row >= a.R || row % a.T >= n) return;
     const float inv = l == 0.f ? 0.f : 1.f / l;
@@ -1276,7 +1290,9 @@ template <int D, bool BF16>
 int launch(const AttnArgs &a, const Shape &s, hipStream_t st) {
     if (int rc = a.p.mask ? launch_attn<D, BF16, true>(a, s, st) : launch_attn<D, BF16, false>(a, s, st)) return rc;
     // (a row group of few rows has fewer than its slots hold)
-    paged_merge_kernel<D, BF16><<<dim3(a.B * a.H * a.RG, (min(s.rows, a.R) + 3) / 4), 256, 0, st>>>(a, s.rows);
+    const int rows = min(s.rows, a.R);
+    if (s.nt) paged_merge_kernel<D, BF16, false><<<dim3(a.B * a.H * a.RG, (rows + 3) / 4), 256, 0, st>>>(a, s.rows);
+    else paged_merge_kernel<D, BF16, true><<<dim3(a.B * a.H * a.RG, (rows + 15) / 16 * 4), 256, 0, st>>>(a, s.rows);
     return ma_check_launch("ma_paged_attention");
 }
 
