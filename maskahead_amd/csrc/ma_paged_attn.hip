@@ -39,7 +39,7 @@ struct AttnArgs {
     int B, H, G, T, R, RG, HR, causal, W;   // HR = H * RG
     int max_len;              // tokens that a table row can name
     int start;                // items that a segment's start is worth (see Items)
-    int dense;                // log2 of the items that one of 16-bit rows is worth
+    int rows0, dense;         // items that a segment's 16-bit rows are worth: rows0, and 1 << dense each
     float sl2;                // scale * log2(e)
     float *wm, *wl, *wo;      // partials of slots [2 W]: per row maximum and sum, unnormalised rows
     int4 *desc;               // [B, H, RG]: what note_segment says of every segment
@@ -62,7 +62,8 @@ __device__ __forceinline__ Items items_from(const AttnArgs &a, int n, int len) {
     r.ng = len / PG_GROUP;
     r.rem = len % PG_GROUP;
     const int cur = a.kc.ptr ? (n + PG_GROUP - 1) / PG_GROUP : 0;
-    r.items = n ? a.start + r.ng + (((r.rem ? 1 : 0) + cur) << a.dense) : 0;
+    const int rows = (r.rem ? 1 : 0) + cur;
+    r.items = n ? a.start + r.ng + (rows ? a.rows0 + (rows << a.dense) : 0) : 0;
     return r;
 }
 __device__ __forceinline__ Items items_of(const AttnArgs &a, int b) {
@@ -604,8 +605,8 @@ __device__ __forceinline__ Part part_of(const AttnArgs &a, const Stretch &st, in
     p.first = i0 == 0;
     p.whole = i0 == 0 && i1 == st.it.items;
     auto work = [&](int i) {     // items of work before place i (one of 16-bit rows lies where it begins)
-        const int u = max(i - a.start, 0), over = u - st.it.ng;
-        return over <= 0 ? u : st.it.ng + ((over + (1 << a.dense) - 1) >> a.dense);
+        const int u = max(i - a.start, 0), over = u - st.it.ng - a.rows0;
+        return over <= 0 ? min(u, st.it.ng) : st.it.ng + ((over + (1 << a.dense) - 1) >> a.dense);
     };
     p.i0 = work(i0);
     p.i1 = work(i1);
@@ -1214,11 +1215,11 @@ __global__ __launch_bounds__(256) void paged_merge_kernel(AttnArgs a, int rows) 
 
 // ------------------------------------------------------------------ host
 struct Shape {
-    int nt, rw, rows, RG, W, start, dense;   // nt > 0: few rows, nt tiles; else many rows, rw waves of 2 tiles; rows of a slot
+    int nt, rw, rows, RG, W, start, rows0, dense;   // nt > 0: few rows, nt tiles; else many rows, rw waves of 2 tiles; rows of a slot
 };
 
 constexpr int FEW_START = 16, MANY_START = 8;   // items that a segment's start is worth
-constexpr int MANY_DENSE = 1;
+constexpr int MANY_ROWS0 = 4, MANY_DENSE = 1;
 
 // Up to 32 rows go to the waves of the few-rows kernel (1 or 2 tiles each); more rows to the
 // many-rows kernel in row groups of at most 16 tiles, the groups as even as its built 4, 8 and
@@ -1232,7 +1233,7 @@ Shape shape_of(int R) {
         s.RG = 1;
         s.W = cus * (tiles == 1 ? 3 : 2);    // as many workgroups as are resident at once
         s.start = FEW_START;
-        s.dense = 0;
+        s.rows0 = s.dense = 0;
         return s;
     }
     const int groups = (tiles + 15) / 16, per = (tiles + groups - 1) / groups;
@@ -1241,6 +1242,7 @@ Shape shape_of(int R) {
     s.RG = (R + s.rows - 1) / s.rows;
     s.W = cus;
     s.start = MANY_START;
+    s.rows0 = MANY_ROWS0;
     s.dense = MANY_DENSE;
     return s;
 }
@@ -1326,7 +1328,7 @@ extern "C" int ma_paged_attention(ma_tensor4 q, int B, int Hq, int T, int D, con
     }
     const Shape s = shape_of(Hq / H * T);
     // the line: every request as long as its table row, with room for what the stretches round up
-    const int64_t most = s.start + (int64_t)p->width * p->page_tokens / PG_GROUP +
+    const int64_t most = s.start + s.rows0 + (int64_t)p->width * p->page_tokens / PG_GROUP +
                          ((1 + (T + PG_GROUP - 1) / PG_GROUP) << s.dense);
     if (most * B * H * s.RG + 64LL * s.W > INT32_MAX) {
         ma_set_error("%s: %d requests of up to %lld tokens and %d row groups of each head are not built (2^31 items)", who,
@@ -1351,6 +1353,7 @@ extern "C" int ma_paged_attention(ma_tensor4 q, int B, int Hq, int T, int D, con
     a.HR = H * s.RG;
     a.max_len = p->width * p->page_tokens;
     a.start = s.start;
+    a.rows0 = s.rows0;
     a.dense = s.dense;
     a.causal = causal_block;
     a.W = s.W;
