@@ -2,13 +2,16 @@
 // tail | the block's own keys], for ragged requests whose lengths lie on the device.
 //
 // The work is a line of items: a group of 32 packed tokens, the tail, or 32 keys of the
-// block, of one segment = (request, KV head, row group of up to 16 NT query rows).  Every
-// workgroup takes an equal stretch of the line, whatever segments it crosses, so ragged
-// lengths need no plan and no read-back: it finds its first request by a scan of the lengths.
-// Its four waves take the stretch's items of a segment in turn, each with its own running
-// maximum, sum and output (registers only, no barrier), and join them in LDS at the segment's
-// end.  A segment that lies in one stretch is written out; one cut between workgroups leaves
-// partials, which page_merge_kernel joins.
+// block, of one segment = (request, KV head, row group); a row is one of the R = (Hq / H) T
+// pairs of a query head of the KV head and a position.  Every workgroup takes an equal stretch
+// of the line, whatever segments it crosses, so ragged lengths need no plan and no read-back:
+// it finds its first request by a scan of the lengths.  A segment that lies in one stretch is
+// written out; one cut between workgroups leaves f32 partials (row maximum, sum, unnormalised
+// output), which paged_merge_kernel joins in a fixed order: the same call gives the same bits.
+//
+// Two kernels walk the line.  Up to 32 rows (single tokens, short blocks) are bound by the
+// cache's bytes: there every wave unpacks records into its own registers.  More rows are bound
+// by the matrix cores: there a record is unpacked once, into LDS, for up to 256 rows.
 //
 // Per item and wave: S^T = K Q^T and O^T += V^T P^T with v_mfma_f32_16x16x32, K and V as A
 // operands.  A lane of S^T holds 8 tokens of one query row, which is the B operand that P^T
@@ -671,8 +674,17 @@ __device__ __forceinline__ void store_out(const AttnArgs &a, int b, int h, int r
 }
 
 // ------------------------------------------------------------------ few rows
-// NT row tiles of 16; the four waves of a workgroup take a segment's items in turn and are
-// joined in LDS at its end.
+// NT row tiles of 16; the four waves of a workgroup take a segment's items in turn, each with
+// its own running maximum, sum and output (registers only, no barrier), and are joined in LDS at
+// the segment's end.  A wave's next record is asked for as soon as the registers of this one are
+// free: keys behind the scores, values behind the second product.
+//
+// bound: 40 D bytes a group and head, once.  One token of 64 requests of 700 to 16 384 tokens
+// (28 query and 4 KV heads, D 128): 206 MB in 52.5 us with the merge, 3.9 TB/s, where a large copy
+// reaches 5.1; 2 requests of 90 000 to 131 072 tokens (32 and 8 heads): 67.5 us, 4.6 TB/s.  Some
+// 10 us are no traffic: two launches, the scan, the first record's three loads in a row (length,
+// table, words), the join and the merge (one token after prompts of up to 700 tokens: 13.9 us in
+// all).  Two records under way a wave were no faster (D 128: 55.2 and 69.0 us).
 template <int D, int NT>
 struct FewShared {
     static constexpr int OS = D + 4;                 // row stride of a wave's output rows, f32
@@ -860,6 +872,16 @@ __global__ __launch_bounds__(256, NT == 1 ? 3 : 2) void paged_few_kernel(AttnArg
 // rows: wave w unpacks the keys (w even) or values (w odd) of item w / 2 of the next step into
 // the other buffer while it computes, one barrier a step.  An item's 16 operands lie as the
 // lanes read them (1 KB each, no bank conflicts).
+//
+// bound: the matrix cores, 4 D operations a row and token.  512 new tokens of 2 requests of 6 000
+// to 16 384 tokens (28 query and 4 KV heads, D 128): 205 GFLOP in 217 to 223 us; each 8 192 tokens
+// more add 104 us, 1.15 PFLOP/s, where a large library product reaches 1.19.  The rest is start
+// and end: partials of 256 rows (128 KB) written and read again, and 16-bit rows, which are not
+// pipelined (a step of up to four items is 5 us).  32 new tokens of 8 requests: 51 us, of which
+// some 25 are that.  Measured and not kept (chunk, then 251 us): two tiles half an item apart, so
+// that one's exponentials lie under the other's products: 268; 4 tiles a wave and one wave a
+// SIMD: 368 (operands copied between the two register files); the next 16-bit rows under way in
+// registers: 20 % slower, the main loop spilled.
 constexpr int MWAVES = 8, STEP = 4;
 
 // place of row rt's channels (D/16) x + (0 .. 3) in a partial: as the tile's wave holds them,
@@ -1215,15 +1237,27 @@ __global__ __launch_bounds__(256) void paged_merge_kernel(AttnArgs a, int rows) 
 
 // ------------------------------------------------------------------ host
 struct Shape {
-    int nt, rw, rows, RG, W, start, rows0, dense;   // nt > 0: few rows, nt tiles; else many rows, rw waves of 2 tiles; rows of a slot
+    int nt, rw;               // nt > 0: few rows, nt tiles; else many rows, rw waves of 2 tiles
+    int rows, RG, W;          // rows of a slot, row groups, workgroups
+    int start, rows0, dense;  // what items are worth (AttnArgs)
 };
 
-constexpr int FEW_START = 16, MANY_START = 8;   // items that a segment's start is worth
+// Items that a segment's start is worth.  Few rows, one token of 64 ragged requests / of 2 long
+// ones: 8 items 54.9 / 68.9 us, 16 52.5 / 67.6, 24 53.1 / 68.1.  Many: 4, 8, 12 and 16 are
+// within 2 % of one another, none (1) is 9 % slower (32 tokens of 8 requests).
+constexpr int FEW_START = 16, MANY_START = 8;
+// ... and its 16-bit rows of the many-rows kernel: 4 and 2 each.  32 tokens of 8 requests 54.9 us
+// (0 and 2 each: 57.6, 8 and 2: 54.5), of 32 requests 143 (150, 147); 512 tokens of 2 requests, 16
+// such items a segment: 2 each 224, 1 each 231, 4 each 234.
 constexpr int MANY_ROWS0 = 4, MANY_DENSE = 1;
 
-// Up to 32 rows go to the waves of the few-rows kernel (1 or 2 tiles each); more rows to the
-// many-rows kernel in row groups of at most 16 tiles, the groups as even as its built 4, 8 and
-// 16 tiles allow.
+// Up to 32 rows go to the waves of the few-rows kernel (1 or 2 tiles each): 28 rows of 64
+// requests 70 us there, 114 in the other; of 16 requests 33 and 42.  More rows go to the many-rows
+// kernel in row groups of at most 16 tiles (of at most 8: 32 tokens of 8 requests 54 -> 63 us,
+// 512 of 2 requests 220 -> 268), the groups as even as its built 4, 8 and 16 tiles allow.
+// Workgroups: two a CU for few rows (three: 54.0 and 71.4 us where two have 52.5 and 67.6; more
+// than are resident at once: 62 and 78), one for many (their LDS; two in turn: 54 -> 67 and
+// 220 -> 233 us).
 Shape shape_of(int R) {
     const int tiles = (R + 15) / 16, cus = ma_num_cus() / 8 * 8;
     Shape s{};
@@ -1231,7 +1265,7 @@ Shape shape_of(int R) {
         s.nt = tiles;
         s.rows = tiles * 16;
         s.RG = 1;
-        s.W = cus * (tiles == 1 ? 3 : 2);    // as many workgroups as are resident at once
+        s.W = cus * 2;
         s.start = FEW_START;
         s.rows0 = s.dense = 0;
         return s;
