@@ -643,6 +643,17 @@ extern "C" int ma_page_plan(const int32_t *lengths, const int32_t *new_lens, int
         ma_set_error("%s: more than 2^31 - 1 tokens of a request, 2^29 pages or 2^42 slots are not built", who);
         return MA_EUNSUPPORTED;
     }
+    // every workgroup reads all lengths, and one writes its requests' ends and table rows
+    const uintptr_t e = (uintptr_t)ends, span = (uintptr_t)B * sizeof(int32_t);
+    for (const uintptr_t x : {(uintptr_t)lengths, (uintptr_t)new_lens})
+        if (e < x + span && x < e + span) {
+            ma_set_error("%s: ends overlaps lengths or new_lens", who);
+            return MA_EINVAL;
+        }
+    if (B > 1 && s_table < width) {
+        ma_set_error("%s: the requests' table rows overlap (stride %lld, width %d)", who, (long long)s_table, width);
+        return MA_EINVAL;
+    }
     PlanArgs a{lengths, new_lens, table, ring, state, ends, slots, s_table, nflat, B, T, page_tokens, width, num_pages};
     page_plan_kernel<<<dim3((unsigned)wgs), PLAN_THREADS, 0, (hipStream_t)stream>>>(a);
     return ma_check_launch(who);

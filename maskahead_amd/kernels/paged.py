@@ -46,6 +46,14 @@ def _check_table(t: torch.Tensor, b: int) -> None:
         raise ValueError(f"block_table must be an int32 [{b}, width] tensor with contiguous rows")
 
 
+def _c_int(name: str, value: int) -> int:
+    """A size that the C entry points take as 32 bits."""
+    value = int(value)
+    if not 0 <= value < 1 << 31:
+        raise ValueError(f"{name} must lie in 0 .. 2^31 - 1, got {value}")
+    return value
+
+
 def _same_device(index: int, **tensors) -> None:
     for name, t in tensors.items():
         if t is not None and t.get_device() != index:
@@ -101,6 +109,8 @@ class PagedPrefix:
         if mask is not None and (mask.ndim != 3 or mask.dtype != torch.uint8 or tuple(mask.shape[:2]) != (b, hkv) or
                                  (mask.shape[2] > 1 and mask.stride(2) != 1)):
             raise ValueError(f"mask must be a uint8 [{b}, {hkv}, tokens] tensor with contiguous tokens")
+        if mask is not None:
+            _c_int("mask's tokens", mask.shape[2])
         N.require_gpu(pool, "pool")
         index = pool.get_device()
         _i32(lengths, "lengths", (b,), index)
@@ -134,7 +144,8 @@ def plan_pages(lengths: torch.Tensor, new_lens: torch.Tensor, block_table: torch
     max(0, lengths[b] + new_lens[b]) tokens.  Returns (slots int64 [B, tokens], ends int32
     [B]): slot = page id * page_tokens + offset of each new token, -1 behind new_lens[b].
 
-    block_table [B, width] gets the pages that appear and -1 for those that go.  free_ring
+    block_table [B, width] gets the pages that appear and -1 for those that go (its rows must
+    not overlap, nor ends lengths or new_lens).  free_ring
     int32 [pages] holds the free pages' ids first in, first out; ring_state int32 [4] =
     (place of the oldest, free pages, 0, status).  Growing requests take the oldest pages, in
     request order; pages given back (new_lens[b] < 0: that many tokens, at most all) enter
@@ -154,9 +165,7 @@ def plan_pages(lengths: torch.Tensor, new_lens: torch.Tensor, block_table: torch
     _check_table(block_table, b)
     _i32(free_ring, "free_ring", (free_ring.numel(),), index)
     _i32(ring_state, "ring_state", (4,), index)
-    tokens = int(tokens)
-    if tokens < 0:
-        raise ValueError("tokens must not be negative")
+    tokens, page_tokens = _c_int("tokens", tokens), _c_int("page_tokens", page_tokens)
     if slots is None:
         slots = torch.empty((b, tokens), device=lengths.device, dtype=torch.int64)
     elif slots.dtype is not torch.int64 or slots.shape != (b, tokens) or not slots.is_contiguous():
@@ -169,7 +178,7 @@ def plan_pages(lengths: torch.Tensor, new_lens: torch.Tensor, block_table: torch
         _same_device(index, block_table=block_table, slots=slots)
     if b == 0:
         return slots, ends
-    _call(index, "ma_page_plan", lengths.data_ptr(), new_lens.data_ptr(), b, tokens, int(page_tokens),
+    _call(index, "ma_page_plan", lengths.data_ptr(), new_lens.data_ptr(), b, tokens, page_tokens,
           block_table.data_ptr(), block_table.stride(0), block_table.shape[1], free_ring.data_ptr(), free_ring.numel(),
           ring_state.data_ptr(), slots.data_ptr() if tokens else None, ends.data_ptr())
     return slots, ends
@@ -229,9 +238,7 @@ def dequantize_pages(prefix: PagedPrefix, tokens: int, *, starts: torch.Tensor |
                      out_value: torch.Tensor | None = None):
     """Tokens starts[b] .. starts[b] + tokens of every request (starts None: from 0) as K and V
     [B, Hkv, tokens, D] in dtype (default: the tails'), zero from the request's length on."""
-    tokens = int(tokens)
-    if tokens < 0:
-        raise ValueError("tokens must not be negative")
+    tokens = _c_int("tokens", tokens)
     shape = (prefix.batch, prefix.heads, tokens, prefix.head_dim)
     dtype = dtype or (out_key.dtype if out_key is not None else prefix.dtype)
     if out_key is None:
@@ -276,8 +283,7 @@ def paged_attention(query: torch.Tensor, prefix: PagedPrefix, current_key: torch
             raise ValueError(f"the block's keys and values must hold {t} positions like its queries")
     if new_lens is not None:
         _i32(new_lens, "new_lens", (b,), prefix.index)
-    if causal_block < 0:
-        raise ValueError("causal_block must not be negative")
+    causal_block = _c_int("causal_block", causal_block)
     if out is None:
         out = torch.empty(shape, device=query.device, dtype=query.dtype)
     elif _check_block("out", out, prefix, hq) != shape:
@@ -290,7 +296,7 @@ def paged_attention(query: torch.Tensor, prefix: PagedPrefix, current_key: torch
         raise N.KernelUnavailableError(f"{hq // h * t} rows for each of {b * h} KV heads are not built")
     ws = torch.empty((need,), device=query.device, dtype=torch.uint8)
     _call(prefix.index, "ma_paged_attention", N.t4(query), b, hq, t, d, prefix._nat, h, N.t4(current_key),
-          N.t4(current_value), N.ptr(new_lens), int(causal_block), scale, N.t4(out), ws.data_ptr(), need)
+          N.t4(current_value), N.ptr(new_lens), causal_block, scale, N.t4(out), ws.data_ptr(), need)
     return out
 
 

@@ -65,10 +65,13 @@ class PagedKVCache:
         self.prefixes = [self.prefix(i) for i in range(num_layers)]
         self._plan: tuple | None = None     # (new_lens, slots, ends, staged layers) of an append in progress
 
-    def prefix(self, layer: int, *, mask: torch.Tensor | None = None) -> PagedPrefix:
-        """The kernels' descriptor of one layer, with an optional mask of dead entries."""
+    def _check_layer(self, layer: int) -> None:
         if not 0 <= layer < self.num_layers:
             raise IndexError(layer)
+
+    def prefix(self, layer: int, *, mask: torch.Tensor | None = None) -> PagedPrefix:
+        """The kernels' descriptor of one layer, with an optional mask of dead entries."""
+        self._check_layer(layer)
         return PagedPrefix(self.pool[layer], self.k_tail[layer], self.v_tail[layer], self.block_table, self.lengths,
                            mask=mask)
 
@@ -80,7 +83,8 @@ class PagedKVCache:
     def begin_append(self, new_lens: torch.Tensor, tokens: int) -> torch.Tensor:
         """Open an append of new_lens[b] (0 .. tokens) tokens to every layer and give their pages
         to the requests.  Returns the slots [B, tokens] (``plan_pages``).  A plan that cannot be
-        met stores nothing and leaves every length as it is; ``check`` reports it."""
+        met stores nothing and leaves every length as it is; ``check`` reports it.  new_lens is
+        read until the commit: it must not change before."""
         if self._plan is not None:
             raise RuntimeError("another cache append is already in progress")
         if tokens <= 0:
@@ -98,8 +102,7 @@ class PagedKVCache:
         new_lens, slots, _, staged = self._plan
         if layer in staged:
             raise RuntimeError(f"layer {layer} was staged twice")
-        if not 0 <= layer < self.num_layers:
-            raise IndexError(layer)
+        self._check_layer(layer)
         append_pages(self.prefixes[layer], key, value, new_lens, slots)
         staged.add(layer)
 
@@ -148,6 +151,7 @@ class PagedKVCache:
         the append in progress."""
         if new_lens is None and self._plan is not None:
             new_lens = self._plan[0]
+        self._check_layer(layer)
         prefix = self.prefixes[layer] if mask is None else self.prefix(layer, mask=mask)
         return paged_attention(query, prefix, current_key, current_value, new_lens=new_lens, scaling=scaling,
                                causal_block=causal_block, out=out)
@@ -155,6 +159,7 @@ class PagedKVCache:
     def dequantize_layer(self, layer: int, tokens: int, *, starts: torch.Tensor | None = None,
                          dtype: torch.dtype | None = None):
         """``dequantize_pages`` of one layer: [B, Hkv, tokens, D] K and V."""
+        self._check_layer(layer)
         return dequantize_pages(self.prefixes[layer], tokens, starts=starts, dtype=dtype)
 
 

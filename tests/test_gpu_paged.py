@@ -539,3 +539,105 @@ def test_refusals_on_the_gpu(gpu):
             call()
             raise AssertionError(f"call {i} was not refused")
     torch.cuda.synchronize()
+
+
+# ------------------------------------------------------------------ what a server does besides
+@pytest.mark.parametrize("b,t,hq", [(65, 1, 1), (300, 1, 2), (600, 3, 1), (70, 40, 1), (600, 34, 1)])
+def test_attention_of_many_requests(gpu, b, t, hq):
+    """More requests than lanes of a wave and than threads of a workgroup, part of them idle or
+    empty, of few rows and of many."""
+    rng = random.Random(b + t)
+    lens = [rng.choice((0, 1, 20, 32, 33, 70)) for _ in range(b)]
+    _attend(gpu, lens=lens, new=[rng.choice((0, t, t, max(1, t // 2))) for _ in lens], t=t, hq=hq, h=1, d=64, dtype=BF,
+            page=32)
+
+
+@pytest.mark.parametrize("b,t,hq,d,dtype", [(4, 1, 8, 64, BF), (4, 1, 16, 128, F16), (2, 8, 40, 128, BF), (2, 8, 40, 64, F16)])
+def test_attention_over_a_table_of_repeated_pages(gpu, b, t, hq, d, dtype):
+    """160 000 tokens of every request, the same 8 pages over and over, shared by all of them: a
+    stretch of the line is longer than what a wave looks up at once.  A softmax over tokens that
+    are repeated equally often is that over one of each; the longest chain of f32 additions is 32
+    products of an instruction, some 80 items of a wave, its workgroup's 4 waves and fewer than 70
+    partials, which the bound's 256 additions cover."""
+    h, page = 8, 32
+    r = Requests(gpu, [256], h=h, d=d, dtype=dtype, page=page)
+    row = r.cache.block_table[0, :8].repeat(625)
+    wide = torch.zeros((b, h, 32, d), dtype=dtype, device=gpu)
+    p = PagedPrefix(r.cache.pool[0], wide, wide, row[None].expand(b, -1), r.i32([5000 * 32] * b))
+    q = torch.randn((b, hq, t, d), generator=r.gen).to(dtype)
+    got = paged_attention(q.to(gpu), p)
+    none = torch.empty((h, 0, d))
+    for i in range(b):
+        want, bound = attend64(q[i], *r.kv64(0), none, none, seen=torch.ones((h, 256), dtype=torch.bool))
+        check_attention(got[i], want, bound, dtype)
+    assert torch.equal(paged_attention(q.to(gpu), p), got)      # (no atomics: the same bits)
+
+
+@pytest.mark.parametrize("t,hq", [(1, 4), (40, 2)])
+@pytest.mark.parametrize("tokens", [1, 5, 8, 33, 90])
+def test_a_mask_shorter_than_the_requests(gpu, tokens, t, hq):
+    """Positions past a mask's end are dead."""
+    r = Requests(gpu, [20, 100, 77], h=2, page=32)
+    q = torch.randn((3, hq, t, 128), generator=r.gen).to(BF)
+    k, v = r.block([t] * 3, t)
+    mask = (torch.rand((3, 2, tokens), generator=r.gen) >= 0.3).to(torch.uint8)
+    got = r.cache.attend(0, q.to(gpu), k.to(gpu), v.to(gpu), mask=mask.to(gpu))
+    for b, n in enumerate(r.lens):
+        seen = torch.zeros((2, n), dtype=torch.bool)
+        m = min(n, tokens)
+        seen[:, :m] = mask[b, :, :m].bool()
+        want, bound = attend64(q[b], *r.kv64(b), k[b], v[b], seen=seen)
+        check_attention(got[b], want, bound, BF)
+
+
+@pytest.mark.parametrize("causal", [1, 32, 250, 1000])
+@pytest.mark.parametrize("t,hq", [(600, 1), (300, 2)])
+def test_attention_causal_over_several_row_groups(gpu, causal, t, hq):
+    """Row groups that end inside a head's positions or cross from one head into the next: what no
+    row of a group sees is left out."""
+    _attend(gpu, lens=[0, 45, 1000], new=[t, t - 77, t], t=t, hq=hq, h=1, d=128, dtype=BF, causal=causal)
+
+
+def test_a_block_is_captured_and_replayed(gpu):
+    """A captured call of many rows over growing requests, replayed with eager work between."""
+    r = Requests(gpu, [50, 3, 200], h=2, d=128, room=300)
+    c, t = r.cache, 40
+    q = torch.randn((3, 4, t, 128), generator=r.gen).to(BF).to(gpu)
+    k, v = (x.to(gpu) for x in r.block([t] * 3, t))
+    out = torch.zeros_like(q)
+    graph = torch.cuda.CUDAGraph()
+    torch.cuda.synchronize()
+    with torch.cuda.graph(graph):
+        c.attend(0, q, k, v, causal_block=32, out=out)
+    for i in range(6):
+        graph.replay()
+        want = c.attend(0, q, k, v, causal_block=32)
+        torch.cuda.synchronize()
+        assert torch.equal(out, want), i
+        r.append([30, i, 9 * i], 60)
+        q.mul_(-0.75)
+
+
+def test_read_back_far_behind_the_end_is_zero(gpu):
+    r = Requests(gpu, [40, 70], d=64, page=32)
+    k, v = r.cache.dequantize_layer(0, 50, starts=r.i32([(1 << 31) - 1, 69]))
+    assert (k[0] == 0).all() and (v[0] == 0).all() and (k[1, :, 1:] == 0).all()
+    assert torch.equal(k[1, :, 0].cpu(), r.k[1][:, 69]) and torch.equal(v[1, :, 0].cpu(), r.v[1][:, 69])
+
+
+def test_sizes_past_32_bits_and_overlapping_arguments_are_refused(gpu):
+    c = PagedKVCache(num_layers=1, batch_size=2, num_kv_heads=1, head_dim=64, num_pages=6, max_tokens=128, page_tokens=32,
+                     device=gpu)
+    q = torch.zeros((2, 2, 1, 64), dtype=BF, device=gpu)
+    new = torch.ones(2, dtype=torch.int32, device=gpu)
+    plan = lambda **kw: plan_pages(c.lengths, new, kw.pop("table", c.block_table), c.free_ring, c.ring_state,  # noqa: E731
+                                   **{**dict(page_tokens=32, tokens=1), **kw})
+    for call in (lambda: c.attend(0, q, causal_block=1 << 32), lambda: plan(page_tokens=(1 << 32) + 32),
+                 lambda: plan(tokens=(1 << 32) + 1), lambda: c.dequantize_layer(0, 1 << 32), lambda: plan(ends=c.lengths),
+                 lambda: plan(ends=new), lambda: plan(table=c.block_table[:1].expand(2, -1))):
+        with pytest.raises(ValueError):
+            call()
+    for call in (lambda: c.attend(1, q), lambda: c.attend(-1, q), lambda: c.dequantize_layer(-1, 1)):
+        with pytest.raises(IndexError):
+            call()
+    assert c.ring_state.tolist() == [0, 6, 0, 0] and c.lengths.tolist() == [0, 0]

@@ -111,3 +111,22 @@ def test_cpu_tensors_and_unbuilt_shapes_are_refused():
                         (dict(num_pages=0), ValueError)):
         with pytest.raises(error):
             PagedKVCache(**{**kw, **more})
+
+
+def test_overlapping_plan_arguments_are_refused(lib):
+    """What one workgroup writes while another reads it: ends over lengths or new_lens, two
+    requests' table rows in one place."""
+    ok = dict(lengths=4096, new=8192, s=4, ends=16384)
+    call = lambda a: lib.ma_page_plan(a["lengths"], a["new"], 2, 1, 64, 4096, a["s"], 4, 4096, 8, 4096, 4096,  # noqa: E731
+                                      a["ends"], None)
+    for kw in (dict(ends=4096), dict(ends=4100), dict(ends=4092), dict(ends=8192), dict(ends=8196), dict(s=0), dict(s=3)):
+        assert call({**ok, **kw}) == N.MA_EINVAL, kw
+
+
+def test_a_line_past_31_bits_is_refused(lib):
+    """64 requests of up to 2^30 tokens and 2 heads are 2^32 groups of tokens."""
+    p = ctypes.byref(_pages(width=1 << 24))
+    assert lib.ma_paged_attention(_t4(), 64, 4, 1, 128, p, 2, _t4(), _t4(), None, 0, 1.0, _t4(), 4096, 1 << 40,
+                                  None) == N.MA_EUNSUPPORTED
+    # rows that no launch holds
+    assert lib.ma_paged_workspace_bytes(1, 1, 1 << 16, 1 << 16, 128) == -1
