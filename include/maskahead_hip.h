@@ -371,7 +371,8 @@ typedef struct ma_pages {
 
 /* Page plan of one step: request b goes from lengths[b] to ends[b] = max(0, lengths[b] +
  * new_lens[b]) tokens (new_lens negative: gives tokens back, all of them with any value of
- * at most -lengths[b]).  ring [num_pages] i32 holds the free pages' ids, first in first out;
+ * at most -lengths[b]; for a step given up before its append, or a request that ends: a packed
+ * group's tokens do not become 16-bit rows of the tail again).  ring [num_pages] i32 holds the free pages' ids, first in first out;
  * state [4] i32 = (place of the oldest, free pages, 0, status).  Growing requests take pages
  * in request order, oldest first; then the pages given back enter the ring, in request and
  * page order, free from the next plan on.  table entries that appear are written, those that
@@ -380,7 +381,8 @@ typedef struct ma_pages {
  * A plan that cannot be met changes nothing (slots -1, ends = lengths) and adds to status:
  * 1 the ring runs out, 2 a request outgrows its table row, 4 new_lens[b] > T, 8 a negative
  * length.  status is never cleared here.  One launch; plans of one ring are ordered by the
- * caller (one stream). */
+ * caller (one stream).  MA_EINVAL: ends overlaps lengths or new_lens, table rows overlap;
+ * MA_EUNSUPPORTED: 2^31 tokens of a request, 2^29 pages. */
 int ma_page_plan(const int32_t *lengths, const int32_t *new_lens, int B, int T, int page_tokens, int32_t *table,
                  int64_t s_table, int width, int32_t *ring, int num_pages, int32_t *state, int64_t *slots,
                  int32_t *ends, void *stream);
@@ -388,7 +390,8 @@ int ma_page_plan(const int32_t *lengths, const int32_t *new_lens, int B, int T, 
  * tokens: every group of 32 that [tail | new] completes is quantized with ma_quantize_keys'
  * and ma_quantize_values' arithmetic into the record that slots (ma_page_plan's) names, and
  * the rest becomes the tail.  Requests without new tokens, and those whose slots are -1, are
- * left as they are.  k, v share p->dtype.  One launch. */
+ * left as they are.  k, v share p->dtype.  One launch.  MA_EUNSUPPORTED (here and below): B
+ * or H > 65535. */
 int ma_page_append(const ma_pages *p, ma_tensor4 k, ma_tensor4 v, int B, int H, int T, int D,
                    const int32_t *new_lens, const int64_t *slots, void *stream);
 /* Tokens starts[b] .. starts[b] + n of every request (starts NULL: from 0) as k_out, v_out
@@ -402,8 +405,10 @@ int ma_page_dequant(const ma_pages *p, int B, int H, int D, const int32_t *start
  * positions: rows t >= new_lens[b] of out stay as they are, keys j >= new_lens[b] are not
  * seen.  causal_block > 0: key j is seen by query t only if (lengths[b] + j) / causal_block <=
  * (lengths[b] + t) / causal_block.  A row that sees nothing is zero.  q, kc, vc, out share
- * p->dtype.  workspace: ma_paged_workspace_bytes() bytes, 256-byte aligned; its contents are
- * not read before they are written. */
+ * p->dtype; D 64 or 128.  workspace: ma_paged_workspace_bytes() bytes, 256-byte aligned; its
+ * contents are not read before they are written, and calls that may run at once need one each.
+ * The same call gives the same bits (no atomics).  Two launches.  MA_EUNSUPPORTED: B * H * row
+ * groups of requests as long as their table rows are 2^31 groups of 32 tokens or more. */
 int64_t ma_paged_workspace_bytes(int B, int H, int Hq, int T, int D);
 int ma_paged_attention(ma_tensor4 q, int B, int Hq, int T, int D, const ma_pages *p, int H, ma_tensor4 kc,
                        ma_tensor4 vc, const int32_t *new_lens, int causal_block, float scale, ma_tensor4 out,

@@ -16,11 +16,13 @@
 // Per item and wave: S^T = K Q^T and O^T += V^T P^T with v_mfma_f32_16x16x32, K and V as A
 // operands.  A lane of S^T holds 8 tokens of one query row, which is the B operand that P^T
 // needs: nothing moves between lanes.  Codes become f16 in place (mask into the mantissa of
-// 1024 or 64, subtract, one fused multiply-add by scale and zero: one rounding of 2^-12
-// relative, where a bf16 copy of the cache has 2^-9); scores, maxima, sums and outputs are
-// f32; probabilities are rounded to f16 (2^-12) for the second product, their sum is not.
+// 1024 or 64, subtract, one fused multiply-add by scale and zero: one rounding of 2^-11
+// relative, where a bf16 copy of the cache has 2^-8); scores, maxima, sums and outputs are
+// f32; probabilities are rounded to f16 (2^-11) for the second product, and their sum is that
+// of what is multiplied.  Together 3.5e-4 of a result in the 2-norm, beside f16's own 2.1e-4
+// (bf16's 1.6e-3): what the matrix cores' full rate costs.
 // The tail and the block's keys are read as they are: f16 like the above, bf16 in bf16
-// products with the probability as a sum of two bf16 (2^-17).
+// products with the probability as a sum of two bf16 (2^-16).
 #include "ma_pages.h"
 
 using namespace ma;
@@ -874,14 +876,14 @@ __global__ __launch_bounds__(256, NT == 1 ? 3 : 2) void paged_few_kernel(AttnArg
 // lanes read them (1 KB each, no bank conflicts).
 //
 // bound: the matrix cores, 4 D operations a row and token.  512 new tokens of 2 requests of 6 000
-// to 16 384 tokens (28 query and 4 KV heads, D 128): 205 GFLOP in 217 to 223 us; each 8 192 tokens
+// to 16 384 tokens (28 query and 4 KV heads, D 128): 205 GFLOP in 217 to 233 us; each 8 192 tokens
 // more add 104 us, 1.15 PFLOP/s, where a large library product reaches 1.19.  The rest is start
 // and end: partials of 256 rows (128 KB) written and read again, and 16-bit rows, which are not
 // pipelined (a step of up to four items is 5 us).  32 new tokens of 8 requests: 51 us, of which
 // some 25 are that.  Measured and not kept (chunk, then 251 us): two tiles half an item apart, so
 // that one's exponentials lie under the other's products: 268; 4 tiles a wave and one wave a
 // SIMD: 368 (operands copied between the two register files); the next 16-bit rows under way in
-// registers: 20 % slower, the main loop spilled.
+// registers: 20 % slower, the main loop spilled; a SIMD's two waves unpacking in turn: no gain.
 constexpr int MWAVES = 8, STEP = 4;
 
 // place of row rt's channels (D/16) x + (0 .. 3) in a partial: as the tile's wave holds them,

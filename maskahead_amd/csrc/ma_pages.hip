@@ -17,6 +17,10 @@ namespace {
 // request, from L2 after the first) and writes the slots of its own PLAN_SLOTS (request,
 // token) pairs.  The ring's state is written by the workgroup that arrives last, when every
 // other has read it.
+//
+// bound: latency (lengths, page ids, writes: three loads in a row behind a scan).  64 requests of
+// one token 6 us, 256 of 2 048 tokens (4 MB of slots) 11, of which the arrivals of 256 workgroups
+// at one counter are 2.6; a second launch instead of the counter would cost more.
 constexpr int PLAN_THREADS = 256;
 constexpr int PLAN_SLOTS = 2048;
 constexpr int PLAN_SCAN = 4 * PLAN_THREADS;   // requests per scan step
@@ -196,7 +200,9 @@ __global__ __launch_bounds__(PLAN_THREADS) void page_plan_kernel(PlanArgs a) {
 // bound: 4 D bytes read and 1.25 D written a token and head.  A quotient rounded to a bf16 code
 // needs no division: with 8-bit significands a / step is never nearer than 2^-17 (relative) to
 // where bf16 rounds the other way, and a * rcp(step) is within 2^-22 of it; a / 15 likewise
-// (2^-13).  f16 quotients come as near as 2^-23 and are divided.
+// (2^-13).  f16 quotients come as near as 2^-23 and are divided.  8 ragged prompts of up to 8 192
+// tokens (8 heads, D 128): 266 MB in 55 to 69 us, 3.9 to 4.8 TB/s (53 without any arithmetic);
+// one token of 64 requests 4.3 us.
 struct AppendArgs {
     PagesDev p;
     const uint16_t *k, *v;
@@ -447,6 +453,9 @@ tail_rows:
 // One wave = one group of 32 tokens of one (request, KV head), K by code words of 8 channels
 // (a lane keeps one octet of channels, so its parameters, for every token), V by lanes of
 // D / 16 channels x 8 tokens; every store instruction writes whole rows.
+//
+// bound: 1.25 D bytes read and 4 D (f32: 8 D) written a token and head.  2 requests' 65 536 tokens
+// (8 heads, D 128, bf16): 697 MB in 143 us, 4.9 TB/s, a large copy's 5.1.
 struct DequantArgs {
     PagesDev p;
     const int32_t *starts;

@@ -149,7 +149,9 @@ def plan_pages(lengths: torch.Tensor, new_lens: torch.Tensor, block_table: torch
     int32 [pages] holds the free pages' ids first in, first out; ring_state int32 [4] =
     (place of the oldest, free pages, 0, status).  Growing requests take the oldest pages, in
     request order; pages given back (new_lens[b] < 0: that many tokens, at most all) enter
-    behind the newest and are free from the next plan on.  lengths is not written.
+    behind the newest and are free from the next plan on: for a step given up before its
+    append, or a request that ends (tokens of a packed group do not return to the tail).
+    lengths is not written.
 
     A plan that cannot be met changes nothing, returns slots of -1 and ends = lengths, and
     adds to the status, which stays until the caller clears it: 1 the pages run out, 2 a
@@ -268,7 +270,7 @@ def paged_attention(query: torch.Tensor, prefix: PagedPrefix, current_key: torch
     [B] (None: T each) counts each request's real positions: rows t >= new_lens[b] of out are
     left as they are, keys j >= new_lens[b] not seen.  causal_block > 0: key j is seen by query
     t only if (lengths[b] + j) // causal_block <= (lengths[b] + t) // causal_block.  A row that
-    sees nothing is zero.  ``out`` [B, Hq, T, D] (not overlapping the inputs) receives the
+    sees nothing is zero.  The same call gives the same bits.  ``out`` [B, Hq, T, D] (not overlapping the inputs) receives the
     result; without it a new tensor does, whose rows t >= new_lens[b] are undefined."""
     shape = _check_block("query", query, prefix)
     b, hq, t, d = shape
