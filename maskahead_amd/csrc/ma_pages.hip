@@ -179,7 +179,7 @@ __global__ __launch_bounds__(PLAN_THREADS) void page_plan_kernel(PlanArgs a) {
         }
     }
     __syncthreads();   // the workgroup's reads of the state are done
-    if (tid == 0 && atomicAdd(&a.state[2], 1) == (int)gridDim.x - 1) {
+    if (tid == 0 && (gridDim.x == 1 || atomicAdd(&a.state[2], 1) == (int)gridDim.x - 1)) {
         if (!bad) {
             a.state[0] = (int)((head + gsum) % a.num_pages);
             a.state[1] = (int)(count - gsum + bsum);
