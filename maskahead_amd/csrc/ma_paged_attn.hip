@@ -682,10 +682,10 @@ __device__ __forceinline__ void store_out(const AttnArgs &a, int b, int h, int r
 // free: keys behind the scores, values behind the second product.
 //
 // bound: 40 D bytes a group and head, once.  One token of 64 requests of 700 to 16 384 tokens
-// (28 query and 4 KV heads, D 128): 206 MB in 52.5 us with the merge, 3.9 TB/s, where a large copy
-// reaches 5.1; 2 requests of 90 000 to 131 072 tokens (32 and 8 heads): 67.5 us, 4.6 TB/s.  Some
+// (28 query and 4 KV heads, D 128): 208 MB in 52.7 us with the merge, 4.0 TB/s, where a large copy
+// reaches 5.1; 2 requests of 90 000 to 131 072 tokens (32 and 8 heads): 66.1 us, 4.7 TB/s.  Some
 // 10 us are no traffic: two launches, the scan, the first record's three loads in a row (length,
-// table, words), the join and the merge (one token after prompts of up to 700 tokens: 13.9 us in
+// table, words), the join and the merge (one token after prompts of up to 700 tokens: 13.8 us in
 // all).  Two records under way a wave were no faster (D 128: 55.2 and 69.0 us).
 template <int D, int NT>
 struct FewShared {
@@ -1163,13 +1163,20 @@ __global__ __launch_bounds__(512, 2) void paged_many_kernel(AttnArgs a) {
 
 // ------------------------------------------------------------------ merge
 // Partials of a cut segment, joined: the first lies in desc.x, the stretch after workgroup w's
-// in slot 2 (w + 1), and so on.  A workgroup joins 64 pairs of a row and D/16 channels; its four
-// waves take every fourth partial and are joined in LDS, in a fixed order.  Partials of few rows
-// lie row by row (4 rows of 16 pairs), those of many as their waves hold them (TILES: 16 rows of
-// a tile's 4 pairs, 256 contiguous bytes a load).
+// in slot 2 (w + 1), and so on.  A workgroup joins 64 pairs of a row and D/16 channels; each of its
+// waves takes every eighth (many rows: fourth) partial, and they are joined in LDS, in a fixed
+// order.  Partials of few rows lie row by row (4 rows of 16 pairs), those of many as their waves
+// hold them (TILES: 16 rows of a tile's 4 pairs, 256 contiguous bytes a load).
+//
+// bound: latency (desc, then partials), many rows: their bytes (8 requests' 224 rows of 4 heads, 33
+// MB in 8.9 us).  Waves of few rows: one token of 2 long requests, some 30 partials a segment, 66.1
+// us with 8, 67.3 with 4, 66.1 with 16; of 64 requests 52.8, 52.3, 53.7.  Of many: 32 tokens of 8
+// requests 50.9 us with 4, 51.2 with 2, 51.9 with 8.
+constexpr int merge_waves(bool tiles) { return tiles ? 4 : 8; }
+
 template <int D, bool BF16, bool TILES>
-__global__ __launch_bounds__(256) void paged_merge_kernel(AttnArgs a, int rows) {
-    constexpr int NC = D / 16, GR = 4;
+__global__ __launch_bounds__(64 * merge_waves(TILES)) void paged_merge_kernel(AttnArgs a, int rows) {
+    constexpr int NC = D / 16, GR = merge_waves(TILES);
     __shared__ float sm[GR][64], sl[GR][64];
     __shared__ f32x4_t so[GR][NC / 4][64];
     const int b = blockIdx.x / a.HR, hr = blockIdx.x - b * a.HR;
@@ -1329,8 +1336,8 @@ int launch(const AttnArgs &a, const Shape &s, hipStream_t st) {
     if (int rc = a.p.mask ? launch_attn<D, BF16, true>(a, s, st) : launch_attn<D, BF16, false>(a, s, st)) return rc;
     // (a row group of few rows has fewer than its slots hold)
     const int rows = min(s.rows, a.R);
-    if (s.nt) paged_merge_kernel<D, BF16, false><<<dim3(a.B * a.H * a.RG, (rows + 3) / 4), 256, 0, st>>>(a, s.rows);
-    else paged_merge_kernel<D, BF16, true><<<dim3(a.B * a.H * a.RG, (rows + 15) / 16 * 4), 256, 0, st>>>(a, s.rows);
+    if (s.nt) paged_merge_kernel<D, BF16, false><<<dim3(a.B * a.H * a.RG, (rows + 3) / 4), 64 * merge_waves(false), 0, st>>>(a, s.rows);
+    else paged_merge_kernel<D, BF16, true><<<dim3(a.B * a.H * a.RG, (rows + 15) / 16 * 4), 64 * merge_waves(true), 0, st>>>(a, s.rows);
     return ma_check_launch("ma_paged_attention");
 }
 
