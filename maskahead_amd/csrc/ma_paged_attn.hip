@@ -43,7 +43,6 @@ struct AttnArgs {
     const int32_t *new_lens;
     int B, H, G, T, R, RG, HR, causal, W;   // HR = H * RG
     int max_len;              // tokens that a table row can name
-    int start;                // items that a segment's start is worth (see Items)
     int rows0, dense;         // items that a segment's 16-bit rows are worth: rows0, and 1 << dense each
     float sl2;                // scale * log2(e)
     float *wm, *wl, *wo;      // partials of slots [2 W]: per row maximum and sum, unnormalised rows
@@ -54,9 +53,14 @@ struct AttnArgs {
 __device__ __forceinline__ int uniform(int x) { return __builtin_amdgcn_readfirstlane(x); }
 
 // What a request has: new tokens, stored tokens, whole groups, tail, and the items of one of its
-// segments.  The first `start` items of a segment are no work: they stand for its start and end
+// segments.  The first START items of a segment are no work: they stand for its start and end
 // (queries, table, first loads; joining, writing), so that stretches of equal length are of
-// equal time.  A request without new tokens has none.
+// equal time; rows0 in front of its 16-bit rows stand for those rows' first loads.  A request
+// without new tokens has none.
+//
+// START 1, 8, 12, 16, 20: one token of 64 ragged requests 58, 52.4, 52.8, 52.4, 54.1 us, of 2 long
+// ones 66.8 to 67.3; of many rows 9 % slower with 1, 4 to 16 within 2 % of one another.
+constexpr int START = 8;
 struct Items {
     int n, len, ng, rem, items;
 };
@@ -68,7 +72,7 @@ __device__ __forceinline__ Items items_from(const AttnArgs &a, int n, int len) {
     r.rem = len % PG_GROUP;
     const int cur = a.kc.ptr ? (n + PG_GROUP - 1) / PG_GROUP : 0;
     const int rows = (r.rem ? 1 : 0) + cur;
-    r.items = n ? a.start + r.ng + (rows ? a.rows0 + (rows << a.dense) : 0) : 0;
+    r.items = n ? START + r.ng + (rows ? a.rows0 + (rows << a.dense) : 0) : 0;
     return r;
 }
 __device__ __forceinline__ Items items_of(const AttnArgs &a, int b) {
@@ -610,7 +614,7 @@ __device__ __forceinline__ Part part_of(const AttnArgs &a, const Stretch &st, in
     p.first = i0 == 0;
     p.whole = i0 == 0 && i1 == st.it.items;
     auto work = [&](int i) {     // items of work before place i (one of 16-bit rows lies where it begins)
-        const int u = max(i - a.start, 0), over = u - st.it.ng - a.rows0;
+        const int u = max(i - START, 0), over = u - st.it.ng - a.rows0;
         return over <= 0 ? min(u, st.it.ng) : st.it.ng + ((over + (1 << a.dense) - 1) >> a.dense);
     };
     p.i0 = work(i0);
@@ -682,8 +686,8 @@ __device__ __forceinline__ void store_out(const AttnArgs &a, int b, int h, int r
 // free: keys behind the scores, values behind the second product.
 //
 // bound: 40 D bytes a group and head, once.  One token of 64 requests of 700 to 16 384 tokens
-// (28 query and 4 KV heads, D 128): 208 MB in 52.7 us with the merge, 4.0 TB/s, where a large copy
-// reaches 5.1; 2 requests of 90 000 to 131 072 tokens (32 and 8 heads): 66.1 us, 4.7 TB/s.  Some
+// (28 query and 4 KV heads, D 128): 208 MB in 52.4 us with the merge, 4.0 TB/s, where a large copy
+// reaches 5.1; 2 requests of 90 000 to 131 072 tokens (32 and 8 heads): 66.8 us, 4.7 TB/s.  Some
 // 10 us are no traffic: two launches, the scan, the first record's three loads in a row (length,
 // table, words), the join and the merge (one token after prompts of up to 700 tokens: 13.8 us in
 // all).  Two records under way a wave were no faster (D 128: 55.2 and 69.0 us).
@@ -1248,17 +1252,15 @@ __global__ __launch_bounds__(64 * merge_waves(TILES)) void paged_merge_kernel(At
 struct Shape {
     int nt, rw;               // nt > 0: few rows, nt tiles; else many rows, rw waves of 2 tiles
     int rows, RG, W;          // rows of a slot, row groups, workgroups
-    int start, rows0, dense;  // what items are worth (AttnArgs)
+    int rows0, dense;         // what 16-bit rows are worth (AttnArgs)
 };
 
-// Items that a segment's start is worth.  Few rows, one token of 64 ragged requests / of 2 long
-// ones: 8 items 54.9 / 68.9 us, 16 52.5 / 67.6, 24 53.1 / 68.1.  Many: 4, 8, 12 and 16 are
-// within 2 % of one another, none (1) is 9 % slower (32 tokens of 8 requests).
-constexpr int FEW_START = 16, MANY_START = 8;
-// ... and its 16-bit rows of the many-rows kernel: 4 and 2 each.  32 tokens of 8 requests 54.9 us
-// (0 and 2 each: 57.6, 8 and 2: 54.5), of 32 requests 143 (150, 147); 512 tokens of 2 requests, 16
+// Items that a segment's 16-bit rows are worth, beside 1 << dense each.  Few rows (1 each): one token
+// of 64 ragged requests 53.2 us with 0 or 4, 52.5 with 8, 54.0 with 12; 8 tokens of 6 requests 19.1, 18.1,
+// 18.2, 18.0; of 2 long requests 66.7, 67.2, 67.2, 67.3.  Many (2 each): 32 tokens of 8 requests 57.6 us
+// with 0, 54.9 with 4, 54.5 with 8, of 32 requests 150, 143, 147; 512 tokens of 2 requests, 16
 // such items a segment: 2 each 224, 1 each 231, 4 each 234.
-constexpr int MANY_ROWS0 = 4, MANY_DENSE = 1;
+constexpr int FEW_ROWS0 = 8, MANY_ROWS0 = 4, MANY_DENSE = 1;
 
 // Up to 32 rows go to the waves of the few-rows kernel (1 or 2 tiles each): 28 rows of 64
 // requests 70 us there, 114 in the other; of 16 requests 33 and 42.  More rows go to the many-rows
@@ -1275,8 +1277,8 @@ Shape shape_of(int R) {
         s.rows = tiles * 16;
         s.RG = 1;
         s.W = cus * 2;
-        s.start = FEW_START;
-        s.rows0 = s.dense = 0;
+        s.rows0 = FEW_ROWS0;
+        s.dense = 0;
         return s;
     }
     const int groups = (tiles + 15) / 16, per = (tiles + groups - 1) / groups;
@@ -1284,7 +1286,6 @@ Shape shape_of(int R) {
     s.rows = s.rw * 32;
     s.RG = (R + s.rows - 1) / s.rows;
     s.W = cus;
-    s.start = MANY_START;
     s.rows0 = MANY_ROWS0;
     s.dense = MANY_DENSE;
     return s;
@@ -1371,7 +1372,7 @@ extern "C" int ma_paged_attention(ma_tensor4 q, int B, int Hq, int T, int D, con
     }
     const Shape s = shape_of(Hq / H * T);
     // the line: every request as long as its table row, with room for what the stretches round up
-    const int64_t most = s.start + s.rows0 + (int64_t)p->width * p->page_tokens / PG_GROUP +
+    const int64_t most = START + s.rows0 + (int64_t)p->width * p->page_tokens / PG_GROUP +
                          ((1 + (T + PG_GROUP - 1) / PG_GROUP) << s.dense);
     if (most * B * H * s.RG + 64LL * s.W > INT32_MAX) {
         ma_set_error("%s: %d requests of up to %lld tokens and %d row groups of each head are not built (2^31 items)", who,
@@ -1395,7 +1396,6 @@ extern "C" int ma_paged_attention(ma_tensor4 q, int B, int Hq, int T, int D, con
     a.RG = s.RG;
     a.HR = H * s.RG;
     a.max_len = p->width * p->page_tokens;
-    a.start = s.start;
     a.rows0 = s.rows0;
     a.dense = s.dense;
     a.causal = causal_block;
