@@ -245,6 +245,8 @@ def dequantize_pages(prefix: PagedPrefix, tokens: int, *, starts: torch.Tensor |
     dtype = dtype or (out_key.dtype if out_key is not None else prefix.dtype)
     if out_key is None:
         out_key = torch.empty(shape, device=prefix.device, dtype=dtype)
+        if out_value is None:
+            out_value = torch.empty_like(out_key)     # (a third cheaper than by its shape)
     if out_value is None:
         out_value = torch.empty(shape, device=prefix.device, dtype=dtype)
     for name, t in (("out_key", out_key), ("out_value", out_value)):
