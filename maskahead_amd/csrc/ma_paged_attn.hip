@@ -1263,7 +1263,8 @@ struct Shape {
 constexpr int FEW_ROWS0 = 8, MANY_ROWS0 = 4, MANY_DENSE = 1;
 
 // Up to 32 rows go to the waves of the few-rows kernel (1 or 2 tiles each): 28 rows of 64
-// requests 70 us there, 114 in the other; of 16 requests 33 and 42.  More rows go to the many-rows
+// requests 70 us there, 114 in the other; of 16 requests 32 and 43; D 64, 32 rows of 48 requests
+// 33 and 49, of 6 requests 18 and 19.  More rows go to the many-rows
 // kernel in row groups of at most 16 tiles (of at most 8: 32 tokens of 8 requests 54 -> 63 us,
 // 512 of 2 requests 220 -> 268), the groups as even as its built 4, 8 and 16 tiles allow.
 // Workgroups: two a CU for few rows (three: 54.0 and 71.4 us where two have 52.5 and 67.6; more

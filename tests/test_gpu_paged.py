@@ -641,3 +641,26 @@ def test_sizes_past_32_bits_and_overlapping_arguments_are_refused(gpu):
         with pytest.raises(IndexError):
             call()
     assert c.ring_state.tolist() == [0, 6, 0, 0] and c.lengths.tolist() == [0, 0]
+
+
+@pytest.mark.parametrize("t,hq", [(1, 4), (20, 8)])
+def test_broadcast_queries_masks_and_tables(gpu, t, hq):
+    """One tensor for all heads or requests (strides of 0) is read as its copies are, and requests
+    that share their pages agree."""
+    r = Requests(gpu, [150], h=2, page=32)
+    c = r.cache
+    rows = lambda x: x.expand(3, *x.shape[1:])  # noqa: E731
+    lens = r.i32([150, 150, 150])
+    q = torch.randn((1, hq, t, 128), generator=r.gen).to(BF).to(gpu)
+    mask = (torch.rand((1, 1, 150), generator=r.gen) >= 0.4).to(torch.uint8).to(gpu)
+    k, v = (x.to(gpu) for x in r.block([t], t))
+    p = PagedPrefix(c.pool[0], rows(c.k_tail[0]), rows(c.v_tail[0]), c.block_table.expand(3, -1), lens,
+                    mask=mask.expand(3, 2, -1))
+    got = paged_attention(rows(q), p, rows(k), rows(v))
+    copies = PagedPrefix(c.pool[0], rows(c.k_tail[0]).contiguous(), rows(c.v_tail[0]).contiguous(),
+                         c.block_table.expand(3, -1).contiguous(), lens, mask=mask.expand(3, 2, -1).contiguous())
+    assert torch.equal(paged_attention(rows(q).contiguous(), copies, rows(k).contiguous(), rows(v).contiguous()), got)
+    seen = mask[0].expand(2, -1).bool().cpu()
+    want, bound = attend64(q[0].cpu(), *r.kv64(0), k[0].cpu(), v[0].cpu(), seen=seen)
+    for b in range(3):
+        check_attention(got[b], want, bound, BF)
