@@ -353,7 +353,8 @@ int ma_rebuild_packed(const ma_prefix *old_store, int B, int H, int D, const ma_
  *   k_tail, v_tail  [B, H, 32, D] in dtype (bf16 or f16), sharing the strides s_tail (b, h, t)
  *   table   [B, width] i32, row stride s_table;  lengths [B] i32
  *   mask    [B, H, mask_tokens] u8 (strides s_mask; 0 = dead, as are positions past
- *           mask_tokens) for ma_paged_attention, or NULL */
+ *           mask_tokens) for ma_paged_attention, or NULL: no mask.  With mask_tokens 0 every
+ *           stored token is dead; mask is then any address but NULL, and not read */
 typedef struct ma_pages {
     void *pool;
     void *k_tail;

@@ -128,7 +128,9 @@ class PagedPrefix:
         p.s_table = block_table.stride(0)
         p.num_pages, p.width, p.page_tokens = pages, block_table.shape[1], per * GROUP
         if mask is not None:
-            p.mask, p.mask_tokens = mask.data_ptr(), mask.shape[2]
+            # (an empty tensor's address is 0, which is no mask: any other stands for one whose positions
+            # are all behind its end, and is not read)
+            p.mask, p.mask_tokens = mask.data_ptr() or lengths.data_ptr(), mask.shape[2]
             p.s_mask[0], p.s_mask[1] = mask.stride(0), mask.stride(1)
         p.dtype = N.dtype_code(k_tail.dtype)
         self._nat = p

@@ -1,0 +1,27 @@
+"""The paged 4-bit cache where its rules are easily missed: masks without a position."""
+
+import pytest
+import torch
+
+from _paged import Requests, attend64, check_attention
+
+pytestmark = pytest.mark.gpu
+
+BF = torch.bfloat16
+
+
+# ------------------------------------------------------------------ masks
+@pytest.mark.parametrize("t,hq", [(1, 4), (40, 2)])
+@pytest.mark.parametrize("sliced", [False, True])
+def test_a_mask_without_positions_leaves_the_block_alone(gpu, t, hq, sliced):
+    """Positions past a mask's end are dead: of a mask of no tokens (an empty tensor or an empty
+    slice of one) every stored token is, the block's own keys are not."""
+    r = Requests(gpu, [20, 100, 0], h=2, page=32)
+    q = torch.randn((3, hq, t, 128), generator=r.gen).to(BF)
+    k, v = r.block([t] * 3, t)
+    mask = torch.ones((3, 2, 8 if sliced else 0), dtype=torch.uint8, device=gpu)[:, :, :0]
+    got = r.cache.attend(0, q.to(gpu), k.to(gpu), v.to(gpu), mask=mask)
+    for b, n in enumerate(r.lens):
+        want, bound = attend64(q[b], *r.kv64(b), k[b], v[b], seen=torch.zeros((2, n), dtype=torch.bool))
+        check_attention(got[b], want, bound, BF)
+    assert (r.cache.attend(0, q.to(gpu), mask=mask, out=torch.full_like(got, 9.0)) == 0).all()
