@@ -75,6 +75,12 @@ class PagedKVCache:
         return PagedPrefix(self.pool[layer], self.k_tail[layer], self.v_tail[layer], self.block_table, self.lengths,
                            mask=mask)
 
+    def _check_readable(self, layer: int) -> None:
+        """A staged layer's tail holds the new tokens while lengths are still the old ones."""
+        self._check_layer(layer)
+        if self._plan is not None and layer in self._plan[3]:
+            raise RuntimeError(f"layer {layer} was staged: it can be read again after commit_append")
+
     @property
     def append_in_progress(self) -> bool:
         return self._plan is not None
@@ -96,7 +102,7 @@ class PagedKVCache:
 
     def stage_layer(self, layer: int, key: torch.Tensor, value: torch.Tensor) -> None:
         """Write one layer's new tokens, key and value [B, Hkv, T, D] (rows behind a request's
-        new_lens are not read)."""
+        new_lens are not read).  The layer is not read again before the commit."""
         if self._plan is None:
             raise RuntimeError("begin_append must be called before stage_layer")
         new_lens, slots, _, staged = self._plan
@@ -148,18 +154,19 @@ class PagedKVCache:
                scaling: float | None = None, causal_block: int = 0, mask: torch.Tensor | None = None,
                out: torch.Tensor | None = None) -> torch.Tensor:
         """``paged_attention`` of one layer over [stored | block]; new_lens defaults to that of
-        the append in progress."""
+        the append in progress.  RuntimeError between a layer's stage_layer and the commit."""
         if new_lens is None and self._plan is not None:
             new_lens = self._plan[0]
-        self._check_layer(layer)
+        self._check_readable(layer)
         prefix = self.prefixes[layer] if mask is None else self.prefix(layer, mask=mask)
         return paged_attention(query, prefix, current_key, current_value, new_lens=new_lens, scaling=scaling,
                                causal_block=causal_block, out=out)
 
     def dequantize_layer(self, layer: int, tokens: int, *, starts: torch.Tensor | None = None,
                          dtype: torch.dtype | None = None):
-        """``dequantize_pages`` of one layer: [B, Hkv, tokens, D] K and V."""
-        self._check_layer(layer)
+        """``dequantize_pages`` of one layer: [B, Hkv, tokens, D] K and V.  RuntimeError between a
+        layer's stage_layer and the commit."""
+        self._check_readable(layer)
         return dequantize_pages(self.prefixes[layer], tokens, starts=starts, dtype=dtype)
 
 
