@@ -18,8 +18,8 @@
 // needs: nothing moves between lanes.  Codes become f16 in place (mask into the mantissa of
 // 1024 or 64, subtract, one fused multiply-add by scale and zero: one rounding of 2^-11
 // relative, where a bf16 copy of the cache has 2^-8); scores, maxima, sums and outputs are
-// f32; probabilities are rounded to f16 (2^-11) for the second product, and their sum is that
-// of what is multiplied.  Together 3.5e-4 of a result in the 2-norm, beside f16's own 2.1e-4
+// f32; weights are rounded to f16 (2^-11; their range: P_MAX below) for the second product, and
+// their sum is that of what is multiplied.  Together 3.5e-4 of a result in the 2-norm, beside f16's own 2.1e-4
 // (bf16's 1.6e-3): what the matrix cores' full rate costs.
 // The tail and the block's keys are read as they are: f16 like the above, bf16 in bf16
 // products with the probability as a sum of two bf16 (2^-16).
@@ -32,9 +32,19 @@ namespace {
 typedef __attribute__((ext_vector_type(8))) __bf16 b16x8_t;
 
 constexpr int WAVES = 4;
-// a row's reference maximum is raised only when a score exceeds it by 2^8: most items leave
-// the accumulators alone, and p <= 2^8 keeps f16's full precision
-constexpr float LAZY = 8.0f;
+// Weights are 2^(score - reference) and become f16, which holds 11 bits from 2^-14 to 2^16 and
+// nothing below 2^-25.  A row's reference therefore follows its items: where the largest weight of
+// an item's 32 tokens (of a lane's 8, as it is looked at) would lie above 2^P_MAX or below 2^P_MIN,
+// the reference is moved to where it is 2^P_NEW (those found below 2^P_LOW then, so that the next
+// items lie well inside); most items leave the accumulators alone.  A weight then carries at most
+// 2^-25 absolute, 2^-17 of the largest of its item, beside f16's 2^-11 relative, however far another
+// item's score is above: with the row's maximum as the only reference, a key that leads by 17 nats and
+// has no value of its own left the others no digits.  Beside such a key, in its own item, what
+// is below 2^-32 of it is lost.  The reference goes down only while the sum stays below P_SUM, which
+// leaves the accumulators 2^67 of room.  The cost of the lower border: one token of 64 requests
+// 52.0 -> 52.4 us, 32 tokens of 8 requests 50.9 -> 52.2, 512 tokens of 2 requests 219.1 -> 219.4.
+constexpr float P_MAX = 15.0f, P_MIN = -8.0f, P_LOW = 0.0f, P_NEW = 7.0f;
+constexpr float P_SUM = 0x1p60f;
 constexpr float NO_MAX = -1e30f;
 
 struct AttnArgs {
@@ -45,7 +55,7 @@ struct AttnArgs {
     int max_len;              // tokens that a table row can name
     int rows0, dense;         // items that a segment's 16-bit rows are worth: rows0, and 1 << dense each
     float sl2;                // scale * log2(e)
-    float *wm, *wl, *wo;      // partials of slots [2 W]: per row maximum and sum, unnormalised rows
+    float *wm, *wl, *wo;      // partials of slots [2 W]: per row reference and sum, unnormalised rows
     int4 *desc;               // [B, H, RG]: what note_segment says of every segment
 };
 
@@ -359,8 +369,8 @@ __device__ __forceinline__ uint32_t causal_live(const Rows &r, int keys, int hh,
 }
 
 // a row tile's running softmax and output: lane (n = lane & 15, h = lane >> 4) holds row n,
-// channels (D/16)(4 h + r) + ct in acc[ct][r]; the row's reference maximum m and, in every
-// component of l, its sum of probabilities (a product with ones: the sum of what is multiplied)
+// channels (D/16)(4 h + r) + ct in acc[ct][r]; the row's reference m and, in every
+// component of l, its sum of weights (a product with ones: the sum of what is multiplied)
 template <int D>
 struct Tile {
     f32x4_t acc[D / 16], l;
@@ -384,8 +394,8 @@ __device__ __forceinline__ float max8(const float (&x)[8]) {
     return max3(max3(x[0], x[1], x[2]), max3(x[3], x[4], x[5]), max3(x[6], x[7], x[7]));
 }
 
-// scores s (x c -> exponents of 2) of a lane's 8 tokens -> probabilities; live (where masked):
-// bit i = token i is seen.  Raises the row's maximum where needed.
+// scores s (x c -> exponents of 2) of a lane's 8 tokens -> weights; live (where masked): bit i =
+// token i is seen.  Moves the row's reference where needed.
 template <int D>
 __device__ __forceinline__ void softmax8(Tile<D> &t, const f32x4_t &s0, const f32x4_t &s1, float c, bool masked,
                                          uint32_t live, float (&p)[8]) {
@@ -397,18 +407,24 @@ __device__ __forceinline__ void softmax8(Tile<D> &t, const f32x4_t &s0, const f3
 #pragma unroll
         for (int i = 0; i < 8; ++i) x[i] = (l >> i) & 1u ? x[i] : -INFINITY;
     }
-    if (__any(max8(x) > LAZY)) {
+    // (a lane's 8 tokens outside [P_MIN, P_MAX]; it is the row's 32 that decide below)
+    if (__any(fabsf(max8(x) - 0.5f * (P_MAX + P_MIN)) > 0.5f * (P_MAX - P_MIN))) {
         // (what is dead stays at -inf, whatever its score)
 #pragma unroll
         for (int i = 0; i < 8; ++i) x[i] = x[i] == -INFINITY ? -INFINITY : (i < 4 ? s0[i & 3] : s1[i & 3]) * c;
-        const float m = fmaxf(t.m, max_rows(max8(x)));
-        const float f = __builtin_amdgcn_exp2f(t.m - m);
+        const float top = max_rows(max8(x)), at = top - t.m;
+        const bool up = __any(at > P_MAX), move = (up && at > P_NEW) || (at < P_LOW && top > -INFINITY);
+        const float f = __builtin_amdgcn_exp2f(P_NEW - at);
+        if (__any(move)) {
+            const bool fits = move && t.l[0] * f < P_SUM;
+            const float g = fits ? f : 1.0f;
 #pragma unroll
-        for (int i = 0; i < 8; ++i) x[i] -= m;
+            for (int ct = 0; ct < D / 16; ++ct) t.acc[ct] *= g;
+            t.l *= g;
+            t.m = fits ? top - P_NEW : t.m;
+        }
 #pragma unroll
-        for (int ct = 0; ct < D / 16; ++ct) t.acc[ct] *= f;
-        t.l *= f;
-        t.m = m;
+        for (int i = 0; i < 8; ++i) x[i] -= t.m;
     }
 #pragma unroll
     for (int i = 0; i < 8; ++i) p[i] = __builtin_amdgcn_exp2f(x[i]);
@@ -681,7 +697,7 @@ __device__ __forceinline__ void store_out(const AttnArgs &a, int b, int h, int r
 
 // ------------------------------------------------------------------ few rows
 // NT row tiles of 16; the four waves of a workgroup take a segment's items in turn, each with
-// its own running maximum, sum and output (registers only, no barrier), and are joined in LDS at
+// its own reference, sum and output (registers only, no barrier), and are joined in LDS at
 // the segment's end.  A wave's next record is asked for as soon as the registers of this one are
 // free: keys behind the scores, values behind the second product.
 //

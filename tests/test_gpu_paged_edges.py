@@ -1,14 +1,16 @@
 """The paged 4-bit cache where its rules are easily missed: masks without a position, layers that
-were written but not committed."""
+were written but not committed, weights far below the largest."""
+
+import math
 
 import pytest
 import torch
 
-from _paged import Requests, attend64, check_attention
+from _paged import Requests, attend64, check_attention, stored
 
 pytestmark = pytest.mark.gpu
 
-BF = torch.bfloat16
+BF, F16 = torch.bfloat16, torch.float16
 
 
 # ------------------------------------------------------------------ masks
@@ -49,3 +51,80 @@ def test_a_staged_layer_is_not_read_before_the_commit(gpu):
     c.attend(0, q)
     kk, _ = c.dequantize_layer(0, 75)
     assert torch.equal(kk[1, :, 64:].cpu(), torch.cat((r.k[1][:, 64:], k[1, :, :5].cpu()), 1))
+
+
+# ------------------------------------------------------------------ weights
+def _led(gen, h, n, d, lead, dtype, at):
+    """Keys of whole numbers -8 .. 7 that every group of 32 stores exactly (each channel has both
+    ends: step 1), values, and the direction u that key `at` has: a query lead * u / (7 sqrt(d)) scores
+    it `lead`.  Its own value is 0."""
+    k = torch.randint(-8, 8, (h, n, d), generator=gen).float()
+    for g in range(n // 32):
+        rows = 1 + torch.rand((h, 31, d), generator=gen).argsort(1)[:, :2] + 32 * g
+        k.scatter_(1, rows[:, :1], -8.0)
+        k.scatter_(1, rows[:, 1:], 7.0)
+    v = torch.randn((h, n, d), generator=gen) * (1000.0 if dtype == F16 else 1.0)
+    u = torch.randint(0, 2, (h, d), generator=gen).float() * 2 - 1
+    if at is not None:
+        k[:, at], v[:, at] = 7 * u, 0.0
+    return k.to(dtype), v.to(dtype), u
+
+
+@pytest.mark.parametrize("dtype,lead", [(BF, 12), (BF, 20), (BF, 29), (F16, 12), (F16, 17)])
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("t,where", [(1, "first"), (1, "middle"), (1, "tail"), (1, "block"), (9, "first"),
+                                     (40, "first"), (40, "middle"), (40, "tail"), (40, "block"), (130, "first")])
+def test_a_leading_key_without_a_value_leaves_the_others_their_digits(gpu, t, where, d, dtype, lead):
+    """One key takes nearly all of the weight and adds nothing (an attention sink): the result is
+    that of the other keys, whose weights lie 2^-17 to 2^-42 below the largest.
+
+    The bound.  Scores are exact up to f32's rounding of exponents below 2^7 (2^-16 of a weight, with
+    the exponential's own).  A weight and a value are each rounded to f16: 2^-11 of them, or, where a
+    weight is subnormal, half of f16's least step, 2^-25, at most the weight itself.  That is on a
+    scale where the largest weight of the row among the item's 32 keys is at least 2^-8 (2^-17 of it);
+    where the item holds the leading key, on the scale that this key or an item with smaller weights
+    moved last, to 2^7 (2^-32 of the leading one: its 31 neighbours keep no digits once it leads by 22
+    nats).  The sum of the weights is that of what is multiplied.  So |do| <= sum_j dp_j |v_j - o| +
+    2^-11 sum_j p_j |v_j|, doubled for the higher orders, and the result's own rounding.  In the
+    2-norm of a row the roundings are independent and of no sign: the result's half step, three of
+    f16, and the absolute parts, which meet independent values, in quadrature (twice that)."""
+    h, g, n = 2, 2, 1000 if where == "tail" else 992
+    gen = torch.Generator().manual_seed(int(lead) + t + d)
+    at = {"first": 0, "middle": 512, "tail": 995, "block": None}[where]
+    k, v, u = _led(gen, h, n, d, lead, dtype, at)
+    ck = torch.randint(-8, 8, (h, t, d), generator=gen).to(dtype)
+    cv = (torch.randn((h, t, d), generator=gen) * (1000.0 if dtype == F16 else 1.0)).to(dtype)
+    if where == "block":
+        ck[:, 0], cv[:, 0] = (7 * u).to(dtype), 0.0
+    alpha = round(lead / (7 * math.sqrt(d)) * 256) / 256
+    q = alpha * u.repeat_interleave(g, 0)[:, None] + torch.round(torch.randn((h * g, t, d), generator=gen) * 4) / 64
+    q = q.to(dtype)
+    r = Requests(gpu, [0, 0], h=h, d=d, dtype=dtype, room=n, page=64)
+    rows = lambda x: torch.stack((x, x)).to(gpu)  # noqa: E731
+    r.cache.begin_append(r.i32([n, n]), n)
+    r.cache.stage_layer(0, rows(k), rows(v))
+    r.cache.commit_append()
+    got = r.cache.attend(0, rows(q), rows(ck), rows(cv)).double().cpu()
+    k64 = stored(k, "k")
+    assert torch.equal(k64, k.double())
+    kk = torch.cat((k64, ck.double()), 1).repeat_interleave(g, 0)
+    vv = torch.cat((stored(v, "v"), cv.double()), 1).repeat_interleave(g, 0)
+    p = torch.softmax(torch.matmul(q.double(), kk.transpose(1, 2)) * d ** -0.5, -1)
+    want = torch.matmul(p, vv)
+    # the largest weight among each key's item: 32 packed tokens, the tail, or 32 of the block's keys
+    sizes = [32] * (n // 32) + [n % 32] * bool(n % 32) + [32] * (t // 32) + [t % 32] * bool(t % 32)
+    top = torch.cat([x.amax(-1, keepdim=True).expand_as(x) for x in p.split(sizes, -1)], -1)
+    step = 2.0 ** -11
+    lead = p.argmax(-1, keepdim=True) == torch.arange(p.shape[-1])
+    led = torch.cat([x.any(-1, keepdim=True).expand_as(x) for x in lead.split(sizes, -1)], -1)
+    lost = torch.minimum(p, torch.where(led, 2.0 ** -32, 2.0 ** -17) * top)
+    dp = (step + 2.0 ** -16) * p + lost
+    bound = 2 * (torch.matmul(dp + step * p, vv.abs()) + dp.sum(-1, keepdim=True) * want.abs())
+    fine = torch.finfo(dtype)
+    bound += fine.eps / 2 * want.abs() + fine.smallest_normal * fine.eps
+    over = ((got - want).abs() / bound).max()
+    assert over <= 1, f"an element is {float(over):.2f} of its bound off"
+    tiny = math.sqrt(d) * fine.smallest_normal * fine.eps / 2
+    lost = torch.matmul(lost ** 2, vv.norm(dim=-1, keepdim=True) ** 2).sqrt()[..., 0]
+    rel = ((got - want).norm(dim=-1) / (want.norm(dim=-1) * (fine.eps / 2 + 3 * step) + 2 * lost + tiny)).max()
+    assert rel <= 1, f"a row is {float(rel):.2f} of its 2-norm's bound off"
