@@ -387,6 +387,11 @@ typedef struct ma_pages {
 int ma_page_plan(const int32_t *lengths, const int32_t *new_lens, int B, int T, int page_tokens, int32_t *table,
                  int64_t s_table, int width, int32_t *ring, int num_pages, int32_t *state, int64_t *slots,
                  int32_t *ends, void *stream);
+/* ma_page_plan of a step that stores tokens: a negative new_lens[b] refuses it as well and adds 16
+ * to status (tokens of a packed group cannot return to the tail). */
+int ma_page_plan_append(const int32_t *lengths, const int32_t *new_lens, int B, int T, int page_tokens,
+                        int32_t *table, int64_t s_table, int width, int32_t *ring, int num_pages, int32_t *state,
+                        int64_t *slots, int32_t *ends, void *stream);
 /* Append of new_lens[b] (0 .. T) tokens k, v [B, H, T, D] behind request b's lengths[b]
  * tokens: every group of 32 that [tail | new] completes is quantized with ma_quantize_keys'
  * and ma_quantize_values' arithmetic into the record that slots (ma_page_plan's) names, and

@@ -111,6 +111,7 @@ SIGNATURES = {
     "ma_rebuild_packed": (_I, [_PREF, _I, _I, _I, _PREF, _P, _I64, _I, _P, _I64, _I, _P, _I64, _I, _P, _I64, _I,
                                _P, _I64, _P, _I64, _I, _P, _P]),
     "ma_page_plan": (_I, [_P, _P, _I, _I, _I, _P, _I64, _I, _P, _I, _P, _P, _P, _P]),
+    "ma_page_plan_append": (_I, [_P, _P, _I, _I, _I, _P, _I64, _I, _P, _I, _P, _P, _P, _P]),
     "ma_page_append": (_I, [_PAGES, _T4, _T4, _I, _I, _I, _I, _P, _P, _P]),
     "ma_page_dequant": (_I, [_PAGES, _I, _I, _I, _P, _I, _T4, _T4, _P]),
     "ma_paged_workspace_bytes": (_I64, [_I, _I, _I, _I, _I]),

@@ -25,7 +25,7 @@ constexpr int PLAN_THREADS = 256;
 constexpr int PLAN_SLOTS = 2048;
 constexpr int PLAN_SCAN = 4 * PLAN_THREADS;   // requests per scan step
 
-enum { PLAN_NO_PAGES = 1, PLAN_WIDTH = 2, PLAN_TOKENS = 4, PLAN_LENGTH = 8 };
+enum { PLAN_NO_PAGES = 1, PLAN_WIDTH = 2, PLAN_TOKENS = 4, PLAN_LENGTH = 8, PLAN_NEGATIVE = 16 };
 
 struct PlanArgs {
     const int32_t *lengths, *new_lens;
@@ -33,6 +33,7 @@ struct PlanArgs {
     int64_t *slots;
     int64_t s_table, nflat;   // nflat = B * max(T, 1)
     int B, T, page, width, num_pages;
+    bool grow;                // no request gives tokens back
 };
 
 // a request's step: tokens after it, pages before and after it (`most` + 1 where there are more
@@ -77,6 +78,7 @@ __global__ __launch_bounds__(PLAN_THREADS) void page_plan_kernel(PlanArgs a) {
                 const Step st = step_of(len, n, a.page, a.width);
                 if (len < 0) bad |= PLAN_LENGTH;
                 if (n > a.T) bad |= PLAN_TOKENS;
+                if (a.grow && n < 0) bad |= PLAN_NEGATIVE;
                 if (max(st.p0, st.p1) > (uint32_t)a.width) bad |= PLAN_WIDTH;
                 gt += st.p1 > st.p0 ? st.p1 - st.p0 : 0;
                 kt += st.p0 > st.p1 ? st.p0 - st.p1 : 0;
@@ -634,10 +636,9 @@ int ma::pg_check(const ma_pages *p, int B, int H, int D, const char *who) {
     return MA_OK;
 }
 
-extern "C" int ma_page_plan(const int32_t *lengths, const int32_t *new_lens, int B, int T, int page_tokens,
-                            int32_t *table, int64_t s_table, int width, int32_t *ring, int num_pages, int32_t *state,
-                            int64_t *slots, int32_t *ends, void *stream) {
-    const char *who = "ma_page_plan";
+static int page_plan(const char *who, bool grow, const int32_t *lengths, const int32_t *new_lens, int B, int T,
+                     int page_tokens, int32_t *table, int64_t s_table, int width, int32_t *ring, int num_pages,
+                     int32_t *state, int64_t *slots, int32_t *ends, void *stream) {
     if (B <= 0 || T < 0 || page_tokens <= 0 || page_tokens % PG_GROUP || width <= 0 || num_pages <= 0) {
         ma_set_error("%s: bad arguments (B=%d T=%d page_tokens=%d, a multiple of 32, width=%d num_pages=%d)", who, B, T,
                      page_tokens, width, num_pages);
@@ -663,9 +664,24 @@ extern "C" int ma_page_plan(const int32_t *lengths, const int32_t *new_lens, int
         ma_set_error("%s: the requests' table rows overlap (stride %lld, width %d)", who, (long long)s_table, width);
         return MA_EINVAL;
     }
-    PlanArgs a{lengths, new_lens, table, ring, state, ends, slots, s_table, nflat, B, T, page_tokens, width, num_pages};
+    PlanArgs a{lengths, new_lens, table, ring, state, ends, slots, s_table, nflat, B, T, page_tokens, width, num_pages,
+               grow};
     page_plan_kernel<<<dim3((unsigned)wgs), PLAN_THREADS, 0, (hipStream_t)stream>>>(a);
     return ma_check_launch(who);
+}
+
+extern "C" int ma_page_plan(const int32_t *lengths, const int32_t *new_lens, int B, int T, int page_tokens,
+                            int32_t *table, int64_t s_table, int width, int32_t *ring, int num_pages, int32_t *state,
+                            int64_t *slots, int32_t *ends, void *stream) {
+    return page_plan("ma_page_plan", false, lengths, new_lens, B, T, page_tokens, table, s_table, width, ring, num_pages,
+                     state, slots, ends, stream);
+}
+
+extern "C" int ma_page_plan_append(const int32_t *lengths, const int32_t *new_lens, int B, int T, int page_tokens,
+                                   int32_t *table, int64_t s_table, int width, int32_t *ring, int num_pages,
+                                   int32_t *state, int64_t *slots, int32_t *ends, void *stream) {
+    return page_plan("ma_page_plan_append", true, lengths, new_lens, B, T, page_tokens, table, s_table, width, ring,
+                     num_pages, state, slots, ends, stream);
 }
 
 extern "C" int ma_page_append(const ma_pages *p, ma_tensor4 k, ma_tensor4 v, int B, int H, int T, int D,

@@ -141,7 +141,7 @@ class PagedPrefix:
 
 def plan_pages(lengths: torch.Tensor, new_lens: torch.Tensor, block_table: torch.Tensor, free_ring: torch.Tensor,
                ring_state: torch.Tensor, *, page_tokens: int, tokens: int, slots: torch.Tensor | None = None,
-               ends: torch.Tensor | None = None):
+               ends: torch.Tensor | None = None, give_back: bool = True):
     """Pages for one step, planned on the GPU: request b goes from lengths[b] to ends[b] =
     max(0, lengths[b] + new_lens[b]) tokens.  Returns (slots int64 [B, tokens], ends int32
     [B]): slot = page id * page_tokens + offset of each new token, -1 behind new_lens[b].
@@ -152,13 +152,14 @@ def plan_pages(lengths: torch.Tensor, new_lens: torch.Tensor, block_table: torch
     (place of the oldest, free pages, 0, status).  Growing requests take the oldest pages, in
     request order; pages given back (new_lens[b] < 0: that many tokens, at most all) enter
     behind the newest and are free from the next plan on: for a step given up before its
-    append, or a request that ends (tokens of a packed group do not return to the tail).
-    lengths is not written.
+    append, or a request that ends (tokens of a packed group do not return to the tail).  A step
+    that stores tokens passes give_back=False: a negative count then refuses it.  lengths is not
+    written.
 
     A plan that cannot be met changes nothing, returns slots of -1 and ends = lengths, and
     adds to the status, which stays until the caller clears it: 1 the pages run out, 2 a
-    request outgrows its table row, 4 new_lens[b] > tokens, 8 a negative length
-    (``check_plan`` reads it and raises)."""
+    request outgrows its table row, 4 new_lens[b] > tokens, 8 a negative length, 16 a negative
+    new_lens[b] without give_back (``check_plan`` reads it and raises)."""
     if lengths.ndim != 1:
         raise ValueError(f"lengths must be [B], got {tuple(lengths.shape)}")
     N.require_gpu(lengths, "lengths")
@@ -182,14 +183,15 @@ def plan_pages(lengths: torch.Tensor, new_lens: torch.Tensor, block_table: torch
         _same_device(index, block_table=block_table, slots=slots)
     if b == 0:
         return slots, ends
-    _call(index, "ma_page_plan", lengths.data_ptr(), new_lens.data_ptr(), b, tokens, page_tokens,
+    _call(index, "ma_page_plan" if give_back else "ma_page_plan_append", lengths.data_ptr(), new_lens.data_ptr(), b, tokens, page_tokens,
           block_table.data_ptr(), block_table.stride(0), block_table.shape[1], free_ring.data_ptr(), free_ring.numel(),
           ring_state.data_ptr(), slots.data_ptr() if tokens else None, ends.data_ptr())
     return slots, ends
 
 
 _PLAN_ERRORS = ((1, "the free pages run out"), (2, "a request outgrows its block table row"),
-                (4, "more new tokens than the plan's tokens"), (8, "a negative length"))
+                (4, "more new tokens than the plan's tokens"), (8, "a negative length"),
+                (16, "a negative number of new tokens"))
 
 
 def check_plan(ring_state: torch.Tensor) -> None:

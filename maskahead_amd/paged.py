@@ -89,14 +89,14 @@ class PagedKVCache:
     def begin_append(self, new_lens: torch.Tensor, tokens: int) -> torch.Tensor:
         """Open an append of new_lens[b] (0 .. tokens) tokens to every layer and give their pages
         to the requests.  Returns the slots [B, tokens] (``plan_pages``).  A plan that cannot be
-        met stores nothing and leaves every length as it is; ``check`` reports it.  new_lens is
+        met (a negative count among what it refuses) stores nothing and leaves every length as it is; ``check`` reports it.  new_lens is
         read until the commit: it must not change before."""
         if self._plan is not None:
             raise RuntimeError("another cache append is already in progress")
         if tokens <= 0:
             raise ValueError("tokens must be positive")
         slots, ends = plan_pages(self.lengths, new_lens, self.block_table, self.free_ring, self.ring_state,
-                                 page_tokens=self.page_tokens, tokens=tokens)
+                                 page_tokens=self.page_tokens, tokens=tokens, give_back=False)
         self._plan = (new_lens, slots, ends, set())
         return slots
 

@@ -1,5 +1,5 @@
 """The paged 4-bit cache where its rules are easily missed: masks without a position, layers that
-were written but not committed, weights far below the largest."""
+were written but not committed, counts below zero, weights far below the largest."""
 
 import math
 
@@ -51,6 +51,29 @@ def test_a_staged_layer_is_not_read_before_the_commit(gpu):
     c.attend(0, q)
     kk, _ = c.dequantize_layer(0, 75)
     assert torch.equal(kk[1, :, 64:].cpu(), torch.cat((r.k[1][:, 64:], k[1, :, :5].cpu()), 1))
+
+
+@pytest.mark.parametrize("new", [[-20, 5], [3, -1], [-40, -10]])
+def test_an_append_of_fewer_than_no_tokens_is_refused(gpu, new):
+    """Tokens of a packed group do not return to the tail, so only abort_append and release give
+    tokens back."""
+    r = Requests(gpu, [40, 10], page=32)
+    c = r.cache
+    before = [x.clone() for x in (c.pool, c.k_tail, c.v_tail, c.lengths, c.block_table, c.free_ring, c.ring_state[:3])]
+    k, v = r.block([8, 8], 8)
+    assert (c.begin_append(r.i32(new), 8) == -1).all()
+    c.stage_layer(0, k.to(gpu), v.to(gpu))
+    c.commit_append()
+    for x, y in zip(before, (c.pool, c.k_tail, c.v_tail, c.lengths, c.block_table, c.free_ring, c.ring_state[:3])):
+        x, y = (t.view(torch.int16) if t.dtype == BF else t for t in (x, y))
+        assert torch.equal(x, y)
+    with pytest.raises(RuntimeError, match="negative number of new tokens"):
+        c.check()
+    c.begin_append(r.i32([8, 8]), 8)
+    c.abort_append()
+    c.release(torch.tensor([True, False], device=gpu))
+    c.check()
+    assert c.lengths.tolist() == [0, 10]
 
 
 # ------------------------------------------------------------------ weights
