@@ -396,8 +396,8 @@ int ma_page_plan_append(const int32_t *lengths, const int32_t *new_lens, int B, 
  * tokens: every group of 32 that [tail | new] completes is quantized with ma_quantize_keys'
  * and ma_quantize_values' arithmetic into the record that slots (ma_page_plan's) names, and
  * the rest becomes the tail.  Requests without new tokens, and those whose slots are -1, are
- * left as they are.  k, v share p->dtype.  One launch.  MA_EUNSUPPORTED (here and below): B
- * or H > 65535. */
+ * left as they are.  k, v share p->dtype.  One launch.  MA_EUNSUPPORTED (here and in
+ * ma_page_dequant): B or H > 65535. */
 int ma_page_append(const ma_pages *p, ma_tensor4 k, ma_tensor4 v, int B, int H, int T, int D,
                    const int32_t *new_lens, const int64_t *slots, void *stream);
 /* Tokens starts[b] .. starts[b] + n of every request (starts NULL: from 0) as k_out, v_out
@@ -414,7 +414,8 @@ int ma_page_dequant(const ma_pages *p, int B, int H, int D, const int32_t *start
  * p->dtype; D 64 or 128.  workspace: ma_paged_workspace_bytes() bytes, 256-byte aligned; its
  * contents are not read before they are written, and calls that may run at once need one each.
  * The same call gives the same bits (no atomics).  Two launches.  MA_EUNSUPPORTED: B * H * row
- * groups of requests as long as their table rows are 2^31 groups of 32 tokens or more. */
+ * groups are 2^23 or more (2^24 where a KV head has more than 32 rows), or 2^31 groups of 32 tokens
+ * in requests as long as their table rows. */
 int64_t ma_paged_workspace_bytes(int B, int H, int Hq, int T, int D);
 int ma_paged_attention(ma_tensor4 q, int B, int Hq, int T, int D, const ma_pages *p, int H, ma_tensor4 kc,
                        ma_tensor4 vc, const int32_t *new_lens, int causal_block, float scale, ma_tensor4 out,

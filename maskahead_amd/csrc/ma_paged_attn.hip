@@ -1396,6 +1396,12 @@ extern "C" int ma_paged_attention(ma_tensor4 q, int B, int Hq, int T, int D, con
                      B, (long long)p->width * p->page_tokens, s.RG);
         return MA_EUNSUPPORTED;
     }
+    // the merge: a workgroup a segment (and rows), threads of one dimension below 2^32
+    if ((int64_t)B * H * s.RG * 64 * merge_waves(s.nt == 0) > UINT32_MAX) {
+        ma_set_error("%s: %d requests, %d heads and %d row groups of each are not built (2^%d segments)", who, B, H, s.RG,
+                     s.nt ? 23 : 24);
+        return MA_EUNSUPPORTED;
+    }
     const Layout l = layout_of(s, (int64_t)B * H * s.RG, D);
     char *ws = (char *)workspace;
     AttnArgs a{};

@@ -130,3 +130,14 @@ def test_a_line_past_31_bits_is_refused(lib):
                                   None) == N.MA_EUNSUPPORTED
     # rows that no launch holds
     assert lib.ma_paged_workspace_bytes(1, 1, 1 << 16, 1 << 16, 128) == -1
+
+
+@pytest.mark.parametrize("heads,t,segments", [(4, 1, 1 << 23), (4, 33, 1 << 24), (1, 300, 1 << 24)])
+def test_more_segments_than_a_launch_holds_are_refused(lib, heads, t, segments):
+    """Before the first launch: 2^32 threads of the merge in one dimension (512 a segment of few rows,
+    256 of many; 300 rows are 2 row groups)."""
+    b = segments // heads // (2 if t == 300 else 1)
+    p = ctypes.byref(_pages(width=1, page_tokens=32))
+    assert lib.ma_paged_attention(_t4(), b, heads, t, 128, p, heads, _t4(ptr=None), _t4(ptr=None), None, 0, 1.0, _t4(),
+                                  4096, 1 << 60, None) == N.MA_EUNSUPPORTED
+    assert b"segments" in lib.ma_last_error()
