@@ -356,6 +356,30 @@ __device__ __forceinline__ uint4 rows_channel(const uint32_t (&vw)[8][D / 32], i
     }
     return uint4{x[0], x[1], x[2], x[3]};
 }
+// A product takes a weight of 0 times a value that is no number to every query row, also to those
+// that do not see it.  So under a causal rule such values of the block are 0 in the products, and are
+// added as they are to the sums (few rows) or to what was written (many) of the rows that see them.
+// Bits 15 and 31 of odd_halves: this half of w is none.
+template <bool BF16>
+__device__ __forceinline__ uint32_t odd_halves(uint32_t w) {
+    return ((w & (BF16 ? 0x7f807f80u : 0x7c007c00u)) + (BF16 ? 0x00800080u : 0x04000400u)) & 0x80008000u;
+}
+__device__ __forceinline__ uint32_t without(uint32_t w, uint32_t odd) { return w & ~(odd | (odd - (odd >> 15))); }
+// the elements e .. e + 3 of a value's row, as f32; odd: bit i = element e + i is no number
+template <bool BF16>
+__device__ __forceinline__ f32x4_t odd_of_four(const uint16_t *src, uint32_t &odd) {
+    const uint2 v = pg_load8(src);
+    const uint32_t x = odd_halves<BF16>(v.x), y = odd_halves<BF16>(v.y);
+    odd = (x >> 15 & 1u) | (x >> 30 & 2u) | (y >> 13 & 4u) | (y >> 28 & 8u);
+    f32x4_t r;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const uint32_t w = i & 2 ? v.y : v.x;
+        const uint16_t e = (uint16_t)(i & 1 ? w >> 16 : w);
+        r[i] = BF16 ? ma_bf16_to_f32(e) : ma_f16_to_f32(e);
+    }
+    return r;
+}
 // how many of the block's keys its position t sees: to the end of its causal block, counted from
 // the request's first token (len + t has 32 bits, its sum with a block has not)
 __device__ __forceinline__ int keys_seen(const AttnArgs &a, const Items &it, int t) {
@@ -407,13 +431,15 @@ __device__ __forceinline__ void softmax8(Tile<D> &t, const f32x4_t &s0, const f3
 #pragma unroll
         for (int i = 0; i < 8; ++i) x[i] = (l >> i) & 1u ? x[i] : -INFINITY;
     }
-    // (a lane's 8 tokens outside [P_MIN, P_MAX]; it is the row's 32 that decide below)
-    if (__any(fabsf(max8(x) - 0.5f * (P_MAX + P_MIN)) > 0.5f * (P_MAX - P_MIN))) {
-        // (what is dead stays at -inf, whatever its score)
+    const float mx = max8(x);
+    if (__any(fabsf(mx - 0.5f * (P_MAX + P_MIN)) > 0.5f * (P_MAX - P_MIN))) {
+        // (what is done to a row depends on its own scores alone; what is dead stays at -inf)
+        float y[8];
 #pragma unroll
-        for (int i = 0; i < 8; ++i) x[i] = x[i] == -INFINITY ? -INFINITY : (i < 4 ? s0[i & 3] : s1[i & 3]) * c;
-        const float top = max_rows(max8(x)), at = top - t.m;
-        const bool up = __any(at > P_MAX), move = (up && at > P_NEW) || (at < P_LOW && top > -INFINITY);
+        for (int i = 0; i < 8; ++i) y[i] = x[i] == -INFINITY ? -INFINITY : (i < 4 ? s0[i & 3] : s1[i & 3]) * c;
+        const float top = max_rows(max8(y)), at = top - t.m;
+        const bool out = at > P_MAX || -max_rows(-mx) < P_MIN;
+        const bool move = out && (at > P_NEW || (at < P_LOW && top > -INFINITY));
         const float f = __builtin_amdgcn_exp2f(P_NEW - at);
         if (__any(move)) {
             const bool fits = move && t.l[0] * f < P_SUM;
@@ -422,9 +448,10 @@ __device__ __forceinline__ void softmax8(Tile<D> &t, const f32x4_t &s0, const f3
             for (int ct = 0; ct < D / 16; ++ct) t.acc[ct] *= g;
             t.l *= g;
             t.m = fits ? top - P_NEW : t.m;
-        }
 #pragma unroll
-        for (int i = 0; i < 8; ++i) x[i] -= t.m;
+            for (int i = 0; i < 8; ++i)
+                x[i] = x[i] == -INFINITY ? -INFINITY : __builtin_fmaf(i < 4 ? s0[i & 3] : s1[i & 3], c, -t.m);
+        }
     }
 #pragma unroll
     for (int i = 0; i < 8; ++i) p[i] = __builtin_amdgcn_exp2f(x[i]);
@@ -682,17 +709,43 @@ __device__ __forceinline__ uint32_t pack_out(float x, float y) {
     const f16x2_t z = {(_Float16)x, (_Float16)y};
     return __builtin_bit_cast(uint32_t, z);
 }
+__device__ __forceinline__ uint16_t *out_row(const AttnArgs &a, int b, int h, int row) {
+    const int g = row / a.T, t = row - g * a.T;
+    return (uint16_t *)a.out.ptr + (int64_t)b * a.out.s[0] + (int64_t)(h * a.G + g) * a.out.s[1] + (int64_t)t * a.out.s[2];
+}
 // NC channels of a row, to its place in out
 template <int NC, bool BF16>
 __device__ __forceinline__ void store_out(const AttnArgs &a, int b, int h, int row, int ch, const float *o) {
-    const int g = row / a.T, t = row - g * a.T;
-    uint16_t *dst = (uint16_t *)a.out.ptr + (int64_t)b * a.out.s[0] + (int64_t)(h * a.G + g) * a.out.s[1] +
-                    (int64_t)t * a.out.s[2] + ch;
+    uint16_t *dst = out_row(a, b, h, row) + ch;
     uint32_t y[NC / 2];
 #pragma unroll
     for (int k = 0; k < NC / 2; ++k) y[k] = pack_out<BF16>(o[2 * k], o[2 * k + 1]);
     if constexpr (NC == 8) pg_store16(dst, uint4{y[0], y[1], y[2], y[3]});
     else pg_store8(dst, uint2{y[0], y[1]});
+}
+
+// f(element, value) of every value that is no number, of the block's rows below keys in items [d0, d1)
+// (every step-th), in the lane's channels (D/4) hh + (0 .. D/4 - 1)
+template <int D, bool BF16, class F>
+__device__ __forceinline__ void each_odd(const AttnArgs &a, const Items &it, int b, int h, int d0, int d1, int step, int keys,
+                                         int hh, F f) {
+#pragma unroll 1
+    for (int i = d0; i < d1; i += step) {
+        const Rows r = rows_of(a, it, b, h, i - it.ng);
+        const int end = r.tail ? 0 : min(r.j0 + PG_GROUP, r.cnt);
+#pragma unroll 1
+        for (int j = r.j0; j < end; ++j) {
+            const uint16_t *src = r.v + (int64_t)j * r.sv + (D / 4) * hh;
+#pragma unroll
+            for (int e = 0; e < D / 4; e += 4) {
+                uint32_t odd;
+                const f32x4_t v = odd_of_four<BF16>(src + e, odd);
+#pragma unroll
+                for (int y = 0; y < 4; ++y) f(e + y, (odd >> y & 1u) && j < keys, v[y]);
+                __builtin_amdgcn_sched_barrier(0);      // (few registers: none of this is in a hurry)
+            }
+        }
+    }
 }
 
 // ------------------------------------------------------------------ few rows
@@ -707,6 +760,8 @@ __device__ __forceinline__ void store_out(const AttnArgs &a, int b, int h, int r
 // 10 us are no traffic: two launches, the scan, the first record's three loads in a row (length,
 // table, words), the join and the merge (one token after prompts of up to 700 tokens: 13.8 us in
 // all).  Two records under way a wave were no faster (D 128: 55.2 and 69.0 us).
+// Registers: for the two workgroups a CU that are launched (for three, the 16-bit rows' path spilled:
+// 52.4 -> 80 us).
 template <int D, int NT>
 struct FewShared {
     static constexpr int OS = D + 4;                 // row stride of a wave's output rows, f32
@@ -716,7 +771,7 @@ struct FewShared {
 };
 
 template <int D, int NT, bool BF16, bool MASK>
-__global__ __launch_bounds__(256, NT == 1 ? 3 : 2) void paged_few_kernel(AttnArgs a) {
+__global__ __launch_bounds__(256, 2) void paged_few_kernel(AttnArgs a) {
     constexpr int CB = D / 32, NC = D / 16;
     __shared__ FewShared<D, NT> sh;
     const int tid = threadIdx.x, lane = tid & 63, wave = uniform(tid >> 6), n16 = lane & 15, hh = lane >> 4;
@@ -796,6 +851,8 @@ __global__ __launch_bounds__(256, NT == 1 ? 3 : 2) void paged_few_kernel(AttnArg
             dead = dead_next;
         }
         // the tail and the block's own keys
+        bool odd = false;
+        const int rows_at = i;
         for (; i < pt.i1; i += WAVES) {
             const Rows r = rows_of(a, it, b, h, i - it.ng);
             if (r.cnt == 0) continue;
@@ -822,12 +879,30 @@ __global__ __launch_bounds__(256, NT == 1 ? 3 : 2) void paged_few_kernel(AttnArg
             __builtin_amdgcn_sched_barrier(0);
             uint32_t vw[8][NC / 2];
             rows_v<D>(r, l, seen, vw);
+            if (a.causal > 0 && !r.tail) {
+                uint32_t any = 0;
+#pragma unroll
+                for (int y = 0; y < 8; ++y)
+#pragma unroll
+                    for (int z = 0; z < NC / 2; ++z) {
+                        const uint32_t x = odd_halves<BF16>(vw[y][z]);
+                        any |= x;
+                        vw[y][z] = without(vw[y][z], x);
+                    }
+                odd |= __any(any);
+            }
 #pragma unroll
             for (int ct = 0; ct < NC; ++ct) {
                 const uint4 v = rows_channel<D>(vw, ct);
 #pragma unroll
                 for (int nt = 0; nt < NT; ++nt) t[nt].acc[ct] = rows_values(v, p[nt], t[nt].acc[ct]);
             }
+        }
+        if (odd) {
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt)
+                each_odd<D, BF16>(a, it, b, h, rows_at, pt.i1, WAVES, keys_seen(a, it, (row0 + nt * 16 + n16) % a.T), hh,
+                                  [&](int e, bool yes, float v) { t[nt].acc[e % NC][e / NC] += yes ? v : 0.f; });
         }
         // the waves' parts joined; whole segments written out, cut ones left as a partial
 #pragma unroll
@@ -918,6 +993,7 @@ struct ManyShared {
     static constexpr int OPS = 2 * (D / 32) + D / 16;     // operands of an item: K [2][D/32], V [D/16]
     uint4 op[2][STEP][OPS][64];
     uint32_t live[2][STEP];                               // bit j: the item's token j is seen
+    uint32_t odd[2][STEP];                                // one of the item's values is no number (causal calls)
     ScanShared scan;
 };
 
@@ -1042,6 +1118,7 @@ __global__ __launch_bounds__(512, 2) void paged_many_kernel(AttnArgs a) {
         const int r1 = min((pt.rg + 1) * (2 * RW * 16), a.R) - 1, t1 = pt.rg * (2 * RW * 16) / a.T == r1 / a.T ? r1 % a.T : a.T - 1;
         const int d0 = max(pt.i0, it.ng);
         const int d1 = min(pt.i1, it.ng + (it.rem ? 1 : 0) + (a.kc.ptr ? (keys_seen(a, it, t1) + PG_GROUP - 1) / PG_GROUP : 0));
+        int odd = 0;
         if (d0 < d1) {
             const int l = hidden(lane), lh = l >> 4;
             int keys[2];
@@ -1053,6 +1130,7 @@ __global__ __launch_bounds__(512, 2) void paged_many_kernel(AttnArgs a) {
                 keys[nt] = keys_seen(a, it, row % a.T);
             }
             for (int i = d0, x = 0; i < d1; i += STEP, ++x) {
+                uint32_t any = 0;
                 if (i + si < d1) {
                     const Rows r = rows_of(a, it, b, h, i + si - it.ng);
                     uint4(*op)[64] = sh.op[x & 1][si];
@@ -1067,11 +1145,25 @@ __global__ __launch_bounds__(512, 2) void paged_many_kernel(AttnArgs a) {
                         uint32_t w[8][NC / 2];
                         rows_v<D>(r, l, live, w);
 #pragma unroll
-                        for (int ct = 0; ct < NC; ++ct) op[2 * CB + ct][l] = rows_channel<D>(w, ct);
+                        for (int ct = 0; ct < NC; ++ct) {
+                            uint4 v = rows_channel<D>(w, ct);
+                            if (a.causal > 0 && !r.tail) {
+                                const uint32_t o[4] = {odd_halves<BF16>(v.x), odd_halves<BF16>(v.y), odd_halves<BF16>(v.z),
+                                                       odd_halves<BF16>(v.w)};
+                                any |= o[0] | o[1] | o[2] | o[3];
+                                v = uint4{without(v.x, o[0]), without(v.y, o[1]), without(v.z, o[2]), without(v.w, o[3])};
+                            }
+                            op[2 * CB + ct][l] = v;
+                        }
                         note_live(x, live);
                     }
                 }
+                if (a.causal > 0 && sv) {
+                    const bool o = __any(any);
+                    if (l == 0) sh.odd[x & 1][si] = o;
+                }
                 __syncthreads();
+                if (a.causal > 0) odd |= uniform((int)(sh.odd[x & 1][0] | sh.odd[x & 1][1] | sh.odd[x & 1][2] | sh.odd[x & 1][3]));
                 const int g1 = busy ? min(d1 - i, STEP) : 0;
                 for (int g = tw; g < g1; g += TW) {
                     const Rows r = rows_of(a, it, b, h, i + g - it.ng);
@@ -1159,6 +1251,12 @@ __global__ __launch_bounds__(512, 2) void paged_many_kernel(AttnArgs a) {
                         for (int ct = 0; ct < NC; ++ct) o[ct] = t[nt].acc[ct][r] * inv;
                         store_out<NC, BF16>(a, b, h, row, NC * (4 * hh + r), o);
                     }
+                    if (odd) {
+                        uint16_t *dst = out_row(a, b, h, row) + (D / 4) * hh;
+                        each_odd<D, BF16>(a, it, b, h, d0, d1, 1, keys_seen(a, it, row % a.T), hh, [&](int e, bool yes, float v) {
+                            if (yes) dst[e] = (uint16_t)pack_out<BF16>((BF16 ? ma_bf16_to_f32(dst[e]) : ma_f16_to_f32(dst[e])) + v, 0.f);
+                        });
+                    }
                 } else {
                     const int64_t slot = (int64_t)pt.slot * (2 * RW * 16);
                     const int rt = rw * 32 + nt * 16 + (hidden(lane) & 15);
@@ -1173,6 +1271,10 @@ __global__ __launch_bounds__(512, 2) void paged_many_kernel(AttnArgs a) {
                         for (int ct = 0; ct < NC; ct += 4)
                             *(f32x4_t *)&dst[(r * (NC / 4) + ct / 4) * 256] =
                                 f32x4_t{t[nt].acc[ct][r], t[nt].acc[ct + 1][r], t[nt].acc[ct + 2][r], t[nt].acc[ct + 3][r]};
+                    if (odd)
+                        each_odd<D, BF16>(a, it, b, h, d0, d1, 1, keys_seen(a, it, row % a.T), hh, [&](int e, bool yes, float v) {
+                            if (yes) dst[(e / 4) * 256 + e % 4] += v;
+                        });
                 }
             }
         }

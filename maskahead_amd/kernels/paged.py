@@ -276,7 +276,8 @@ def paged_attention(query: torch.Tensor, prefix: PagedPrefix, current_key: torch
     [B] (None: T each) counts each request's real positions: rows t >= new_lens[b] of out are
     left as they are, keys j >= new_lens[b] not seen.  causal_block > 0: key j is seen by query
     t only if (lengths[b] + j) // causal_block <= (lengths[b] + t) // causal_block.  A row that
-    sees nothing is zero.  The same call gives the same bits.  ``out`` [B, Hq, T, D] (not overlapping the inputs) receives the
+    sees nothing is zero; what a row does not see may hold anything, NaN and infinities too.  The
+    same call gives the same bits.  ``out`` [B, Hq, T, D] (not overlapping the inputs) receives the
     result; without it a new tensor does, whose rows t >= new_lens[b] are undefined."""
     shape = _check_block("query", query, prefix)
     b, hq, t, d = shape

@@ -1,5 +1,6 @@
 """The paged 4-bit cache where its rules are easily missed: masks without a position, layers that
-were written but not committed, counts below zero, weights far below the largest."""
+were written but not committed, counts below zero, weights far below the largest,
+values that a causal row does not see."""
 
 import math
 
@@ -151,3 +152,37 @@ def test_a_leading_key_without_a_value_leaves_the_others_their_digits(gpu, t, wh
     lost = torch.matmul(lost ** 2, vv.norm(dim=-1, keepdim=True) ** 2).sqrt()[..., 0]
     rel = ((got - want).norm(dim=-1) / (want.norm(dim=-1) * (fine.eps / 2 + 3 * step) + 2 * lost + tiny)).max()
     assert rel <= 1, f"a row is {float(rel):.2f} of its 2-norm's bound off"
+
+
+# ------------------------------------------------------------------ values that are not numbers
+@pytest.mark.parametrize("d,dtype", [(128, BF), (64, F16), (64, BF), (128, F16)])
+@pytest.mark.parametrize("t,hq,causal", [(8, 2, 4), (12, 4, 5), (70, 2, 32), (40, 8, 1), (300, 2, 100)])
+@pytest.mark.parametrize("what", [float("nan"), float("inf"), float("-inf")])
+def test_what_a_causal_row_does_not_see_may_be_no_number(gpu, t, hq, causal, what, d, dtype):
+    """A key or value of a later causal block changes no row of an earlier one, whatever it holds;
+    the rows that see it are no numbers either, and in the other channels what they are beside a
+    number: fewer than 512 products summed in another order, 2^-24 of them each on both sides, may
+    round to the next value of the type."""
+    lens = [45, 3, 64]
+    r = Requests(gpu, lens, h=2, d=d, dtype=dtype, page=32)
+    q = torch.randn((3, hq, t, d), generator=r.gen).to(dtype).to(gpu)
+    k, v = (x.to(gpu) for x in r.block([t, t - 1, t], t))
+    new = r.i32([t, t - 1, t])
+    want = r.cache.attend(0, q, k, v, new_lens=new, causal_block=causal)
+    biggest = max(float(x.abs().nan_to_num().max()) for x in (v, *r.v))
+    for place, part in (((t - 2, t - 3), "v"), ((t - 2,), "k"), ((t // 2, t - 2), "v")):
+        kb, vb = k.clone(), v.clone()
+        for j in place:
+            (kb if part == "k" else vb)[:, 1, j, 3 if part == "k" else slice(0, 5)] = what
+        got = r.cache.attend(0, q, kb, vb, new_lens=new, causal_block=causal)
+        for b, n in enumerate([t, t - 1, t]):
+            assert torch.equal(got[b, :hq // 2, :n], want[b, :hq // 2, :n])          # the other KV head's
+            for i in range(n):
+                sees = any((lens[b] + j) // causal <= (lens[b] + i) // causal for j in place)
+                row, was = got[b, hq // 2:, i], want[b, hq // 2:, i]
+                if not sees:
+                    assert torch.equal(row, was), (b, i, part)
+                elif part == "v":
+                    assert not torch.isfinite(row[:, :5]).any(), (b, i)
+                    off = (row[:, 5:].float() - was[:, 5:].float()).abs() - torch.finfo(dtype).eps * was[:, 5:].float().abs()
+                    assert off.max() <= 1024 * 2.0 ** -24 * biggest, (b, i)
