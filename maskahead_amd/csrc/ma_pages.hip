@@ -237,7 +237,14 @@ __device__ __forceinline__ QuantGroup group_params(float lo, float hi) {
     step = ma_round_bf16(fmaxf(step, 1e-8f));
     return {lo, step, __builtin_amdgcn_rcpf(step)};
 }
-// minimum / maximum of three, without the quieting that fminf / fmaxf put before each argument
+// the same for a minimum: a signalling NaN as a quiet one, which v_min3 and v_max3 pass over (they
+// answer a signalling one with NaN, and the numbers beside it are lost); f16's conversion does so
+template <int DT>
+__device__ __forceinline__ void unpack2_quiet(uint32_t w, float &a, float &b) {
+    unpack2<DT>(w, a, b);
+    if constexpr (DT == MA_BF16) a = __builtin_canonicalizef(a), b = __builtin_canonicalizef(b);
+}
+// minimum / maximum of three quiet values (fminf and fmaxf quiet each argument again)
 __device__ __forceinline__ float min3(float x, float y, float z) {
     float r;
     asm("v_min3_f32 %0, %1, %2, %3" : "=v"(r) : "v"(x), "v"(y), "v"(z));
@@ -329,8 +336,8 @@ __global__ __launch_bounds__(256) void page_append_kernel(AppendArgs a) {
                 float v[2][4];
 #pragma unroll
                 for (int e = 0; e < 2; ++e) {
-                    unpack2<DT>(x[i + e].x, v[e][0], v[e][1]);
-                    unpack2<DT>(x[i + e].y, v[e][2], v[e][3]);
+                    unpack2_quiet<DT>(x[i + e].x, v[e][0], v[e][1]);
+                    unpack2_quiet<DT>(x[i + e].y, v[e][2], v[e][3]);
                 }
 #pragma unroll
                 for (int c = 0; c < 4; ++c) {
@@ -394,7 +401,7 @@ __global__ __launch_bounds__(256) void page_append_kernel(AppendArgs a) {
 #pragma unroll
                 for (int c = 0; c < NC / 2; ++c) {
                     float v0, v1;
-                    unpack2<DT>(x[i][c], v0, v1);
+                    unpack2_quiet<DT>(x[i][c], v0, v1);
                     lo = min3(lo, v0, v1);
                     hi = max3(hi, v0, v1);
                 }

@@ -1,11 +1,15 @@
 """The paged 4-bit cache where its rules are easily missed: masks without a position, layers that
 were written but not committed, counts below zero, weights far below the largest,
-values that a causal row does not see."""
+values that a causal row does not see, and groups whose parameters are not ordinary numbers."""
 
 import math
 
 import pytest
 import torch
+
+from maskahead_amd.cache import PackedKVCache
+from maskahead_amd.config import QuantizationConfig
+from maskahead_amd.paged import PagedKVCache
 
 from _paged import Requests, attend64, check_attention, stored
 
@@ -186,3 +190,79 @@ def test_what_a_causal_row_does_not_see_may_be_no_number(gpu, t, hq, causal, wha
                     assert not torch.isfinite(row[:, :5]).any(), (b, i)
                     off = (row[:, 5:].float() - was[:, 5:].float()).abs() - torch.finfo(dtype).eps * was[:, 5:].float().abs()
                     assert off.max() <= 1024 * 2.0 ** -24 * biggest, (b, i)
+
+
+# ------------------------------------------------------------------ quantization
+def _read_back(x, dtype):
+    """Groups x [..., 32] as they are stored and read, NaN passed over (its code is 0), every operation
+    rounded to dtype."""
+    r = lambda y: y.to(dtype).float()  # noqa: E731
+    x = x.float()
+    lo = torch.where(x.isnan(), math.inf, x).amin(-1, keepdim=True)
+    hi = torch.where(x.isnan(), -math.inf, x).amax(-1, keepdim=True)
+    step = r(r(r(hi - lo) / 15).clamp_min(1e-8))
+    code = torch.nan_to_num(r(r(x - lo) / step)).round().clamp(0, 15)
+    return code * step.half().float() + lo.half().float()
+
+
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("dtype", [BF, F16])
+@pytest.mark.parametrize("pieces", [[160], [31, 1, 70, 58]])
+def test_groups_of_any_values_are_stored_as_the_packed_cache_stores_them(gpu, d, dtype, pieces):
+    """Constant, zero and signed-zero groups, infinities, NaN, the type's largest and smallest
+    values: the codes and parameters of the contiguous cache's quantizers, in the first group and
+    in ones that a tail completes.  A signalling NaN is passed over like a quiet one (the contiguous
+    cache's minimum loses numbers beside it): that group against the rule itself."""
+    h, n = 2, 160
+    gen = torch.Generator().manual_seed(d)
+    fine = torch.finfo(dtype)
+    signalling = torch.tensor([0x7F81 if dtype == BF else 0x7C01], dtype=torch.int16).view(dtype)[0]
+
+    def special(x):      # x [..., 32] of ordinary values: one kind of group a row
+        y = x.clone()
+        y[0] = 1.5
+        y[1] = 0.0
+        y[2] = 0.0
+        y[2, ..., ::3] = -0.0
+        y[3, ..., 7] = float("inf")
+        y[4, ..., 9] = float("-inf")
+        y[5, ..., 0], y[5, ..., 31] = float("inf"), float("-inf")
+        y[6, ..., 5] = float("nan")
+        y[7] = float("nan")
+        y[8, ..., 3], y[8, ..., 30] = fine.max, fine.min
+        y[9] = fine.smallest_normal * fine.eps * torch.arange(32).to(dtype)
+        y[10] = 1.0
+        y[10, ..., 4] = 1.0 + fine.eps
+        y[11] = float("inf")
+        y[12, ..., 17] = signalling
+        y[13] = 1e-4
+        y[13, ..., 1] = 1e-4 + 1e-7
+        return y
+
+    k, v = (torch.randn((1, h, n, d), generator=gen).to(dtype) for _ in range(2))
+    for g in (0, 32, 96):
+        # keys: a group is 32 tokens of a channel; values: 32 channels of a token
+        k[0, :, g:g + 32] = special(k[0, :, g:g + 32].permute(2, 0, 1).contiguous()).permute(1, 2, 0)
+        x = v[0, :, g:g + 32].unflatten(-1, (d // 32, 32)).permute(1, 0, 2, 3).contiguous()
+        v[0, :, g:g + 32] = special(x).permute(1, 0, 2, 3).flatten(-2)
+    c = PagedKVCache(num_layers=1, batch_size=1, num_kv_heads=h, head_dim=d, num_pages=6, max_tokens=192, page_tokens=32,
+                     device=gpu, compute_dtype=dtype)
+    f = PackedKVCache(num_layers=1, batch_size=1, num_kv_heads=h, head_dim=d, max_tokens=192,
+                      quant=QuantizationConfig(residual_tokens=0), device=gpu, compute_dtype=dtype)
+    k, v = k.to(gpu), v.to(gpu)
+    f.begin_append(n)
+    f.stage_layer(0, k, v)
+    f.commit_append()
+    at = 0
+    for t in pieces:
+        c.begin_append(torch.tensor([t], dtype=torch.int32, device=gpu), t)
+        c.stage_layer(0, k[:, :, at:at + t], v[:, :, at:at + t])
+        c.commit_append()
+        at += t
+    got, want = c.dequantize_layer(0, n, dtype=torch.float32), f.dequantize_layer(0, dtype=torch.float32)
+    for x, y, src, key in zip(got, want, (k, v), (True, False)):
+        x, y = x.cpu(), y[:, :, :n].cpu()
+        for g in (0, 32, 96):
+            at = (0, slice(None), slice(g, g + 32), 12) if key else (0, slice(None), g + 12)
+            y[at] = _read_back(src[at].cpu().unflatten(-1, (-1, 32)), dtype).flatten(-2)
+        torch.testing.assert_close(x, y, rtol=0, atol=0, equal_nan=True)
