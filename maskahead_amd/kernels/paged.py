@@ -282,7 +282,7 @@ def paged_attention(query: torch.Tensor, prefix: PagedPrefix, current_key: torch
     shape = _check_block("query", query, prefix)
     b, hq, t, d = shape
     h = prefix.heads
-    if hq == 0 or hq % h:
+    if h == 0 or hq == 0 or hq % h:
         raise ValueError("Hq must be a positive multiple of Hkv")
     if (current_key is None) != (current_value is None):
         raise ValueError("current_key and current_value go together")

@@ -9,6 +9,7 @@ import torch
 
 from maskahead_amd.cache import PackedKVCache
 from maskahead_amd.config import QuantizationConfig
+from maskahead_amd.kernels.paged import PagedPrefix, paged_attention
 from maskahead_amd.paged import PagedKVCache
 
 from _paged import Requests, attend64, check_attention, stored
@@ -79,6 +80,15 @@ def test_an_append_of_fewer_than_no_tokens_is_refused(gpu, new):
     c.release(torch.tensor([True, False], device=gpu))
     c.check()
     assert c.lengths.tolist() == [0, 10]
+
+
+def test_a_cache_without_heads_is_refused(gpu):
+    i32 = lambda *x: torch.zeros(x, dtype=torch.int32, device=gpu)  # noqa: E731
+    tail = torch.zeros((2, 0, 32, 64), dtype=BF, device=gpu)
+    p = PagedPrefix(torch.zeros((4, 0, 2, 2560), dtype=torch.uint8, device=gpu), tail, tail, i32(2, 3), i32(2))
+    for heads in (0, 4):
+        with pytest.raises(ValueError, match="Hq"):
+            paged_attention(torch.zeros((2, heads, 1, 64), dtype=BF, device=gpu), p)
 
 
 # ------------------------------------------------------------------ weights
