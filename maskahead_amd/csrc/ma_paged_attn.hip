@@ -33,17 +33,18 @@ typedef __attribute__((ext_vector_type(8))) __bf16 b16x8_t;
 
 constexpr int WAVES = 4;
 // Weights are 2^(score - reference) and become f16, which holds 11 bits from 2^-14 to 2^16 and
-// nothing below 2^-25.  A row's reference therefore follows its items: where the largest weight of
-// an item's 32 tokens (of a lane's 8, as it is looked at) would lie above 2^P_MAX or below 2^P_MIN,
-// the reference is moved to where it is 2^P_NEW (those found below 2^P_LOW then, so that the next
-// items lie well inside); most items leave the accumulators alone.  A weight then carries at most
-// 2^-25 absolute, 2^-17 of the largest of its item, beside f16's 2^-11 relative, however far another
-// item's score is above: with the row's maximum as the only reference, a key that leads by 17 nats and
-// has no value of its own left the others no digits.  Beside such a key, in its own item, what
-// is below 2^-32 of it is lost.  The reference goes down only while the sum stays below P_SUM, which
-// leaves the accumulators 2^67 of room.  The cost of the lower border: one token of 64 requests
-// 52.0 -> 52.4 us, 32 tokens of 8 requests 50.9 -> 52.2, 512 tokens of 2 requests 219.1 -> 219.4.
-constexpr float P_MAX = 15.0f, P_MIN = -8.0f, P_LOW = 0.0f, P_NEW = 7.0f;
+// nothing below 2^-25.  A row's reference therefore follows its items.  It begins where a score of 0
+// weighs 2^P_NEW.  Where the largest weight of an item's 32 tokens (of a lane's 8, as it is looked at)
+// would lie above 2^P_MAX or below 2^P_MIN (of the first item: 2^P_FIRST), the reference is moved to
+// where it is 2^P_NEW (those found below 2^P_LOW then, so that the next items lie well inside).  Most
+// items, and most first ones, leave the reference and the accumulators alone.  A weight then carries
+// at most 2^-25 absolute, 2^-17 of the largest of its item, beside f16's 2^-11 relative, however far
+// another item's score is above: with the row's maximum as the only reference, a key that leads by 17
+// nats and has no value of its own left the others no digits.  Beside such a key, in its own item, what
+// is below 2^-25 of it can be lost.  The reference goes down only while the sum stays below P_SUM, which
+// leaves the accumulators 2^67 of room.  Following costs 32 tokens of 8 requests 51.2 -> 52.7 us, 512
+// tokens of 2 requests 217 -> 222, one token of 64 requests nothing.
+constexpr float P_MAX = 15.0f, P_MIN = -8.0f, P_FIRST = 0.0f, P_LOW = 0.0f, P_NEW = 7.0f;
 constexpr float P_SUM = 0x1p60f;
 constexpr float NO_MAX = -1e30f;
 
@@ -358,28 +359,13 @@ __device__ __forceinline__ uint4 rows_channel(const uint32_t (&vw)[8][D / 32], i
 }
 // A product takes a weight of 0 times a value that is no number to every query row, also to those
 // that do not see it.  So under a causal rule such values of the block are 0 in the products, and are
-// added as they are to the sums (few rows) or to what was written (many) of the rows that see them.
+// added as they are to what was written of the rows that see them (each_odd).
 // Bits 15 and 31 of odd_halves: this half of w is none.
 template <bool BF16>
 __device__ __forceinline__ uint32_t odd_halves(uint32_t w) {
     return ((w & (BF16 ? 0x7f807f80u : 0x7c007c00u)) + (BF16 ? 0x00800080u : 0x04000400u)) & 0x80008000u;
 }
 __device__ __forceinline__ uint32_t without(uint32_t w, uint32_t odd) { return w & ~(odd | (odd - (odd >> 15))); }
-// the elements e .. e + 3 of a value's row, as f32; odd: bit i = element e + i is no number
-template <bool BF16>
-__device__ __forceinline__ f32x4_t odd_of_four(const uint16_t *src, uint32_t &odd) {
-    const uint2 v = pg_load8(src);
-    const uint32_t x = odd_halves<BF16>(v.x), y = odd_halves<BF16>(v.y);
-    odd = (x >> 15 & 1u) | (x >> 30 & 2u) | (y >> 13 & 4u) | (y >> 28 & 8u);
-    f32x4_t r;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        const uint32_t w = i & 2 ? v.y : v.x;
-        const uint16_t e = (uint16_t)(i & 1 ? w >> 16 : w);
-        r[i] = BF16 ? ma_bf16_to_f32(e) : ma_f16_to_f32(e);
-    }
-    return r;
-}
 // how many of the block's keys its position t sees: to the end of its causal block, counted from
 // the request's first token (len + t has 32 bits, its sum with a block has not)
 __device__ __forceinline__ int keys_seen(const AttnArgs &a, const Items &it, int t) {
@@ -405,7 +391,7 @@ __device__ __forceinline__ void clear(Tile<D> &t) {
 #pragma unroll
     for (int ct = 0; ct < D / 16; ++ct) t.acc[ct] = f32x4_t{};
     t.l = f32x4_t{};
-    t.m = NO_MAX;
+    t.m = -P_NEW;
 }
 
 // max of three without the quieting that fmaxf puts before each of its arguments
@@ -419,9 +405,9 @@ __device__ __forceinline__ float max8(const float (&x)[8]) {
 }
 
 // scores s (x c -> exponents of 2) of a lane's 8 tokens -> weights; live (where masked): bit i =
-// token i is seen.  Moves the row's reference where needed.
+// token i is seen.  Moves the row's reference where needed; lo: P_FIRST for the first item, then P_MIN.
 template <int D>
-__device__ __forceinline__ void softmax8(Tile<D> &t, const f32x4_t &s0, const f32x4_t &s1, float c, bool masked,
+__device__ __forceinline__ void softmax8(Tile<D> &t, const f32x4_t &s0, const f32x4_t &s1, float c, float lo, bool masked,
                                          uint32_t live, float (&p)[8]) {
     float x[8];
 #pragma unroll
@@ -432,22 +418,20 @@ __device__ __forceinline__ void softmax8(Tile<D> &t, const f32x4_t &s0, const f3
         for (int i = 0; i < 8; ++i) x[i] = (l >> i) & 1u ? x[i] : -INFINITY;
     }
     const float mx = max8(x);
-    if (__any(fabsf(mx - 0.5f * (P_MAX + P_MIN)) > 0.5f * (P_MAX - P_MIN))) {
-        // (what is done to a row depends on its own scores alone; what is dead stays at -inf)
-        float y[8];
-#pragma unroll
-        for (int i = 0; i < 8; ++i) y[i] = x[i] == -INFINITY ? -INFINITY : (i < 4 ? s0[i & 3] : s1[i & 3]) * c;
-        const float top = max_rows(max8(y)), at = top - t.m;
-        const bool out = at > P_MAX || -max_rows(-mx) < P_MIN;
-        const bool move = out && (at > P_NEW || (at < P_LOW && top > -INFINITY));
-        const float f = __builtin_amdgcn_exp2f(P_NEW - at);
+    if (__any((mx > P_MAX) | (mx < lo))) {
+        // (what is done to a row depends on its own scores alone)
+        const float top = max_rows(mx);
+        const bool out = top > P_MAX || -max_rows(-mx) < lo;
+        const bool move = out && (top > P_NEW || (top < P_LOW && top > -INFINITY));
         if (__any(move)) {
+            const float f = t.l[0] == 0.f ? 0.f : __builtin_amdgcn_exp2f(P_NEW - top);
             const bool fits = move && t.l[0] * f < P_SUM;
             const float g = fits ? f : 1.0f;
 #pragma unroll
             for (int ct = 0; ct < D / 16; ++ct) t.acc[ct] *= g;
             t.l *= g;
-            t.m = fits ? top - P_NEW : t.m;
+            t.m = fits ? t.m + (top - P_NEW) : t.m;
+            // (what is dead stays at -inf, whatever its score)
 #pragma unroll
             for (int i = 0; i < 8; ++i)
                 x[i] = x[i] == -INFINITY ? -INFINITY : __builtin_fmaf(i < 4 ? s0[i & 3] : s1[i & 3], c, -t.m);
@@ -455,6 +439,11 @@ __device__ __forceinline__ void softmax8(Tile<D> &t, const f32x4_t &s0, const f3
     }
 #pragma unroll
     for (int i = 0; i < 8; ++i) p[i] = __builtin_amdgcn_exp2f(x[i]);
+}
+// a row that saw nothing says so, when its sums are to be joined with others'
+template <int D>
+__device__ __forceinline__ void settle(Tile<D> &t) {
+    if (t.l[0] == 0.f) t.m = NO_MAX;
 }
 
 __device__ __forceinline__ f16x8_t as_f16(const float (&p)[8]) {
@@ -491,10 +480,10 @@ __device__ __forceinline__ f32x4_t rows_scores(const uint4 *k, const uint4 *q) {
     return s;
 }
 template <int D, bool BF16>
-__device__ __forceinline__ Probs<BF16> rows_probs(Tile<D> &t, const f32x4_t &s0, const f32x4_t &s1, float c, uint32_t live) {
+__device__ __forceinline__ Probs<BF16> rows_probs(Tile<D> &t, const f32x4_t &s0, const f32x4_t &s1, float c, float lo, uint32_t live) {
     Probs<BF16> r;
     float p[8];
-    softmax8(t, s0, s1, c, true, live, p);
+    softmax8(t, s0, s1, c, lo, true, live, p);
     if constexpr (BF16) {
         b16x8_t one;
 #pragma unroll
@@ -724,28 +713,47 @@ __device__ __forceinline__ void store_out(const AttnArgs &a, int b, int h, int r
     else pg_store8(dst, uint2{y[0], y[1]});
 }
 
-// f(element, value) of every value that is no number, of the block's rows below keys in items [d0, d1)
-// (every step-th), in the lane's channels (D/4) hh + (0 .. D/4 - 1)
-template <int D, bool BF16, class F>
-__device__ __forceinline__ void each_odd(const AttnArgs &a, const Items &it, int b, int h, int d0, int d1, int step, int keys,
-                                         int hh, F f) {
+// f(element, value) of every value that is no number, of channels ch + (0 .. n - 1) of the block's rows
+// below keys in items [d0, d1).  (Rare: loops that are small beside the code around them.)
+template <bool BF16, class F>
+__device__ __forceinline__ void each_odd(const AttnArgs &a, const Items &it, int b, int h, int d0, int d1, int keys, int ch,
+                                         int n, F f) {
 #pragma unroll 1
-    for (int i = d0; i < d1; i += step) {
+    for (int i = d0; i < d1; ++i) {
+        const Rows r = rows_of(a, it, b, h, i - it.ng);
+        const int end = r.tail ? 0 : min(min(r.j0 + PG_GROUP, r.cnt), keys);
+#pragma unroll 1
+        for (int j = r.j0; j < end; ++j)
+#pragma unroll 1
+            for (int e = 0; e < n; ++e) {
+                const uint16_t v = r.v[(int64_t)j * r.sv + ch + e];
+                if (odd_halves<BF16>(v)) f(e, BF16 ? ma_bf16_to_f32(v) : ma_f16_to_f32(v));
+            }
+    }
+}
+// ... added to a tile's sums, of a wave's items d0, d0 + WAVES, ...
+template <int D, bool BF16>
+__device__ __forceinline__ void add_odd(const AttnArgs &a, const Items &it, int b, int h, int d0, int d1, int keys, int hh,
+                                        Tile<D> &t) {
+    constexpr int NC = D / 16;
+#pragma unroll 1
+    for (int i = d0; i < d1; i += WAVES) {
         const Rows r = rows_of(a, it, b, h, i - it.ng);
         const int end = r.tail ? 0 : min(r.j0 + PG_GROUP, r.cnt);
 #pragma unroll 1
-        for (int j = r.j0; j < end; ++j) {
-            const uint16_t *src = r.v + (int64_t)j * r.sv + (D / 4) * hh;
+        for (int j = r.j0; j < end; ++j)
 #pragma unroll
-            for (int e = 0; e < D / 4; e += 4) {
-                uint32_t odd;
-                const f32x4_t v = odd_of_four<BF16>(src + e, odd);
-#pragma unroll
-                for (int y = 0; y < 4; ++y) f(e + y, (odd >> y & 1u) && j < keys, v[y]);
-                __builtin_amdgcn_sched_barrier(0);      // (few registers: none of this is in a hurry)
+            for (int e = 0; e < D / 4; ++e) {
+                const uint16_t v = r.v[(int64_t)j * r.sv + (D / 4) * hh + e];
+                t.acc[e % NC][e / NC] += odd_halves<BF16>(v) && j < keys ? (BF16 ? ma_bf16_to_f32(v) : ma_f16_to_f32(v)) : 0.f;
+                if (e % 4 == 3) __builtin_amdgcn_sched_barrier(0);     // (few registers: none of this is in a hurry)
             }
-        }
     }
+}
+// ... added to an element of out
+template <bool BF16>
+__device__ __forceinline__ void add_to(uint16_t &x, float v) {
+    x = (uint16_t)pack_out<BF16>((BF16 ? ma_bf16_to_f32(x) : ma_f16_to_f32(x)) + v, 0.f);
 }
 
 // ------------------------------------------------------------------ few rows
@@ -804,6 +812,7 @@ __global__ __launch_bounds__(256, 2) void paged_few_kernel(AttnArgs a) {
             c[nt] = (BF16 ? q_as_f16<D>(q[nt]) : 1.f) * a.sl2;
             clear(t[nt]);
         }
+        float lo = P_FIRST;
         for (; i < last; i += WAVES) {
             if (++k == 64) {
                 recs = find_records<D>(a, b, h, i + WAVES, last, lane);
@@ -837,10 +846,11 @@ __global__ __launch_bounds__(256, 2) void paged_few_kernel(AttnArgs a) {
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt) {
                 float p[8];
-                softmax8(t[nt], s0[nt], s1[nt], c[nt], masked, live, p);
+                softmax8(t[nt], s0[nt], s1[nt], c[nt], lo, masked, live, p);
                 pf[nt] = as_f16(p);
                 t[nt].l = mfma16(ones_f16(), pf[nt], t[nt].l);
             }
+            lo = P_MIN;
 #pragma unroll
             for (int ct = 0; ct < NC; ++ct) {
                 const f16x8_t vf = word_values(v_word(rv, ct), rv.s, rv.z);
@@ -873,8 +883,9 @@ __global__ __launch_bounds__(256, 2) void paged_few_kernel(AttnArgs a) {
             Probs<BF16> p[NT];
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt)
-                p[nt] = rows_probs<D, BF16>(t[nt], s[0][nt], s[1][nt], a.sl2,
+                p[nt] = rows_probs<D, BF16>(t[nt], s[0][nt], s[1][nt], a.sl2, lo,
                                             causal_live(r, keys_seen(a, it, (row0 + nt * 16 + (l & 15)) % a.T), lh, seen));
+            lo = P_MIN;
             // (the values' loads stay behind the scores' registers: ahead of them the main loop spilled)
             __builtin_amdgcn_sched_barrier(0);
             uint32_t vw[8][NC / 2];
@@ -884,12 +895,14 @@ __global__ __launch_bounds__(256, 2) void paged_few_kernel(AttnArgs a) {
 #pragma unroll
                 for (int y = 0; y < 8; ++y)
 #pragma unroll
-                    for (int z = 0; z < NC / 2; ++z) {
-                        const uint32_t x = odd_halves<BF16>(vw[y][z]);
-                        any |= x;
-                        vw[y][z] = without(vw[y][z], x);
-                    }
-                odd |= __any(any);
+                    for (int z = 0; z < NC / 2; ++z) any |= odd_halves<BF16>(vw[y][z]);
+                if (__any(any)) {
+                    odd = true;
+#pragma unroll
+                    for (int y = 0; y < 8; ++y)
+#pragma unroll
+                        for (int z = 0; z < NC / 2; ++z) vw[y][z] = without(vw[y][z], odd_halves<BF16>(vw[y][z]));
+                }
             }
 #pragma unroll
             for (int ct = 0; ct < NC; ++ct) {
@@ -900,13 +913,12 @@ __global__ __launch_bounds__(256, 2) void paged_few_kernel(AttnArgs a) {
         }
         if (odd) {
 #pragma unroll
-            for (int nt = 0; nt < NT; ++nt)
-                each_odd<D, BF16>(a, it, b, h, rows_at, pt.i1, WAVES, keys_seen(a, it, (row0 + nt * 16 + n16) % a.T), hh,
-                                  [&](int e, bool yes, float v) { t[nt].acc[e % NC][e / NC] += yes ? v : 0.f; });
+            for (int nt = 0; nt < NT; ++nt) add_odd<D, BF16>(a, it, b, h, rows_at, pt.i1, keys_seen(a, it, (row0 + nt * 16 + n16) % a.T), hh, t[nt]);
         }
         // the waves' parts joined; whole segments written out, cut ones left as a partial
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
+            settle(t[nt]);
             __syncthreads();
             if (hh == 0) {
                 sh.m[wave][n16] = t[nt].m;
@@ -1064,6 +1076,7 @@ __global__ __launch_bounds__(512, 2) void paged_many_kernel(AttnArgs a) {
             c[nt] = (BF16 ? q_as_f16<D>(q[nt]) : 1.f) * a.sl2;
             clear(t[nt]);
         }
+        float lo = P_FIRST;
         for (int x = -1; x < steps; ++x) {
             if (x + 1 < steps) {
                 unpack(x + 1);
@@ -1098,10 +1111,11 @@ __global__ __launch_bounds__(512, 2) void paged_many_kernel(AttnArgs a) {
 #pragma unroll
                 for (int nt = 0; nt < 2; ++nt) {
                     float p[8];
-                    softmax8(t[nt], s0[nt], s1[nt], c[nt], all != 0xffffffffu, live, p);
+                    softmax8(t[nt], s0[nt], s1[nt], c[nt], lo, all != 0xffffffffu, live, p);
                     pf[nt] = as_f16(p);
                     t[nt].l = mfma16(ones_f16(), pf[nt], t[nt].l);
                 }
+                lo = P_MIN;
                 const uint4(*next)[64] = sh.op[x & 1][min(g + TW, STEP - 1)];
 #pragma unroll
                 for (int y = 0; y < 2 * CB; ++y) kf[y] = __builtin_bit_cast(f16x8_t, next[y][lane]);
@@ -1183,7 +1197,8 @@ __global__ __launch_bounds__(512, 2) void paged_many_kernel(AttnArgs a) {
                     Probs<BF16> p[2];
 #pragma unroll
                     for (int nt = 0; nt < 2; ++nt)
-                        p[nt] = rows_probs<D, BF16>(t[nt], s[nt][0], s[nt][1], a.sl2, see[nt]);
+                        p[nt] = rows_probs<D, BF16>(t[nt], s[nt][0], s[nt][1], a.sl2, lo, see[nt]);
+                    lo = P_MIN;
                     __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
                     for (int ct = 0; ct < NC; ++ct) {
@@ -1195,6 +1210,8 @@ __global__ __launch_bounds__(512, 2) void paged_many_kernel(AttnArgs a) {
             }
             __syncthreads();
         }
+        settle(t[0]);
+        settle(t[1]);
         // waves that share rows joined (lane by lane, through the operands' space), then each row
         // tile written out or left as a partial
         if constexpr (TW > 1) {
@@ -1251,12 +1268,6 @@ __global__ __launch_bounds__(512, 2) void paged_many_kernel(AttnArgs a) {
                         for (int ct = 0; ct < NC; ++ct) o[ct] = t[nt].acc[ct][r] * inv;
                         store_out<NC, BF16>(a, b, h, row, NC * (4 * hh + r), o);
                     }
-                    if (odd) {
-                        uint16_t *dst = out_row(a, b, h, row) + (D / 4) * hh;
-                        each_odd<D, BF16>(a, it, b, h, d0, d1, 1, keys_seen(a, it, row % a.T), hh, [&](int e, bool yes, float v) {
-                            if (yes) dst[e] = (uint16_t)pack_out<BF16>((BF16 ? ma_bf16_to_f32(dst[e]) : ma_f16_to_f32(dst[e])) + v, 0.f);
-                        });
-                    }
                 } else {
                     const int64_t slot = (int64_t)pt.slot * (2 * RW * 16);
                     const int rt = rw * 32 + nt * 16 + (hidden(lane) & 15);
@@ -1271,10 +1282,18 @@ __global__ __launch_bounds__(512, 2) void paged_many_kernel(AttnArgs a) {
                         for (int ct = 0; ct < NC; ct += 4)
                             *(f32x4_t *)&dst[(r * (NC / 4) + ct / 4) * 256] =
                                 f32x4_t{t[nt].acc[ct][r], t[nt].acc[ct + 1][r], t[nt].acc[ct + 2][r], t[nt].acc[ct + 3][r]};
-                    if (odd)
-                        each_odd<D, BF16>(a, it, b, h, d0, d1, 1, keys_seen(a, it, row % a.T), hh, [&](int e, bool yes, float v) {
-                            if (yes) dst[(e / 4) * 256 + e % 4] += v;
-                        });
+                }
+            }
+            if (odd) {
+#pragma unroll 1
+                for (int rt = rw * 32 + (lane & 15); rt < rw * 32 + 32; rt += 16) {
+                    const int row = row0 - rw * 32 + rt;
+                    if (row >= a.R || (pt.whole && row % a.T >= it.n)) continue;
+                    float *dst = a.wo + (int64_t)pt.slot * (2 * RW * 16) * D + partial_at<D>(rt, 4 * hh);
+                    each_odd<BF16>(a, it, b, h, d0, d1, keys_seen(a, it, row % a.T), (D / 4) * hh, D / 4, [&](int e, float v) {
+                        if (pt.whole) add_to<BF16>(out_row(a, b, h, row)[(D / 4) * hh + e], v);
+                        else dst[(e / 4) * 256 + e % 4] += v;
+                    });
                 }
             }
         }

@@ -168,6 +168,45 @@ def test_a_leading_key_without_a_value_leaves_the_others_their_digits(gpu, t, wh
     assert rel <= 1, f"a row is {float(rel):.2f} of its 2-norm's bound off"
 
 
+@pytest.mark.parametrize("dtype", [BF, F16])
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("t", [1, 9, 40, 130])
+@pytest.mark.parametrize("offset", [-400, -90, -20, 20, 90, 400])
+def test_scores_far_from_zero(gpu, offset, t, d, dtype):
+    """All of a row's scores lie `offset` nats from zero (a channel that is 7 in every key): the weights
+    are those without the offset.  An exponent of up to 2^10 is rounded to f32 in its product and in its
+    difference to the reference: 2^-13 of a weight; otherwise as above, without a leading key."""
+    h, g, n = 2, 2, 203
+    gen = torch.Generator().manual_seed(t + d)
+    k, v, _ = _led(gen, h, n, d, 0, dtype, None)
+    ck = torch.randint(-8, 8, (h, t, d), generator=gen).to(dtype)
+    cv = torch.randn((h, t, d), generator=gen).to(dtype)
+    k[..., 0], ck[..., 0] = 7.0, 7.0
+    if dtype == F16:
+        v = v / 1000.0
+    q = (torch.round(torch.randn((h * g, t, d), generator=gen) * 8) / 64).to(dtype)
+    q[..., 0] = round(offset * math.sqrt(d) / 7)
+    r = Requests(gpu, [0, 0], h=h, d=d, dtype=dtype, room=n, page=64)
+    rows = lambda x: torch.stack((x, x)).to(gpu)  # noqa: E731
+    r.cache.begin_append(r.i32([n, n]), n)
+    r.cache.stage_layer(0, rows(k), rows(v))
+    r.cache.commit_append()
+    got = r.cache.attend(0, rows(q), rows(ck), rows(cv)).double().cpu()
+    assert torch.equal(stored(k, "k"), k.double())
+    kk = torch.cat((k.double(), ck.double()), 1).repeat_interleave(g, 0)
+    vv = torch.cat((stored(v, "v"), cv.double()), 1).repeat_interleave(g, 0)
+    p = torch.softmax(torch.matmul(q.double(), kk.transpose(1, 2)) * d ** -0.5, -1)
+    want = torch.matmul(p, vv)
+    step = 2.0 ** -11
+    dp = (step + 2.0 ** -13) * p + 2.0 ** -17 * p.amax(-1, keepdim=True)
+    bound = 2 * (torch.matmul(dp + step * p, vv.abs()) + dp.sum(-1, keepdim=True) * want.abs())
+    bound += torch.finfo(dtype).eps / 2 * want.abs() + 2.0 ** -24
+    over = ((got - want).abs() / bound).max()
+    assert over <= 1, f"an element is {float(over):.2f} of its bound off"
+    rel = ((got - want).norm(dim=-1) / want.norm(dim=-1)).max()
+    assert rel <= torch.finfo(dtype).eps / 2 + 3 * step + 2.0 ** -13
+
+
 # ------------------------------------------------------------------ values that are not numbers
 @pytest.mark.parametrize("d,dtype", [(128, BF), (64, F16), (64, BF), (128, F16)])
 @pytest.mark.parametrize("t,hq,causal", [(8, 2, 4), (12, 4, 5), (70, 2, 32), (40, 8, 1), (300, 2, 100)])
