@@ -411,9 +411,10 @@ int ma_page_dequant(const ma_pages *p, int B, int H, int D, const int32_t *start
  * positions: rows t >= new_lens[b] of out stay as they are, keys j >= new_lens[b] are not
  * seen.  causal_block > 0: key j is seen by query t only if (lengths[b] + j) / causal_block <=
  * (lengths[b] + t) / causal_block.  A row that sees nothing is zero; what a row does not see may
- * hold anything, NaN and infinities too.  q, kc, vc, out share
- * p->dtype; D 64 or 128.  workspace: ma_paged_workspace_bytes() bytes, 256-byte aligned; its
- * contents are not read before they are written, and calls that may run at once need one each.
+ * hold anything, NaN and infinities too.  A packed value is an f16: one whose code * scale + zero
+ * passes 65504 is infinite.  q, kc, vc, out share p->dtype; D 64 or 128.  workspace:
+ * ma_paged_workspace_bytes() bytes, 256-byte aligned; its contents are not read before they are
+ * written, and calls that may run at once need one each.
  * The same call gives the same bits (no atomics).  Two launches.  MA_EUNSUPPORTED: B * H * row
  * groups are 2^23 or more (2^24 where a KV head has more than 32 rows), or 2^31 groups of 32 tokens
  * in requests as long as their table rows. */

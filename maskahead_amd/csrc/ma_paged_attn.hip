@@ -41,7 +41,7 @@ constexpr int WAVES = 4;
 // at most 2^-25 absolute, 2^-17 of the largest of its item, beside f16's 2^-11 relative, however far
 // another item's score is above: with the row's maximum as the only reference, a key that leads by 17
 // nats and has no value of its own left the others no digits.  Beside such a key, in its own item, what
-// is below 2^-25 of it can be lost.  The reference goes down only while the sum stays below P_SUM, which
+// is below 2^-25 of it can be lost (2^-17 where all before it was dead).  The reference goes down only while the sum stays below P_SUM, which
 // leaves the accumulators 2^67 of room.  Following costs 32 tokens of 8 requests 51.2 -> 52.7 us, 512
 // tokens of 2 requests 217 -> 222, one token of 64 requests nothing.
 constexpr float P_MAX = 15.0f, P_MIN = -8.0f, P_FIRST = 0.0f, P_LOW = 0.0f, P_NEW = 7.0f;
@@ -763,10 +763,10 @@ __device__ __forceinline__ void add_to(uint16_t &x, float v) {
 // free: keys behind the scores, values behind the second product.
 //
 // bound: 40 D bytes a group and head, once.  One token of 64 requests of 700 to 16 384 tokens
-// (28 query and 4 KV heads, D 128): 208 MB in 52.4 us with the merge, 4.0 TB/s, where a large copy
-// reaches 5.1; 2 requests of 90 000 to 131 072 tokens (32 and 8 heads): 66.8 us, 4.7 TB/s.  Some
+// (28 query and 4 KV heads, D 128): 208 MB in 52.3 us with the merge, 4.0 TB/s, where a large copy
+// reaches 5.1; 2 requests of 90 000 to 131 072 tokens (32 and 8 heads): 66.3 us, 4.7 TB/s.  Some
 // 10 us are no traffic: two launches, the scan, the first record's three loads in a row (length,
-// table, words), the join and the merge (one token after prompts of up to 700 tokens: 13.8 us in
+// table, words), the join and the merge (one token after prompts of up to 700 tokens: 14.0 us in
 // all).  Two records under way a wave were no faster (D 128: 55.2 and 69.0 us).
 // Registers: for the two workgroups a CU that are launched (for three, the 16-bit rows' path spilled:
 // 52.4 -> 80 us).
@@ -983,14 +983,16 @@ __global__ __launch_bounds__(256, 2) void paged_few_kernel(AttnArgs a) {
 // lanes read them (1 KB each, no bank conflicts).
 //
 // bound: the matrix cores, 4 D operations a row and token.  512 new tokens of 2 requests of 6 000
-// to 16 384 tokens (28 query and 4 KV heads, D 128): 205 GFLOP in 217 to 233 us; each 8 192 tokens
+// to 16 384 tokens (28 query and 4 KV heads, D 128): 205 GFLOP in 222 to 239 us; each 8 192 tokens
 // more add 104 us, 1.15 PFLOP/s, where a large library product reaches 1.19.  The rest is start
 // and end: partials of 256 rows (128 KB) written and read again, and 16-bit rows, which are not
-// pipelined (a step of up to four items is 5 us).  32 new tokens of 8 requests: 51 us, of which
+// pipelined (a step of up to four items is 5 us).  32 new tokens of 8 requests: 53 us, of which
 // some 25 are that.  Measured and not kept (chunk, then 251 us): two tiles half an item apart, so
 // that one's exponentials lie under the other's products: 268; 4 tiles a wave and one wave a
 // SIMD: 368 (operands copied between the two register files); the next 16-bit rows under way in
 // registers: 20 % slower, the main loop spilled; a SIMD's two waves unpacking in turn: no gain.
+// Registers: at D 128 all 256 are in use and 5 to 17 spilled.  What lives across the packed loop
+// costs at once: 40 to 60 spilled were 53 -> 61 us (block).
 constexpr int MWAVES = 8, STEP = 4;
 
 // place of row rt's channels (D/16) x + (0 .. 3) in a partial: as the tile's wave holds them,
@@ -1285,6 +1287,7 @@ __global__ __launch_bounds__(512, 2) void paged_many_kernel(AttnArgs a) {
                 }
             }
             if (odd) {
+                asm volatile("" ::: "memory");      // (what the lane just stored is read again as other types)
 #pragma unroll 1
                 for (int rt = rw * 32 + (lane & 15); rt < rw * 32 + 32; rt += 16) {
                     const int row = row0 - rw * 32 + rt;
@@ -1406,7 +1409,8 @@ constexpr int FEW_ROWS0 = 8, MANY_ROWS0 = 4, MANY_DENSE = 1;
 // 512 of 2 requests 220 -> 268), the groups as even as its built 4, 8 and 16 tiles allow.
 // Workgroups: two a CU for few rows (three: 54.0 and 71.4 us where two have 52.5 and 67.6; more
 // than are resident at once: 62 and 78), one for many (their LDS; two in turn: 54 -> 67 and
-// 220 -> 233 us).
+// 220 -> 233 us).  D 64, whose registers and LDS would hold more: few rows 34.4 us with two, 33.4
+// with three or four where 64 requests are read, 17.2, 17.2 and 18.9 where 5 are; many 42 -> 49 us.
 Shape shape_of(int R) {
     const int tiles = (R + 15) / 16, cus = ma_num_cus() / 8 * 8;
     Shape s{};

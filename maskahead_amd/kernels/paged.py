@@ -8,7 +8,8 @@ The reference's cache holds one scalar length for all its batch rows (cache.py:9
 ``splitk_attention`` follows it; here every request has its own, read by the kernels, so a
 step of a ragged batch needs no padding, no host copy of a length and one launch per layer
 and operator.  The codes, scales and zeros are those of the framework's other quantizers
-(``quantize_key_groups_into``, ``quantize_values_into``), bit for bit; they are stored in
+(``quantize_key_groups_into``, ``quantize_values_into``), bit for bit (but beside a signalling
+NaN, which is passed over like any other here); they are stored in
 records of 32 tokens of one KV head in the order in which the matrix instructions read them
 (``csrc/ma_pages.h``).  ``maskahead_amd.paged.PagedKVCache`` keeps the planes of every layer
 and the step protocol; these functions are its kernels.
@@ -276,9 +277,10 @@ def paged_attention(query: torch.Tensor, prefix: PagedPrefix, current_key: torch
     [B] (None: T each) counts each request's real positions: rows t >= new_lens[b] of out are
     left as they are, keys j >= new_lens[b] not seen.  causal_block > 0: key j is seen by query
     t only if (lengths[b] + j) // causal_block <= (lengths[b] + t) // causal_block.  A row that
-    sees nothing is zero; what a row does not see may hold anything, NaN and infinities too.  The
-    same call gives the same bits.  ``out`` [B, Hq, T, D] (not overlapping the inputs) receives the
-    result; without it a new tensor does, whose rows t >= new_lens[b] are undefined."""
+    sees nothing is zero; what a row does not see may hold anything, NaN and infinities too.  A
+    packed value is an f16 here (beyond 65504: infinite).  The same call gives the same bits.
+    ``out`` [B, Hq, T, D] (not overlapping the inputs) receives the result; without it a new
+    tensor does, whose rows t >= new_lens[b] are undefined."""
     shape = _check_block("query", query, prefix)
     b, hq, t, d = shape
     h = prefix.heads

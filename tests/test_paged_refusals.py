@@ -141,3 +141,10 @@ def test_more_segments_than_a_launch_holds_are_refused(lib, heads, t, segments):
     assert lib.ma_paged_attention(_t4(), b, heads, t, 128, p, heads, _t4(ptr=None), _t4(ptr=None), None, 0, 1.0, _t4(),
                                   4096, 1 << 60, None) == N.MA_EUNSUPPORTED
     assert b"segments" in lib.ma_last_error()
+
+
+def test_the_plan_of_an_append_refuses_what_a_plan_does(lib):
+    for page, b, ring, rc in ((33, 2, 4096, N.MA_EINVAL), (64, 0, 4096, N.MA_EINVAL), (64, 2, None, N.MA_EINVAL)):
+        assert lib.ma_page_plan_append(4096, 8192, b, 1, page, 4096, 4, 4, ring, 8, 4096, 4096, 16384, None) == rc
+    assert lib.ma_page_plan_append(4096, 8192, 2, 1, 64, 4096, 4, 4, 4096, 8, 4096, 4096, 4096, None) == N.MA_EINVAL
+    assert b"ma_page_plan_append" in lib.ma_last_error()
