@@ -19,10 +19,11 @@
 // 1024 or 64, subtract, one fused multiply-add by scale and zero: one rounding of 2^-11
 // relative, where a bf16 copy of the cache has 2^-8); scores, maxima, sums and outputs are
 // f32; weights are rounded to f16 (2^-11; their range: P_MAX below) for the second product, and
-// their sum is that of what is multiplied.  Together 3.5e-4 of a result in the 2-norm, beside f16's own 2.1e-4
-// (bf16's 1.6e-3): what the matrix cores' full rate costs.
-// The tail and the block's keys are read as they are: f16 like the above, bf16 in bf16
-// products with the probability as a sum of two bf16 (2^-16).
+// their sum is that of what is multiplied.  Together 3.5e-4 of a result in the 2-norm, where bf16
+// results are rounded by 1.6e-3: what the matrix cores' full rate costs.  f16 results are rounded by
+// 2.1e-4 alone, so for them keys, values and weights are sums of two f16 (2.1e-4 in all; more than 32
+// rows: values are one, whose second half has no room in the LDS at D 128: 3.0e-4).
+// The tail and the block's keys are read as they are, the weight a sum of two of their type.
 #include "ma_pages.h"
 
 using namespace ma;
@@ -130,6 +131,37 @@ __device__ __forceinline__ f16x8_t word_values(uint32_t w, uint4 s, uint4 z) {
         r[2 * k + 1] = v[1];
     }
     return r;
+}
+
+// f16 results: a value in two parts.  Few rows: code * scale with the scale's upper 7 bits and with
+// its lower 4, both exact, the zero being a product of its own.
+__device__ __forceinline__ f16x2_t as_f16x2(uint32_t w) { return __builtin_bit_cast(f16x2_t, w); }
+__device__ __forceinline__ void split_scale(uint4 s, uint4 &hi, uint4 &lo) {
+    hi = uint4{s.x & 0xfff0fff0u, s.y & 0xfff0fff0u, s.z & 0xfff0fff0u, s.w & 0xfff0fff0u};
+    auto rest = [](uint32_t x, uint32_t y) { return __builtin_bit_cast(uint32_t, as_f16x2(x) - as_f16x2(y)); };
+    lo = uint4{rest(s.x, hi.x), rest(s.y, hi.y), rest(s.z, hi.z), rest(s.w, hi.w)};
+}
+__device__ __forceinline__ void word_products(uint32_t w, uint4 s_hi, uint4 s_lo, f16x8_t &hi, f16x8_t &lo) {
+    const uint32_t hw[4] = {s_hi.x, s_hi.y, s_hi.z, s_hi.w}, lw[4] = {s_lo.x, s_lo.y, s_lo.z, s_lo.w};
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+        const f16x2_t c = code_pair(w, k), x = c * as_f16x2(hw[k]), y = c * as_f16x2(lw[k]);
+        hi[2 * k] = x[0], hi[2 * k + 1] = x[1];
+        lo[2 * k] = y[0], lo[2 * k + 1] = y[1];
+    }
+}
+// Many rows: the value rounded, and what the rounding left (product and sum with their errors).
+__device__ __forceinline__ void word_values2(uint32_t w, uint4 s, uint4 z, f16x8_t &hi, f16x8_t &lo) {
+#pragma clang fp contract(off)
+    const uint32_t sw[4] = {s.x, s.y, s.z, s.w}, zw[4] = {z.x, z.y, z.z, z.w};
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+        const f16x2_t c = code_pair(w, k), a = as_f16x2(sw[k]), b = as_f16x2(zw[k]);
+        const f16x2_t x = c * a, dx = __builtin_elementwise_fma(c, a, -x);
+        const f16x2_t v = x + b, y = v - x, dv = (x - (v - y)) + (b - y), r = dv + dx;
+        hi[2 * k] = v[0], hi[2 * k + 1] = v[1];
+        lo[2 * k] = r[0], lo[2 * k + 1] = r[1];
+    }
 }
 
 __device__ __forceinline__ f32x4_t mfma16(f16x8_t a, f16x8_t b, f32x4_t c) {
@@ -383,14 +415,14 @@ __device__ __forceinline__ uint32_t causal_live(const Rows &r, int keys, int hh,
 // component of l, its sum of weights (a product with ones: the sum of what is multiplied)
 template <int D>
 struct Tile {
-    f32x4_t acc[D / 16], l;
+    f32x4_t acc[D / 16], l, z;      // z (f16, few rows): the zeros' part of the lane's channels
     float m;
 };
 template <int D>
 __device__ __forceinline__ void clear(Tile<D> &t) {
 #pragma unroll
     for (int ct = 0; ct < D / 16; ++ct) t.acc[ct] = f32x4_t{};
-    t.l = f32x4_t{};
+    t.l = t.z = f32x4_t{};
     t.m = -P_NEW;
 }
 
@@ -430,6 +462,7 @@ __device__ __forceinline__ void softmax8(Tile<D> &t, const f32x4_t &s0, const f3
 #pragma unroll
             for (int ct = 0; ct < D / 16; ++ct) t.acc[ct] *= g;
             t.l *= g;
+            t.z *= g;
             t.m = fits ? t.m + (top - P_NEW) : t.m;
             // (what is dead stays at -inf, whatever its score)
 #pragma unroll
@@ -459,11 +492,17 @@ __device__ __forceinline__ f16x8_t ones_f16() {
     return r;
 }
 
-// 16-bit rows as they are: f16 like the packed ones, bf16 in bf16 products with each
-// probability as a sum of two bf16
+// weights as a sum of two f16 (22 bits; below 2^-14: the first one's absolute 2^-25)
+__device__ __forceinline__ void as_two_f16(const float (&p)[8], f16x8_t &hi, f16x8_t &lo) {
+    hi = as_f16(p);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) lo[i] = (_Float16)(p[i] - (float)hi[i]);
+}
+
+// 16-bit rows as they are, with each weight as a sum of two of their type
 template <bool BF16>
 struct Probs {
-    f16x8_t p;
+    f16x8_t hi, lo;
 };
 template <>
 struct Probs<true> {
@@ -494,8 +533,8 @@ __device__ __forceinline__ Probs<BF16> rows_probs(Tile<D> &t, const f32x4_t &s0,
         }
         t.l = mfma16(one, r.lo, mfma16(one, r.hi, t.l));
     } else {
-        r.p = as_f16(p);
-        t.l = mfma16(ones_f16(), r.p, t.l);
+        as_two_f16(p, r.hi, r.lo);
+        t.l = mfma16(ones_f16(), r.lo, mfma16(ones_f16(), r.hi, t.l));
     }
     return r;
 }
@@ -504,7 +543,8 @@ __device__ __forceinline__ f32x4_t rows_values(uint4 v, const Probs<true> &p, f3
     return mfma16(x, p.lo, mfma16(x, p.hi, acc));
 }
 __device__ __forceinline__ f32x4_t rows_values(uint4 v, const Probs<false> &p, f32x4_t acc) {
-    return mfma16(__builtin_bit_cast(f16x8_t, v), p.p, acc);
+    const f16x8_t x = __builtin_bit_cast(f16x8_t, v);
+    return mfma16(x, p.lo, mfma16(x, p.hi, acc));
 }
 
 // ---- Q of one row tile as B operands: lane (n, h) = row n, channels (D/4) h + 8 cb + (0..7);
@@ -669,16 +709,16 @@ __device__ __forceinline__ void next_part(const AttnArgs &a, Stretch &st, const 
     while (st.it.items == 0);
 }
 
-// The records of a wave's next 64 packed items, one a lane: items first, first + 4, ... below
+// The records of a wave's next 64 packed items, one a lane: items first, first + EVERY, ... below
 // last of one (request, head).  Looked up at once, so that no item waits for its table entry
 // (a load in the loop also waits for every load before it).  Records are 16-byte aligned: bit 0
 // says that the table names no page, and the address is then the pool's first record.
 struct Records {
     uint32_t lo, hi;
 };
-template <int D>
+template <int D, int EVERY>
 __device__ __forceinline__ Records find_records(const AttnArgs &a, int b, int h, int first, int last, int lane) {
-    const int per = a.p.page_tokens / PG_GROUP, i = first + 4 * lane, pg = i / per;
+    const int per = a.p.page_tokens / PG_GROUP, i = first + EVERY * lane, pg = i / per;
     uint64_t r = (uint64_t)a.p.pool | 1u;
     if (i < last) {
         const uint8_t *rec = pg_record(a.p, a.p.table[(int64_t)b * a.p.s_table + pg], i - pg * per, h, 40 * D);
@@ -768,6 +808,8 @@ __device__ __forceinline__ void add_to(uint16_t &x, float v) {
 // 10 us are no traffic: two launches, the scan, the first record's three loads in a row (length,
 // table, words), the join and the merge (one token after prompts of up to 700 tokens: 14.0 us in
 // all).  Two records under way a wave were no faster (D 128: 55.2 and 69.0 us).
+// f16, whose operands are sums of two: the first two 59.0 and 78.6 us (51.5 and 66 with one rounding
+// each, and twice the error): bound by the instructions that unpack.
 // Registers: for the two workgroups a CU that are launched (for three, the 16-bit rows' path spilled:
 // 52.4 -> 80 us).
 template <int D, int NT>
@@ -798,7 +840,7 @@ __global__ __launch_bounds__(256, 2) void paged_few_kernel(AttnArgs a) {
         for (int nt = 0; nt < NT; ++nt) load_q<D>(a, b, h, row0 + nt * 16 + (hidden(lane) & 15), it.n, hh, q[nt]);
         const int last = min(pt.i1, it.ng);
         int i = pt.i0 + wave, k = 0;
-        Records recs = find_records<D>(a, b, h, i, last, lane);
+        Records recs = find_records<D, WAVES>(a, b, h, i, last, lane);
         RawK<D> rk;
         RawV<D> rv;
         bool dead = false;
@@ -815,7 +857,7 @@ __global__ __launch_bounds__(256, 2) void paged_few_kernel(AttnArgs a) {
         float lo = P_FIRST;
         for (; i < last; i += WAVES) {
             if (++k == 64) {
-                recs = find_records<D>(a, b, h, i + WAVES, last, lane);
+                recs = find_records<D, WAVES>(a, b, h, i + WAVES, last, lane);
                 k = 0;
             }
             // (behind the last one the pool's first record is loaded: no branch around the loads)
@@ -824,15 +866,39 @@ __global__ __launch_bounds__(256, 2) void paged_few_kernel(AttnArgs a) {
             f32x4_t s0[NT], s1[NT];
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt) s0[nt] = s1[nt] = f32x4_t{};
+            if constexpr (BF16) {
 #pragma unroll
-            for (int cb = 0; cb < CB; ++cb) {
-                const f16x8_t k0 = word_values(rk.k[0][cb], rk.s[cb], rk.z[cb]);
-                const f16x8_t k1 = word_values(rk.k[1][cb], rk.s[cb], rk.z[cb]);
+                for (int cb = 0; cb < CB; ++cb) {
+                    const f16x8_t k0 = word_values(rk.k[0][cb], rk.s[cb], rk.z[cb]);
+                    const f16x8_t k1 = word_values(rk.k[1][cb], rk.s[cb], rk.z[cb]);
 #pragma unroll
-                for (int nt = 0; nt < NT; ++nt) {
-                    const f16x8_t qf = __builtin_bit_cast(f16x8_t, q[nt][cb]);
-                    s0[nt] = mfma16(k0, qf, s0[nt]);
-                    s1[nt] = mfma16(k1, qf, s1[nt]);
+                    for (int nt = 0; nt < NT; ++nt) {
+                        const f16x8_t qf = __builtin_bit_cast(f16x8_t, q[nt][cb]);
+                        s0[nt] = mfma16(k0, qf, s0[nt]);
+                        s1[nt] = mfma16(k1, qf, s1[nt]);
+                    }
+                }
+            } else {
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt) {       // (the zeros are those of all 32 tokens)
+#pragma unroll
+                    for (int cb = 0; cb < CB; ++cb)
+                        s0[nt] = mfma16(__builtin_bit_cast(f16x8_t, rk.z[cb]), __builtin_bit_cast(f16x8_t, q[nt][cb]), s0[nt]);
+                    s1[nt] = s0[nt];
+                }
+#pragma unroll
+                for (int cb = 0; cb < CB; ++cb) {
+                    uint4 s_hi, s_lo;
+                    split_scale(rk.s[cb], s_hi, s_lo);
+                    f16x8_t h0, l0, h1, l1;
+                    word_products(rk.k[0][cb], s_hi, s_lo, h0, l0);
+                    word_products(rk.k[1][cb], s_hi, s_lo, h1, l1);
+#pragma unroll
+                    for (int nt = 0; nt < NT; ++nt) {
+                        const f16x8_t qf = __builtin_bit_cast(f16x8_t, q[nt][cb]);
+                        s0[nt] = mfma16(l0, qf, mfma16(h0, qf, s0[nt]));
+                        s1[nt] = mfma16(l1, qf, mfma16(h1, qf, s1[nt]));
+                    }
                 }
             }
             load_k(rk, next, lane);
@@ -842,23 +908,47 @@ __global__ __launch_bounds__(256, 2) void paged_few_kernel(AttnArgs a) {
                 if (MASK) live &= mask_bits(a.p, b, h, i * PG_GROUP + 8 * (hidden(lane) >> 4));
                 clear_dead(rv, live);
             }
-            f16x8_t pf[NT];
+            f16x8_t pf[NT], pl[NT];
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt) {
                 float p[8];
                 softmax8(t[nt], s0[nt], s1[nt], c[nt], lo, masked, live, p);
-                pf[nt] = as_f16(p);
+                if constexpr (BF16) pf[nt] = as_f16(p);
+                else as_two_f16(p, pf[nt], pl[nt]);
                 t[nt].l = mfma16(ones_f16(), pf[nt], t[nt].l);
+                if constexpr (!BF16) t[nt].l = mfma16(ones_f16(), pl[nt], t[nt].l);
             }
             lo = P_MIN;
+            if constexpr (BF16) {
 #pragma unroll
-            for (int ct = 0; ct < NC; ++ct) {
-                const f16x8_t vf = word_values(v_word(rv, ct), rv.s, rv.z);
+                for (int ct = 0; ct < NC; ++ct) {
+                    const f16x8_t vf = word_values(v_word(rv, ct), rv.s, rv.z);
 #pragma unroll
-                for (int nt = 0; nt < NT; ++nt) t[nt].acc[ct] = mfma16(vf, pf[nt], t[nt].acc[ct]);
+                    for (int nt = 0; nt < NT; ++nt) t[nt].acc[ct] = mfma16(vf, pf[nt], t[nt].acc[ct]);
+                }
+            } else {
+                const f16x8_t z = __builtin_bit_cast(f16x8_t, rv.z);
+                uint4 s_hi, s_lo;
+                split_scale(rv.s, s_hi, s_lo);
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt) t[nt].z = mfma16(z, pl[nt], mfma16(z, pf[nt], t[nt].z));
+#pragma unroll
+                for (int ct = 0; ct < NC; ++ct) {
+                    f16x8_t vh, vl;
+                    word_products(v_word(rv, ct), s_hi, s_lo, vh, vl);
+#pragma unroll
+                    for (int nt = 0; nt < NT; ++nt)
+                        t[nt].acc[ct] = mfma16(vl, pf[nt], mfma16(vh, pl[nt], mfma16(vh, pf[nt], t[nt].acc[ct])));
+                }
             }
             load_v(rv, next, lane);
             dead = dead_next;
+        }
+        if constexpr (!BF16) {
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                for (int ct = 0; ct < NC; ++ct) t[nt].acc[ct] += t[nt].z;
         }
         // the tail and the block's own keys
         bool odd = false;
@@ -991,9 +1081,12 @@ __global__ __launch_bounds__(256, 2) void paged_few_kernel(AttnArgs a) {
 // that one's exponentials lie under the other's products: 268; 4 tiles a wave and one wave a
 // SIMD: 368 (operands copied between the two register files); the next 16-bit rows under way in
 // registers: 20 % slower, the main loop spilled; a SIMD's two waves unpacking in turn: no gain.
-// Registers: at D 128 all 256 are in use and 5 to 17 spilled.  What lives across the packed loop
+// f16: twice the products and 3 items a step, 32 new tokens of 8 requests 85.6 us (49.8 with one
+// rounding each, and twice the error).
+// Registers: at D 128 all 256 are in use and 4 to 17 spilled.  What lives across the packed loop
 // costs at once: 40 to 60 spilled were 53 -> 61 us (block).
-constexpr int MWAVES = 8, STEP = 4;
+constexpr int MWAVES = 8;
+constexpr int step_of(int D, bool BF16) { return D == 128 && !BF16 ? 3 : 4; }      // (what the LDS holds twice)
 
 // place of row rt's channels (D/16) x + (0 .. 3) in a partial: as the tile's wave holds them,
 // [tile][channels mod 4][4 channels] of 64 lanes' 16 bytes
@@ -1002,9 +1095,10 @@ __device__ __forceinline__ int partial_at(int rt, int x) {
     return ((rt >> 4) * (D / 16) + (x & 3) * (D / 64)) * 256 + ((x >> 2) * 16 + (rt & 15)) * 4;
 }
 
-template <int D>
+template <int D, bool BF16>
 struct ManyShared {
-    static constexpr int OPS = 2 * (D / 32) + D / 16;     // operands of an item: K [2][D/32], V [D/16]
+    // operands of an item: K [2][D/32], V [D/16], and what rounding left of K (f16)
+    static constexpr int OPS = 2 * (D / 32) + D / 16 + (BF16 ? 0 : 2 * (D / 32)), STEP = step_of(D, BF16);
     uint4 op[2][STEP][OPS][64];
     uint32_t live[2][STEP];                               // bit j: the item's token j is seen
     uint32_t odd[2][STEP];                                // one of the item's values is no number (causal calls)
@@ -1013,12 +1107,12 @@ struct ManyShared {
 
 template <int D, int RW, bool BF16, bool MASK>
 __global__ __launch_bounds__(512, 2) void paged_many_kernel(AttnArgs a) {
-    constexpr int CB = D / 32, NC = D / 16, TW = MWAVES / RW;
+    constexpr int CB = D / 32, NC = D / 16, TW = MWAVES / RW, STEP = step_of(D, BF16), LEFT = 2 * CB + NC;
     extern __shared__ __attribute__((aligned(16))) char lds[];
-    ManyShared<D> &sh = *(ManyShared<D> *)lds;
+    ManyShared<D, BF16> &sh = *(ManyShared<D, BF16> *)lds;
     const int tid = threadIdx.x, lane = tid & 63, wave = uniform(tid >> 6), hh = lane >> 4;
     const int rw = wave % RW, tw = wave / RW;
-    const int si = wave >> 1;              // the item of a step that this wave unpacks
+    const int si = wave >> 1;              // the item of a step that this wave unpacks (STEP and more: none)
     const bool sv = wave & 1;              // its values (else its keys)
     Stretch st = find_stretch<512>(a, sh.scan, STEP);
     int pos = st.s;
@@ -1048,19 +1142,29 @@ __global__ __launch_bounds__(512, 2) void paged_many_kernel(AttnArgs a) {
         Records recs;
         // the words of step x's item of this wave (behind the last one: of the pool's first record)
         auto fetch = [&](int x) {
-            if (x % 64 == 0) recs = find_records<D>(a, b, h, pt.i0 + x * STEP + si, last, lane);
+            if (si >= STEP) return;
+            if (x % 64 == 0) recs = find_records<D, STEP>(a, b, h, pt.i0 + x * STEP + si, last, lane);
             const rec_t rec = record_at(recs, x % 64, dead);
             load_either(raw, rec, lane, sv, poff);
         };
         // ... as operands in buffer x & 1
         auto unpack = [&](int x) {
+            if (si >= STEP) return;
             uint4(*op)[64] = sh.op[x & 1][si];
             if (!sv) {
 #pragma unroll
                 for (int mt = 0; mt < 2; ++mt)
 #pragma unroll
-                    for (int cb = 0; cb < CB; ++cb)
-                        op[mt * CB + cb][lane] = __builtin_bit_cast(uint4, word_values(raw.k[mt][cb], raw.s[cb], raw.z[cb]));
+                    for (int cb = 0; cb < CB; ++cb) {
+                        if constexpr (BF16) {
+                            op[mt * CB + cb][lane] = __builtin_bit_cast(uint4, word_values(raw.k[mt][cb], raw.s[cb], raw.z[cb]));
+                        } else {
+                            f16x8_t hi, left;
+                            word_values2(raw.k[mt][cb], raw.s[cb], raw.z[cb], hi, left);
+                            op[mt * CB + cb][lane] = __builtin_bit_cast(uint4, hi);
+                            op[LEFT + mt * CB + cb][lane] = __builtin_bit_cast(uint4, left);
+                        }
+                    }
             } else {
                 uint32_t live = dead ? 0u : 255u;
                 RawV<D> rv = v_from(raw);
@@ -1104,18 +1208,30 @@ __global__ __launch_bounds__(512, 2) void paged_many_kernel(AttnArgs a) {
                         s0[nt] = mfma16(kf[cb], qf, s0[nt]);
                         s1[nt] = mfma16(kf[CB + cb], qf, s1[nt]);
                     }
+                    if constexpr (!BF16) {
+                        const f16x8_t l0 = __builtin_bit_cast(f16x8_t, op[LEFT + cb][lane]);
+                        const f16x8_t l1 = __builtin_bit_cast(f16x8_t, op[LEFT + CB + cb][lane]);
+#pragma unroll
+                        for (int nt = 0; nt < 2; ++nt) {
+                            const f16x8_t qf = __builtin_bit_cast(f16x8_t, q[nt][cb]);
+                            s0[nt] = mfma16(l0, qf, s0[nt]);
+                            s1[nt] = mfma16(l1, qf, s1[nt]);
+                        }
+                    }
                 }
                 // the values' operands come while the scores become probabilities
                 f16x8_t vf[NC];
 #pragma unroll
                 for (int ct = 0; ct < NC; ++ct) vf[ct] = __builtin_bit_cast(f16x8_t, op[2 * CB + ct][lane]);
-                f16x8_t pf[2];
+                f16x8_t pf[2], pl[2];
 #pragma unroll
                 for (int nt = 0; nt < 2; ++nt) {
                     float p[8];
                     softmax8(t[nt], s0[nt], s1[nt], c[nt], lo, all != 0xffffffffu, live, p);
-                    pf[nt] = as_f16(p);
+                    if constexpr (BF16) pf[nt] = as_f16(p);
+                    else as_two_f16(p, pf[nt], pl[nt]);
                     t[nt].l = mfma16(ones_f16(), pf[nt], t[nt].l);
+                    if constexpr (!BF16) t[nt].l = mfma16(ones_f16(), pl[nt], t[nt].l);
                 }
                 lo = P_MIN;
                 const uint4(*next)[64] = sh.op[x & 1][min(g + TW, STEP - 1)];
@@ -1124,7 +1240,10 @@ __global__ __launch_bounds__(512, 2) void paged_many_kernel(AttnArgs a) {
 #pragma unroll
                 for (int ct = 0; ct < NC; ++ct)
 #pragma unroll
-                    for (int nt = 0; nt < 2; ++nt) t[nt].acc[ct] = mfma16(vf[ct], pf[nt], t[nt].acc[ct]);
+                    for (int nt = 0; nt < 2; ++nt) {
+                        t[nt].acc[ct] = mfma16(vf[ct], pf[nt], t[nt].acc[ct]);
+                        if constexpr (!BF16) t[nt].acc[ct] = mfma16(vf[ct], pl[nt], t[nt].acc[ct]);
+                    }
             }
             __syncthreads();
         }
@@ -1147,7 +1266,7 @@ __global__ __launch_bounds__(512, 2) void paged_many_kernel(AttnArgs a) {
             }
             for (int i = d0, x = 0; i < d1; i += STEP, ++x) {
                 uint32_t any = 0;
-                if (i + si < d1) {
+                if (si < STEP && i + si < d1) {
                     const Rows r = rows_of(a, it, b, h, i + si - it.ng);
                     uint4(*op)[64] = sh.op[x & 1][si];
                     if (!sv) {
@@ -1174,12 +1293,17 @@ __global__ __launch_bounds__(512, 2) void paged_many_kernel(AttnArgs a) {
                         note_live(x, live);
                     }
                 }
-                if (a.causal > 0 && sv) {
+                if (a.causal > 0 && sv && si < STEP) {
                     const bool o = __any(any);
                     if (l == 0) sh.odd[x & 1][si] = o;
                 }
                 __syncthreads();
-                if (a.causal > 0) odd |= uniform((int)(sh.odd[x & 1][0] | sh.odd[x & 1][1] | sh.odd[x & 1][2] | sh.odd[x & 1][3]));
+                if (a.causal > 0) {
+                    uint32_t o = 0;
+#pragma unroll
+                    for (int y = 0; y < STEP; ++y) o |= sh.odd[x & 1][y];
+                    odd |= uniform((int)o);
+                }
                 const int g1 = busy ? min(d1 - i, STEP) : 0;
                 for (int g = tw; g < g1; g += TW) {
                     const Rows r = rows_of(a, it, b, h, i + g - it.ng);
@@ -1450,7 +1574,7 @@ Layout layout_of(const Shape &s, int64_t segments, int D) {
 
 template <int D, int RW, bool BF16, bool MASK>
 int launch_many(const AttnArgs &a, hipStream_t st) {
-    constexpr int LDS = (int)sizeof(ManyShared<D>);
+    constexpr int LDS = (int)sizeof(ManyShared<D, BF16>);
     static_assert(LDS <= 160 * 1024, "two steps of operands in one CU's LDS");
     if (LDS > 64 * 1024) {
         const hipError_t e = hipFuncSetAttribute((const void *)paged_many_kernel<D, RW, BF16, MASK>,

@@ -207,6 +207,27 @@ def test_scores_far_from_zero(gpu, offset, t, d, dtype):
     assert rel <= torch.finfo(dtype).eps / 2 + 3 * step + 2.0 ** -13
 
 
+@pytest.mark.parametrize("t,hq,most", [(1, 4, 1.1), (1, 14, 1.1), (8, 8, 1.1), (12, 14, 1.5), (40, 8, 1.5), (130, 4, 1.5)])
+@pytest.mark.parametrize("d", [64, 128])
+def test_f16_results_have_f16s_digits(gpu, t, hq, most, d):
+    """The error in the 2-norm, beside what rounding the exact result to f16 leaves.  Up to 32 rows keys,
+    values and weights are products and sums of two f16 each, exact to 2^-18 of a weight or value:
+    nothing beside the result's own rounding (a tenth is allowed).  More rows round each value
+    once: as much again, independent of it, is a factor of 2^(1/2)."""
+    lens = [0, 700, 333, 64]
+    r = Requests(gpu, lens, h=2, d=d, dtype=F16, room=t)
+    q = (1.5 * torch.randn((4, hq, t, d), generator=r.gen)).to(F16)
+    k, v = r.block([t] * 4, t)
+    got = r.cache.attend(0, q.to(gpu), k.to(gpu), v.to(gpu)).double().cpu()
+    off = rounded = 0.0
+    for b, n in enumerate(lens):
+        want, _ = attend64(q[b], *r.kv64(b), k[b], v[b], seen=torch.ones((2, n), dtype=torch.bool))
+        if n:
+            off += float((got[b] - want).norm() ** 2)
+            rounded += float((want.half().double() - want).norm() ** 2)
+    assert off ** 0.5 <= most * rounded ** 0.5, (off / rounded) ** 0.5
+
+
 # ------------------------------------------------------------------ values that are not numbers
 @pytest.mark.parametrize("d,dtype", [(128, BF), (64, F16), (64, BF), (128, F16)])
 @pytest.mark.parametrize("t,hq,causal", [(8, 2, 4), (12, 4, 5), (70, 2, 32), (40, 8, 1), (300, 2, 100)])
