@@ -228,6 +228,30 @@ def test_f16_results_have_f16s_digits(gpu, t, hq, most, d):
     assert off ** 0.5 <= most * rounded ** 0.5, (off / rounded) ** 0.5
 
 
+@pytest.mark.parametrize("scale_k,scale_v", [(2e-5, 1.0), (1e-3, 1e-4), (30.0, 1000.0), (2000.0, 6000.0), (1.0, 3e-6)])
+@pytest.mark.parametrize("t,hq,most", [(1, 8, 1.1), (40, 4, 1.5)])
+@pytest.mark.parametrize("d", [64, 128])
+def test_f16_digits_of_large_and_small_values(gpu, t, hq, most, d, scale_k, scale_v):
+    """Keys and values from the subnormal ones to a range of f16's largest (beyond it the cache stores
+    no numbers), the scores ordinary: as above, and half of f16's least step beside."""
+    h, n = 2, 500
+    gen = torch.Generator().manual_seed(d)
+    k, ck = ((torch.randn((h, x, d), generator=gen) * scale_k).to(F16) for x in (n, t))
+    v, cv = ((torch.randn((h, x, d), generator=gen) * scale_v).to(F16) for x in (n, t))
+    q = torch.randn((hq, t, d), generator=gen).to(F16)
+    r = Requests(gpu, [0], h=h, d=d, dtype=F16, room=n, page=64)
+    one = lambda x: x[None].to(gpu)  # noqa: E731
+    r.cache.begin_append(r.i32([n]), n)
+    r.cache.stage_layer(0, one(k), one(v))
+    r.cache.commit_append()
+    scale = d ** -0.5 / scale_k
+    got = r.cache.attend(0, one(q), one(ck), one(cv), scaling=scale)[0].double().cpu()
+    want, _ = attend64(q, stored(k, "k"), stored(v, "v"), ck, cv, seen=torch.ones((h, n), dtype=torch.bool), scale=scale)
+    assert torch.isfinite(got).all()
+    least = math.sqrt(want.numel()) * 2.0 ** -25
+    assert float((got - want).norm()) <= most * float((want.half().double() - want).norm()) + least
+
+
 # ------------------------------------------------------------------ values that are not numbers
 @pytest.mark.parametrize("d,dtype", [(128, BF), (64, F16), (64, BF), (128, F16)])
 @pytest.mark.parametrize("t,hq,causal", [(8, 2, 4), (12, 4, 5), (70, 2, 32), (40, 8, 1), (300, 2, 100)])
