@@ -400,6 +400,33 @@ int ma_page_plan_append(const int32_t *lengths, const int32_t *new_lens, int B, 
  * ma_page_dequant): B or H > 65535. */
 int ma_page_append(const ma_pages *p, ma_tensor4 k, ma_tensor4 v, int B, int H, int T, int D,
                    const int32_t *new_lens, const int64_t *slots, void *stream);
+/* The rotation of rows at their positions (no counterpart in the reference, whose models rotate
+ * before they call its cache): pairs of channels (i, i + dim/2), or (2 i, 2 i + 1) where interleaved,
+ * of the first dim turn by x' = x c - y s, y' = y c + x s in f32, each operation rounded, then once to
+ * the type; the other channels stay.
+ *   table  [rows, dim] f32, cosines then sines of a position's dim/2 angles; row stride s_row, rows
+ *          16-byte aligned, dim a multiple of 16
+ *   first  [B] i32, the position of every request's new token 0, or NULL: the lengths
+ * Positions outside the table take its nearest row. */
+typedef struct ma_rotary {
+    const float *table;
+    const int32_t *first;
+    int64_t s_row;
+    int32_t rows, dim, interleaved, reserved;
+} ma_rotary;
+/* q [B, Hq, T, D] and k [B, Hk, T, D] (Hk 0: none) rotated into q_out and k_out, which may be q and k
+ * themselves (but must not overlap them otherwise): token t of request b at position lengths[b] + t (or
+ * r->first's).  All share one dtype of bf16 and f16; D 64 or 128.  One launch.  MA_EUNSUPPORTED: B >
+ * 65535, or more than 65535 groups of 4 heads. */
+int ma_rotate_block(ma_tensor4 q, int Hq, ma_tensor4 q_out, ma_tensor4 k, int Hk, ma_tensor4 k_out, int B, int T, int D,
+                    const int32_t *lengths, const ma_rotary *r, void *stream);
+/* ma_page_append whose keys are rotated on the way (codes, scales, zeros and tail rows are those of
+ * ma_rotate_block's keys, bit for bit), and in the same launch all T rows of q [B, Hq, T, D] (Hq 0:
+ * none) rotated into q_out as ma_rotate_block does.  k is not written.  MA_EUNSUPPORTED also: H and the
+ * groups of 4 query heads are more than 65535. */
+int ma_page_append_rotary(const ma_pages *p, ma_tensor4 k, ma_tensor4 v, int B, int H, int T, int D,
+                          const int32_t *new_lens, const int64_t *slots, const ma_rotary *r, ma_tensor4 q, int Hq,
+                          ma_tensor4 q_out, void *stream);
 /* Tokens starts[b] .. starts[b] + n of every request (starts NULL: from 0) as k_out, v_out
  * [B, H, n, D] in bf16, f16 or f32 (f32(code) * f32(scale) + f32(zero), rounded once), zero
  * from lengths[b] on. */

@@ -58,6 +58,12 @@ class MaPages(ctypes.Structure):
     ]
 
 
+class MaRotary(ctypes.Structure):
+    _fields_ = [("table", ctypes.c_void_p), ("first", ctypes.c_void_p), ("s_row", ctypes.c_int64),
+                ("rows", ctypes.c_int32), ("dim", ctypes.c_int32), ("interleaved", ctypes.c_int32),
+                ("reserved", ctypes.c_int32)]
+
+
 _P = ctypes.c_void_p
 _I = ctypes.c_int
 _I64 = ctypes.c_int64
@@ -65,6 +71,7 @@ _F = ctypes.c_float
 _PREF = ctypes.POINTER(MaPrefix)
 _T4 = MaTensor4
 _PAGES = ctypes.POINTER(MaPages)
+_ROT = ctypes.POINTER(MaRotary)
 _I64P = ctypes.POINTER(ctypes.c_int64)
 
 # name -> (restype, argtypes); must match include/maskahead_hip.h
@@ -113,6 +120,8 @@ SIGNATURES = {
     "ma_page_plan": (_I, [_P, _P, _I, _I, _I, _P, _I64, _I, _P, _I, _P, _P, _P, _P]),
     "ma_page_plan_append": (_I, [_P, _P, _I, _I, _I, _P, _I64, _I, _P, _I, _P, _P, _P, _P]),
     "ma_page_append": (_I, [_PAGES, _T4, _T4, _I, _I, _I, _I, _P, _P, _P]),
+    "ma_rotate_block": (_I, [_T4, _I, _T4, _T4, _I, _T4, _I, _I, _I, _P, _ROT, _P]),
+    "ma_page_append_rotary": (_I, [_PAGES, _T4, _T4, _I, _I, _I, _I, _P, _P, _ROT, _T4, _I, _T4, _P]),
     "ma_page_dequant": (_I, [_PAGES, _I, _I, _I, _P, _I, _T4, _T4, _P]),
     "ma_paged_workspace_bytes": (_I64, [_I, _I, _I, _I, _I]),
     "ma_paged_attention": (_I, [_T4, _I, _I, _I, _I, _PAGES, _I, _T4, _T4, _P, _I, _F, _T4, _P, _I64, _P]),

@@ -3,6 +3,7 @@
 // is in ma_pages.h.
 #include "ma_pages.h"
 #include "ma_quant.h"
+#include "ma_rotary.h"
 
 using namespace ma;
 
@@ -212,6 +213,10 @@ struct AppendArgs {
     const int32_t *new_lens;
     const int64_t *slots;
     int T;
+    // an append that rotates: its keys, and the rows of q beside them
+    int H;
+    RotaryDev rot;
+    RotaryRows q;
 };
 
 template <int DT>
@@ -285,9 +290,43 @@ __device__ __forceinline__ uint32_t f16x2_bits(float a, float b) {
     return __builtin_bit_cast(uint32_t, v);
 }
 
-template <int D, int DT>
+// A keys wave's rows of 4 channels, turned at their positions: row i is new token t0 + i (below 0: a
+// row of the old tail, turned when it was new).  The partners of channels i lie dim / 8 lanes on.
+template <int D, int DT, int N>
+__device__ __forceinline__ void turn_rows(const RotaryDev &r, int first, int t0, int lane, uint2 (&x)[N]) {
+    constexpr int CL = D / 4;
+    const int c4 = lane % CL, q = r.dim / 8, ch = 4 * c4;
+    const bool turned = ch < r.dim, ahead = c4 >= q;
+    const int partner = turned && !r.next ? (ahead ? lane - q : lane + q) : lane;
+    const int at = !turned ? 0 : r.next ? 2 * c4 : ahead ? ch - 4 * q : ch;
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+        const float *row = rotary_row(r, first, max(t0 + i, 0)) + at;
+        uint2 y;
+        if (r.next) {
+            typedef __attribute__((ext_vector_type(2))) float f32x2_t;
+            const f32x2_t c = *(const f32x2_t *)row, s = *(const f32x2_t *)(row + r.dim / 2);
+            y = uint2{rotary_pair<DT>(x[i].x, c[0], s[0]), rotary_pair<DT>(x[i].y, c[1], s[1])};
+        } else {
+            const f32x4_t c = *(const f32x4_t *)row, s = *(const f32x4_t *)(row + r.dim / 2);
+            const uint2 z = {(uint32_t)__shfl((int)x[i].x, partner), (uint32_t)__shfl((int)x[i].y, partner)};
+            y = uint2{rotary_halves<DT>(x[i].x, z.x, c[0], c[1], s[0], s[1], ahead),
+                      rotary_halves<DT>(x[i].y, z.y, c[2], c[3], s[2], s[3], ahead)};
+        }
+        if (turned && t0 + i >= 0) x[i] = y;
+    }
+}
+
+template <int D, int DT, bool ROT>
 __global__ __launch_bounds__(256) void page_append_kernel(AppendArgs a) {
     constexpr int NC = D / 16, CL = D / 4, SL = 64 / CL, TPL = PG_GROUP / SL;   // CL lanes a row, SL slices of the tokens
+    if (ROT && (int)blockIdx.y >= a.H) {      // 64 rows of 4 query heads
+        constexpr int U = D / 16;
+        const int first = a.rot.first[blockIdx.z];
+        for (int t = 64 * blockIdx.x + threadIdx.x / U, y = 0; y < U / 4; ++y, t += 256 / U)
+            if (t < a.T) rotary_heads<D, DT>(a.rot, a.q, first, blockIdx.z, (blockIdx.y - a.H) * ROTARY_HEADS, t, threadIdx.x % U);
+        return;
+    }
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int u = blockIdx.x * 2 + (wave >> 1), h = blockIdx.y, b = blockIdx.z;
     const bool val = wave & 1;
@@ -328,6 +367,7 @@ __global__ __launch_bounds__(256) void page_append_kernel(AppendArgs a) {
             const int c4 = lane % CL, sl = lane / CL, odd = c4 & 1;
             uint2 x[TPL];
             rows(sl * TPL, TPL, 4 * c4, [&](int i, const uint16_t *src) { x[i] = pg_load8(src); });
+            if constexpr (ROT) turn_rows<D, DT>(a.rot, a.rot.first[b], j0 + sl * TPL, lane, x);
             float lo[4], hi[4];
 #pragma unroll
             for (int c = 0; c < 4; ++c) lo[c] = INFINITY, hi[c] = -INFINITY;
@@ -451,11 +491,36 @@ tail_rows:
     // the tail: new tokens behind the last whole group (in front of them, where none was
     // completed, the tail's own rows stay); its old rows were read above, by this wave alone
     const int first = whole ? 0 : r, j0 = whole ? whole * PG_GROUP - r : 0, cnt = n - j0;
+    if (ROT && !val) {
+        constexpr int U = D / 16;
+        const RotaryRows x{fresh + (int64_t)j0 * st, tail + (int64_t)first * a.p.s_tt, 0, 0, st, 0, 0, a.p.s_tt, 1};
+        const int pos = (int)min((int64_t)a.rot.first[b] + j0, (int64_t)INT32_MAX);
+        for (int i = lane; i < cnt * U; i += 64) rotary_heads<D, DT>(a.rot, x, pos, 0, 0, i / U, i % U);
+        return;
+    }
     constexpr int CH = D / 8;           // 16-byte chunks of a row
     for (int x = lane; x < cnt * CH; x += 64) {
         const int rw = x / CH, c = x % CH;
         pg_store16(tail + (int64_t)(first + rw) * a.p.s_tt + 8 * c, pg_load16(fresh + (int64_t)(j0 + rw) * st + 8 * c));
     }
+}
+
+// ------------------------------------------------------------------ rotation alone
+// A thread: 16 channels of one token of 4 heads (rotary_heads); blockIdx.y: 4 heads of q, then of k.
+struct RotateArgs {
+    RotaryDev r;
+    RotaryRows q, k;
+    int T, qgroups;
+};
+template <int D, int DT>
+__global__ __launch_bounds__(256) void rotate_kernel(RotateArgs a) {
+    constexpr int U = D / 16;
+    const int64_t t = ((int64_t)blockIdx.x * blockDim.x + threadIdx.x) / U;
+    if (t >= a.T) return;
+    const int g = blockIdx.y, b = blockIdx.z;
+    const bool key = g >= a.qgroups;
+    rotary_heads<D, DT>(a.r, key ? a.k : a.q, a.r.first[b], b, (key ? g - a.qgroups : g) * ROTARY_HEADS, (int)t,
+                        threadIdx.x % U);
 }
 
 // ------------------------------------------------------------------ read-back
@@ -691,9 +756,68 @@ extern "C" int ma_page_plan_append(const int32_t *lengths, const int32_t *new_le
                      num_pages, state, slots, ends, stream);
 }
 
-extern "C" int ma_page_append(const ma_pages *p, ma_tensor4 k, ma_tensor4 v, int B, int H, int T, int D,
-                              const int32_t *new_lens, const int64_t *slots, void *stream) {
-    const char *who = "ma_page_append";
+static int rotary_check(const ma_rotary *r, int D, const char *who) {
+    if (!r || !r->table || r->rows <= 0 || r->dim <= 0 || r->dim > D || r->dim % 16) {
+        ma_set_error("%s: bad rotary table (rows=%d dim=%d, a multiple of 16 up to %d)", who, r ? r->rows : 0,
+                     r ? r->dim : 0, D);
+        return MA_EINVAL;
+    }
+    if ((uintptr_t)r->table % 16 || r->s_row % 4) {
+        ma_set_error("%s: the rotary table's rows must be 16-byte aligned", who);
+        return MA_EINVAL;
+    }
+    return MA_OK;
+}
+
+static RotaryRows rotary_rows(const ma_tensor4 &in, const ma_tensor4 &out, int heads) {
+    return RotaryRows{(const uint16_t *)in.ptr, (uint16_t *)out.ptr, in.s[0], in.s[1], in.s[2],
+                      out.s[0], out.s[1], out.s[2], heads};
+}
+
+extern "C" int ma_rotate_block(ma_tensor4 q, int Hq, ma_tensor4 q_out, ma_tensor4 k, int Hk, ma_tensor4 k_out, int B,
+                               int T, int D, const int32_t *lengths, const ma_rotary *r, void *stream) {
+    const char *who = "ma_rotate_block";
+    if (B <= 0 || T <= 0 || Hq <= 0 || Hk < 0 || no_data(q) || no_data(q_out) || (Hk && (no_data(k) || no_data(k_out)))) {
+        ma_set_error("%s: bad arguments (B=%d T=%d Hq=%d Hk=%d, or a NULL tensor)", who, B, T, Hq, Hk);
+        return MA_EINVAL;
+    }
+    if (D != 64 && D != 128) {
+        ma_set_error("%s: head_dim %d is not built (64, 128)", who, D);
+        return MA_EUNSUPPORTED;
+    }
+    if (int rc = rotary_check(r, D, who)) return rc;
+    if (!lengths && !r->first) {
+        ma_set_error("%s: neither lengths nor positions", who);
+        return MA_EINVAL;
+    }
+    if (q.dtype != MA_BF16 && q.dtype != MA_F16) {
+        ma_set_error("%s: rows must be bf16 or f16", who);
+        return MA_EUNSUPPORTED;
+    }
+    if (q_out.dtype != q.dtype || (Hk && (k.dtype != q.dtype || k_out.dtype != q.dtype))) {
+        ma_set_error("%s: queries, keys and outputs must share one dtype", who);
+        return MA_EINVAL;
+    }
+    const int64_t qg = ((int64_t)Hq + ROTARY_HEADS - 1) / ROTARY_HEADS, kg = ((int64_t)Hk + ROTARY_HEADS - 1) / ROTARY_HEADS;
+    const int64_t threads = (int64_t)T * (D / 16);
+    if (B > 65535 || qg + kg > 65535) {
+        ma_set_error("%s: more than 65535 requests or groups of %d heads are not built", who, ROTARY_HEADS);
+        return MA_EUNSUPPORTED;
+    }
+    const RotateArgs a{rotary_dev(r, lengths), rotary_rows(q, q_out, Hq), rotary_rows(k, k_out, Hk), T, (int)qg};
+    const int wg = threads <= 64 ? 64 : 256;
+    const dim3 grid((unsigned)((threads + wg - 1) / wg), (unsigned)(qg + kg), B);
+    hipStream_t st = (hipStream_t)stream;
+    if (D == 128 && q.dtype == MA_BF16) rotate_kernel<128, MA_BF16><<<grid, wg, 0, st>>>(a);
+    else if (D == 128) rotate_kernel<128, MA_F16><<<grid, wg, 0, st>>>(a);
+    else if (q.dtype == MA_BF16) rotate_kernel<64, MA_BF16><<<grid, wg, 0, st>>>(a);
+    else rotate_kernel<64, MA_F16><<<grid, wg, 0, st>>>(a);
+    return ma_check_launch(who);
+}
+
+static int page_append(const char *who, const ma_pages *p, const ma_tensor4 &k, const ma_tensor4 &v, int B, int H, int T,
+                       int D, const int32_t *new_lens, const int64_t *slots, const ma_rotary *r, const ma_tensor4 &q, int Hq,
+                       const ma_tensor4 &q_out, void *stream) {
     if (int rc = pg_check(p, B, H, D, who)) return rc;
     if (T <= 0 || no_data(k) || no_data(v) || !new_lens || !slots) {
         ma_set_error("%s: bad arguments (T=%d, or a NULL tensor)", who, T);
@@ -703,21 +827,58 @@ extern "C" int ma_page_append(const ma_pages *p, ma_tensor4 k, ma_tensor4 v, int
         ma_set_error("%s: new tokens and tails must share one dtype", who);
         return MA_EINVAL;
     }
+    if (r) {
+        if (int rc = rotary_check(r, D, who)) return rc;
+        if (Hq < 0 || (Hq && (no_data(q) || no_data(q_out)))) {
+            ma_set_error("%s: bad queries (Hq=%d, or a NULL tensor)", who, Hq);
+            return MA_EINVAL;
+        }
+        if (Hq && (q.dtype != p->dtype || q_out.dtype != p->dtype)) {
+            ma_set_error("%s: queries and tails must share one dtype", who);
+            return MA_EINVAL;
+        }
+    }
     const int64_t units = ((int64_t)T + PG_GROUP - 1) / PG_GROUP;
-    if (B > 65535 || H > 65535) {
+    const int64_t heads = H + ((int64_t)Hq + ROTARY_HEADS - 1) / ROTARY_HEADS;
+    if (B > 65535 || heads > 65535) {
         ma_set_error("%s: more than 65535 requests or heads are not built", who);
         return MA_EUNSUPPORTED;
     }
     AppendArgs a{pages_dev(p), (const uint16_t *)k.ptr, (const uint16_t *)v.ptr, k.s[0], k.s[1], k.s[2], v.s[0],
-                 v.s[1], v.s[2], new_lens, slots, T};
+                 v.s[1], v.s[2], new_lens, slots, T, H, {}, {}};
     // (31 + T) / 32 groups can become whole, one at least writes the tail; two groups a workgroup
-    const dim3 grid((unsigned)((units + 1) / 2), H, B);
+    const dim3 grid((unsigned)((units + 1) / 2), (unsigned)heads, B);
     hipStream_t st = (hipStream_t)stream;
-    if (D == 128 && p->dtype == MA_BF16) page_append_kernel<128, MA_BF16><<<grid, 256, 0, st>>>(a);
-    else if (D == 128) page_append_kernel<128, MA_F16><<<grid, 256, 0, st>>>(a);
-    else if (p->dtype == MA_BF16) page_append_kernel<64, MA_BF16><<<grid, 256, 0, st>>>(a);
-    else page_append_kernel<64, MA_F16><<<grid, 256, 0, st>>>(a);
+    if (r) {
+        a.rot = rotary_dev(r, p->lengths);
+        a.q = rotary_rows(q, q_out, Hq);
+        if (D == 128 && p->dtype == MA_BF16) page_append_kernel<128, MA_BF16, true><<<grid, 256, 0, st>>>(a);
+        else if (D == 128) page_append_kernel<128, MA_F16, true><<<grid, 256, 0, st>>>(a);
+        else if (p->dtype == MA_BF16) page_append_kernel<64, MA_BF16, true><<<grid, 256, 0, st>>>(a);
+        else page_append_kernel<64, MA_F16, true><<<grid, 256, 0, st>>>(a);
+        return ma_check_launch(who);
+    }
+    if (D == 128 && p->dtype == MA_BF16) page_append_kernel<128, MA_BF16, false><<<grid, 256, 0, st>>>(a);
+    else if (D == 128) page_append_kernel<128, MA_F16, false><<<grid, 256, 0, st>>>(a);
+    else if (p->dtype == MA_BF16) page_append_kernel<64, MA_BF16, false><<<grid, 256, 0, st>>>(a);
+    else page_append_kernel<64, MA_F16, false><<<grid, 256, 0, st>>>(a);
     return ma_check_launch(who);
+}
+
+extern "C" int ma_page_append(const ma_pages *p, ma_tensor4 k, ma_tensor4 v, int B, int H, int T, int D,
+                              const int32_t *new_lens, const int64_t *slots, void *stream) {
+    return page_append("ma_page_append", p, k, v, B, H, T, D, new_lens, slots, nullptr, {}, 0, {}, stream);
+}
+
+extern "C" int ma_page_append_rotary(const ma_pages *p, ma_tensor4 k, ma_tensor4 v, int B, int H, int T, int D,
+                                     const int32_t *new_lens, const int64_t *slots, const ma_rotary *r, ma_tensor4 q,
+                                     int Hq, ma_tensor4 q_out, void *stream) {
+    const char *who = "ma_page_append_rotary";
+    if (!r) {
+        ma_set_error("%s: no rotary table", who);
+        return MA_EINVAL;
+    }
+    return page_append(who, p, k, v, B, H, T, D, new_lens, slots, r, q, Hq, q_out, stream);
 }
 
 extern "C" int ma_page_dequant(const ma_pages *p, int B, int H, int D, const int32_t *starts, int n, ma_tensor4 k_out,

@@ -19,6 +19,8 @@ All calls run on the current stream of their tensors' device and return without 
 
 from __future__ import annotations
 
+import struct
+
 import torch
 
 from .. import _native as N
@@ -218,13 +220,98 @@ def _check_block(name: str, t: torch.Tensor, prefix: PagedPrefix, heads: int | N
     return s
 
 
+def rotary_table(positions: int, head_dim: int, *, base: float = 10000.0, rotary_dim: int | None = None,
+                 inv_freq: torch.Tensor | None = None, device: torch.device | str = "cuda") -> torch.Tensor:
+    """The f32 [positions, rotary_dim] table of ``rotate_block`` and ``append_pages``: row p holds
+    the cosines, then the sines, of p * inv_freq (default: base ** (-2 i / rotary_dim), i = 0 ..
+    rotary_dim / 2 - 1), angles and functions in 64 bits.  rotary_dim: a multiple of 16 up to
+    head_dim, its default.  Made once; a program keeps it for all layers and steps."""
+    positions, dim = _c_int("positions", positions), int(head_dim if rotary_dim is None else rotary_dim)
+    if positions == 0 or dim <= 0 or dim > head_dim or dim % 16:
+        raise ValueError(f"a rotary table needs a position and a multiple of 16 up to {head_dim} channels, got "
+                         f"{positions} and {dim}")
+    if inv_freq is None:
+        inv_freq = base ** (-torch.arange(0, dim, 2, dtype=torch.float64, device=device) / dim)
+    elif tuple(inv_freq.shape) != (dim // 2,):
+        raise ValueError(f"inv_freq must be [{dim // 2}], got {tuple(inv_freq.shape)}")
+    at = torch.arange(positions, dtype=torch.float64, device=device)
+    angle = at[:, None] * inv_freq.to(device=device, dtype=torch.float64)[None]
+    return torch.cat((angle.cos(), angle.sin()), 1).float()
+
+
+_ROTARY_PACK = struct.Struct("=QQqiiii").pack
+
+
+def _rotary(prefix: PagedPrefix, table: torch.Tensor, interleaved: bool, positions: torch.Tensor | None) -> N.MaRotary:
+    """The kernels' descriptor of a rotary table (positions None: the prefix's lengths)."""
+    s = table.shape
+    if len(s) != 2 or table.dtype is not torch.float32 or not s[0] or not 0 < s[1] <= prefix.head_dim or s[1] % 16 or \
+            table.stride(1) != 1:
+        raise ValueError(f"rotary must be a float32 [positions, channels] tensor with contiguous rows of a multiple of 16 "
+                         f"up to {prefix.head_dim} channels, got {table.dtype} {tuple(s)}")
+    if table.get_device() != prefix.index:
+        N.require_gpu(table, "rotary")
+        raise ValueError(f"rotary is on {table.device}, expected {prefix.device}")
+    if positions is not None:
+        _i32(positions, "positions", (prefix.batch,), prefix.index)
+    return N.MaRotary.from_buffer_copy(_ROTARY_PACK(
+        table.data_ptr(), 0 if positions is None else positions.data_ptr(), table.stride(0) if s[0] > 1 else s[1],
+        _c_int("rotary's positions", s[0]), s[1], bool(interleaved), 0))
+
+
+def _check_rows(name: str, t: torch.Tensor, prefix: PagedPrefix, out: torch.Tensor | None) -> torch.Tensor:
+    """The output of rotated rows t [B, H, T, D]: `out`, or a new tensor."""
+    shape = _check_block(name, t, prefix)
+    if out is None:
+        return torch.empty(shape, device=t.device, dtype=t.dtype)
+    if _check_block(f"out_{name}", out, prefix, shape[1]) != shape:
+        raise ValueError(f"out_{name} must be {tuple(shape)}")
+    return out
+
+
+def rotate_block(prefix: PagedPrefix, query: torch.Tensor, key: torch.Tensor | None = None, *, rotary: torch.Tensor,
+                 interleaved: bool = False, positions: torch.Tensor | None = None,
+                 out_query: torch.Tensor | None = None, out_key: torch.Tensor | None = None):
+    """query [B, Hq, T, D] and key [B, Hk, T, D] (or None) rotated at their positions: position t of
+    request b is prefix.lengths[b] + t (positions int32 [B]: positions[b] + t).  Returns (query, key).
+
+    rotary is a ``rotary_table``; channels i and i + rotary_dim / 2 are a pair (interleaved: 2 i
+    and 2 i + 1), channels from rotary_dim on stay as they are.  x' = x cos - y sin, y' = y cos + x
+    sin, each operation rounded to f32, the result once to its type.  Positions outside the table
+    take its nearest row.  All T rows are rotated.  out_query may be query, out_key key; otherwise
+    they must not overlap them."""
+    out_query = _check_rows("query", query, prefix, out_query)
+    if key is None and out_key is not None:
+        raise ValueError("out_key without a key")
+    if key is not None:
+        out_key = _check_rows("key", key, prefix, out_key)
+        if key.shape[2] != query.shape[2]:
+            raise ValueError(f"key must hold {query.shape[2]} positions like the queries")
+    rot = _rotary(prefix, rotary, interleaved, positions)
+    b, hq, t, d = query.shape
+    hk = 0 if key is None else key.shape[1]
+    if hq == 0 and hk:      # (the kernel wants rows in its first place)
+        rotate_block(prefix, key, None, rotary=rotary, interleaved=interleaved, positions=positions, out_query=out_key)
+    elif b and t and hq:
+        _call(prefix.index, "ma_rotate_block", N.t4(query), hq, N.t4(out_query), N.t4(key if hk else None), hk,
+              N.t4(out_key if hk else None), b, t, d, prefix.lengths.data_ptr(), rot)
+    return out_query, out_key
+
+
 def append_pages(prefix: PagedPrefix, key: torch.Tensor, value: torch.Tensor, new_lens: torch.Tensor,
-                 slots: torch.Tensor) -> None:
+                 slots: torch.Tensor, *, rotary: torch.Tensor | None = None, interleaved: bool = False,
+                 positions: torch.Tensor | None = None, query: torch.Tensor | None = None,
+                 out_query: torch.Tensor | None = None) -> torch.Tensor | None:
     """Store new_lens[b] (0 .. T) tokens of key, value [B, Hkv, T, D] behind request b's
     prefix.lengths[b] tokens: every 32-token group that they complete is quantized into the
     page that ``slots`` (``plan_pages``) names, the rest stays in the tail at 16 bits.
     prefix.lengths is not written: it is to become plan_pages' ends when every layer has been
-    appended to.  Requests without new tokens, or whose slots are -1, are left as they are."""
+    appended to.  Requests without new tokens, or whose slots are -1, are left as they are.
+
+    rotary (a ``rotary_table``): the keys are rotated at their positions on the way; what is stored
+    is what ``rotate_block`` and an append of its result would store, bit for bit, and key is not
+    written.  interleaved, positions: as there.  With query [B, Hq, T, D] the same launch rotates all
+    its rows, and they are returned (in out_query, if given, which may be query)."""
     shape = _check_block("key", key, prefix, prefix.heads)
     if _check_block("value", value, prefix, prefix.heads) != shape:
         raise ValueError("key and value shapes differ")
@@ -234,10 +321,25 @@ def append_pages(prefix: PagedPrefix, key: torch.Tensor, value: torch.Tensor, ne
         raise ValueError(f"slots must be a contiguous int64 [{b}, {t}] tensor")
     if slots.get_device() != prefix.index:
         raise ValueError(f"slots is on {slots.device}, expected {prefix.device}")
-    if b == 0 or t == 0:
-        return
-    _call(prefix.index, "ma_page_append", prefix._nat, N.t4(key), N.t4(value), b, h, t, d, new_lens.data_ptr(),
-          slots.data_ptr())
+    if rotary is None:
+        if query is not None or out_query is not None or positions is not None:
+            raise ValueError("query, out_query and positions need a rotary table")
+        if b and t:
+            _call(prefix.index, "ma_page_append", prefix._nat, N.t4(key), N.t4(value), b, h, t, d, new_lens.data_ptr(),
+                  slots.data_ptr())
+        return None
+    rot, hq = _rotary(prefix, rotary, interleaved, positions), 0
+    if query is not None:
+        out_query = _check_rows("query", query, prefix, out_query)
+        hq = query.shape[1]
+        if query.shape[2] != t:
+            raise ValueError(f"query must hold {t} positions like the keys")
+    elif out_query is not None:
+        raise ValueError("out_query without a query")
+    if b and t:
+        _call(prefix.index, "ma_page_append_rotary", prefix._nat, N.t4(key), N.t4(value), b, h, t, d, new_lens.data_ptr(),
+              slots.data_ptr(), rot, N.t4(query if hq else None), hq, N.t4(out_query if hq else None))
+    return out_query
 
 
 def dequantize_pages(prefix: PagedPrefix, tokens: int, *, starts: torch.Tensor | None = None,
@@ -312,4 +414,4 @@ def paged_attention(query: torch.Tensor, prefix: PagedPrefix, current_key: torch
 
 
 __all__ = ["PagedPrefix", "append_pages", "check_plan", "dequantize_pages", "paged_attention", "plan_pages",
-           "record_bytes"]
+           "record_bytes", "rotary_table", "rotate_block"]

@@ -16,6 +16,12 @@ tokens, bit for bit: whole groups of 32 are 4-bit, the newest length % 32 tokens
         cache.stage_layer(layer, k, v)
     cache.commit_append()
     cache.release(finished)                                # bool [B]: their pages go back
+
+Queries and keys that are not rotated yet: ``rotate`` before ``attend``, or, where a step is one
+token of every request, on the way into the pages:
+
+    q = cache.stage_layer(layer, k, v, rotary=table, query=q)
+    out = cache.attend(layer, q, staged=True)              # the new token among the stored ones
 """
 
 from __future__ import annotations
@@ -24,7 +30,7 @@ import torch
 
 from ._native import KernelUnavailableError
 from .kernels.paged import (GROUP, PagedPrefix, append_pages, check_plan, dequantize_pages, paged_attention,
-                            plan_pages, record_bytes)
+                            plan_pages, record_bytes, rotate_block)
 
 
 class PagedKVCache:
@@ -63,23 +69,35 @@ class PagedKVCache:
         self.free_ring = torch.arange(num_pages, device=dev, dtype=torch.int32)
         self.ring_state = torch.tensor([0, num_pages, 0, 0], device=dev, dtype=torch.int32)
         self.prefixes = [self.prefix(i) for i in range(num_layers)]
+        self._ends = torch.zeros_like(self.lengths)     # lengths of the append in progress
+        self._after = [self.prefix(i, staged=True) for i in range(num_layers)]
         self._plan: tuple | None = None     # (new_lens, slots, ends, staged layers) of an append in progress
 
     def _check_layer(self, layer: int) -> None:
         if not 0 <= layer < self.num_layers:
             raise IndexError(layer)
 
-    def prefix(self, layer: int, *, mask: torch.Tensor | None = None) -> PagedPrefix:
-        """The kernels' descriptor of one layer, with an optional mask of dead entries."""
+    def prefix(self, layer: int, *, mask: torch.Tensor | None = None, staged: bool = False) -> PagedPrefix:
+        """The kernels' descriptor of one layer, with an optional mask of dead entries; staged: as
+        it is once the append in progress has staged it, new tokens included."""
         self._check_layer(layer)
-        return PagedPrefix(self.pool[layer], self.k_tail[layer], self.v_tail[layer], self.block_table, self.lengths,
-                           mask=mask)
+        return PagedPrefix(self.pool[layer], self.k_tail[layer], self.v_tail[layer], self.block_table,
+                           self._ends if staged else self.lengths, mask=mask)
 
-    def _check_readable(self, layer: int) -> None:
+    def _check_readable(self, layer: int, staged: bool = False) -> None:
         """A staged layer's tail holds the new tokens while lengths are still the old ones."""
         self._check_layer(layer)
-        if self._plan is not None and layer in self._plan[3]:
+        is_staged = self._plan is not None and layer in self._plan[3]
+        if is_staged and not staged:
             raise RuntimeError(f"layer {layer} was staged: it can be read again after commit_append")
+        if staged and not is_staged:
+            raise RuntimeError(f"layer {layer} was not staged by an append in progress")
+
+    def _readable(self, layer: int, mask: torch.Tensor | None, staged: bool) -> PagedPrefix:
+        self._check_readable(layer, staged)
+        if mask is not None:
+            return self.prefix(layer, mask=mask, staged=staged)
+        return (self._after if staged else self.prefixes)[layer]
 
     @property
     def append_in_progress(self) -> bool:
@@ -96,21 +114,31 @@ class PagedKVCache:
         if tokens <= 0:
             raise ValueError("tokens must be positive")
         slots, ends = plan_pages(self.lengths, new_lens, self.block_table, self.free_ring, self.ring_state,
-                                 page_tokens=self.page_tokens, tokens=tokens, give_back=False)
+                                 page_tokens=self.page_tokens, tokens=tokens, ends=self._ends, give_back=False)
         self._plan = (new_lens, slots, ends, set())
         return slots
 
-    def stage_layer(self, layer: int, key: torch.Tensor, value: torch.Tensor) -> None:
+    def rotate(self, query: torch.Tensor, key: torch.Tensor | None = None, *, rotary: torch.Tensor,
+               interleaved: bool = False, positions: torch.Tensor | None = None):
+        """``rotate_block`` of a block behind the stored tokens: (query, key), for ``attend``."""
+        return rotate_block(self.prefixes[0], query, key, rotary=rotary, interleaved=interleaved, positions=positions)
+
+    def stage_layer(self, layer: int, key: torch.Tensor, value: torch.Tensor, *, rotary: torch.Tensor | None = None,
+                    interleaved: bool = False, positions: torch.Tensor | None = None,
+                    query: torch.Tensor | None = None) -> torch.Tensor | None:
         """Write one layer's new tokens, key and value [B, Hkv, T, D] (rows behind a request's
-        new_lens are not read).  The layer is not read again before the commit."""
+        new_lens are not stored).  Before the commit the layer is read with staged=True alone.
+        rotary: the keys are rotated on the way, and query, which is returned (``append_pages``)."""
         if self._plan is None:
             raise RuntimeError("begin_append must be called before stage_layer")
         new_lens, slots, _, staged = self._plan
         if layer in staged:
             raise RuntimeError(f"layer {layer} was staged twice")
         self._check_layer(layer)
-        append_pages(self.prefixes[layer], key, value, new_lens, slots)
+        query = append_pages(self.prefixes[layer], key, value, new_lens, slots, rotary=rotary, interleaved=interleaved,
+                             positions=positions, query=query)
         staged.add(layer)
+        return query
 
     def commit_append(self) -> None:
         """Take the new lengths, when every layer has been staged."""
@@ -152,13 +180,18 @@ class PagedKVCache:
     def attend(self, layer: int, query: torch.Tensor, current_key: torch.Tensor | None = None,
                current_value: torch.Tensor | None = None, *, new_lens: torch.Tensor | None = None,
                scaling: float | None = None, causal_block: int = 0, mask: torch.Tensor | None = None,
-               out: torch.Tensor | None = None) -> torch.Tensor:
+               out: torch.Tensor | None = None, staged: bool = False) -> torch.Tensor:
         """``paged_attention`` of one layer over [stored | block]; new_lens defaults to that of
-        the append in progress.  RuntimeError between a layer's stage_layer and the commit."""
+        the append in progress.  RuntimeError between a layer's stage_layer and the commit.
+
+        staged=True, between the two: over what is stored by then, where every query sees all
+        the new tokens (so without current_key, current_value and causal_block).  A group of 32 that
+        they completed is read from its 4 bits."""
         if new_lens is None and self._plan is not None:
             new_lens = self._plan[0]
-        self._check_readable(layer)
-        prefix = self.prefixes[layer] if mask is None else self.prefix(layer, mask=mask)
+        if staged and (current_key is not None or current_value is not None or causal_block):
+            raise ValueError("a staged layer holds the block: no current_key, current_value or causal_block")
+        prefix = self._readable(layer, mask, staged)
         return paged_attention(query, prefix, current_key, current_value, new_lens=new_lens, scaling=scaling,
                                causal_block=causal_block, out=out)
 

@@ -171,3 +171,21 @@ class Requests:
 
     def kv64(self, b):
         return stored(self.k[b], "k"), stored(self.v[b], "v")
+
+
+def rotated(x, table, first, interleaved, add=False):
+    """x [B, H, T, D] with token t of row b turned by row first[b] + t of the table (the nearest one
+    there is), in the table's type, then in x's; add: |x c| + |y s| in the places of the results."""
+    rd = table.shape[1]
+    out = x.clone()
+    for b, f in enumerate(first):
+        pos = [min(max(f + t, 0), table.shape[0] - 1) for t in range(x.shape[2])]
+        c, s = table[pos][:, :rd // 2], table[pos][:, rd // 2:]
+        f = x[b, ..., :rd].to(table.dtype)
+        u, w = (f[..., 0::2], f[..., 1::2]) if interleaved else (f[..., :rd // 2], f[..., rd // 2:])
+        p, r = u * c, w * s
+        q, z = w * c, u * s
+        u, w = (p + r if add else p - r), q + z
+        y = torch.stack((u, w), -1).flatten(-2) if interleaved else torch.cat((u, w), -1)
+        out[b, ..., :rd] = y.to(x.dtype)
+    return out
