@@ -450,6 +450,28 @@ int ma_paged_attention(ma_tensor4 q, int B, int Hq, int T, int D, const ma_pages
                        ma_tensor4 vc, const int32_t *new_lens, int causal_block, float scale, ma_tensor4 out,
                        void *workspace, int64_t workspace_bytes, void *stream);
 
+/* The blocks of block_tokens (a multiple of 32) stored tokens that a run of query_block positions
+ * (0: all T) should read, of every request, KV head and run: blocks [B, H, runs, count] i32, ascending,
+ * -1 behind the last, runs = ceil(T / query_block).  Block i holds tokens i block_tokens ... of the
+ * request's whole groups of 32 (the tail is in none).  No counterpart in the reference, whose selection
+ * scores every key (splitk.py:582-614).
+ * A block's score is the largest, over its groups and the run's rows (positions t < new_lens[b], new_lens
+ * NULL: all, of the KV head's Hq / H query heads), of sum q_c zero_c + max(q_c, 0) 15 scale_c over a
+ * group's key parameters: what q k can be at most.  Queries and parameters are taken as whole numbers
+ * times a power of two (the row's, the group's largest in [2^13, 2^14); that power is at least 2^-100
+ * and 2^-24), so a score does not depend on an order of sums; it is rounded once to f32, and at
+ * least -FLT_MAX.  A row or group with infinities or NaN scores +inf.  The count largest are taken, ties
+ * to the lowest index; before them keep_first blocks from the start and keep_last to the end (together at
+ * most count).  No block: those all of whose groups lie in no page, or have no live token in p->mask.
+ * scores [B, H, runs, nb] f32, or NULL: every block's, -inf where there is none; nb = ceil(width *
+ * page_tokens / block_tokens).  workspace: ma_select_workspace_bytes(B, H, runs, width * page_tokens)
+ * bytes, 256-byte aligned, written before it is read; calls that may run at once need one each.  Two
+ * launches.  MA_EUNSUPPORTED: 2^31 selections, or 2^27 rows of a selection. */
+int64_t ma_select_workspace_bytes(int B, int H, int runs, int64_t tokens);
+int ma_select_blocks(ma_tensor4 q, int B, int Hq, int T, int D, const ma_pages *p, int H, const int32_t *new_lens,
+                     int query_block, int block_tokens, int count, int keep_first, int keep_last, int32_t *blocks,
+                     float *scores, void *workspace, int64_t workspace_bytes, void *stream);
+
 #ifdef __cplusplus
 }
 #endif

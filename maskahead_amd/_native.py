@@ -123,6 +123,8 @@ SIGNATURES = {
     "ma_rotate_block": (_I, [_T4, _I, _T4, _T4, _I, _T4, _I, _I, _I, _P, _ROT, _P]),
     "ma_page_append_rotary": (_I, [_PAGES, _T4, _T4, _I, _I, _I, _I, _P, _P, _ROT, _T4, _I, _T4, _P]),
     "ma_page_dequant": (_I, [_PAGES, _I, _I, _I, _P, _I, _T4, _T4, _P]),
+    "ma_select_workspace_bytes": (_I64, [_I, _I, _I, _I64]),
+    "ma_select_blocks": (_I, [_T4, _I, _I, _I, _I, _PAGES, _I, _P, _I, _I, _I, _I, _I, _P, _P, _P, _I64, _P]),
     "ma_paged_workspace_bytes": (_I64, [_I, _I, _I, _I, _I]),
     "ma_paged_attention": (_I, [_T4, _I, _I, _I, _I, _PAGES, _I, _T4, _T4, _P, _I, _F, _T4, _P, _I64, _P]),
 }

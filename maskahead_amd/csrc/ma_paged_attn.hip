@@ -293,28 +293,6 @@ __device__ __forceinline__ void clear_dead(RawV<D> &w, uint32_t live) {
     w.z = uint4{w.z.x & h0, w.z.y & h1, w.z.z & h2, w.z.w & h3};
 }
 
-// the nonzero bytes of x, as 4 bits
-__device__ __forceinline__ uint32_t byte_bits(uint32_t x) {
-    x |= x >> 4;
-    x |= x >> 2;
-    x |= x >> 1;
-    return ((x & 0x01010101u) * 0x10204080u) >> 28;
-}
-// the seen ones of a lane's 8 tokens from position pos on, of a request with a mask
-__device__ __forceinline__ uint32_t mask_bits(const PagesDev &p, int b, int h, int pos) {
-    const uint8_t *m = p.mask + (int64_t)b * p.s_mb + (int64_t)h * p.s_mh;
-    const int n = p.mask_tokens;
-    if (n >= 8) {     // 8 bytes that the mask has, moved to where they belong
-        const int at = min(pos, n - 8), out = min(pos - at, 8);
-        const pg_b8 v = *(const pg_b8 *)(m + (uint32_t)at);
-        return (byte_bits(v.x) | byte_bits(v.y) << 4) >> out;
-    }
-    uint32_t bits = 0;
-    for (int i = 0; i < 8; ++i)
-        if (pos + i < n && m[pos + i]) bits |= 1u << i;
-    return bits;
-}
-
 // ---- rows of 16-bit K and V (the tail, or 32 keys of the block) as operands
 struct Rows {
     const uint16_t *k, *v;
@@ -346,7 +324,7 @@ __device__ __forceinline__ Rows rows_of(const AttnArgs &a, const Items &it, int 
 template <bool MASK>
 __device__ __forceinline__ uint32_t rows_live(const AttnArgs &a, const Items &it, const Rows &r, int b, int h, int hh) {
     uint32_t seen = 255u >> min(max(r.j0 + 8 * hh + 8 - r.cnt, 0), 8);
-    if (MASK && r.tail) seen &= mask_bits(a.p, b, h, it.ng * PG_GROUP + 8 * hh);
+    if (MASK && r.tail) seen &= pg_mask_bits(a.p, b, h, it.ng * PG_GROUP + 8 * hh);
     return seen;
 }
 // (rows behind the last are read from the last one, so that no load waits for a branch; their
@@ -905,7 +883,7 @@ __global__ __launch_bounds__(256, 2) void paged_few_kernel(AttnArgs a) {
             const bool masked = MASK || dead;
             uint32_t live = dead ? 0u : 255u;
             if (masked) {
-                if (MASK) live &= mask_bits(a.p, b, h, i * PG_GROUP + 8 * (hidden(lane) >> 4));
+                if (MASK) live &= pg_mask_bits(a.p, b, h, i * PG_GROUP + 8 * (hidden(lane) >> 4));
                 clear_dead(rv, live);
             }
             f16x8_t pf[NT], pl[NT];
@@ -1168,7 +1146,7 @@ __global__ __launch_bounds__(512, 2) void paged_many_kernel(AttnArgs a) {
             } else {
                 uint32_t live = dead ? 0u : 255u;
                 RawV<D> rv = v_from(raw);
-                if (MASK) live &= mask_bits(a.p, b, h, (pt.i0 + x * STEP + si) * PG_GROUP + 8 * (hidden(lane) >> 4));
+                if (MASK) live &= pg_mask_bits(a.p, b, h, (pt.i0 + x * STEP + si) * PG_GROUP + 8 * (hidden(lane) >> 4));
                 if (MASK || dead) clear_dead(rv, live);
 #pragma unroll
                 for (int ct = 0; ct < NC; ++ct)

@@ -89,6 +89,28 @@ __device__ __forceinline__ const uint8_t *pg_record(const PagesDev &p, int page_
     return p.pool + (int64_t)page_id * p.s_page + (int64_t)h * p.s_head + (int64_t)gi * rec;
 }
 
+// the nonzero bytes of x, as 4 bits
+__device__ __forceinline__ uint32_t pg_byte_bits(uint32_t x) {
+    x |= x >> 4;
+    x |= x >> 2;
+    x |= x >> 1;
+    return ((x & 0x01010101u) * 0x10204080u) >> 28;
+}
+// the seen ones of 8 tokens from position pos on, of a request with a mask
+__device__ __forceinline__ uint32_t pg_mask_bits(const PagesDev &p, int b, int h, int pos) {
+    const uint8_t *m = p.mask + (int64_t)b * p.s_mb + (int64_t)h * p.s_mh;
+    const int n = p.mask_tokens;
+    if (n >= 8) {     // 8 bytes that the mask has, moved to where they belong
+        const int at = min(pos, n - 8), out = min(pos - at, 8);
+        const pg_b8 v = *(const pg_b8 *)(m + (uint32_t)at);
+        return (pg_byte_bits(v.x) | pg_byte_bits(v.y) << 4) >> out;
+    }
+    uint32_t bits = 0;
+    for (int i = 0; i < 8; ++i)
+        if (pos + i < n && m[pos + i]) bits |= 1u << i;
+    return bits;
+}
+
 // inclusive prefix sum over the wave of values >= 0: by lane moves where 32 bits hold every sum
 __device__ __forceinline__ int64_t pg_wave_scan(int64_t x, int lane) {
     if (!__any(x >= (int64_t)1 << 25)) return (int64_t)ma_wave_prefix_u32((uint32_t)x);

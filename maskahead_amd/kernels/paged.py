@@ -368,6 +368,57 @@ def dequantize_pages(prefix: PagedPrefix, tokens: int, *, starts: torch.Tensor |
     return out_key, out_value
 
 
+def select_blocks(query: torch.Tensor, prefix: PagedPrefix, count: int, *, new_lens: torch.Tensor | None = None,
+                  block_tokens: int = GROUP, query_block: int = 0, keep_first: int = 0, keep_last: int = 0,
+                  return_scores: bool = False):
+    """The blocks of stored tokens that the queries [B, Hq, T, D] of every request should read:
+    int32 [B, Hkv, runs, count], ascending, -1 behind the last.  A run is query_block positions
+    (0: all T) of the Hq / Hkv query heads of a KV head, runs = ceil(T / query_block); positions t >=
+    new_lens[b] (None: T) count for nothing.  Block i is the tokens i * block_tokens ... (a multiple of
+    32) of a request's whole groups of 32; the newest lengths % 32 tokens are in no block
+    (``paged_attention`` reads them always).
+
+    A block's score is what q . k could be at most for its keys' channel ranges, which the 4-bit
+    records hold: a tenth of the cache is read.  It is the largest over the run's rows and the block's
+    groups, computed in whole numbers (14 bits of the row's and of the group's largest), so the
+    same blocks are taken whatever the batch.  The count best are taken, ties to the lowest index;
+    the keep_first oldest and keep_last newest blocks in any case.  Blocks without a live token
+    (prefix.mask) are not.  A row or a group with NaN or infinities scores infinity.
+
+    return_scores: also the scores, float32 [B, Hkv, runs, blocks that a table row can name], -inf
+    where there is no block."""
+    b, hq, t, d = _check_block("query", query, prefix)
+    h, width = prefix.heads, prefix._nat.width
+    if h == 0 or hq == 0 or hq % h:
+        raise ValueError("Hq must be a positive multiple of Hkv")
+    count, block_tokens, query_block = _c_int("count", count), _c_int("block_tokens", block_tokens), _c_int("query_block", query_block)
+    keep_first, keep_last = _c_int("keep_first", keep_first), _c_int("keep_last", keep_last)
+    if not block_tokens or block_tokens % GROUP:
+        raise ValueError(f"block_tokens must be a positive multiple of {GROUP}, got {block_tokens}")
+    if count < 1 or keep_first + keep_last > count:
+        raise ValueError(f"count must be positive and hold keep_first and keep_last, got {count}, {keep_first} and {keep_last}")
+    if new_lens is not None:
+        _i32(new_lens, "new_lens", (b,), prefix.index)
+    runs = -(-t // query_block) if query_block else min(t, 1)
+    tokens = width * prefix.page_tokens
+    blocks = torch.empty((b, h, runs, count), device=query.device, dtype=torch.int32)
+    scores = torch.empty((b, h, runs, -(-tokens // block_tokens)), device=query.device, dtype=torch.float32) \
+        if return_scores else None
+    if b and t:
+        if tokens == 0 or prefix._nat.num_pages == 0:
+            blocks.fill_(-1)
+            if return_scores:
+                scores.fill_(float("-inf"))
+            return (blocks, scores) if return_scores else blocks
+        need = N.size_query("ma_select_workspace_bytes", b, h, runs, tokens)
+        if need < 0:
+            raise N.KernelUnavailableError(f"{b * h * runs} selections over {tokens} tokens are not built")
+        ws = torch.empty((need,), device=query.device, dtype=torch.uint8)
+        _call(prefix.index, "ma_select_blocks", N.t4(query), b, hq, t, d, prefix._nat, h, N.ptr(new_lens), query_block,
+              block_tokens, count, keep_first, keep_last, blocks.data_ptr(), N.ptr(scores), ws.data_ptr(), need)
+    return (blocks, scores) if return_scores else blocks
+
+
 def paged_attention(query: torch.Tensor, prefix: PagedPrefix, current_key: torch.Tensor | None = None,
                     current_value: torch.Tensor | None = None, *, new_lens: torch.Tensor | None = None,
                     scaling: float | None = None, causal_block: int = 0, out: torch.Tensor | None = None):
@@ -414,4 +465,4 @@ def paged_attention(query: torch.Tensor, prefix: PagedPrefix, current_key: torch
 
 
 __all__ = ["PagedPrefix", "append_pages", "check_plan", "dequantize_pages", "paged_attention", "plan_pages",
-           "record_bytes", "rotary_table", "rotate_block"]
+           "record_bytes", "rotary_table", "rotate_block", "select_blocks"]

@@ -30,7 +30,7 @@ import torch
 
 from ._native import KernelUnavailableError
 from .kernels.paged import (GROUP, PagedPrefix, append_pages, check_plan, dequantize_pages, paged_attention,
-                            plan_pages, record_bytes, rotate_block)
+                            plan_pages, record_bytes, rotate_block, select_blocks)
 
 
 class PagedKVCache:
@@ -194,6 +194,14 @@ class PagedKVCache:
         prefix = self._readable(layer, mask, staged)
         return paged_attention(query, prefix, current_key, current_value, new_lens=new_lens, scaling=scaling,
                                causal_block=causal_block, out=out)
+
+    def select(self, layer: int, query: torch.Tensor, count: int, *, new_lens: torch.Tensor | None = None,
+               mask: torch.Tensor | None = None, staged: bool = False, **how):
+        """``select_blocks`` of one layer for the block's (rotated) queries; new_lens, mask and staged
+        as in ``attend``, which takes what this returns."""
+        if new_lens is None and self._plan is not None:
+            new_lens = self._plan[0]
+        return select_blocks(query, self._readable(layer, mask, staged), count, new_lens=new_lens, **how)
 
     def dequantize_layer(self, layer: int, tokens: int, *, starts: torch.Tensor | None = None,
                          dtype: torch.dtype | None = None):

@@ -189,3 +189,55 @@ def rotated(x, table, first, interleaved, add=False):
         y = torch.stack((u, w), -1).flatten(-2) if interleaved else torch.cat((u, w), -1)
         out[b, ..., :rd] = y.to(x.dtype)
     return out
+
+
+def group_scores(pool, row, ng, h, q):
+    """[ng] float64: the largest score of the rows q [R, D] against each of the first ng groups of KV
+    head h of the request whose pages `row` names, in whole numbers (None: the group lies in no page)."""
+    import numpy as np
+
+    pages, _, per, rec = pool.shape
+    d = rec // 40
+    half = lambda g, at: np.frombuffer(pool[row[g // per], h, g % per].numpy().tobytes(), np.float16, d, at).astype(np.float64)  # noqa: E731
+    rows = [r.to(torch.float64).numpy() for r in q]
+
+    def whole(x, top, least):
+        if not np.isfinite(top):
+            return None, 0
+        e = max(int(np.floor(np.log2(top))) if top else least, least)
+        if top and 2.0 ** (e + 1) <= top:
+            e += 1
+        return [int(v) for v in np.rint(x * 2.0 ** (13 - e))], e
+
+    fixed = [whole(r, np.abs(r).max(), -100) for r in rows]
+    out = []
+    for g in range(ng):
+        if not 0 <= row[g // per] < pages:
+            out.append(None)
+            continue
+        with np.errstate(all="ignore"):
+            s, z = 15 * half(g, 32 * d), half(g, 34 * d)
+        top = max(np.abs(s).max(), np.abs(z).max())
+        zc, f = whole(z, top, -24)
+        sc, _ = whole(s, top, -24)
+        best = -math.inf
+        for qc, e in fixed:
+            if zc is None or qc is None:
+                v = math.inf
+            else:
+                v = sum(a * b + max(a, 0) * c for a, b, c in zip(qc, zc, sc)) * 2.0 ** (e + f - 26)
+                with np.errstate(over="ignore"):
+                    v = max(float(np.float32(v)), -3.4028234663852886e38)
+            best = max(best, v)
+        out.append(best)
+    return out
+
+
+def select_rule(scores, m, count, first, last):
+    """The blocks of m groups that are taken, and every block's score."""
+    nb = -(-len(scores) // m)
+    block = [max([s for s in scores[i * m:(i + 1) * m] if s is not None], default=-math.inf) for i in range(nb)]
+    there = [i for i in range(nb) if block[i] > -math.inf]
+    must = [i for i in there if i < first or i >= nb - last]
+    rest = sorted((i for i in there if i not in must), key=lambda i: (-block[i], i))
+    return sorted(must + rest[:count - len(must)]), block
