@@ -450,6 +450,18 @@ int ma_paged_attention(ma_tensor4 q, int B, int Hq, int T, int D, const ma_pages
                        ma_tensor4 vc, const int32_t *new_lens, int causal_block, float scale, ma_tensor4 out,
                        void *workspace, int64_t workspace_bytes, void *stream);
 
+/* ma_paged_attention over [the blocks that blocks [B, H, runs, count] i32 lists for each request, KV
+ * head and run of query_block positions (0: all T; runs = ceil(T / query_block)) | the tail | the block's
+ * own keys]: entry i stands for tokens i block_tokens ... (a multiple of 32) of the request's whole groups
+ * of 32 (ma_select_blocks lists them so, in any order here).  Entries below 0 or behind the request's
+ * last block are none; one listed twice weighs twice.  No more than the first ceil(whole groups /
+ * block) entries are looked at.  workspace: ma_paged_blocks_workspace_bytes() bytes.  MA_EUNSUPPORTED as
+ * there, with every run's row groups and what the lists hold. */
+int64_t ma_paged_blocks_workspace_bytes(int B, int H, int Hq, int T, int D, int query_block);
+int ma_paged_attention_blocks(ma_tensor4 q, int B, int Hq, int T, int D, const ma_pages *p, int H, ma_tensor4 kc,
+                              ma_tensor4 vc, const int32_t *new_lens, int causal_block, float scale, ma_tensor4 out,
+                              const int32_t *blocks, int count, int block_tokens, int query_block, void *workspace,
+                              int64_t workspace_bytes, void *stream);
 /* The blocks of block_tokens (a multiple of 32) stored tokens that a run of query_block positions
  * (0: all T) should read, of every request, KV head and run: blocks [B, H, runs, count] i32, ascending,
  * -1 behind the last, runs = ceil(T / query_block).  Block i holds tokens i block_tokens ... of the

@@ -59,6 +59,10 @@ struct AttnArgs {
     float sl2;                // scale * log2(e)
     float *wm, *wl, *wo;      // partials of slots [2 W]: per row reference and sum, unnormalised rows
     int4 *desc;               // [B, H, RG]: what note_segment says of every segment
+    // Over selected blocks (SEL): every run of `run` positions has a list of its own, rows are those of
+    // a run (R = G run), and RG = runs * RGR.
+    const int32_t *blocks;    // [B, H, runs, count]
+    int count, m, run, RGR;   // entries of a list, groups of a block
 };
 
 // values that every lane holds alike, as scalars
@@ -73,28 +77,39 @@ __device__ __forceinline__ int uniform(int x) { return __builtin_amdgcn_readfirs
 // START 1, 8, 12, 16, 20: one token of 64 ragged requests 58, 52.4, 52.8, 52.4, 54.1 us, of 2 long
 // ones 66.8 to 67.3; of many rows 9 % slower with 1, 4 to 16 within 2 % of one another.
 constexpr int START = 8;
+//
+// Over selected blocks the packed items are the groups of the list's entries, those that a request
+// has no block for left out; an entry that names none, and groups behind the request's last, are
+// items that nothing is seen of.
 struct Items {
-    int n, len, ng, rem, items;
+    int n, len, ng, rem, items;      // ng: packed items
 };
+template <bool SEL>
 __device__ __forceinline__ Items items_from(const AttnArgs &a, int n, int len) {
     Items r;
     r.n = n;
     r.len = len;
     r.ng = len / PG_GROUP;
+    if (SEL) r.ng = (int)min((unsigned)a.count, ((unsigned)r.ng + (unsigned)a.m - 1) / (unsigned)a.m) * a.m;
     r.rem = len % PG_GROUP;
     const int cur = a.kc.ptr ? (n + PG_GROUP - 1) / PG_GROUP : 0;
     const int rows = (r.rem ? 1 : 0) + cur;
     r.items = n ? START + r.ng + (rows ? a.rows0 + (rows << a.dense) : 0) : 0;
     return r;
 }
+template <bool SEL>
 __device__ __forceinline__ Items items_of(const AttnArgs &a, int b) {
-    return items_from(a, a.new_lens ? min(max(a.new_lens[b], 0), a.T) : a.T, min(max(a.p.lengths[b], 0), a.max_len));
+    return items_from<SEL>(a, a.new_lens ? min(max(a.new_lens[b], 0), a.T) : a.T, min(max(a.p.lengths[b], 0), a.max_len));
 }
 // ... of a request that the whole wave looks at
+template <bool SEL>
 __device__ __forceinline__ Items items_at(const AttnArgs &a, int b) {
-    const Items r = items_of(a, b);
-    return items_from(a, uniform(r.n), uniform(r.len));
+    const Items r = items_of<SEL>(a, b);
+    return items_from<SEL>(a, uniform(r.n), uniform(r.len));
 }
+// positions of a segment's rows: row = query head * positions + position
+template <bool SEL>
+__device__ __forceinline__ int positions(const AttnArgs &a) { return SEL ? a.run : a.T; }
 
 // The lane's number, as a value that nothing is known of: what is computed from it stays where
 // it is used, where the compiler would otherwise keep every address of the rare paths in
@@ -324,7 +339,7 @@ __device__ __forceinline__ Rows rows_of(const AttnArgs &a, const Items &it, int 
 template <bool MASK>
 __device__ __forceinline__ uint32_t rows_live(const AttnArgs &a, const Items &it, const Rows &r, int b, int h, int hh) {
     uint32_t seen = 255u >> min(max(r.j0 + 8 * hh + 8 - r.cnt, 0), 8);
-    if (MASK && r.tail) seen &= pg_mask_bits(a.p, b, h, it.ng * PG_GROUP + 8 * hh);
+    if (MASK && r.tail) seen &= pg_mask_bits(a.p, b, h, it.len / PG_GROUP * PG_GROUP + 8 * hh);
     return seen;
 }
 // (rows behind the last are read from the last one, so that no load waits for a branch; their
@@ -528,12 +543,13 @@ __device__ __forceinline__ f32x4_t rows_values(uint4 v, const Probs<false> &p, f
 // ---- Q of one row tile as B operands: lane (n, h) = row n, channels (D/4) h + 8 cb + (0..7);
 // rows behind the request's new tokens are zero
 // (WORDS: as they lie there, where such rows are left out later)
-template <int D, bool WORDS = false>
-__device__ __forceinline__ void load_q(const AttnArgs &a, int b, int h, int row, int n, int hh, uint4 *q) {
-    const int rc = min(row, a.R - 1), g = rc / a.T, t = rc - g * a.T;
+// t0: position of the segment's first
+template <int D, bool SEL, bool WORDS = false>
+__device__ __forceinline__ void load_q(const AttnArgs &a, int b, int h, int t0, int row, int n, int hh, uint4 *q) {
+    const int rc = min(row, a.R - 1), g = rc / positions<SEL>(a), t = (SEL ? t0 : 0) + rc - g * positions<SEL>(a);
     const uint32_t ok = WORDS || (row < a.R && t < n) ? 0xffffffffu : 0u;
     const uint16_t *src = (const uint16_t *)a.q.ptr + (int64_t)b * a.q.s[0] + (int64_t)(h * a.G + g) * a.q.s[1] +
-                          (int64_t)t * a.q.s[2] + (D / 4) * hh;
+                          (int64_t)(SEL ? min(t, a.T - 1) : t) * a.q.s[2] + (D / 4) * hh;
 #pragma unroll
     for (int cb = 0; cb < D / 32; ++cb) {
         const uint4 x = pg_load16(src + 8 * cb);
@@ -590,13 +606,13 @@ __device__ __forceinline__ void cut_line(const AttnArgs &a, Stretch &r, int tota
 }
 // Items of all requests, by a scan of the lengths in every workgroup (8 B a request, from L2): of
 // up to 64 requests in every wave, without a barrier
-template <int THREADS>
+template <int THREADS, bool SEL>
 __device__ __forceinline__ Stretch find_stretch(const AttnArgs &a, ScanShared &sh, int unit) {
     constexpr int NW = THREADS / 64;
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     Stretch r;
     if (a.B <= 64) {
-        const Items own = lane < a.B ? items_of(a, lane) : Items{};
+        const Items own = lane < a.B ? items_of<SEL>(a, lane) : Items{};
         const int inc = (int)ma_wave_prefix_u32((uint32_t)own.items);
         cut_line(a, r, __builtin_amdgcn_readlane(inc, 63) * a.HR, unit);
         const int want = (int)((unsigned)r.s / (unsigned)a.HR);
@@ -605,7 +621,7 @@ __device__ __forceinline__ Stretch find_stretch(const AttnArgs &a, ScanShared &s
         const int l = here ? __ffsll((unsigned long long)here) - 1 : 0;
         r.b = l;
         r.pre = __builtin_amdgcn_readlane(inc - own.items, l);
-        r.it = items_from(a, __builtin_amdgcn_readlane(own.n, l), __builtin_amdgcn_readlane(own.len, l));
+        r.it = items_from<SEL>(a, __builtin_amdgcn_readlane(own.n, l), __builtin_amdgcn_readlane(own.len, l));
         return r;
     }
     const int per = (a.B + THREADS - 1) / THREADS, first = tid * per;
@@ -613,7 +629,7 @@ __device__ __forceinline__ Stretch find_stretch(const AttnArgs &a, ScanShared &s
     Items own{};   // of this thread's first request
     for (int i = 0; i < per; ++i)
         if (first + i < a.B) {
-            const Items it = items_of(a, first + i);
+            const Items it = items_of<SEL>(a, first + i);
             if (i == 0) own = it;
             sum += it.items;
         }
@@ -632,7 +648,7 @@ __device__ __forceinline__ Stretch find_stretch(const AttnArgs &a, ScanShared &s
         int pre = before, b = first;
         while (want >= pre + own.items) {
             pre += own.items;
-            own = items_of(a, ++b);
+            own = items_of<SEL>(a, ++b);
         }
         sh.b = b;
         sh.pre = pre;
@@ -642,17 +658,19 @@ __device__ __forceinline__ Stretch find_stretch(const AttnArgs &a, ScanShared &s
     __syncthreads();
     r.b = uniform(sh.b);
     r.pre = uniform(sh.pre);
-    r.it = items_from(a, uniform(sh.n), uniform(sh.len));
+    r.it = items_from<SEL>(a, uniform(sh.n), uniform(sh.len));
     return r;
 }
 
 // the part of a segment that lies in a stretch
 struct Part {
-    int h, rg, hr, i0, i1;   // its items of work [i0, i1)
+    int h, rg, hr, i0, i1;   // its items of work [i0, i1); rg: the row group of the head's (SEL: of the run's)
+    int run, t0;             // SEL: the run and its first position; else 0
     int next;                // where the stretch goes on
     bool first, whole;       // the segment begins here; all of it lies here
     int slot;                // of its partial, where it is not whole: the first or the last of the stretch
 };
+template <bool SEL>
 __device__ __forceinline__ Part part_of(const AttnArgs &a, const Stretch &st, int pos) {
     Part p;
     const int rel = pos - a.HR * st.pre;
@@ -660,6 +678,12 @@ __device__ __forceinline__ Part part_of(const AttnArgs &a, const Stretch &st, in
     const int i0 = rel - p.hr * st.it.items, i1 = min(st.it.items, i0 + (st.e - pos));
     p.h = a.RG == 1 ? p.hr : (int)((unsigned)p.hr / (unsigned)a.RG);
     p.rg = p.hr - p.h * a.RG;
+    p.run = p.t0 = 0;
+    if (SEL) {
+        p.run = (int)((unsigned)p.rg / (unsigned)a.RGR);
+        p.rg -= p.run * a.RGR;
+        p.t0 = p.run * a.run;
+    }
     p.next = pos + i1 - i0;
     p.first = i0 == 0;
     p.whole = i0 == 0 && i1 == st.it.items;
@@ -679,11 +703,12 @@ __device__ __forceinline__ void note_segment(const AttnArgs &a, const Stretch &s
     const int n = p.whole ? 0 : (int)((unsigned)(pos + st.it.items - 1) / (unsigned)st.chunk) - st.w + 1;
     a.desc[(int64_t)st.b * a.HR + p.hr] = int4{p.slot, n, st.w, 0};
 }
+template <bool SEL>
 __device__ __forceinline__ void next_part(const AttnArgs &a, Stretch &st, const Part &p, int &pos) {
     pos = p.next;
     if (pos >= st.e || pos - a.HR * st.pre < a.HR * st.it.items) return;
     st.pre += st.it.items;
-    do st.it = items_at(a, ++st.b);
+    do st.it = items_at<SEL>(a, ++st.b);
     while (st.it.items == 0);
 }
 
@@ -691,18 +716,32 @@ __device__ __forceinline__ void next_part(const AttnArgs &a, Stretch &st, const 
 // last of one (request, head).  Looked up at once, so that no item waits for its table entry
 // (a load in the loop also waits for every load before it).  Records are 16-byte aligned: bit 0
 // says that the table names no page, and the address is then the pool's first record.
+// (SEL: by way of the list's entry, and the group's number, which a mask is looked up by.)
 struct Records {
     uint32_t lo, hi;
+    int group;
 };
-template <int D, int EVERY>
-__device__ __forceinline__ Records find_records(const AttnArgs &a, int b, int h, int first, int last, int lane) {
-    const int per = a.p.page_tokens / PG_GROUP, i = first + EVERY * lane, pg = i / per;
+template <int D, int EVERY, bool SEL>
+__device__ __forceinline__ Records find_records(const AttnArgs &a, const Items &it, int b, int h, int run, int first, int last,
+                                                int lane) {
+    const int per = a.p.page_tokens / PG_GROUP;
+    int i = first + EVERY * lane;
     uint64_t r = (uint64_t)a.p.pool | 1u;
-    if (i < last) {
+    bool there = i < last;
+    if (SEL && there) {
+        const int e = (int)((unsigned)i / (unsigned)a.m), ng = it.len / PG_GROUP;
+        const int block = a.blocks[(((int64_t)b * a.H + h) * (a.RG / a.RGR) + run) * a.count + e];
+        // (a block behind the request's last is none: its first group's number is not computed)
+        there = block >= 0 && block <= (ng - 1) / a.m;
+        i = there ? block * a.m + (i - e * a.m) : 0;
+        there = there && i < ng;
+    }
+    if (there) {
+        const int pg = i / per;
         const uint8_t *rec = pg_record(a.p, a.p.table[(int64_t)b * a.p.s_table + pg], i - pg * per, h, 40 * D);
         if (rec) r = (uint64_t)rec;
     }
-    return Records{(uint32_t)r, (uint32_t)(r >> 32)};
+    return Records{(uint32_t)r, (uint32_t)(r >> 32), i};
 }
 __device__ __forceinline__ rec_t record_at(const Records &r, int k, bool &dead) {
     const uint32_t lo = (uint32_t)__builtin_amdgcn_readlane((int)r.lo, k), hi = (uint32_t)__builtin_amdgcn_readlane((int)r.hi, k);
@@ -716,14 +755,15 @@ __device__ __forceinline__ uint32_t pack_out(float x, float y) {
     const f16x2_t z = {(_Float16)x, (_Float16)y};
     return __builtin_bit_cast(uint32_t, z);
 }
-__device__ __forceinline__ uint16_t *out_row(const AttnArgs &a, int b, int h, int row) {
-    const int g = row / a.T, t = row - g * a.T;
+template <bool SEL>
+__device__ __forceinline__ uint16_t *out_row(const AttnArgs &a, int b, int h, int t0, int row) {
+    const int g = row / positions<SEL>(a), t = (SEL ? t0 : 0) + row - g * positions<SEL>(a);
     return (uint16_t *)a.out.ptr + (int64_t)b * a.out.s[0] + (int64_t)(h * a.G + g) * a.out.s[1] + (int64_t)t * a.out.s[2];
 }
 // NC channels of a row, to its place in out
-template <int NC, bool BF16>
-__device__ __forceinline__ void store_out(const AttnArgs &a, int b, int h, int row, int ch, const float *o) {
-    uint16_t *dst = out_row(a, b, h, row) + ch;
+template <int NC, bool BF16, bool SEL>
+__device__ __forceinline__ void store_out(const AttnArgs &a, int b, int h, int t0, int row, int ch, const float *o) {
+    uint16_t *dst = out_row<SEL>(a, b, h, t0, row) + ch;
     uint32_t y[NC / 2];
 #pragma unroll
     for (int k = 0; k < NC / 2; ++k) y[k] = pack_out<BF16>(o[2 * k], o[2 * k + 1]);
@@ -798,31 +838,37 @@ struct FewShared {
     ScanShared scan;
 };
 
-template <int D, int NT, bool BF16, bool MASK>
+template <int D, int NT, bool BF16, bool MASK, bool SEL>
 __global__ __launch_bounds__(256, 2) void paged_few_kernel(AttnArgs a) {
     constexpr int CB = D / 32, NC = D / 16;
     __shared__ FewShared<D, NT> sh;
     const int tid = threadIdx.x, lane = tid & 63, wave = uniform(tid >> 6), n16 = lane & 15, hh = lane >> 4;
-    Stretch st = find_stretch<256>(a, sh.scan, WAVES);
+    Stretch st = find_stretch<256, SEL>(a, sh.scan, WAVES);
     int pos = st.s;
     while (pos < st.e) {
         const Items it = st.it;
-        const Part pt = part_of(a, st, pos);
-        const int b = st.b, h = pt.h, row0 = pt.rg * NT * 16;
+        const Part pt = part_of<SEL>(a, st, pos);
+        const int b = st.b, h = pt.h, row0 = pt.rg * NT * 16, t0 = pt.t0;
+        if (SEL && t0 >= it.n) {           // a run behind the new tokens
+            next_part<SEL>(a, st, pt, pos);
+            continue;
+        }
         uint4 q[NT][CB];
         float c[NT];
         Tile<D> t[NT];
         // (the queries' loads and the table's are under way together, the first record's behind
         // them while the queries are scaled)
 #pragma unroll
-        for (int nt = 0; nt < NT; ++nt) load_q<D>(a, b, h, row0 + nt * 16 + (hidden(lane) & 15), it.n, hh, q[nt]);
+        for (int nt = 0; nt < NT; ++nt) load_q<D, SEL>(a, b, h, t0, row0 + nt * 16 + (hidden(lane) & 15), it.n, hh, q[nt]);
         const int last = min(pt.i1, it.ng);
         int i = pt.i0 + wave, k = 0;
-        Records recs = find_records<D, WAVES>(a, b, h, i, last, lane);
+        Records recs = find_records<D, WAVES, SEL>(a, it, b, h, pt.run, i, last, lane);
         RawK<D> rk;
         RawV<D> rv;
         bool dead = false;
+        int group = i;
         if (i < last) {
+            if (SEL && MASK) group = __builtin_amdgcn_readlane(recs.group, 0);
             const rec_t rec = record_at(recs, 0, dead);
             load_k(rk, rec, lane);
             load_v(rv, rec, lane);
@@ -835,7 +881,7 @@ __global__ __launch_bounds__(256, 2) void paged_few_kernel(AttnArgs a) {
         float lo = P_FIRST;
         for (; i < last; i += WAVES) {
             if (++k == 64) {
-                recs = find_records<D, WAVES>(a, b, h, i + WAVES, last, lane);
+                recs = find_records<D, WAVES, SEL>(a, it, b, h, pt.run, i + WAVES, last, lane);
                 k = 0;
             }
             // (behind the last one the pool's first record is loaded: no branch around the loads)
@@ -883,7 +929,7 @@ __global__ __launch_bounds__(256, 2) void paged_few_kernel(AttnArgs a) {
             const bool masked = MASK || dead;
             uint32_t live = dead ? 0u : 255u;
             if (masked) {
-                if (MASK) live &= pg_mask_bits(a.p, b, h, i * PG_GROUP + 8 * (hidden(lane) >> 4));
+                if (MASK) live &= pg_mask_bits(a.p, b, h, (SEL ? group : i) * PG_GROUP + 8 * (hidden(lane) >> 4));
                 clear_dead(rv, live);
             }
             f16x8_t pf[NT], pl[NT];
@@ -921,6 +967,7 @@ __global__ __launch_bounds__(256, 2) void paged_few_kernel(AttnArgs a) {
             }
             load_v(rv, next, lane);
             dead = dead_next;
+            if (SEL && MASK) group = __builtin_amdgcn_readlane(recs.group, k);
         }
         if constexpr (!BF16) {
 #pragma unroll
@@ -944,7 +991,7 @@ __global__ __launch_bounds__(256, 2) void paged_few_kernel(AttnArgs a) {
 #pragma unroll
                 for (int nt = 0; nt < NT; ++nt) {
                     uint4 qr[CB];
-                    load_q<D>(a, b, h, row0 + nt * 16 + (l & 15), it.n, lh, qr);
+                    load_q<D, SEL>(a, b, h, t0, row0 + nt * 16 + (l & 15), it.n, lh, qr);
                     s[mt][nt] = rows_scores<CB, BF16>(k, qr);
                 }
             }
@@ -952,7 +999,7 @@ __global__ __launch_bounds__(256, 2) void paged_few_kernel(AttnArgs a) {
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt)
                 p[nt] = rows_probs<D, BF16>(t[nt], s[0][nt], s[1][nt], a.sl2, lo,
-                                            causal_live(r, keys_seen(a, it, (row0 + nt * 16 + (l & 15)) % a.T), lh, seen));
+                                            causal_live(r, keys_seen(a, it, t0 + (row0 + nt * 16 + (l & 15)) % positions<SEL>(a)), lh, seen));
             lo = P_MIN;
             // (the values' loads stay behind the scores' registers: ahead of them the main loop spilled)
             __builtin_amdgcn_sched_barrier(0);
@@ -981,7 +1028,7 @@ __global__ __launch_bounds__(256, 2) void paged_few_kernel(AttnArgs a) {
         }
         if (odd) {
 #pragma unroll
-            for (int nt = 0; nt < NT; ++nt) add_odd<D, BF16>(a, it, b, h, rows_at, pt.i1, keys_seen(a, it, (row0 + nt * 16 + n16) % a.T), hh, t[nt]);
+            for (int nt = 0; nt < NT; ++nt) add_odd<D, BF16>(a, it, b, h, rows_at, pt.i1, keys_seen(a, it, t0 + (row0 + nt * 16 + n16) % positions<SEL>(a)), hh, t[nt]);
         }
         // the waves' parts joined; whole segments written out, cut ones left as a partial
 #pragma unroll
@@ -1025,7 +1072,7 @@ __global__ __launch_bounds__(256, 2) void paged_few_kernel(AttnArgs a) {
                     const float inv = lt == 0.f ? 0.f : 1.f / lt;
 #pragma unroll
                     for (int k = 0; k < NC; ++k) o[k] *= inv;
-                    if (row % a.T < it.n) store_out<NC, BF16>(a, b, h, row, NC * x, o);
+                    if (t0 + row % positions<SEL>(a) < it.n) store_out<NC, BF16, SEL>(a, b, h, t0, row, NC * x, o);
                 } else {
                     const int64_t at = (int64_t)pt.slot * (NT * 16) + nt * 16 + r;
                     if (x == 0) {
@@ -1039,7 +1086,7 @@ __global__ __launch_bounds__(256, 2) void paged_few_kernel(AttnArgs a) {
             }
         }
         note_segment(a, st, pt, pos);
-        next_part(a, st, pt, pos);
+        next_part<SEL>(a, st, pt, pos);
     }
 }
 
@@ -1083,7 +1130,7 @@ struct ManyShared {
     ScanShared scan;
 };
 
-template <int D, int RW, bool BF16, bool MASK>
+template <int D, int RW, bool BF16, bool MASK, bool SEL>
 __global__ __launch_bounds__(512, 2) void paged_many_kernel(AttnArgs a) {
     constexpr int CB = D / 32, NC = D / 16, TW = MWAVES / RW, STEP = step_of(D, BF16), LEFT = 2 * CB + NC;
     extern __shared__ __attribute__((aligned(16))) char lds[];
@@ -1092,18 +1139,22 @@ __global__ __launch_bounds__(512, 2) void paged_many_kernel(AttnArgs a) {
     const int rw = wave % RW, tw = wave / RW;
     const int si = wave >> 1;              // the item of a step that this wave unpacks (STEP and more: none)
     const bool sv = wave & 1;              // its values (else its keys)
-    Stretch st = find_stretch<512>(a, sh.scan, STEP);
+    Stretch st = find_stretch<512, SEL>(a, sh.scan, STEP);
     int pos = st.s;
     while (pos < st.e) {
         const Items it = st.it;
-        const Part pt = part_of(a, st, pos);
-        const int b = st.b, h = pt.h, row0 = pt.rg * (2 * RW * 16) + rw * 32;
+        const Part pt = part_of<SEL>(a, st, pos);
+        const int b = st.b, h = pt.h, row0 = pt.rg * (2 * RW * 16) + rw * 32, t0 = pt.t0;
+        if (SEL && t0 >= it.n) {           // a run behind the new tokens
+            next_part<SEL>(a, st, pt, pos);
+            continue;
+        }
         const bool busy = row0 < a.R;      // this wave has rows
         uint4 q[2][CB];
         float c[2];
         Tile<D> t[2];
 #pragma unroll
-        for (int nt = 0; nt < 2; ++nt) load_q<D>(a, b, h, row0 + nt * 16 + (hidden(lane) & 15), it.n, hh, q[nt]);
+        for (int nt = 0; nt < 2; ++nt) load_q<D, SEL>(a, b, h, t0, row0 + nt * 16 + (hidden(lane) & 15), it.n, hh, q[nt]);
         // the seen tokens of an item, from its values' wave
         auto note_live = [&](int x, uint32_t live) {
             uint32_t all = 0;
@@ -1117,11 +1168,13 @@ __global__ __launch_bounds__(512, 2) void paged_many_kernel(AttnArgs a) {
         const int poff = sv ? 2 * (32 * (NC * (lane & 15) / 32) + 8 * hh) : (D / 2) * hh;
         RawK<D> raw;
         bool dead = false;
+        int group = 0;
         Records recs;
         // the words of step x's item of this wave (behind the last one: of the pool's first record)
         auto fetch = [&](int x) {
             if (si >= STEP) return;
-            if (x % 64 == 0) recs = find_records<D, STEP>(a, b, h, pt.i0 + x * STEP + si, last, lane);
+            if (x % 64 == 0) recs = find_records<D, STEP, SEL>(a, it, b, h, pt.run, pt.i0 + x * STEP + si, last, lane);
+            if (SEL && MASK) group = __builtin_amdgcn_readlane(recs.group, x % 64);
             const rec_t rec = record_at(recs, x % 64, dead);
             load_either(raw, rec, lane, sv, poff);
         };
@@ -1146,7 +1199,7 @@ __global__ __launch_bounds__(512, 2) void paged_many_kernel(AttnArgs a) {
             } else {
                 uint32_t live = dead ? 0u : 255u;
                 RawV<D> rv = v_from(raw);
-                if (MASK) live &= pg_mask_bits(a.p, b, h, (pt.i0 + x * STEP + si) * PG_GROUP + 8 * (hidden(lane) >> 4));
+                if (MASK) live &= pg_mask_bits(a.p, b, h, (SEL ? group : pt.i0 + x * STEP + si) * PG_GROUP + 8 * (hidden(lane) >> 4));
                 if (MASK || dead) clear_dead(rv, live);
 #pragma unroll
                 for (int ct = 0; ct < NC; ++ct)
@@ -1228,7 +1281,8 @@ __global__ __launch_bounds__(512, 2) void paged_many_kernel(AttnArgs a) {
 
         // ---- the tail and the block's own keys, four items a step too; what no row of the group
         // sees is left out, what none of the wave's sees too
-        const int r1 = min((pt.rg + 1) * (2 * RW * 16), a.R) - 1, t1 = pt.rg * (2 * RW * 16) / a.T == r1 / a.T ? r1 % a.T : a.T - 1;
+        const int tq = positions<SEL>(a), r1 = min((pt.rg + 1) * (2 * RW * 16), a.R) - 1;
+        const int t1 = t0 + (pt.rg * (2 * RW * 16) / tq == r1 / tq ? r1 % tq : tq - 1);
         const int d0 = max(pt.i0, it.ng);
         const int d1 = min(pt.i1, it.ng + (it.rem ? 1 : 0) + (a.kc.ptr ? (keys_seen(a, it, t1) + PG_GROUP - 1) / PG_GROUP : 0));
         int odd = 0;
@@ -1239,8 +1293,8 @@ __global__ __launch_bounds__(512, 2) void paged_many_kernel(AttnArgs a) {
             for (int nt = 0; nt < 2; ++nt) {
                 const int row = row0 + nt * 16 + (l & 15);
                 // (as they are, not as f16; a row that is none is left out when results are stored)
-                if (BF16) load_q<D, true>(a, b, h, row, it.n, lh, q[nt]);
-                keys[nt] = keys_seen(a, it, row % a.T);
+                if (BF16) load_q<D, SEL, true>(a, b, h, t0, row, it.n, lh, q[nt]);
+                keys[nt] = keys_seen(a, it, t0 + row % tq);
             }
             for (int i = d0, x = 0; i < d1; i += STEP, ++x) {
                 uint32_t any = 0;
@@ -1363,14 +1417,14 @@ __global__ __launch_bounds__(512, 2) void paged_many_kernel(AttnArgs a) {
                 if (row >= a.R) continue;
                 const float l = t[nt].l[0];
                 if (pt.whole) {
-                    if (row % a.T >= it.n) continue;
+                    if (t0 + row % tq >= it.n) continue;
                     const float inv = l == 0.f ? 0.f : 1.f / l;
 #pragma unroll
                     for (int r = 0; r < 4; ++r) {
                         float o[NC];
 #pragma unroll
                         for (int ct = 0; ct < NC; ++ct) o[ct] = t[nt].acc[ct][r] * inv;
-                        store_out<NC, BF16>(a, b, h, row, NC * (4 * hh + r), o);
+                        store_out<NC, BF16, SEL>(a, b, h, t0, row, NC * (4 * hh + r), o);
                     }
                 } else {
                     const int64_t slot = (int64_t)pt.slot * (2 * RW * 16);
@@ -1393,17 +1447,17 @@ __global__ __launch_bounds__(512, 2) void paged_many_kernel(AttnArgs a) {
 #pragma unroll 1
                 for (int rt = rw * 32 + (lane & 15); rt < rw * 32 + 32; rt += 16) {
                     const int row = row0 - rw * 32 + rt;
-                    if (row >= a.R || (pt.whole && row % a.T >= it.n)) continue;
+                    if (row >= a.R || (pt.whole && t0 + row % tq >= it.n)) continue;
                     float *dst = a.wo + (int64_t)pt.slot * (2 * RW * 16) * D + partial_at<D>(rt, 4 * hh);
-                    each_odd<BF16>(a, it, b, h, d0, d1, keys_seen(a, it, row % a.T), (D / 4) * hh, D / 4, [&](int e, float v) {
-                        if (pt.whole) add_to<BF16>(out_row(a, b, h, row)[(D / 4) * hh + e], v);
+                    each_odd<BF16>(a, it, b, h, d0, d1, keys_seen(a, it, t0 + row % tq), (D / 4) * hh, D / 4, [&](int e, float v) {
+                        if (pt.whole) add_to<BF16>(out_row<SEL>(a, b, h, t0, row)[(D / 4) * hh + e], v);
                         else dst[(e / 4) * 256 + e % 4] += v;
                     });
                 }
             }
         }
         note_segment(a, st, pt, pos);
-        next_part(a, st, pt, pos);
+        next_part<SEL>(a, st, pt, pos);
     }
 }
 
@@ -1420,19 +1474,21 @@ __global__ __launch_bounds__(512, 2) void paged_many_kernel(AttnArgs a) {
 // requests 50.9 us with 4, 51.2 with 2, 51.9 with 8.
 constexpr int merge_waves(bool tiles) { return tiles ? 4 : 8; }
 
-template <int D, bool BF16, bool TILES>
+template <int D, bool BF16, bool TILES, bool SEL>
 __global__ __launch_bounds__(64 * merge_waves(TILES)) void paged_merge_kernel(AttnArgs a, int rows) {
     constexpr int NC = D / 16, GR = merge_waves(TILES);
     __shared__ float sm[GR][64], sl[GR][64];
     __shared__ f32x4_t so[GR][NC / 4][64];
     const int b = blockIdx.x / a.HR, hr = blockIdx.x - b * a.HR;
     const int n = a.new_lens ? min(max(a.new_lens[b], 0), a.T) : a.T;
+    const int h = hr / a.RG, run = SEL ? (hr - h * a.RG) / a.RGR : 0, rg = hr - h * a.RG - (SEL ? run * a.RGR : 0);
+    const int t0 = SEL ? run * a.run : 0;
     const int4 d = a.desc[blockIdx.x];
-    if ((n == 0) | (d.y == 0)) return;      // (n 0: nobody wrote its segments)
+    if ((n <= t0) | (d.y == 0)) return;      // (no new tokens: nobody wrote its segments)
     const int grp = threadIdx.x >> 6, u = threadIdx.x & 63;
     const int x = TILES ? 4 * (blockIdx.y & 3) + (u >> 4) : u & 15;
     const int rt = TILES ? 16 * (blockIdx.y >> 2) + (u & 15) : 4 * blockIdx.y + (u >> 4);
-    const int h = hr / a.RG, rg = hr - h * a.RG, row = rg * rows + rt;
+    const int row = rg * rows + rt;
     const int off = TILES ? partial_at<D>(rt, x) : rt * D + NC * x;      // ... of its first 4 channels
     constexpr int next = TILES ? 256 : 4;                                // from 4 channels to the next 4
     float m = NO_MAX, l = 0.f, o[NC];
@@ -1483,11 +1539,11 @@ __global__ __launch_bounds__(64 * merge_waves(TILES)) void paged_merge_kernel(At
 #pragma unroll
         for (int k = 0; k < NC; ++k) o[k] += so[v][k / 4][u][k % 4] * f;
     }
-    if (row >= a.R || row % a.T >= n) return;
+    if (row >= a.R || t0 + row % positions<SEL>(a) >= n) return;
     const float inv = l == 0.f ? 0.f : 1.f / l;
 #pragma unroll
     for (int k = 0; k < NC; ++k) o[k] *= inv;
-    store_out<NC, BF16>(a, b, h, row, NC * x, o);
+    store_out<NC, BF16, SEL>(a, b, h, t0, row, NC * x, o);
 }
 
 // ------------------------------------------------------------------ host
@@ -1550,57 +1606,78 @@ Layout layout_of(const Shape &s, int64_t segments, int D) {
     return l;
 }
 
-template <int D, int RW, bool BF16, bool MASK>
+template <int D, int RW, bool BF16, bool MASK, bool SEL>
 int launch_many(const AttnArgs &a, hipStream_t st) {
     constexpr int LDS = (int)sizeof(ManyShared<D, BF16>);
     static_assert(LDS <= 160 * 1024, "two steps of operands in one CU's LDS");
     if (LDS > 64 * 1024) {
-        const hipError_t e = hipFuncSetAttribute((const void *)paged_many_kernel<D, RW, BF16, MASK>,
+        const hipError_t e = hipFuncSetAttribute((const void *)paged_many_kernel<D, RW, BF16, MASK, SEL>,
                                                  hipFuncAttributeMaxDynamicSharedMemorySize, LDS);
         if (e != hipSuccess) {
             ma_set_error("ma_paged_attention: %d bytes of LDS refused: %s", LDS, hipGetErrorString(e));
             return MA_EHIP;
         }
     }
-    paged_many_kernel<D, RW, BF16, MASK><<<a.W, 512, LDS, st>>>(a);
+    paged_many_kernel<D, RW, BF16, MASK, SEL><<<a.W, 512, LDS, st>>>(a);
     return MA_OK;
 }
 
-template <int D, bool BF16, bool MASK>
+template <int D, bool BF16, bool MASK, bool SEL>
 int launch_attn(const AttnArgs &a, const Shape &s, hipStream_t st) {
-    if (s.nt == 1) paged_few_kernel<D, 1, BF16, MASK><<<a.W, 256, 0, st>>>(a);
-    else if (s.nt == 2) paged_few_kernel<D, 2, BF16, MASK><<<a.W, 256, 0, st>>>(a);
-    else if (s.rw == 2) return launch_many<D, 2, BF16, MASK>(a, st);
-    else if (s.rw == 4) return launch_many<D, 4, BF16, MASK>(a, st);
-    else return launch_many<D, 8, BF16, MASK>(a, st);
+    if (s.nt == 1) paged_few_kernel<D, 1, BF16, MASK, SEL><<<a.W, 256, 0, st>>>(a);
+    else if (s.nt == 2) paged_few_kernel<D, 2, BF16, MASK, SEL><<<a.W, 256, 0, st>>>(a);
+    else if (s.rw == 2) return launch_many<D, 2, BF16, MASK, SEL>(a, st);
+    else if (s.rw == 4) return launch_many<D, 4, BF16, MASK, SEL>(a, st);
+    else return launch_many<D, 8, BF16, MASK, SEL>(a, st);
     return MA_OK;
 }
 
-template <int D, bool BF16>
+template <int D, bool BF16, bool SEL>
 int launch(const AttnArgs &a, const Shape &s, hipStream_t st) {
-    if (int rc = a.p.mask ? launch_attn<D, BF16, true>(a, s, st) : launch_attn<D, BF16, false>(a, s, st)) return rc;
+    if (int rc = a.p.mask ? launch_attn<D, BF16, true, SEL>(a, s, st) : launch_attn<D, BF16, false, SEL>(a, s, st)) return rc;
     // (a row group of few rows has fewer than its slots hold)
     const int rows = min(s.rows, a.R);
-    if (s.nt) paged_merge_kernel<D, BF16, false><<<dim3(a.B * a.H * a.RG, (rows + 3) / 4), 64 * merge_waves(false), 0, st>>>(a, s.rows);
-    else paged_merge_kernel<D, BF16, true><<<dim3(a.B * a.H * a.RG, (rows + 15) / 16 * 4), 64 * merge_waves(true), 0, st>>>(a, s.rows);
-    return ma_check_launch("ma_paged_attention");
+    if (s.nt) paged_merge_kernel<D, BF16, false, SEL><<<dim3(a.B * a.H * a.RG, (rows + 3) / 4), 64 * merge_waves(false), 0, st>>>(a, s.rows);
+    else paged_merge_kernel<D, BF16, true, SEL><<<dim3(a.B * a.H * a.RG, (rows + 15) / 16 * 4), 64 * merge_waves(true), 0, st>>>(a, s.rows);
+    return ma_check_launch(SEL ? "ma_paged_attention_blocks" : "ma_paged_attention");
 }
 
 }  // namespace
 
-extern "C" int64_t ma_paged_workspace_bytes(int B, int H, int Hq, int T, int D) {
-    if (B <= 0 || H <= 0 || Hq <= 0 || Hq % H || T <= 0 || (D != 64 && D != 128)) return -1;
-    if ((int64_t)(Hq / H) * T > INT32_MAX / 16) return -1;
-    const Shape s = shape_of(Hq / H * T);
-    return (int64_t)B * H * s.RG > INT32_MAX ? -1 : layout_of(s, (int64_t)B * H * s.RG, D).bytes;
+// positions of a run, and runs
+struct Runs {
+    int run, runs;
+};
+static Runs runs_of(int T, int query_block) {
+    const int run = query_block <= 0 || query_block > T ? T : query_block;
+    return {run, (T + run - 1) / run};
 }
 
-extern "C" int ma_paged_attention(ma_tensor4 q, int B, int Hq, int T, int D, const ma_pages *p, int H, ma_tensor4 kc,
-                                  ma_tensor4 vc, const int32_t *new_lens, int causal_block, float scale,
-                                  ma_tensor4 out, void *workspace, int64_t workspace_bytes, void *stream) {
-    const char *who = "ma_paged_attention";
+static int64_t workspace_bytes_of(int B, int H, int Hq, int T, int D, int query_block) {
+    if (B <= 0 || H <= 0 || Hq <= 0 || Hq % H || T <= 0 || (D != 64 && D != 128) || query_block < 0) return -1;
+    const Runs r = runs_of(T, query_block);
+    if ((int64_t)(Hq / H) * r.run > INT32_MAX / 16) return -1;
+    const Shape s = shape_of(Hq / H * r.run);
+    const int64_t groups = (int64_t)s.RG * r.runs;
+    if (groups > INT32_MAX || groups * H > INT32_MAX || groups * H * B > INT32_MAX) return -1;
+    return layout_of(s, (int64_t)B * H * groups, D).bytes;
+}
+
+extern "C" int64_t ma_paged_workspace_bytes(int B, int H, int Hq, int T, int D) {
+    return workspace_bytes_of(B, H, Hq, T, D, 0);
+}
+
+extern "C" int64_t ma_paged_blocks_workspace_bytes(int B, int H, int Hq, int T, int D, int query_block) {
+    return workspace_bytes_of(B, H, Hq, T, D, query_block);
+}
+
+// m: groups of a selected block, 0 where every stored token is read
+static int paged_attention(const char *who, const ma_tensor4 &q, int B, int Hq, int T, int D, const ma_pages *p, int H,
+                           const ma_tensor4 &kc, const ma_tensor4 &vc, const int32_t *new_lens, int causal_block,
+                           float scale, const ma_tensor4 &out, const int32_t *blocks, int count, int m, int query_block,
+                           void *workspace, int64_t workspace_bytes, void *stream) {
     if (int rc = pg_check(p, B, H, D, who)) return rc;
-    const int64_t need = ma_paged_workspace_bytes(B, H, Hq, T, D);
+    const int64_t need = workspace_bytes_of(B, H, Hq, T, D, query_block);
     if (need < 0 || !q.ptr || !out.ptr || causal_block < 0 || (kc.ptr == nullptr) != (vc.ptr == nullptr)) {
         ma_set_error("%s: bad arguments (B=%d H=%d Hq=%d T=%d D=%d causal_block=%d)", who, B, H, Hq, T, D, causal_block);
         return MA_EINVAL;
@@ -1614,22 +1691,25 @@ extern "C" int ma_paged_attention(ma_tensor4 q, int B, int Hq, int T, int D, con
                      (long long)workspace_bytes);
         return MA_EWORKSPACE;
     }
-    const Shape s = shape_of(Hq / H * T);
-    // the line: every request as long as its table row, with room for what the stretches round up
-    const int64_t most = START + s.rows0 + (int64_t)p->width * p->page_tokens / PG_GROUP +
-                         ((1 + (T + PG_GROUP - 1) / PG_GROUP) << s.dense);
-    if (most * B * H * s.RG + 64LL * s.W > INT32_MAX) {
-        ma_set_error("%s: %d requests of up to %lld tokens and %d row groups of each head are not built (2^31 items)", who,
-                     B, (long long)p->width * p->page_tokens, s.RG);
+    const Runs runs = runs_of(T, query_block);
+    const Shape s = shape_of(Hq / H * runs.run);
+    const int64_t RG = (int64_t)s.RG * runs.runs;
+    // the line: every request as long as its table row (and lists), with room for what the stretches round up
+    int64_t groups = (int64_t)p->width * p->page_tokens / PG_GROUP;
+    if (m) groups = min((int64_t)count, (groups + m - 1) / m) * m;
+    const int64_t most = START + s.rows0 + groups + ((1 + (T + PG_GROUP - 1) / PG_GROUP) << s.dense);
+    if (groups > INT32_MAX / 2 || RG * B * H > INT32_MAX || most * B * H * RG + 64LL * s.W > INT32_MAX) {
+        ma_set_error("%s: %d requests of up to %lld tokens and %lld row groups of each head are not built (2^31 items)", who,
+                     B, (long long)p->width * p->page_tokens, (long long)RG);
         return MA_EUNSUPPORTED;
     }
     // the merge: a workgroup a segment (and rows), threads of one dimension below 2^32
-    if ((int64_t)B * H * s.RG * 64 * merge_waves(s.nt == 0) > UINT32_MAX) {
-        ma_set_error("%s: %d requests, %d heads and %d row groups of each are not built (2^%d segments)", who, B, H, s.RG,
-                     s.nt ? 23 : 24);
+    if ((int64_t)B * H * RG * 64 * merge_waves(s.nt == 0) > UINT32_MAX) {
+        ma_set_error("%s: %d requests, %d heads and %lld row groups of each are not built (2^%d segments)", who, B, H,
+                     (long long)RG, s.nt ? 23 : 24);
         return MA_EUNSUPPORTED;
     }
-    const Layout l = layout_of(s, (int64_t)B * H * s.RG, D);
+    const Layout l = layout_of(s, (int64_t)B * H * RG, D);
     char *ws = (char *)workspace;
     AttnArgs a{};
     a.q = q;
@@ -1642,9 +1722,9 @@ extern "C" int ma_paged_attention(ma_tensor4 q, int B, int Hq, int T, int D, con
     a.H = H;
     a.G = Hq / H;
     a.T = T;
-    a.R = a.G * T;
-    a.RG = s.RG;
-    a.HR = H * s.RG;
+    a.R = a.G * runs.run;
+    a.RG = (int)RG;
+    a.HR = H * a.RG;
     a.max_len = p->width * p->page_tokens;
     a.rows0 = s.rows0;
     a.dense = s.dense;
@@ -1656,6 +1736,36 @@ extern "C" int ma_paged_attention(ma_tensor4 q, int B, int Hq, int T, int D, con
     a.wo = (float *)(ws + l.wo);
     a.desc = (int4 *)(ws + l.desc);
     hipStream_t st = (hipStream_t)stream;
-    if (D == 128) return p->dtype == MA_BF16 ? launch<128, true>(a, s, st) : launch<128, false>(a, s, st);
-    return p->dtype == MA_BF16 ? launch<64, true>(a, s, st) : launch<64, false>(a, s, st);
+    if (m) {
+        a.blocks = blocks;
+        a.count = count;
+        a.m = m;
+        a.run = runs.run;
+        a.RGR = s.RG;
+        if (D == 128) return p->dtype == MA_BF16 ? launch<128, true, true>(a, s, st) : launch<128, false, true>(a, s, st);
+        return p->dtype == MA_BF16 ? launch<64, true, true>(a, s, st) : launch<64, false, true>(a, s, st);
+    }
+    if (D == 128) return p->dtype == MA_BF16 ? launch<128, true, false>(a, s, st) : launch<128, false, false>(a, s, st);
+    return p->dtype == MA_BF16 ? launch<64, true, false>(a, s, st) : launch<64, false, false>(a, s, st);
+}
+
+extern "C" int ma_paged_attention(ma_tensor4 q, int B, int Hq, int T, int D, const ma_pages *p, int H, ma_tensor4 kc,
+                                  ma_tensor4 vc, const int32_t *new_lens, int causal_block, float scale,
+                                  ma_tensor4 out, void *workspace, int64_t workspace_bytes, void *stream) {
+    return paged_attention("ma_paged_attention", q, B, Hq, T, D, p, H, kc, vc, new_lens, causal_block, scale, out, nullptr, 0,
+                           0, 0, workspace, workspace_bytes, stream);
+}
+
+extern "C" int ma_paged_attention_blocks(ma_tensor4 q, int B, int Hq, int T, int D, const ma_pages *p, int H, ma_tensor4 kc,
+                                         ma_tensor4 vc, const int32_t *new_lens, int causal_block, float scale,
+                                         ma_tensor4 out, const int32_t *blocks, int count, int block_tokens,
+                                         int query_block, void *workspace, int64_t workspace_bytes, void *stream) {
+    const char *who = "ma_paged_attention_blocks";
+    if (!blocks || count <= 0 || block_tokens <= 0 || block_tokens % PG_GROUP || query_block < 0) {
+        ma_set_error("%s: bad blocks (count=%d block_tokens=%d, a multiple of 32, query_block=%d)", who, count, block_tokens,
+                     query_block);
+        return MA_EINVAL;
+    }
+    return paged_attention(who, q, B, Hq, T, D, p, H, kc, vc, new_lens, causal_block, scale, out, blocks, count,
+                           block_tokens / PG_GROUP, query_block, workspace, workspace_bytes, stream);
 }

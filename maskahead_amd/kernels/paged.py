@@ -421,7 +421,8 @@ def select_blocks(query: torch.Tensor, prefix: PagedPrefix, count: int, *, new_l
 
 def paged_attention(query: torch.Tensor, prefix: PagedPrefix, current_key: torch.Tensor | None = None,
                     current_value: torch.Tensor | None = None, *, new_lens: torch.Tensor | None = None,
-                    scaling: float | None = None, causal_block: int = 0, out: torch.Tensor | None = None):
+                    scaling: float | None = None, causal_block: int = 0, out: torch.Tensor | None = None,
+                    blocks: torch.Tensor | None = None, block_tokens: int = GROUP, query_block: int = 0):
     """softmax over [request b's stored tokens | the block's own keys] for every query row of
     query [B, Hq, T, D] (``splitk_attention`` with one length per request; Hq a multiple of
     Hkv, head_dim 64 or 128, one dtype of bf16 and f16 throughout).
@@ -433,12 +434,28 @@ def paged_attention(query: torch.Tensor, prefix: PagedPrefix, current_key: torch
     sees nothing is zero; what a row does not see may hold anything, NaN and infinities too.  A
     packed value is an f16 here (beyond 65504: infinite).  The same call gives the same bits.
     ``out`` [B, Hq, T, D] (not overlapping the inputs) receives the result; without it a new
-    tensor does, whose rows t >= new_lens[b] are undefined."""
+    tensor does, whose rows t >= new_lens[b] are undefined.
+
+    blocks int32 [B, Hkv, runs, count] (``select_blocks``, with the same block_tokens and query_block)
+    names the stored tokens that each run of query_block positions (0: all T) reads, beside the tail and
+    the block's own keys, in the place of all: entry i is tokens i * block_tokens ... of the request's
+    whole groups of 32.  Entries that are no block (-1) read nothing, entries behind as many as the
+    request has blocks are not looked at, one listed twice weighs twice."""
     shape = _check_block("query", query, prefix)
     b, hq, t, d = shape
     h = prefix.heads
     if h == 0 or hq == 0 or hq % h:
         raise ValueError("Hq must be a positive multiple of Hkv")
+    if blocks is not None:
+        block_tokens, query_block = _c_int("block_tokens", block_tokens), _c_int("query_block", query_block)
+        if not block_tokens or block_tokens % GROUP:
+            raise ValueError(f"block_tokens must be a positive multiple of {GROUP}, got {block_tokens}")
+        runs = -(-t // query_block) if query_block else min(t, 1)
+        if blocks.ndim != 4:
+            raise ValueError(f"blocks must be [{b}, {h}, {runs}, count], got {tuple(blocks.shape)}")
+        _i32(blocks, "blocks", (b, h, runs, blocks.shape[3]), prefix.index)
+    elif query_block:
+        raise ValueError("query_block without blocks")
     if (current_key is None) != (current_value is None):
         raise ValueError("current_key and current_value go together")
     if current_key is not None:
@@ -455,10 +472,20 @@ def paged_attention(query: torch.Tensor, prefix: PagedPrefix, current_key: torch
     if b == 0 or t == 0:
         return out
     scale = float(scaling) if scaling is not None else d ** -0.5
-    need = N.size_query("ma_paged_workspace_bytes", b, h, hq, t, d)
+    if blocks is not None:
+        need = N.size_query("ma_paged_blocks_workspace_bytes", b, h, hq, t, d, query_block)
+    else:
+        need = N.size_query("ma_paged_workspace_bytes", b, h, hq, t, d)
     if need < 0:
         raise N.KernelUnavailableError(f"{hq // h * t} rows for each of {b * h} KV heads are not built")
     ws = torch.empty((need,), device=query.device, dtype=torch.uint8)
+    if blocks is not None:
+        if blocks.shape[3] == 0:
+            blocks = torch.full((b, h, runs, 1), -1, device=query.device, dtype=torch.int32)
+        _call(prefix.index, "ma_paged_attention_blocks", N.t4(query), b, hq, t, d, prefix._nat, h, N.t4(current_key),
+              N.t4(current_value), N.ptr(new_lens), causal_block, scale, N.t4(out), blocks.data_ptr(), blocks.shape[3],
+              block_tokens, query_block, ws.data_ptr(), need)
+        return out
     _call(prefix.index, "ma_paged_attention", N.t4(query), b, hq, t, d, prefix._nat, h, N.t4(current_key),
           N.t4(current_value), N.ptr(new_lens), causal_block, scale, N.t4(out), ws.data_ptr(), need)
     return out

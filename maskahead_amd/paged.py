@@ -180,9 +180,11 @@ class PagedKVCache:
     def attend(self, layer: int, query: torch.Tensor, current_key: torch.Tensor | None = None,
                current_value: torch.Tensor | None = None, *, new_lens: torch.Tensor | None = None,
                scaling: float | None = None, causal_block: int = 0, mask: torch.Tensor | None = None,
-               out: torch.Tensor | None = None, staged: bool = False) -> torch.Tensor:
+               out: torch.Tensor | None = None, staged: bool = False, blocks: torch.Tensor | None = None,
+               block_tokens: int = GROUP, query_block: int = 0) -> torch.Tensor:
         """``paged_attention`` of one layer over [stored | block]; new_lens defaults to that of
-        the append in progress.  RuntimeError between a layer's stage_layer and the commit.
+        the append in progress.  RuntimeError between a layer's stage_layer and the commit.  blocks,
+        block_tokens, query_block: the stored tokens to read (``select``).
 
         staged=True, between the two: over what is stored by then, where every query sees all
         the new tokens (so without current_key, current_value and causal_block).  A group of 32 that
@@ -193,7 +195,8 @@ class PagedKVCache:
             raise ValueError("a staged layer holds the block: no current_key, current_value or causal_block")
         prefix = self._readable(layer, mask, staged)
         return paged_attention(query, prefix, current_key, current_value, new_lens=new_lens, scaling=scaling,
-                               causal_block=causal_block, out=out)
+                               causal_block=causal_block, out=out, blocks=blocks, block_tokens=block_tokens,
+                               query_block=query_block)
 
     def select(self, layer: int, query: torch.Tensor, count: int, *, new_lens: torch.Tensor | None = None,
                mask: torch.Tensor | None = None, staged: bool = False, **how):
