@@ -40,7 +40,7 @@ def _t4(dtype=N.MA_BF16, ptr=4096):
     (E, dict(out=_t4(N.MA_F16))), (U, dict(d=96)), (E, dict(p=dict(pool=None))), (E, dict(q=_t4(ptr=None))),
     # (a head's rows, segments and items that the kernels do not count)
     (E, dict(t=1 << 28)), (U, dict(b=1 << 13, h=32, hq=32, t=64, run=1)),
-    (U, dict(count=1 << 20, b=64, hq=8, t=4, p=dict(width=1 << 24))),
+    (U, dict(count=1 << 20, b=1024, hq=8, t=4, p=dict(width=1 << 24))),
     (N.MA_EWORKSPACE, dict(ws=None)), (N.MA_EWORKSPACE, dict(ws=4100)), (N.MA_EWORKSPACE, dict(bytes=256))])
 def test_bad_lists_are_refused(lib, rc, change):
     a = dict(q=_t4(), b=2, hq=4, t=2, d=64, p={}, h=2, kc=_t4(), vc=_t4(), causal=0, out=_t4(), blocks=4096, count=4, per=64,
