@@ -90,7 +90,7 @@ __device__ __forceinline__ Items items_from(const AttnArgs &a, int n, int len) {
     r.n = n;
     r.len = len;
     r.ng = len / PG_GROUP;
-    if (SEL) r.ng = (int)min((unsigned)a.count, ((unsigned)r.ng + (unsigned)a.m - 1) / (unsigned)a.m) * a.m;
+    if (SEL) r.ng = (int)min((unsigned)a.count, ((unsigned)r.ng + (unsigned)a.m - 1) / (unsigned)a.m) * min(a.m, r.ng);
     r.rem = len % PG_GROUP;
     const int cur = a.kc.ptr ? (n + PG_GROUP - 1) / PG_GROUP : 0;
     const int rows = (r.rem ? 1 : 0) + cur;
@@ -1696,7 +1696,7 @@ static int paged_attention(const char *who, const ma_tensor4 &q, int B, int Hq, 
     const int64_t RG = (int64_t)s.RG * runs.runs;
     // the line: every request as long as its table row (and lists), with room for what the stretches round up
     int64_t groups = (int64_t)p->width * p->page_tokens / PG_GROUP;
-    if (m) groups = min((int64_t)count, (groups + m - 1) / m) * m;
+    if (m) groups = min((int64_t)count, (groups + m - 1) / m) * min((int64_t)m, groups);
     const int64_t most = START + s.rows0 + groups + ((1 + (T + PG_GROUP - 1) / PG_GROUP) << s.dense);
     if (groups > INT32_MAX / 2 || RG * B * H > INT32_MAX || most * B * H * RG + 64LL * s.W > INT32_MAX) {
         ma_set_error("%s: %d requests of up to %lld tokens and %lld row groups of each head are not built (2^31 items)", who,

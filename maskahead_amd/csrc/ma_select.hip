@@ -8,19 +8,17 @@
 // Which blocks are read must not hang on the order of a sum, so the products are of whole numbers:
 // q_c times 2^(13 - e), rounded, where 2^e is the power of two at or below the row's largest (e at
 // least -100), and z_c and 15 s_c times 2^(13 - f) with the group's largest alike (f at least -24).
-// Codes of at most 2^14 are two digits of 7 bits (sign with both), which f16 holds; each of the
-// four products of digits sums to at most 2^22 over 2 D channels, which f32 accumulates without
-// rounding whatever the order (two share an accumulator).  The score, a whole number below 2^37
-// times 2^(e + f - 26), is rounded once, to f32.
+// A code of at most 2^14 is two digits, 256 hi + lo with lo of -128 .. 127, so the product of 8-bit
+// integers computes it: four of digits, each at most 2^22 over 2 D channels.  The score, a whole number
+// below 2^37 times 2^(e + f - 26), is rounded once, to f32.
 #include "ma_pages.h"
 
 using namespace ma;
 
 namespace {
 
-constexpr int SEL_WAVES = 4, SEL_TILES = 4;             // 16 groups a wave; row tiles in LDS at once
-constexpr int SEL_SPAN = 16 * SEL_WAVES;                // groups of a workgroup
-constexpr int ROW_ABSENT = INT32_MIN, ROW_ODD = INT32_MAX;
+constexpr int SEL_WAVES = 4, SEL_TILES = 4;             // row tiles in LDS at once: one a wave
+constexpr int SEL_FEW_ROWS = 32;
 constexpr float LEAST = -3.4028234663852886e38f;
 
 struct SelectArgs {
@@ -32,40 +30,12 @@ struct SelectArgs {
     int32_t *blocks;            // [B, H, runs, count]
     int64_t ngcap, nbcap;
     int B, H, G, T, run, runs, m, count, first, last;
+    int units;                  // workgroups' worth of groups in a batch of requests as long as their table rows
 };
 
 __device__ __forceinline__ int uniform(int x) { return __builtin_amdgcn_readfirstlane(x); }
 __device__ __forceinline__ int new_of(const SelectArgs &a, int b) {
     return a.new_lens ? min(max(a.new_lens[b], 0), a.T) : a.T;
-}
-
-typedef __attribute__((ext_vector_type(2))) __fp16 fp16x2_t;
-__device__ __forceinline__ f16x2_t pk(float a, float b) {      // (whole numbers below 2^11: exact)
-    return __builtin_bit_cast(f16x2_t, __builtin_amdgcn_cvt_pkrtz(a, b));
-}
-// 8 values times scale, rounded to whole numbers, as two digits: code = 128 hi + lo, both of its sign
-__device__ __forceinline__ void digits8(const float (&x)[8], float scale, f16x8_t &hi, f16x8_t &lo) {
-#pragma unroll
-    for (int i = 0; i < 8; i += 2) {
-        float h[2], l[2];
-#pragma unroll
-        for (int k = 0; k < 2; ++k) {
-            const float c = rintf(x[i + k] * scale);
-            h[k] = truncf(c * 0.0078125f);
-            l[k] = __builtin_fmaf(h[k], -128.0f, c);
-        }
-        const f16x2_t hv = pk(h[0], h[1]), lv = pk(l[0], l[1]);
-        hi[i] = hv[0], hi[i + 1] = hv[1];
-        lo[i] = lv[0], lo[i + 1] = lv[1];
-    }
-}
-__device__ __forceinline__ f16x8_t relu(f16x8_t x) { return __builtin_elementwise_max(x, (f16x8_t)(_Float16)0.0f); }
-__device__ __forceinline__ float pow2(int e) { return __uint_as_float((uint32_t)(127 + e) << 23); }
-
-// maximum over the four lanes of a row (lane ^ 16, lane ^ 32)
-__device__ __forceinline__ float max_rows(float v) {
-    const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
-    return ma_max_xor32(fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1])));
 }
 
 template <int DT>
@@ -83,234 +53,379 @@ __device__ __forceinline__ void unpack8(uint4 w, float (&x)[8]) {
     }
 }
 
+typedef __attribute__((ext_vector_type(4))) int i32x4_t;
+// 16 codes x scale, rounded half to even, as digits: the sum with 1.5 2^23 + 128 leaves code + 128 in
+// the lowest 16 bits, whose upper byte is hi, and whose lower is lo + 128.
+__device__ __forceinline__ uint32_t code_bits(float x, float scale) {
+    return __float_as_uint(__builtin_fmaf(x, scale, 12583040.0f));
+}
+// (four codes into byte i of the digits)
+__device__ __forceinline__ void put_digits(uint32_t a, uint32_t b, uint32_t c, uint32_t d, int i, i32x4_t &hi, i32x4_t &lo) {
+    const uint32_t x = __builtin_amdgcn_perm(b, a, 0x05010400u), y = __builtin_amdgcn_perm(d, c, 0x05010400u);
+    lo[i] = (int)(__builtin_amdgcn_perm(y, x, 0x05040100u) ^ 0x80808080u);
+    hi[i] = (int)__builtin_amdgcn_perm(y, x, 0x07060302u);
+}
+// 16 channels of a row (RELU: 0 where they are negative)
+template <int DT>
+__device__ __forceinline__ void row_digits(const uint4 (&w)[2], float scale, bool relu, i32x4_t &hi, i32x4_t &lo) {
+#pragma unroll
+    for (int y = 0; y < 2; ++y) {
+        float v[8];
+        unpack8<DT>(w[y], v);
+        if (relu) {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) v[i] = fmaxf(v[i], 0.0f);
+        }
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+            put_digits(code_bits(v[4 * i], scale), code_bits(v[4 * i + 1], scale), code_bits(v[4 * i + 2], scale),
+                       code_bits(v[4 * i + 3], scale), 2 * y + i, hi, lo);
+    }
+}
+__device__ __forceinline__ i32x4_t mfma_i8(i32x4_t a, i32x4_t b, i32x4_t c) {
+    return __builtin_amdgcn_mfma_i32_16x16x64_i8(a, b, c, 0, 0, 0);
+}
+__device__ __forceinline__ float pow2(int e) { return __uint_as_float((uint32_t)(127 + e) << 23); }
+
+// maximum over the four lanes of a row (lane ^ 16, lane ^ 32)
+__device__ __forceinline__ float max_rows(float v) {
+    const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    return ma_max_xor32(fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1])));
+}
+// Largest magnitude of 16-bit floats, as bits of one: without its sign a float is ordered like a whole
+// number, infinities and NaN above all.
+typedef __attribute__((ext_vector_type(2))) uint16_t u16x2_t;
+__device__ __forceinline__ void most_of(uint4 w, u16x2_t &most) {
+    const uint32_t u[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) most = __builtin_elementwise_max(most, __builtin_bit_cast(u16x2_t, u[i] & 0x7fff7fffu));
+}
+// ... over the four lanes of a row, as f32; not finite: infinite
+template <int DT>
+__device__ __forceinline__ float most_float(u16x2_t most) {
+    const float x = max_rows((float)max(most[0], most[1]));         // (16 bits: a whole number of f32)
+    const uint16_t h = (uint16_t)x;
+    if constexpr (DT == MA_BF16) return h >= 0x7f80 ? INFINITY : ma_bf16_to_f32(h);
+    return h >= 0x7c00 ? INFINITY : ma_f16_to_f32(h);
+}
+
+// a workgroup's work: spans of its groups, runs of positions, heads, requests (fastest to slowest: runs,
+// heads, spans, so that what is under way together reads the same pages)
+struct Unit {
+    int b, len, n;       // request, its stored tokens and new positions; b < 0: behind the last
+    int run, h, span;
+};
+__device__ __forceinline__ Unit find_unit(const SelectArgs &a, int u, int span, int lane) {
+    Unit r{-1, 0, 0, 0, 0, 0};
+    unsigned pre = 0;
+    for (int b0 = 0; b0 < a.B; b0 += 64) {       // 64 requests at a time, the units of those before
+        int len = 0, n = 0;
+        unsigned units = 0;
+        if (b0 + lane < a.B) {
+            len = pg_length(a.p, b0 + lane);
+            n = new_of(a, b0 + lane);
+            units = (unsigned)((len / PG_GROUP + span - 1) / span) * a.H * ((unsigned)(n + a.run - 1) / (unsigned)a.run);
+        }
+        const unsigned inc = pre + ma_wave_prefix_u32(units);
+        const uint64_t here = __ballot((unsigned)u >= inc - units && (unsigned)u < inc);
+        if (here) {
+            const int l = __ffsll((unsigned long long)here) - 1;
+            r.b = b0 + l;
+            r.len = __builtin_amdgcn_readlane(len, l);
+            r.n = __builtin_amdgcn_readlane(n, l);
+            const unsigned rel = (unsigned)u - (unsigned)__builtin_amdgcn_readlane((int)(inc - units), l);
+            const unsigned runs = (unsigned)(r.n + a.run - 1) / (unsigned)a.run, rest = rel / runs;
+            r.run = (int)(rel - rest * runs);
+            r.span = (int)(rest / (unsigned)a.H);
+            r.h = (int)(rest - (unsigned)r.span * (unsigned)a.H);
+            break;
+        }
+        pre = (unsigned)__builtin_amdgcn_readlane((int)inc, 63);
+    }
+    return r;
+}
+
 // ------------------------------------------------------------------ scores of groups
-// A workgroup: 64 groups of one (request, head) and the rows of one run; a wave holds the digits of
-// its 16 groups' parameters and passes all rows by them, whose digits lie in LDS, 64 rows at a time.
-template <int D, int DT>
-__global__ __launch_bounds__(64 * SEL_WAVES, 2) void select_score_kernel(SelectArgs a) {
-    constexpr int KB = D / 32;
-    __shared__ f16x8_t dig[SEL_TILES][2][KB][64];
-    __shared__ int expo[SEL_TILES][16];
+// A workgroup: 64 GW groups of one (request, head) and the rows of one run; a wave holds the digits of
+// its 16 GW groups' parameters and passes all rows by them, whose digits lie in LDS, 64 rows at a time.
+struct RowScale {
+    double by, add;      // a row's power of two and 0; no row: 0 and -inf; one that is not finite: 0 and inf
+};
+template <int D, int DT, int GW>
+__global__ __launch_bounds__(64 * SEL_WAVES, GW == 1 ? 4 : 2) void select_score_kernel(SelectArgs a) {
+    constexpr int KB = D / 64, SPAN = 16 * GW * SEL_WAVES;
+    __shared__ i32x4_t dig[SEL_TILES][4][KB][64];         // hi, lo, and those of the positive codes
+    __shared__ RowScale scales[SEL_TILES][16];
     const int tid = threadIdx.x, lane = tid & 63, wave = uniform(tid >> 6), n16 = lane & 15, hh = lane >> 4;
     const int R = a.G * a.run, tiles = (R + 15) / 16, per = a.p.page_tokens / PG_GROUP;
-    for (int64_t u = blockIdx.x;; u += gridDim.x) {
-        // the unit's request: units of those before it, 64 requests at a time
-        int64_t pre = 0;
-        int b = -1, len = 0, n = 0;
-        for (int b0 = 0; b0 < a.B; b0 += 64) {
-            int own_len = 0, own_n = 0;
-            int64_t units = 0;
-            if (b0 + lane < a.B) {
-                own_len = pg_length(a.p, b0 + lane);
-                own_n = new_of(a, b0 + lane);
-                units = (int64_t)((own_len / PG_GROUP + SEL_SPAN - 1) / SEL_SPAN) * a.H * ((own_n + a.run - 1) / a.run);
-            }
-            const int64_t inc = pre + pg_wave_scan(units, lane);
-            const uint64_t here = __ballot(u >= inc - units && u < inc);
-            if (here) {
-                const int l = __ffsll((unsigned long long)here) - 1;
-                b = b0 + l;
-                len = __builtin_amdgcn_readlane(own_len, l);
-                n = __builtin_amdgcn_readlane(own_n, l);
-                const int64_t before = inc - units;
-                pre = (int64_t)((uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(before >> 32), l) << 32 |
-                                (uint32_t)__builtin_amdgcn_readlane((int)before, l));
-                break;
-            }
-            pre = (int64_t)((uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(inc >> 32), 63) << 32 |
-                            (uint32_t)__builtin_amdgcn_readlane((int)inc, 63));
-        }
-        if (b < 0) return;       // behind the last unit (all waves alike)
-        const int ng = len / PG_GROUP, runs = (n + a.run - 1) / a.run;
-        const int64_t rel = u - pre;
-        const int run = (int)(rel % runs), h = (int)(rel / runs % a.H), span = (int)(rel / runs / a.H);
+    for (int u = blockIdx.x; u < a.units; u += gridDim.x) {
+        const Unit x = find_unit(a, u, SPAN, lane);
+        if (x.b < 0) return;         // (all waves alike)
+        const int b = x.b, h = x.h, n = x.n, ng = x.len / PG_GROUP;
         // the wave's groups
-        const int g = span * SEL_SPAN + 16 * wave + n16, gc = min(g, ng - 1), pg = gc / per;
-        const uint8_t *rec = pg_record(a.p, a.p.table[(int64_t)b * a.p.s_table + pg], gc - pg * per, h, 40 * D);
-        const bool there = rec != nullptr;
-        if (!there) rec = a.p.pool;
-        uint4 sw[KB], zw[KB];
+        const int g0 = x.span * SPAN + 16 * GW * wave + n16;
+        int gi[GW], page[GW];
 #pragma unroll
-        for (int kb = 0; kb < KB; ++kb) {
-            sw[kb] = *(const uint4 *)(rec + 32 * D + 2 * (32 * kb + 8 * hh));
-            zw[kb] = *(const uint4 *)(rec + 34 * D + 2 * (32 * kb + 8 * hh));
+        for (int y = 0; y < GW; ++y) {
+            const int g = min(g0 + 16 * y, ng - 1), pg = g / per;
+            gi[y] = g - pg * per;
+            page[y] = a.p.table[(int64_t)b * a.p.s_table + pg];
         }
-        float top = 0.f;
+        // the rows of tile t (this wave's), or of the only one
+        uint4 w[KB][2];
+        auto load_rows = [&](int t) {
+            const int rc = min(16 * t + n16, R - 1), qh = rc / a.run, pos = x.run * a.run + rc - qh * a.run;
+            const uint16_t *src = (const uint16_t *)a.q.ptr + (int64_t)b * a.q.s[0] + (int64_t)(h * a.G + qh) * a.q.s[1] +
+                                  (int64_t)min(pos, a.T - 1) * a.q.s[2] + 16 * hh;
 #pragma unroll
-        for (int kb = 0; kb < KB; ++kb) {
-            float s[8], z[8];
-            unpack8<MA_F16>(sw[kb], s);
-            unpack8<MA_F16>(zw[kb], z);
+            for (int kb = 0; kb < KB; ++kb)
 #pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                // (a NaN becomes infinite, so that the maximum shows it)
-                const float x = fmaxf(fabsf(15.0f * s[i]), fabsf(z[i]));
-                top = s[i] != s[i] || z[i] != z[i] ? INFINITY : fmaxf(top, x);
+                for (int y = 0; y < 2; ++y) w[kb][y] = pg_load16(src + 64 * kb + 8 * y);
+        };
+        load_rows(tiles == 1 ? 0 : wave);       // (behind the last tile: the last row)
+        bool live[GW];
+        uint4 sw[GW][KB][2], zw[GW][KB][2];
+#pragma unroll
+        for (int y = 0; y < GW; ++y) {
+            const uint8_t *rec = pg_record(a.p, page[y], gi[y], h, 40 * D);
+            live[y] = rec != nullptr;
+            if (!rec) rec = a.p.pool;
+#pragma unroll
+            for (int kb = 0; kb < KB; ++kb)
+#pragma unroll
+                for (int z = 0; z < 2; ++z) {
+                    sw[y][kb][z] = *(const uint4 *)(rec + 32 * D + 2 * (64 * kb + 16 * hh + 8 * z));
+                    zw[y][kb][z] = *(const uint4 *)(rec + 34 * D + 2 * (64 * kb + 16 * hh + 8 * z));
+                }
+        }
+        if (a.p.mask) {
+#pragma unroll
+            for (int y = 0; y < GW; ++y) {
+                const bool any = pg_mask_bits(a.p, b, h, min(g0 + 16 * y, ng - 1) * PG_GROUP + 8 * hh) != 0;
+                live[y] = live[y] && max_rows(any ? 1.f : 0.f) != 0.f;
             }
         }
-        top = max_rows(top);
-        const bool odd = top == INFINITY;
-        const int f = max((int)(__float_as_uint(top) >> 23) - 127, -24);
-        const float scale = odd ? 0.f : pow2(13 - f);
-        f16x8_t zh[KB], zl[KB], sh[KB], sl[KB];
+        // the rows' digits into LDS: a tile a wave, or 64 channels of the only one, as they are or the positive ones
+        auto put_rows = [&](int t0) {
+            const int t = tiles == 1 ? 0 : wave;
+            if (t0 + t >= tiles || (tiles == 1 && wave >= 2 * KB)) return;
+            u16x2_t most{};
 #pragma unroll
-        for (int kb = 0; kb < KB; ++kb) {
-            float x[8];
-            unpack8<MA_F16>(zw[kb], x);
-            digits8(x, scale, zh[kb], zl[kb]);
-            unpack8<MA_F16>(sw[kb], x);
-            digits8(x, 15.0f * scale, sh[kb], sl[kb]);
+            for (int kb = 0; kb < KB; ++kb) most_of(w[kb][0], most), most_of(w[kb][1], most);
+            const float mx = most_float<DT>(most);
+            const bool odd = mx == INFINITY;
+            const int e = max((int)(__float_as_uint(mx) >> 23) - 127, -100);
+            const float scale = odd ? 0.f : pow2(13 - e);
+#pragma unroll
+            for (int kb = 0; kb < KB; ++kb)
+#pragma unroll
+                for (int relu = 0; relu < 2; ++relu) {
+                    if (tiles == 1 && kb + KB * relu != wave) continue;
+                    i32x4_t hi, lo;
+                    row_digits<DT>(w[kb], scale, relu, hi, lo);
+                    dig[t][2 * relu][kb][lane] = hi;
+                    dig[t][2 * relu + 1][kb][lane] = lo;
+                }
+            const int row = 16 * (t0 + t) + n16, pos = x.run * a.run + row % a.run;
+            const bool none = row >= R || pos >= n;
+            if (hh == 0) scales[t][n16] = RowScale{none || odd ? 0.0 : (double)pow2(e), none ? -INFINITY : odd ? INFINITY : 0.0};
+        };
+        __syncthreads();         // the unit's before is read
+        put_rows(0);
+        i32x4_t zh[GW][KB], zl[GW][KB], sh[GW][KB], sl[GW][KB];
+        int f[GW];
+        bool odd[GW];
+#pragma unroll
+        for (int y = 0; y < GW; ++y) {
+            u16x2_t ms{}, mz{};
+#pragma unroll
+            for (int kb = 0; kb < KB; ++kb)
+#pragma unroll
+                for (int z = 0; z < 2; ++z) most_of(sw[y][kb][z], ms), most_of(zw[y][kb][z], mz);
+            const float top = fmaxf(15.0f * most_float<MA_F16>(ms), most_float<MA_F16>(mz));
+            odd[y] = top == INFINITY;
+            f[y] = max((int)(__float_as_uint(top) >> 23) - 127, -24);
+            const float scale = odd[y] ? 0.f : pow2(13 - f[y]);
+#pragma unroll
+            for (int kb = 0; kb < KB; ++kb) {
+                row_digits<MA_F16>(zw[y][kb], scale, false, zh[y][kb], zl[y][kb]);
+                row_digits<MA_F16>(sw[y][kb], 15.0f * scale, false, sh[y][kb], sl[y][kb]);
+            }
         }
-        bool live = there;
-        if (a.p.mask) {
-            const bool any = pg_mask_bits(a.p, b, h, gc * PG_GROUP + 8 * hh) != 0;
-            live = live && max_rows(any ? 1.f : 0.f) != 0.f;
-        }
-        float best = -INFINITY;
+        // (the rows' largest exact score, before the group's power of two)
+        double best[GW];
+#pragma unroll
+        for (int y = 0; y < GW; ++y) best[y] = -INFINITY;
         for (int t0 = 0; t0 < tiles; t0 += SEL_TILES) {
-            __syncthreads();          // the rows before are read
-            for (int t = wave; t < min(SEL_TILES, tiles - t0); t += SEL_WAVES) {
-                const int row = 16 * (t0 + t) + n16, rc = min(row, R - 1), qh = rc / a.run, pos = run * a.run + rc - qh * a.run;
-                const uint16_t *src = (const uint16_t *)a.q.ptr + (int64_t)b * a.q.s[0] + (int64_t)(h * a.G + qh) * a.q.s[1] +
-                                      (int64_t)min(pos, a.T - 1) * a.q.s[2] + 8 * hh;
-                uint4 w[KB];
-#pragma unroll
-                for (int kb = 0; kb < KB; ++kb) w[kb] = pg_load16(src + 32 * kb);
-                float mx = 0.f;
-#pragma unroll
-                for (int kb = 0; kb < KB; ++kb) {
-                    float x[8];
-                    unpack8<DT>(w[kb], x);
-#pragma unroll
-                    for (int i = 0; i < 8; ++i) mx = x[i] != x[i] ? INFINITY : fmaxf(mx, fabsf(x[i]));
-                }
-                mx = max_rows(mx);
-                const bool odd_row = mx == INFINITY;
-                const int e = max((int)(__float_as_uint(mx) >> 23) - 127, -100);
-                const float qs = odd_row ? 0.f : pow2(13 - e);
-#pragma unroll
-                for (int kb = 0; kb < KB; ++kb) {
-                    float x[8];
-                    f16x8_t hi, lo;
-                    unpack8<DT>(w[kb], x);
-                    digits8(x, qs, hi, lo);
-                    dig[t][0][kb][lane] = hi;
-                    dig[t][1][kb][lane] = lo;
-                }
-                if (hh == 0) expo[t][n16] = row >= R || pos >= n ? ROW_ABSENT : odd_row ? ROW_ODD : e;
+            if (t0) {
+                __syncthreads();          // the rows before are read
+                put_rows(t0);
             }
             __syncthreads();
+            if (t0 + SEL_TILES < tiles) load_rows(t0 + SEL_TILES + wave);
             for (int t = 0; t < min(SEL_TILES, tiles - t0); ++t) {
-                f32x4_t c2{}, c1{}, c0{};
+                i32x4_t c2[GW], c1[GW], c0[GW];
+#pragma unroll
+                for (int y = 0; y < GW; ++y) c2[y] = c1[y] = c0[y] = i32x4_t{};
 #pragma unroll
                 for (int kb = 0; kb < KB; ++kb) {
-                    const f16x8_t qh = dig[t][0][kb][lane], ql = dig[t][1][kb][lane], rh = relu(qh), rl = relu(ql);
-                    c2 = __builtin_amdgcn_mfma_f32_16x16x32_f16(qh, zh[kb], c2, 0, 0, 0);
-                    c1 = __builtin_amdgcn_mfma_f32_16x16x32_f16(qh, zl[kb], c1, 0, 0, 0);
-                    c1 = __builtin_amdgcn_mfma_f32_16x16x32_f16(ql, zh[kb], c1, 0, 0, 0);
-                    c0 = __builtin_amdgcn_mfma_f32_16x16x32_f16(ql, zl[kb], c0, 0, 0, 0);
-                    c2 = __builtin_amdgcn_mfma_f32_16x16x32_f16(rh, sh[kb], c2, 0, 0, 0);
-                    c1 = __builtin_amdgcn_mfma_f32_16x16x32_f16(rh, sl[kb], c1, 0, 0, 0);
-                    c1 = __builtin_amdgcn_mfma_f32_16x16x32_f16(rl, sh[kb], c1, 0, 0, 0);
-                    c0 = __builtin_amdgcn_mfma_f32_16x16x32_f16(rl, sl[kb], c0, 0, 0, 0);
+                    const i32x4_t qh = dig[t][0][kb][lane], ql = dig[t][1][kb][lane];
+                    const i32x4_t rh = dig[t][2][kb][lane], rl = dig[t][3][kb][lane];
+#pragma unroll
+                    for (int y = 0; y < GW; ++y) {
+                        c1[y] = mfma_i8(qh, zl[y][kb], c1[y]);
+                        c2[y] = mfma_i8(qh, zh[y][kb], c2[y]);
+                        c0[y] = mfma_i8(ql, zl[y][kb], c0[y]);
+                        c1[y] = mfma_i8(ql, zh[y][kb], c1[y]);
+                        c2[y] = mfma_i8(rh, sh[y][kb], c2[y]);
+                        c1[y] = mfma_i8(rh, sl[y][kb], c1[y]);
+                        c0[y] = mfma_i8(rl, sl[y][kb], c0[y]);
+                        c1[y] = mfma_i8(rl, sh[y][kb], c1[y]);
+                    }
                 }
-                // lane (n, h): rows 4 h + r by group n
+                // lane (n, h): rows 4 h + r by group n (256 c1 + c0 is below 2^31)
 #pragma unroll
                 for (int r = 0; r < 4; ++r) {
-                    const int e = expo[t][4 * hh + r];
-                    const double s = (double)c2[r] * 16384.0 + ((double)c1[r] * 128.0 + (double)c0[r]);
-                    float v = fmaxf((float)__builtin_ldexp(s, (e == ROW_ODD || e == ROW_ABSENT ? 0 : e) + f - 26), LEAST);
-                    if (odd || e == ROW_ODD) v = INFINITY;
-                    if (e != ROW_ABSENT) best = fmaxf(best, v);
+                    const RowScale e = scales[t][4 * hh + r];
+#pragma unroll
+                    for (int y = 0; y < GW; ++y) {
+                        const double s = __builtin_fma((double)c2[y][r], 65536.0, (double)(c1[y][r] * 256 + c0[y][r]));
+                        best[y] = __builtin_fmax(best[y], __builtin_fma(s, e.by, e.add));
+                    }
                 }
             }
         }
-        best = max_rows(best);
-        if (hh == 0 && g < ng)
-            a.group[(((int64_t)b * a.H + h) * a.runs + run) * a.ngcap + g] = live ? best : -INFINITY;
+#pragma unroll
+        for (int y = 0; y < GW; ++y) {
+            float v = best[y] == -INFINITY ? -INFINITY : fmaxf((float)__builtin_ldexp(best[y], f[y] - 26), LEAST);
+            v = max_rows(odd[y] && v > -INFINITY ? INFINITY : v);
+            const int g = g0 + 16 * y;
+            if (hh == 0 && g < ng)
+                a.group[(((int64_t)b * a.H + h) * a.runs + x.run) * a.ngcap + g] = live[y] ? v : -INFINITY;
+        }
     }
 }
 
 // ------------------------------------------------------------------ selection
 // One workgroup a (request, head, run): the count largest block scores, ties to the lowest index, in
 // ascending order.  A key is the score's place in the order of floats, 0 for no block; blocks that are
-// always taken stand outside the search.  The search counts keys in 1 024 equal ranges between the
-// smallest and the largest, then within the range that the last one lies in, and so on: three
-// turns at most, and scores alike do not meet in one counter as they would by their leading bits.
-constexpr int SEL_BINS = 1024;
+// always taken stand outside the search.  The search counts keys in equal ranges between the
+// smallest and the largest, four a thread, then within the range that the last one lies in, and so on:
+// three turns (1 024 ranges: four) at most, mostly one, as a range that is taken whole ends it; and scores
+// alike do not meet in one counter as they would by their leading bits.
 constexpr uint32_t KEY_TAKEN = 0xffffffffu;
 
 template <int THREADS>
 struct TopShared {
-    uint32_t bin[SEL_BINS], wsum[2][THREADS / 64], red[2][THREADS / 64];
+    static constexpr int WAVES = THREADS / 64, BINS = 4 * THREADS;
+    uint32_t bin[BINS], red[4][WAVES], sum[WAVES], pick[2][WAVES];
     uint32_t at, above, in;
 };
-
-// sum of the threads before this one, and of all; both of two counts
-template <int THREADS>
-__device__ __forceinline__ void block_scan(TopShared<THREADS> &sh, uint32_t x, uint32_t y, uint32_t &bx, uint32_t &by,
-                                           uint32_t &tx, uint32_t &ty) {
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    const uint32_t ix = ma_wave_prefix_u32(x), iy = ma_wave_prefix_u32(y);
-    __syncthreads();
-    if (lane == 63) sh.wsum[0][wave] = ix, sh.wsum[1][wave] = iy;
-    __syncthreads();
-    bx = ix - x, by = iy - y, tx = ty = 0;
-#pragma unroll
-    for (int w = 0; w < THREADS / 64; ++w) {
-        if (w < wave) bx += sh.wsum[0][w], by += sh.wsum[1][w];
-        tx += sh.wsum[0][w];
-        ty += sh.wsum[1][w];
-    }
+// the waves' values of one array, one a lane (0 behind the last)
+template <int WAVES>
+__device__ __forceinline__ uint32_t of_waves(const uint32_t (&x)[WAVES], int lane) {
+    const uint32_t v = x[min(lane, WAVES - 1)];
+    return lane < WAVES ? v : 0;
+}
+// what the waves before this one have, and all
+__device__ __forceinline__ void wave_offsets(uint32_t v, int wave, uint32_t &before, uint32_t &all) {
+    const uint32_t inc = ma_wave_prefix_u32(v);
+    before = wave ? (uint32_t)__builtin_amdgcn_readlane((int)inc, wave - 1) : 0;
+    all = (uint32_t)__builtin_amdgcn_readlane((int)inc, 63);
 }
 
-// PER > 0: a thread keeps its keys, at most PER; 0: they are read again in every turn
+// PER > 0: a thread keeps its keys, at most PER, of at most THREADS * PER blocks; 0: they are read again in
+// every turn.  Scores are read a wave's width at a time and handed over in LDS (dynamic, THREADS * PER keys)
+// to the threads that hold PER neighbours; the first are asked for before the request's length is known.
 template <int THREADS, int PER>
 __global__ __launch_bounds__(THREADS) void select_top_kernel(SelectArgs a) {
-    __shared__ TopShared<THREADS> sh;
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    using Shared = TopShared<THREADS>;
+    constexpr int BINS = Shared::BINS, BPT = BINS / THREADS, BIN_BITS = THREADS == 256 ? 10 : 12;
+    static_assert(BINS == 1 << BIN_BITS, "ranges are told apart by a shift");
+    __shared__ Shared sh;
+    extern __shared__ uint32_t all_keys[];
+    const int tid = threadIdx.x, lane = tid & 63, wave = uniform(tid >> 6);
     const int64_t row = blockIdx.x;
-    const int run = (int)(row % a.runs), b = (int)(row / a.runs / a.H);
-    const int n = new_of(a, b), ng = run * a.run < n ? pg_length(a.p, b) / PG_GROUP : 0, nb = (ng + a.m - 1) / a.m;
     const float *group = a.group + row * a.ngcap;
+    constexpr int U = PER < 8 ? PER : 8;             // blocks of a thread whose loads are under way together
+    float v[U ? U : 1][2];
+    // groups j and j + 1 of blocks y0 THREADS + tid + ..., below `blocks` and `groups` (a last one twice)
+    auto load = [&](int y0, int j, int blocks, int groups) {
+#pragma unroll
+        for (int y = 0; y < U; ++y)
+#pragma unroll
+            for (int z = 0; z < 2; ++z)
+                v[y][z] = group[min(min(tid + (y0 + y) * THREADS, blocks - 1) * a.m + min(j + z, a.m - 1), groups - 1)];
+    };
+    if constexpr (PER > 0) load(0, 0, (int)a.nbcap, (int)a.ngcap);
+    const int run = (int)((unsigned)blockIdx.x % (unsigned)a.runs), b = (int)((unsigned)blockIdx.x / (unsigned)a.runs / (unsigned)a.H);
+    const int n = new_of(a, b), len = pg_length(a.p, b), ng = run * a.run < n ? len / PG_GROUP : 0;
+    const int nb = (int)((unsigned)(ng + a.m - 1) / (unsigned)a.m);
+#pragma unroll
+    for (int y = 0; y < BPT; ++y) sh.bin[tid + y * THREADS] = 0;
     // this thread's blocks [i0, i1)
     const int each = (nb + THREADS - 1) / THREADS, i0 = min(tid * each, nb), i1 = min(i0 + each, nb);
-    auto score_of = [&](int i) {
-        float s = -INFINITY;
-        for (int y = i * a.m; y < min((i + 1) * a.m, ng); ++y) s = fmaxf(s, group[y]);
-        return s;
-    };
     auto key_of = [&](int i, float s) -> uint32_t {
         if (s == -INFINITY) return 0;
         return i < a.first || i >= nb - a.last ? KEY_TAKEN : ma_order_key(s);
     };
     uint32_t key[PER ? PER : 1];
     uint32_t lo = 0xffffffffu, hi = 0, some = 0, taken = 0;
-    auto note = [&](int i, uint32_t k) {
+    auto note = [&](uint32_t k) {
         if (k == 0) return;
         ++some;
         if (k == KEY_TAKEN) ++taken;
         else lo = min(lo, k), hi = max(hi, k);
     };
+    auto score_of = [&](int i) {
+        float s = -INFINITY;
+        for (int y = i * a.m; y < min((i + 1) * a.m, ng); ++y) s = fmaxf(s, group[y]);
+        return s;
+    };
     if constexpr (PER > 0) {
-        float s[PER];
 #pragma unroll
-        for (int y = 0; y < PER; ++y) s[y] = i0 + y < i1 ? score_of(i0 + y) : -INFINITY;
+        for (int y0 = 0; y0 < PER; y0 += U) {
+            if (y0 * THREADS >= nb) break;
+            float s[U];
 #pragma unroll
-        for (int y = 0; y < PER; ++y) {
-            key[y] = i0 + y < i1 ? key_of(i0 + y, s[y]) : 0;
-            note(i0 + y, key[y]);
-            if (a.scores && i0 + y < i1) a.scores[row * a.nbcap + i0 + y] = s[y];
+            for (int y = 0; y < U; ++y) s[y] = -INFINITY;
+            for (int j = 0; j < min(a.m, ng); j += 2) {
+                if (y0 + j > 0) load(y0, j, nb, ng);
+#pragma unroll
+                for (int y = 0; y < U; ++y)
+#pragma unroll
+                    for (int z = 0; z < 2; ++z) {
+                        // (what was asked for early may lie behind the length)
+                        const int i = tid + (y0 + y) * THREADS;
+                        if (i < nb && i * a.m + min(j + z, a.m - 1) < ng) s[y] = fmaxf(s[y], v[y][z]);
+                    }
+            }
+#pragma unroll
+            for (int y = 0; y < U; ++y) {
+                const int i = tid + (y0 + y) * THREADS;
+                const uint32_t k = i < nb ? key_of(i, s[y]) : 0;
+                all_keys[i] = k;
+                note(k);
+                if (a.scores && i < nb) a.scores[row * a.nbcap + i] = s[y];
+            }
         }
     } else {
         for (int i = i0; i < i1; ++i) {
             const float s = score_of(i);
-            note(i, key_of(i, s));
+            note(key_of(i, s));
             if (a.scores) a.scores[row * a.nbcap + i] = s;
         }
     }
-    if (a.scores)
-        for (int64_t i = nb + tid; i < a.nbcap; i += THREADS) a.scores[row * a.nbcap + i] = -INFINITY;
+    some = ma_wave_sum_u32(some);
+    taken = ma_wave_sum_u32(taken);
+    lo = ma_wave_max_u32(~lo);
+    hi = ma_wave_max_u32(hi);
+    if (lane == 0) sh.red[0][wave] = some, sh.red[1][wave] = taken, sh.red[2][wave] = lo, sh.red[3][wave] = hi;
+    __syncthreads();
+    if constexpr (PER > 0) {
+#pragma unroll
+        for (int y = 0; y < PER; ++y) key[y] = i0 + y < i1 ? all_keys[i0 + y] : 0;
+    }
     auto each_key = [&](auto f) {
         if constexpr (PER > 0) {
 #pragma unroll
@@ -319,42 +434,44 @@ __global__ __launch_bounds__(THREADS) void select_top_kernel(SelectArgs a) {
             for (int i = i0; i < i1; ++i) f(i, key_of(i, score_of(i)));
         }
     };
-    uint32_t before, before2, all, forced;
-    block_scan<THREADS>(sh, some, taken, before, before2, all, forced);
-    const uint32_t wlo = ~ma_wave_max_u32(~lo), whi = ma_wave_max_u32(hi);
-    if (lane == 0) sh.red[0][wave] = wlo, sh.red[1][wave] = whi;
-    __syncthreads();
-#pragma unroll
-    for (int w = 0; w < THREADS / 64; ++w) lo = min(lo, sh.red[0][w]), hi = max(hi, sh.red[1][w]);
+    const uint32_t all = ma_wave_sum_u32(of_waves(sh.red[0], lane)), forced = ma_wave_sum_u32(of_waves(sh.red[1], lane));
+    lo = ~ma_wave_max_u32(of_waves(sh.red[2], lane));
+    hi = ma_wave_max_u32(of_waves(sh.red[3], lane));
     // what is taken: keys above cut, and the first `ties` of those equal to it
     uint32_t cut = 0, ties = 0;
     const uint32_t want = min((uint32_t)a.count, all);
     if (want < all) {
         uint32_t need = want - min(forced, want);
         if (need == 0) cut = KEY_TAKEN - 1;
-        while (need) {
+        for (bool again = false; need; again = true) {
+            if (again) {
+#pragma unroll
+                for (int y = 0; y < BPT; ++y) sh.bin[tid + y * THREADS] = 0;
+                __syncthreads();
+            }
             const uint32_t range = hi - lo;
-            const int bits = range ? 32 - __builtin_clz(range) : 0, s = max(bits - 10, 0);
-            for (int i = tid; i < SEL_BINS; i += THREADS) sh.bin[i] = 0;
-            __syncthreads();
+            const int bits = range ? 32 - __builtin_clz(range) : 0, s = max(bits - BIN_BITS, 0);
             each_key([&](int, uint32_t k) {
                 if (k >= lo && k <= hi && k != 0) atomicAdd(&sh.bin[(k - lo) >> s], 1u);
             });
             __syncthreads();
-            // bins from the top, BPT a thread: the one in which the need-th lies
-            constexpr int BPT = SEL_BINS / THREADS;
+            // ranges from the top, BPT a thread: the one in which the need-th lies
             uint32_t c[BPT], sum = 0;
 #pragma unroll
             for (int y = 0; y < BPT; ++y) {
-                c[y] = sh.bin[SEL_BINS - 1 - (tid * BPT + y)];
+                c[y] = sh.bin[BINS - 1 - (tid * BPT + y)];
                 sum += c[y];
             }
-            uint32_t above, unused, total, unused2;
-            block_scan<THREADS>(sh, sum, 0, above, unused, total, unused2);
+            const uint32_t inc = ma_wave_prefix_u32(sum);
+            if (lane == 63) sh.sum[wave] = inc;
+            __syncthreads();
+            uint32_t above, total;
+            wave_offsets(of_waves(sh.sum, lane), wave, above, total);
+            above += inc - sum;
 #pragma unroll
             for (int y = 0; y < BPT; ++y) {
                 if (above < need && need <= above + c[y]) {
-                    sh.at = SEL_BINS - 1 - (tid * BPT + y);
+                    sh.at = BINS - 1 - (tid * BPT + y);
                     sh.above = above;
                     sh.in = c[y];
                 }
@@ -373,7 +490,6 @@ __global__ __launch_bounds__(THREADS) void select_top_kernel(SelectArgs a) {
                 ties = need;
                 break;
             }
-            __syncthreads();             // at, above and in are read
         }
     }
     uint32_t over = 0, equal = 0;
@@ -381,8 +497,14 @@ __global__ __launch_bounds__(THREADS) void select_top_kernel(SelectArgs a) {
         if (k > cut) ++over;
         else if (k == cut && k != 0) ++equal;
     });
-    uint32_t ob, eb, ot, et;
-    block_scan<THREADS>(sh, over, equal, ob, eb, ot, et);
+    const uint32_t oi = ma_wave_prefix_u32(over), ei = ma_wave_prefix_u32(equal);
+    if (lane == 63) sh.pick[0][wave] = oi, sh.pick[1][wave] = ei;
+    __syncthreads();
+    uint32_t ob, eb, unused;
+    wave_offsets(of_waves(sh.pick[0], lane), wave, ob, unused);
+    wave_offsets(of_waves(sh.pick[1], lane), wave, eb, unused);
+    ob += oi - over;
+    eb += ei - equal;
     int32_t *out = a.blocks + row * a.count;
     each_key([&](int i, uint32_t k) {
         if (k > cut) {
@@ -394,13 +516,32 @@ __global__ __launch_bounds__(THREADS) void select_top_kernel(SelectArgs a) {
         }
     });
     for (int i = (int)want + tid; i < a.count; i += THREADS) out[i] = -1;
+    if (a.scores)
+        for (int64_t i = nb + tid; i < a.nbcap; i += THREADS) a.scores[row * a.nbcap + i] = -INFINITY;
 }
 
 int64_t align256(int64_t x) { return (x + 255) / 256 * 256; }
 
+// groups of a wave: 16 of few rows, whose time is that of the loads, 32 of many
+int groups_of(int rows) { return rows <= SEL_FEW_ROWS ? 1 : 2; }
 template <int D, int DT>
 void launch_score(const SelectArgs &a, unsigned grid, hipStream_t st) {
-    select_score_kernel<D, DT><<<grid, 64 * SEL_WAVES, 0, st>>>(a);
+    if (groups_of(a.G * a.run) == 1) select_score_kernel<D, DT, 1><<<grid, 64 * SEL_WAVES, 0, st>>>(a);
+    else select_score_kernel<D, DT, 2><<<grid, 64 * SEL_WAVES, 0, st>>>(a);
+}
+template <int THREADS, int PER>
+int launch_top(const SelectArgs &a, unsigned rows, hipStream_t st) {
+    constexpr int LDS = THREADS * PER * 4;
+    if (LDS > 48 * 1024) {
+        const hipError_t e = hipFuncSetAttribute((const void *)select_top_kernel<THREADS, PER>,
+                                                 hipFuncAttributeMaxDynamicSharedMemorySize, LDS);
+        if (e != hipSuccess) {
+            ma_set_error("ma_select_blocks: %d bytes of LDS refused: %s", LDS, hipGetErrorString(e));
+            return MA_EHIP;
+        }
+    }
+    select_top_kernel<THREADS, PER><<<rows, THREADS, LDS, st>>>(a);
+    return MA_OK;
 }
 
 }  // namespace
@@ -458,14 +599,23 @@ extern "C" int ma_select_blocks(ma_tensor4 q, int B, int Hq, int T, int D, const
     a.count = count;
     a.first = keep_first;
     a.last = keep_last;
-    const int64_t rows = (int64_t)B * H * runs, units = rows * ((a.ngcap + SEL_SPAN - 1) / SEL_SPAN);
+    const int span = 16 * groups_of(a.G * run) * SEL_WAVES;
+    const int64_t rows = (int64_t)B * H * runs, units = rows * ((a.ngcap + span - 1) / span);
+    if (units > INT32_MAX / 2) {
+        ma_set_error("%s: %lld selections over %lld tokens are not built (2^30 times %d groups)", who, (long long)rows,
+                     (long long)tokens, span);
+        return MA_EUNSUPPORTED;
+    }
+    a.units = (int)units;
     const unsigned grid = (unsigned)min(units, (int64_t)ma_num_cus() * 4);
     hipStream_t st = (hipStream_t)stream;
     if (D == 128) p->dtype == MA_BF16 ? launch_score<128, MA_BF16>(a, grid, st) : launch_score<128, MA_F16>(a, grid, st);
     else p->dtype == MA_BF16 ? launch_score<64, MA_BF16>(a, grid, st) : launch_score<64, MA_F16>(a, grid, st);
     if (int rc = ma_check_launch(who)) return rc;
-    if (a.nbcap <= 256 * 4) select_top_kernel<256, 4><<<(unsigned)rows, 256, 0, st>>>(a);
-    else if (a.nbcap <= 256 * 16) select_top_kernel<256, 16><<<(unsigned)rows, 256, 0, st>>>(a);
-    else select_top_kernel<1024, 0><<<(unsigned)rows, 1024, 0, st>>>(a);
-    return ma_check_launch(who);
+    int rc;
+    if (a.nbcap <= 1024) rc = launch_top<256, 4>(a, (unsigned)rows, st);
+    else if (a.nbcap <= 4096) rc = launch_top<1024, 4>(a, (unsigned)rows, st);
+    else if (a.nbcap <= 32768) rc = launch_top<1024, 32>(a, (unsigned)rows, st);
+    else rc = launch_top<1024, 0>(a, (unsigned)rows, st);
+    return rc ? rc : ma_check_launch(who);
 }

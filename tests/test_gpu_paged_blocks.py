@@ -282,3 +282,19 @@ def test_refused_lists(gpu):
     assert paged_attention(q[:, :, :0], p, blocks=ok[:, :, :0]).shape == (2, 4, 0, 128)
     blocks = select_blocks(q, p, 4)
     assert paged_attention(q, p, blocks=blocks).shape == q.shape
+
+
+@pytest.mark.parametrize("per", [2048, 2 ** 31 - 32])
+def test_blocks_longer_than_requests(gpu, per):
+    lens = [0, 40, 1000, 320]
+    r = Requests(gpu, lens, h=1, d=64, page=32)
+    q = torch.randn((4, 2, 1, 64), generator=r.gen).to(BF)
+    lists, scores = select_blocks(q.to(gpu), r.cache.prefixes[0], 3, block_tokens=per, return_scores=True)
+    assert lists[:, 0, 0].tolist() == [[-1] * 3] + [[0, -1, -1]] * 3 and scores.shape[3] == 1
+    for b, x in enumerate(lens[1:], 1):
+        s = group_scores(r.cache.pool[0].cpu(), r.cache.block_table[b].tolist(), x // 32, 0, q[b, :, 0])
+        assert scores[b, 0, 0, 0] == torch.tensor(max(s), dtype=torch.float64).float()
+    out = paged_attention(q.to(gpu), r.cache.prefixes[0], blocks=lists, block_tokens=per)
+    assert torch.equal(out, paged_attention(q.to(gpu), r.cache.prefixes[0], blocks=lists[..., :1].contiguous(), block_tokens=per))
+    full = paged_attention(q.to(gpu), r.cache.prefixes[0])
+    assert ((out.double() - full.double()).abs() <= 2 * torch.finfo(BF).eps * full.double().abs() + 2.0 ** -9).all()
