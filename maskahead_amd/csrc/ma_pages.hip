@@ -290,30 +290,86 @@ __device__ __forceinline__ uint32_t f16x2_bits(float a, float b) {
     return __builtin_bit_cast(uint32_t, v);
 }
 
-// A keys wave's rows of 4 channels, turned at their positions: row i is new token t0 + i (below 0: a
-// row of the old tail, turned when it was new).  The partners of channels i lie dim / 8 lanes on.
-template <int D, int DT, int N>
-__device__ __forceinline__ void turn_rows(const RotaryDev &r, int first, int t0, int lane, uint2 (&x)[N]) {
-    constexpr int CL = D / 4;
-    const int c4 = lane % CL, q = r.dim / 8, ch = 4 * c4;
-    const bool turned = ch < r.dim, ahead = c4 >= q;
-    const int partner = turned && !r.next ? (ahead ? lane - q : lane + q) : lane;
-    const int at = !turned ? 0 : r.next ? 2 * c4 : ahead ? ch - 4 * q : ch;
+// All 128 channels turned, halves in neighbouring rows of 16 lanes, positions that the table holds: a lane
+// reads the 4 cosines or sines that lie where its channels lie, and both halves' values are swapped by
+// lane moves.  The table's rows are asked for before the keys, all 32 of a group together.
+template <int N>
+struct TableRows {
+    f32x4_t v[N];
+};
+template <int D>
+__device__ __forceinline__ bool table_in_step(const RotaryDev &r, int64_t p0) {
+    return D == 128 && !r.next && r.dim == D && p0 >= 0 && p0 + PG_GROUP <= r.rows && r.s_row >= 0 && r.s_row < 1 << 24;
+}
+template <int N>
+__device__ __forceinline__ void table_rows(const RotaryDev &r, int64_t p0, int first, int ch, TableRows<N> &t) {
+    const float *base = r.table + p0 * r.s_row;
+    const uint32_t off = (uint32_t)first * (uint32_t)r.s_row + (uint32_t)ch;
+#pragma unroll
+    for (int i = 0; i < N; ++i) t.v[i] = *(const f32x4_t *)(base + i * r.s_row + off);
+}
+template <int DT, int N>
+__device__ __forceinline__ void turn_in_step(const TableRows<N> &t, int t0, int lane, uint2 (&x)[N]) {
+    const bool ahead = lane & 16;
+    const uint32_t sign = ahead ? 0u : 0x80000000u;
+    auto swap = [](uint32_t v) { return __builtin_amdgcn_permlane16_swap(v, v, false, false); };
 #pragma unroll
     for (int i = 0; i < N; ++i) {
-        const float *row = rotary_row(r, first, max(t0 + i, 0)) + at;
-        uint2 y;
-        if (r.next) {
-            typedef __attribute__((ext_vector_type(2))) float f32x2_t;
-            const f32x2_t c = *(const f32x2_t *)row, s = *(const f32x2_t *)(row + r.dim / 2);
-            y = uint2{rotary_pair<DT>(x[i].x, c[0], s[0]), rotary_pair<DT>(x[i].y, c[1], s[1])};
-        } else {
-            const f32x4_t c = *(const f32x4_t *)row, s = *(const f32x4_t *)(row + r.dim / 2);
-            const uint2 z = {(uint32_t)__shfl((int)x[i].x, partner), (uint32_t)__shfl((int)x[i].y, partner)};
-            y = uint2{rotary_halves<DT>(x[i].x, z.x, c[0], c[1], s[0], s[1], ahead),
-                      rotary_halves<DT>(x[i].y, z.y, c[2], c[3], s[2], s[3], ahead)};
+        float c[4], g[4];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            const auto cs = swap(__float_as_uint(t.v[i][k]));
+            c[k] = __uint_as_float(cs[0]);
+            g[k] = __uint_as_float(cs[1] ^ sign);
         }
-        if (turned && t0 + i >= 0) x[i] = y;
+        const auto a = swap(x[i].x), b = swap(x[i].y);
+        const uint2 y = {rotary_halves<DT>(x[i].x, ahead ? a[0] : a[1], c[0], c[1], g[0], g[1]),
+                         rotary_halves<DT>(x[i].y, ahead ? b[0] : b[1], c[2], c[3], g[2], g[3])};
+        if (t0 + i >= 0) x[i] = y;
+    }
+}
+
+// A keys wave's rows of 4 channels, turned at their positions: row i of a lane is new token t0 + first + i
+// (below 0: a row of the old tail, turned when it was new).  The partners of channels i lie dim / 8 lanes
+// on.  Where the table holds the group's 32 positions their rows follow one another from a scalar base, a
+// quarter of the instructions of an address for each.
+template <int D, int DT, int N>
+__device__ __forceinline__ void turn_rows(const RotaryDev &r, int pos, int t0, int first, int lane, uint2 (&x)[N]) {
+    constexpr int CL = D / 4;
+    typedef __attribute__((ext_vector_type(2))) float f32x2_t;
+    const int c4 = lane % CL, q = r.dim / 8, ch = 4 * c4, half = r.dim / 2;
+    const bool turned = ch < r.dim, ahead = c4 >= q;
+    const int partner = turned && !r.next ? (ahead ? lane - q : lane + q) : lane;
+    const int at = !turned ? 0 : r.next ? 2 * c4 : ahead ? ch - half : ch;
+    const uint32_t sign = ahead ? 0u : 0x80000000u;
+    const int64_t p0 = (int64_t)pos + t0;
+    const bool inside = p0 >= 0 && p0 + PG_GROUP <= r.rows && r.s_row >= 0 && r.s_row < 1 << 24;
+    const float *base = r.table + (inside ? p0 * r.s_row : 0);
+    auto rows = [&](auto row_of) {
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            const float *row = row_of(i);
+            uint2 y;
+            if (r.next) {
+                const f32x2_t c = *(const f32x2_t *)row, s = *(const f32x2_t *)(row + half);
+                y = uint2{rotary_pair<DT>(x[i].x, c[0], s[0]), rotary_pair<DT>(x[i].y, c[1], s[1])};
+            } else {
+                const f32x4_t c = *(const f32x4_t *)row, s = *(const f32x4_t *)(row + half);
+                const uint2 z = {(uint32_t)__shfl((int)x[i].x, partner), (uint32_t)__shfl((int)x[i].y, partner)};
+                float g[4];
+#pragma unroll
+                for (int k = 0; k < 4; ++k) g[k] = __uint_as_float(__float_as_uint(s[k]) ^ sign);
+                y = uint2{rotary_halves<DT>(x[i].x, z.x, c[0], c[1], g[0], g[1]),
+                          rotary_halves<DT>(x[i].y, z.y, c[2], c[3], g[2], g[3])};
+            }
+            if (turned && t0 + first + i >= 0) x[i] = y;
+        }
+    };
+    if (inside) {
+        const uint32_t off = (uint32_t)first * (uint32_t)r.s_row + (uint32_t)at;
+        rows([&](int i) { return base + i * r.s_row + off; });
+    } else {
+        rows([&](int i) { return rotary_row(r, pos, max(t0 + first + i, 0)) + at; });
     }
 }
 
@@ -366,8 +422,22 @@ __global__ __launch_bounds__(256) void page_append_kernel(AppendArgs a) {
         if (!val) {
             const int c4 = lane % CL, sl = lane / CL, odd = c4 & 1;
             uint2 x[TPL];
-            rows(sl * TPL, TPL, 4 * c4, [&](int i, const uint16_t *src) { x[i] = pg_load8(src); });
-            if constexpr (ROT) turn_rows<D, DT>(a.rot, a.rot.first[b], j0 + sl * TPL, lane, x);
+            auto keys = [&] { rows(sl * TPL, TPL, 4 * c4, [&](int i, const uint16_t *src) { x[i] = pg_load8(src); }); };
+            if constexpr (ROT) {
+                const int pos = a.rot.first[b];
+                if (table_in_step<D>(a.rot, (int64_t)pos + j0)) {
+                    TableRows<TPL> t;
+                    table_rows(a.rot, (int64_t)pos + j0, sl * TPL, 4 * c4, t);
+                    __builtin_amdgcn_sched_barrier(0);
+                    keys();
+                    turn_in_step<DT>(t, j0 + sl * TPL, lane, x);
+                } else {
+                    keys();
+                    turn_rows<D, DT>(a.rot, pos, j0, sl * TPL, lane, x);
+                }
+            } else {
+                keys();
+            }
             float lo[4], hi[4];
 #pragma unroll
             for (int c = 0; c < 4; ++c) lo[c] = INFINITY, hi[c] = -INFINITY;

@@ -54,13 +54,13 @@ __device__ __forceinline__ float rotary_turn(float x, float c, float y, float s)
     return a + b;
 }
 
-// two channels x and their partners y (ahead: the partners are the first of the pairs)
+// two channels x and their partners y (the first of the pairs: with -s)
 template <int DT>
-__device__ __forceinline__ uint32_t rotary_halves(uint32_t x, uint32_t y, float c0, float c1, float s0, float s1, bool ahead) {
+__device__ __forceinline__ uint32_t rotary_halves(uint32_t x, uint32_t y, float c0, float c1, float s0, float s1) {
     float x0, x1, y0, y1;
     rotary_unpack<DT>(x, x0, x1);
     rotary_unpack<DT>(y, y0, y1);
-    return rotary_pack<DT>(rotary_turn(x0, c0, ahead ? y0 : -y0, s0), rotary_turn(x1, c1, ahead ? y1 : -y1, s1));
+    return rotary_pack<DT>(rotary_turn(x0, c0, y0, s0), rotary_turn(x1, c1, y1, s1));
 }
 // two channels that are a pair
 template <int DT>
@@ -81,8 +81,8 @@ __device__ __forceinline__ void rotary_unit(uint4 &a, uint4 &b, const float (&c)
             bw[i] = rotary_pair<DT>(bw[i], c[4 + i], s[4 + i]);
         } else {
             const uint32_t x = aw[i], y = bw[i];
-            aw[i] = rotary_halves<DT>(x, y, c[2 * i], c[2 * i + 1], s[2 * i], s[2 * i + 1], false);
-            bw[i] = rotary_halves<DT>(y, x, c[2 * i], c[2 * i + 1], s[2 * i], s[2 * i + 1], true);
+            aw[i] = rotary_halves<DT>(x, y, c[2 * i], c[2 * i + 1], -s[2 * i], -s[2 * i + 1]);
+            bw[i] = rotary_halves<DT>(y, x, c[2 * i], c[2 * i + 1], s[2 * i], s[2 * i + 1]);
         }
     }
     a = uint4{aw[0], aw[1], aw[2], aw[3]};
