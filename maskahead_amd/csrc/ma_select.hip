@@ -406,14 +406,14 @@ __global__ __launch_bounds__(THREADS) void select_top_kernel(SelectArgs a) {
                 const uint32_t k = i < nb ? key_of(i, s[y]) : 0;
                 all_keys[i] = k;
                 note(k);
-                if (a.scores && i < nb) a.scores[row * a.nbcap + i] = s[y];
+                if (a.scores && a.scores != a.group && i < nb) a.scores[row * a.nbcap + i] = s[y];
             }
         }
     } else {
         for (int i = i0; i < i1; ++i) {
             const float s = score_of(i);
             note(key_of(i, s));
-            if (a.scores) a.scores[row * a.nbcap + i] = s;
+            if (a.scores && a.scores != a.group) a.scores[row * a.nbcap + i] = s;
         }
     }
     some = ma_wave_sum_u32(some);
@@ -575,7 +575,9 @@ extern "C" int ma_select_blocks(ma_tensor4 q, int B, int Hq, int T, int D, const
         ma_set_error("%s: %d rows of %d heads, or 2^31 selections, are not built", who, run, Hq / H);
         return MA_EUNSUPPORTED;
     }
-    if (!workspace || workspace_bytes < need || (uintptr_t)workspace % 256) {
+    // blocks of one group: the groups' scores are the blocks', where they are asked for
+    const bool same = scores && block_tokens == PG_GROUP;
+    if (!same && (!workspace || workspace_bytes < need || (uintptr_t)workspace % 256)) {
         ma_set_error("%s: workspace of %lld bytes (256-byte aligned) needed, got %lld", who, (long long)need,
                      (long long)workspace_bytes);
         return MA_EWORKSPACE;
@@ -584,7 +586,7 @@ extern "C" int ma_select_blocks(ma_tensor4 q, int B, int Hq, int T, int D, const
     a.q = q;
     a.p = pages_dev(p);
     a.new_lens = new_lens;
-    a.group = (float *)workspace;
+    a.group = same ? scores : (float *)workspace;
     a.scores = scores;
     a.blocks = blocks;
     a.ngcap = tokens / PG_GROUP;
