@@ -455,9 +455,10 @@ int ma_paged_attention(ma_tensor4 q, int B, int Hq, int T, int D, const ma_pages
  * own keys]: entry i stands for tokens i block_tokens ... (a multiple of 32) of the request's whole groups
  * of 32 (ma_select_blocks lists them so, in any order here).  Entries below 0 or behind the request's
  * last block are none; one listed twice weighs twice.  No more than the first ceil(whole groups /
- * block) entries are looked at.  workspace: ma_paged_blocks_workspace_bytes() bytes.  MA_EUNSUPPORTED as
- * there, with every run's row groups and what the lists hold. */
-int64_t ma_paged_blocks_workspace_bytes(int B, int H, int Hq, int T, int D, int query_block);
+ * block) entries are looked at.  workspace: ma_paged_blocks_workspace_bytes() bytes, which may be 0 (it is
+ * not looked at then).  One or two launches.  MA_EUNSUPPORTED: 2^23 segments (requests x heads x runs x row
+ * groups) or more, 2^29 groups of a list. */
+int64_t ma_paged_blocks_workspace_bytes(int B, int H, int Hq, int T, int D, int count, int block_tokens, int query_block);
 int ma_paged_attention_blocks(ma_tensor4 q, int B, int Hq, int T, int D, const ma_pages *p, int H, ma_tensor4 kc,
                               ma_tensor4 vc, const int32_t *new_lens, int causal_block, float scale, ma_tensor4 out,
                               const int32_t *blocks, int count, int block_tokens, int query_block, void *workspace,

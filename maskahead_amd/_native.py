@@ -126,7 +126,7 @@ SIGNATURES = {
     "ma_select_workspace_bytes": (_I64, [_I, _I, _I, _I64]),
     "ma_select_blocks": (_I, [_T4, _I, _I, _I, _I, _PAGES, _I, _P, _I, _I, _I, _I, _I, _P, _P, _P, _I64, _P]),
     "ma_paged_workspace_bytes": (_I64, [_I, _I, _I, _I, _I]),
-    "ma_paged_blocks_workspace_bytes": (_I64, [_I, _I, _I, _I, _I, _I]),
+    "ma_paged_blocks_workspace_bytes": (_I64, [_I, _I, _I, _I, _I, _I, _I, _I]),
     "ma_paged_attention_blocks": (_I, [_T4, _I, _I, _I, _I, _PAGES, _I, _T4, _T4, _P, _I, _F, _T4, _P, _I, _I, _I, _P, _I64,
                                        _P]),
     "ma_paged_attention": (_I, [_T4, _I, _I, _I, _I, _PAGES, _I, _T4, _T4, _P, _I, _F, _T4, _P, _I64, _P]),

@@ -63,6 +63,7 @@ struct AttnArgs {
     // a run (R = G run), and RG = runs * RGR.
     const int32_t *blocks;    // [B, H, runs, count]
     int count, m, run, RGR;   // entries of a list, groups of a block
+    int parts;                // workgroups of a segment
 };
 
 // values that every lane holds alike, as scalars
@@ -84,28 +85,27 @@ constexpr int START = 8;
 struct Items {
     int n, len, ng, rem, items;      // ng: packed items
 };
+// (seen: the block's keys that any row of a segment sees)
 template <bool SEL>
-__device__ __forceinline__ Items items_from(const AttnArgs &a, int n, int len) {
+__device__ __forceinline__ Items items_from(const AttnArgs &a, int n, int len, int seen = 0) {
     Items r;
     r.n = n;
     r.len = len;
     r.ng = len / PG_GROUP;
     if (SEL) r.ng = (int)min((unsigned)a.count, ((unsigned)r.ng + (unsigned)a.m - 1) / (unsigned)a.m) * min(a.m, r.ng);
     r.rem = len % PG_GROUP;
-    const int cur = a.kc.ptr ? (n + PG_GROUP - 1) / PG_GROUP : 0;
+    const int cur = a.kc.ptr ? ((SEL ? seen : n) + PG_GROUP - 1) / PG_GROUP : 0;
     const int rows = (r.rem ? 1 : 0) + cur;
-    r.items = n ? START + r.ng + (rows ? a.rows0 + (rows << a.dense) : 0) : 0;
+    r.items = n ? (SEL ? 0 : START) + r.ng + (rows ? a.rows0 + (rows << a.dense) : 0) : 0;
     return r;
 }
-template <bool SEL>
 __device__ __forceinline__ Items items_of(const AttnArgs &a, int b) {
-    return items_from<SEL>(a, a.new_lens ? min(max(a.new_lens[b], 0), a.T) : a.T, min(max(a.p.lengths[b], 0), a.max_len));
+    return items_from<false>(a, a.new_lens ? min(max(a.new_lens[b], 0), a.T) : a.T, min(max(a.p.lengths[b], 0), a.max_len));
 }
 // ... of a request that the whole wave looks at
-template <bool SEL>
 __device__ __forceinline__ Items items_at(const AttnArgs &a, int b) {
-    const Items r = items_of<SEL>(a, b);
-    return items_from<SEL>(a, uniform(r.n), uniform(r.len));
+    const Items r = items_of(a, b);
+    return items_from<false>(a, uniform(r.n), uniform(r.len));
 }
 // positions of a segment's rows: row = query head * positions + position
 template <bool SEL>
@@ -606,13 +606,13 @@ __device__ __forceinline__ void cut_line(const AttnArgs &a, Stretch &r, int tota
 }
 // Items of all requests, by a scan of the lengths in every workgroup (8 B a request, from L2): of
 // up to 64 requests in every wave, without a barrier
-template <int THREADS, bool SEL>
+template <int THREADS>
 __device__ __forceinline__ Stretch find_stretch(const AttnArgs &a, ScanShared &sh, int unit) {
     constexpr int NW = THREADS / 64;
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     Stretch r;
     if (a.B <= 64) {
-        const Items own = lane < a.B ? items_of<SEL>(a, lane) : Items{};
+        const Items own = lane < a.B ? items_of(a, lane) : Items{};
         const int inc = (int)ma_wave_prefix_u32((uint32_t)own.items);
         cut_line(a, r, __builtin_amdgcn_readlane(inc, 63) * a.HR, unit);
         const int want = (int)((unsigned)r.s / (unsigned)a.HR);
@@ -621,7 +621,7 @@ __device__ __forceinline__ Stretch find_stretch(const AttnArgs &a, ScanShared &s
         const int l = here ? __ffsll((unsigned long long)here) - 1 : 0;
         r.b = l;
         r.pre = __builtin_amdgcn_readlane(inc - own.items, l);
-        r.it = items_from<SEL>(a, __builtin_amdgcn_readlane(own.n, l), __builtin_amdgcn_readlane(own.len, l));
+        r.it = items_from<false>(a, __builtin_amdgcn_readlane(own.n, l), __builtin_amdgcn_readlane(own.len, l));
         return r;
     }
     const int per = (a.B + THREADS - 1) / THREADS, first = tid * per;
@@ -629,7 +629,7 @@ __device__ __forceinline__ Stretch find_stretch(const AttnArgs &a, ScanShared &s
     Items own{};   // of this thread's first request
     for (int i = 0; i < per; ++i)
         if (first + i < a.B) {
-            const Items it = items_of<SEL>(a, first + i);
+            const Items it = items_of(a, first + i);
             if (i == 0) own = it;
             sum += it.items;
         }
@@ -648,7 +648,7 @@ __device__ __forceinline__ Stretch find_stretch(const AttnArgs &a, ScanShared &s
         int pre = before, b = first;
         while (want >= pre + own.items) {
             pre += own.items;
-            own = items_of<SEL>(a, ++b);
+            own = items_of(a, ++b);
         }
         sh.b = b;
         sh.pre = pre;
@@ -658,7 +658,7 @@ __device__ __forceinline__ Stretch find_stretch(const AttnArgs &a, ScanShared &s
     __syncthreads();
     r.b = uniform(sh.b);
     r.pre = uniform(sh.pre);
-    r.it = items_from<SEL>(a, uniform(sh.n), uniform(sh.len));
+    r.it = items_from<false>(a, uniform(sh.n), uniform(sh.len));
     return r;
 }
 
@@ -670,7 +670,12 @@ struct Part {
     bool first, whole;       // the segment begins here; all of it lies here
     int slot;                // of its partial, where it is not whole: the first or the last of the stretch
 };
-template <bool SEL>
+// items of work before place i of a segment, whose first `start` items are none (one of 16-bit rows lies
+// where it begins)
+__device__ __forceinline__ int work_before(const AttnArgs &a, const Items &it, int start, int i) {
+    const int u = max(i - start, 0), over = u - it.ng - a.rows0;
+    return over <= 0 ? min(u, it.ng) : it.ng + ((over + (1 << a.dense) - 1) >> a.dense);
+}
 __device__ __forceinline__ Part part_of(const AttnArgs &a, const Stretch &st, int pos) {
     Part p;
     const int rel = pos - a.HR * st.pre;
@@ -679,20 +684,11 @@ __device__ __forceinline__ Part part_of(const AttnArgs &a, const Stretch &st, in
     p.h = a.RG == 1 ? p.hr : (int)((unsigned)p.hr / (unsigned)a.RG);
     p.rg = p.hr - p.h * a.RG;
     p.run = p.t0 = 0;
-    if (SEL) {
-        p.run = (int)((unsigned)p.rg / (unsigned)a.RGR);
-        p.rg -= p.run * a.RGR;
-        p.t0 = p.run * a.run;
-    }
     p.next = pos + i1 - i0;
     p.first = i0 == 0;
     p.whole = i0 == 0 && i1 == st.it.items;
-    auto work = [&](int i) {     // items of work before place i (one of 16-bit rows lies where it begins)
-        const int u = max(i - START, 0), over = u - st.it.ng - a.rows0;
-        return over <= 0 ? min(u, st.it.ng) : st.it.ng + ((over + (1 << a.dense) - 1) >> a.dense);
-    };
-    p.i0 = work(i0);
-    p.i1 = work(i1);
+    p.i0 = work_before(a, st.it, START, i0);
+    p.i1 = work_before(a, st.it, START, i1);
     p.slot = 2 * st.w + (pos > st.s ? 1 : 0);
     return p;
 }
@@ -703,13 +699,62 @@ __device__ __forceinline__ void note_segment(const AttnArgs &a, const Stretch &s
     const int n = p.whole ? 0 : (int)((unsigned)(pos + st.it.items - 1) / (unsigned)st.chunk) - st.w + 1;
     a.desc[(int64_t)st.b * a.HR + p.hr] = int4{p.slot, n, st.w, 0};
 }
-template <bool SEL>
 __device__ __forceinline__ void next_part(const AttnArgs &a, Stretch &st, const Part &p, int &pos) {
     pos = p.next;
     if (pos >= st.e || pos - a.HR * st.pre < a.HR * st.it.items) return;
     st.pre += st.it.items;
-    do st.it = items_at<SEL>(a, ++st.b);
+    do st.it = items_at(a, ++st.b);
     while (st.it.items == 0);
+}
+
+// Over selected blocks every segment holds about as many items as its list, so no line is cut: a segment
+// has a.parts workgroups of equal shares, known from the workgroup's number and its request's length.
+// False: a run behind the new tokens.
+__device__ __forceinline__ bool own_part(const AttnArgs &a, int unit, Stretch &st, Part &p) {
+    // (workgroups of one XCD next to one another: runs of a head list the same pages)
+    const unsigned w = (unsigned)(blockIdx.x % 8) * (gridDim.x / 8) + blockIdx.x / 8;
+    const unsigned seg = w / (unsigned)a.parts, part = w - seg * a.parts;
+    if (seg >= (unsigned)a.B * a.HR) return false;
+    st = Stretch{};
+    st.b = (int)(seg / (unsigned)a.HR);
+    p.hr = (int)(seg - (unsigned)st.b * a.HR);
+    p.h = (int)((unsigned)p.hr / (unsigned)a.RG);
+    p.rg = p.hr - p.h * a.RG;
+    p.run = (int)((unsigned)p.rg / (unsigned)a.RGR);
+    p.rg -= p.run * a.RGR;
+    p.t0 = p.run * a.run;
+    const int n = a.new_lens ? min(max(a.new_lens[st.b], 0), a.T) : a.T, len = min(max(a.p.lengths[st.b], 0), a.max_len);
+    if (p.t0 >= n) return false;
+    Items it{};
+    it.n = n;
+    it.len = len;
+    st.it = items_from<true>(a, n, len, keys_seen(a, it, min(p.t0 + a.run, n) - 1));
+    const int share = max((((st.it.items + a.parts - 1) / a.parts) + unit - 1) / unit, 1) * unit;
+    p.first = false;
+    p.whole = a.parts == 1;
+    p.i0 = work_before(a, st.it, 0, min((int)part * share, st.it.items));
+    p.i1 = work_before(a, st.it, 0, min((int)(part + 1) * share, st.it.items));
+    p.slot = (int)w;
+    return true;
+}
+// The parts of a workgroup, one after the other: of its stretch, or its own alone
+template <int THREADS, bool SEL>
+__device__ __forceinline__ bool first_part(const AttnArgs &a, ScanShared &sh, int unit, Stretch &st, Part &p, int &pos) {
+    if constexpr (SEL) return own_part(a, unit, st, p);
+    st = find_stretch<THREADS>(a, sh, unit);
+    pos = st.s;
+    if (pos >= st.e) return false;
+    p = part_of(a, st, pos);
+    return true;
+}
+template <bool SEL>
+__device__ __forceinline__ bool another_part(const AttnArgs &a, Stretch &st, Part &p, int &pos) {
+    if (SEL) return false;
+    note_segment(a, st, p, pos);
+    next_part(a, st, p, pos);
+    if (pos >= st.e) return false;
+    p = part_of(a, st, pos);
+    return true;
 }
 
 // The records of a wave's next 64 packed items, one a lane: items first, first + EVERY, ... below
@@ -843,16 +888,12 @@ __global__ __launch_bounds__(256, 2) void paged_few_kernel(AttnArgs a) {
     constexpr int CB = D / 32, NC = D / 16;
     __shared__ FewShared<D, NT> sh;
     const int tid = threadIdx.x, lane = tid & 63, wave = uniform(tid >> 6), n16 = lane & 15, hh = lane >> 4;
-    Stretch st = find_stretch<256, SEL>(a, sh.scan, WAVES);
-    int pos = st.s;
-    while (pos < st.e) {
+    Stretch st;
+    Part pt;
+    int pos;
+    for (bool more = first_part<256, SEL>(a, sh.scan, WAVES, st, pt, pos); more; more = another_part<SEL>(a, st, pt, pos)) {
         const Items it = st.it;
-        const Part pt = part_of<SEL>(a, st, pos);
         const int b = st.b, h = pt.h, row0 = pt.rg * NT * 16, t0 = pt.t0;
-        if (SEL && t0 >= it.n) {           // a run behind the new tokens
-            next_part<SEL>(a, st, pt, pos);
-            continue;
-        }
         uint4 q[NT][CB];
         float c[NT];
         Tile<D> t[NT];
@@ -1085,8 +1126,6 @@ __global__ __launch_bounds__(256, 2) void paged_few_kernel(AttnArgs a) {
                 }
             }
         }
-        note_segment(a, st, pt, pos);
-        next_part<SEL>(a, st, pt, pos);
     }
 }
 
@@ -1139,16 +1178,12 @@ __global__ __launch_bounds__(512, 2) void paged_many_kernel(AttnArgs a) {
     const int rw = wave % RW, tw = wave / RW;
     const int si = wave >> 1;              // the item of a step that this wave unpacks (STEP and more: none)
     const bool sv = wave & 1;              // its values (else its keys)
-    Stretch st = find_stretch<512, SEL>(a, sh.scan, STEP);
-    int pos = st.s;
-    while (pos < st.e) {
+    Stretch st;
+    Part pt;
+    int pos;
+    for (bool more = first_part<512, SEL>(a, sh.scan, STEP, st, pt, pos); more; more = another_part<SEL>(a, st, pt, pos)) {
         const Items it = st.it;
-        const Part pt = part_of<SEL>(a, st, pos);
         const int b = st.b, h = pt.h, row0 = pt.rg * (2 * RW * 16) + rw * 32, t0 = pt.t0;
-        if (SEL && t0 >= it.n) {           // a run behind the new tokens
-            next_part<SEL>(a, st, pt, pos);
-            continue;
-        }
         const bool busy = row0 < a.R;      // this wave has rows
         uint4 q[2][CB];
         float c[2];
@@ -1456,8 +1491,6 @@ __global__ __launch_bounds__(512, 2) void paged_many_kernel(AttnArgs a) {
                 }
             }
         }
-        note_segment(a, st, pt, pos);
-        next_part<SEL>(a, st, pt, pos);
     }
 }
 
@@ -1483,7 +1516,7 @@ __global__ __launch_bounds__(64 * merge_waves(TILES)) void paged_merge_kernel(At
     const int n = a.new_lens ? min(max(a.new_lens[b], 0), a.T) : a.T;
     const int h = hr / a.RG, run = SEL ? (hr - h * a.RG) / a.RGR : 0, rg = hr - h * a.RG - (SEL ? run * a.RGR : 0);
     const int t0 = SEL ? run * a.run : 0;
-    const int4 d = a.desc[blockIdx.x];
+    const int4 d = SEL ? int4{(int)blockIdx.x * a.parts, a.parts, 0, 0} : a.desc[blockIdx.x];
     if ((n <= t0) | (d.y == 0)) return;      // (no new tokens: nobody wrote its segments)
     const int grp = threadIdx.x >> 6, u = threadIdx.x & 63;
     const int x = TILES ? 4 * (blockIdx.y & 3) + (u >> 4) : u & 15;
@@ -1502,7 +1535,7 @@ __global__ __launch_bounds__(64 * merge_waves(TILES)) void paged_merge_kernel(At
 #pragma unroll
             for (int z = 0; z < 2; ++z) {
                 const int k = min(k0 + z * GR, d.y - 1);
-                const int64_t at = (k ? 2 * (int64_t)(d.z + k) : (int64_t)d.x) * rows;
+                const int64_t at = (SEL ? (int64_t)d.x + k : k ? 2 * (int64_t)(d.z + k) : (int64_t)d.x) * rows;
                 pm[z] = a.wm[at + rt];
                 pl[z] = a.wl[at + rt];
 #pragma unroll
@@ -1596,14 +1629,20 @@ int64_t align256(int64_t x) { return (x + 255) / 256 * 256; }
 struct Layout {
     int64_t wl, wo, desc, bytes;   // wm at 0
 };
-Layout layout_of(const Shape &s, int64_t segments, int D) {
-    const int64_t rows = 2LL * s.W * s.rows;
+Layout layout_of(const Shape &s, int64_t segments, int64_t slots, int D) {
+    const int64_t rows = slots * s.rows;
     Layout l;
     l.wl = align256(rows * 4);
     l.wo = l.wl + align256(rows * 4);
     l.desc = l.wo + align256(rows * D * 4);
     l.bytes = l.desc + align256(segments * sizeof(int4));
     return l;
+}
+
+// (SEL: a multiple of 8, for the XCDs)
+template <bool SEL>
+unsigned grid_of(const AttnArgs &a) {
+    return SEL ? ((unsigned)a.B * a.HR * a.parts + 7) / 8 * 8 : (unsigned)a.W;
 }
 
 template <int D, int RW, bool BF16, bool MASK, bool SEL>
@@ -1618,14 +1657,14 @@ int launch_many(const AttnArgs &a, hipStream_t st) {
             return MA_EHIP;
         }
     }
-    paged_many_kernel<D, RW, BF16, MASK, SEL><<<a.W, 512, LDS, st>>>(a);
+    paged_many_kernel<D, RW, BF16, MASK, SEL><<<grid_of<SEL>(a), 512, LDS, st>>>(a);
     return MA_OK;
 }
 
 template <int D, bool BF16, bool MASK, bool SEL>
 int launch_attn(const AttnArgs &a, const Shape &s, hipStream_t st) {
-    if (s.nt == 1) paged_few_kernel<D, 1, BF16, MASK, SEL><<<a.W, 256, 0, st>>>(a);
-    else if (s.nt == 2) paged_few_kernel<D, 2, BF16, MASK, SEL><<<a.W, 256, 0, st>>>(a);
+    if (s.nt == 1) paged_few_kernel<D, 1, BF16, MASK, SEL><<<grid_of<SEL>(a), 256, 0, st>>>(a);
+    else if (s.nt == 2) paged_few_kernel<D, 2, BF16, MASK, SEL><<<grid_of<SEL>(a), 256, 0, st>>>(a);
     else if (s.rw == 2) return launch_many<D, 2, BF16, MASK, SEL>(a, st);
     else if (s.rw == 4) return launch_many<D, 4, BF16, MASK, SEL>(a, st);
     else return launch_many<D, 8, BF16, MASK, SEL>(a, st);
@@ -1635,6 +1674,7 @@ int launch_attn(const AttnArgs &a, const Shape &s, hipStream_t st) {
 template <int D, bool BF16, bool SEL>
 int launch(const AttnArgs &a, const Shape &s, hipStream_t st) {
     if (int rc = a.p.mask ? launch_attn<D, BF16, true, SEL>(a, s, st) : launch_attn<D, BF16, false, SEL>(a, s, st)) return rc;
+    if (SEL && a.parts == 1) return ma_check_launch("ma_paged_attention_blocks");      // (nothing to join)
     // (a row group of few rows has fewer than its slots hold)
     const int rows = min(s.rows, a.R);
     if (s.nt) paged_merge_kernel<D, BF16, false, SEL><<<dim3(a.B * a.H * a.RG, (rows + 3) / 4), 64 * merge_waves(false), 0, st>>>(a, s.rows);
@@ -1644,31 +1684,48 @@ int launch(const AttnArgs &a, const Shape &s, hipStream_t st) {
 
 }  // namespace
 
-// positions of a run, and runs
-struct Runs {
-    int run, runs;
+// What a call over selected blocks is cut into (count 0: over all): positions of a run, runs, row groups of
+// all runs, segments, workgroups of a segment.
+struct Plan {
+    Shape s;
+    int run, parts;
+    int64_t runs, RG, segments;
+    Layout l;
 };
-static Runs runs_of(int T, int query_block) {
-    const int run = query_block <= 0 || query_block > T ? T : query_block;
-    return {run, (T + run - 1) / run};
-}
+// Items that a workgroup's share holds at least.
+constexpr int FEW_SHARE = 8, MANY_SHARE = 16;
 
-static int64_t workspace_bytes_of(int B, int H, int Hq, int T, int D, int query_block) {
-    if (B <= 0 || H <= 0 || Hq <= 0 || Hq % H || T <= 0 || (D != 64 && D != 128) || query_block < 0) return -1;
-    const Runs r = runs_of(T, query_block);
-    if ((int64_t)(Hq / H) * r.run > INT32_MAX / 16) return -1;
-    const Shape s = shape_of(Hq / H * r.run);
-    const int64_t groups = (int64_t)s.RG * r.runs;
-    if (groups > INT32_MAX || groups * H > INT32_MAX || groups * H * B > INT32_MAX) return -1;
-    return layout_of(s, (int64_t)B * H * groups, D).bytes;
+// false: not built
+static bool plan_of(int B, int H, int Hq, int T, int D, int query_block, int count, int64_t m, Plan &p) {
+    if (B <= 0 || H <= 0 || Hq <= 0 || Hq % H || T <= 0 || (D != 64 && D != 128) || query_block < 0) return false;
+    p.run = query_block == 0 || query_block > T ? T : query_block;
+    p.runs = (T + p.run - 1) / p.run;
+    if ((int64_t)(Hq / H) * p.run > INT32_MAX / 16) return false;
+    p.s = shape_of(Hq / H * p.run);
+    p.RG = p.s.RG * p.runs;
+    if (p.RG * H > INT32_MAX || p.RG * H * B > INT32_MAX) return false;
+    p.segments = p.RG * H * B;
+    p.parts = 1;
+    if (count) {
+        const int64_t items = min((int64_t)count * m, (int64_t)INT32_MAX) + p.s.rows0 + ((1 + (T + PG_GROUP - 1) / PG_GROUP) << p.s.dense);
+        const int share = p.s.nt ? FEW_SHARE : MANY_SHARE;
+        p.parts = (int)max(min(p.s.W / p.segments, (items + share - 1) / share), (int64_t)1);
+        if (p.segments * p.parts > INT32_MAX - 8) return false;
+    }
+    p.l = layout_of(p.s, count ? 0 : p.segments, !count ? 2LL * p.s.W : p.parts > 1 ? p.segments * p.parts : 0, D);
+    return true;
 }
 
 extern "C" int64_t ma_paged_workspace_bytes(int B, int H, int Hq, int T, int D) {
-    return workspace_bytes_of(B, H, Hq, T, D, 0);
+    Plan p;
+    return plan_of(B, H, Hq, T, D, 0, 0, 0, p) ? p.l.bytes : -1;
 }
 
-extern "C" int64_t ma_paged_blocks_workspace_bytes(int B, int H, int Hq, int T, int D, int query_block) {
-    return workspace_bytes_of(B, H, Hq, T, D, query_block);
+extern "C" int64_t ma_paged_blocks_workspace_bytes(int B, int H, int Hq, int T, int D, int count, int block_tokens,
+                                                   int query_block) {
+    Plan p;
+    if (count <= 0 || block_tokens <= 0 || block_tokens % PG_GROUP) return -1;
+    return plan_of(B, H, Hq, T, D, query_block, count, block_tokens / PG_GROUP, p) ? p.l.bytes : -1;
 }
 
 // m: groups of a selected block, 0 where every stored token is read
@@ -1677,8 +1734,9 @@ static int paged_attention(const char *who, const ma_tensor4 &q, int B, int Hq, 
                            float scale, const ma_tensor4 &out, const int32_t *blocks, int count, int m, int query_block,
                            void *workspace, int64_t workspace_bytes, void *stream) {
     if (int rc = pg_check(p, B, H, D, who)) return rc;
-    const int64_t need = workspace_bytes_of(B, H, Hq, T, D, query_block);
-    if (need < 0 || !q.ptr || !out.ptr || causal_block < 0 || (kc.ptr == nullptr) != (vc.ptr == nullptr)) {
+    Plan plan;
+    const bool built = plan_of(B, H, Hq, T, D, query_block, count, m, plan);
+    if (!built || !q.ptr || !out.ptr || causal_block < 0 || (kc.ptr == nullptr) != (vc.ptr == nullptr)) {
         ma_set_error("%s: bad arguments (B=%d H=%d Hq=%d T=%d D=%d causal_block=%d)", who, B, H, Hq, T, D, causal_block);
         return MA_EINVAL;
     }
@@ -1686,30 +1744,34 @@ static int paged_attention(const char *who, const ma_tensor4 &q, int B, int Hq, 
         ma_set_error("%s: queries, the block's keys and values, out and tails must share one dtype", who);
         return MA_EINVAL;
     }
-    if (!workspace || workspace_bytes < need || (uintptr_t)workspace % 256) {
+    const int64_t need = plan.l.bytes;
+    if (need && (!workspace || workspace_bytes < need || (uintptr_t)workspace % 256)) {
         ma_set_error("%s: workspace of %lld bytes (256-byte aligned) needed, got %lld", who, (long long)need,
                      (long long)workspace_bytes);
         return MA_EWORKSPACE;
     }
-    const Runs runs = runs_of(T, query_block);
-    const Shape s = shape_of(Hq / H * runs.run);
-    const int64_t RG = (int64_t)s.RG * runs.runs;
-    // the line: every request as long as its table row (and lists), with room for what the stretches round up
+    const Shape &s = plan.s;
+    const Layout &l = plan.l;
+    const int64_t RG = plan.RG;
+    // the line: every request as long as its table row, with room for what the stretches round up; or one segment
     int64_t groups = (int64_t)p->width * p->page_tokens / PG_GROUP;
     if (m) groups = min((int64_t)count, (groups + m - 1) / m) * min((int64_t)m, groups);
     const int64_t most = START + s.rows0 + groups + ((1 + (T + PG_GROUP - 1) / PG_GROUP) << s.dense);
-    if (groups > INT32_MAX / 2 || RG * B * H > INT32_MAX || most * B * H * RG + 64LL * s.W > INT32_MAX) {
+    if (groups > INT32_MAX / 4 || (m ? most + 64LL * plan.parts : most * plan.segments + 64LL * s.W) > INT32_MAX) {
         ma_set_error("%s: %d requests of up to %lld tokens and %lld row groups of each head are not built (2^31 items)", who,
                      B, (long long)p->width * p->page_tokens, (long long)RG);
         return MA_EUNSUPPORTED;
     }
     // the merge: a workgroup a segment (and rows), threads of one dimension below 2^32
-    if ((int64_t)B * H * RG * 64 * merge_waves(s.nt == 0) > UINT32_MAX) {
+    if (plan.segments * 64 * merge_waves(s.nt == 0) > UINT32_MAX) {
         ma_set_error("%s: %d requests, %d heads and %lld row groups of each are not built (2^%d segments)", who, B, H,
                      (long long)RG, s.nt ? 23 : 24);
         return MA_EUNSUPPORTED;
     }
-    const Layout l = layout_of(s, (int64_t)B * H * RG, D);
+    if (m && plan.segments * plan.parts * (s.nt ? 256 : 512) > UINT32_MAX - 8 * 512) {
+        ma_set_error("%s: %lld segments are not built (2^32 threads)", who, (long long)plan.segments);
+        return MA_EUNSUPPORTED;
+    }
     char *ws = (char *)workspace;
     AttnArgs a{};
     a.q = q;
@@ -1722,7 +1784,7 @@ static int paged_attention(const char *who, const ma_tensor4 &q, int B, int Hq, 
     a.H = H;
     a.G = Hq / H;
     a.T = T;
-    a.R = a.G * runs.run;
+    a.R = a.G * plan.run;
     a.RG = (int)RG;
     a.HR = H * a.RG;
     a.max_len = p->width * p->page_tokens;
@@ -1740,8 +1802,9 @@ static int paged_attention(const char *who, const ma_tensor4 &q, int B, int Hq, 
         a.blocks = blocks;
         a.count = count;
         a.m = m;
-        a.run = runs.run;
+        a.run = plan.run;
         a.RGR = s.RG;
+        a.parts = plan.parts;
         if (D == 128) return p->dtype == MA_BF16 ? launch<128, true, true>(a, s, st) : launch<128, false, true>(a, s, st);
         return p->dtype == MA_BF16 ? launch<64, true, true>(a, s, st) : launch<64, false, true>(a, s, st);
     }

@@ -473,18 +473,18 @@ def paged_attention(query: torch.Tensor, prefix: PagedPrefix, current_key: torch
         return out
     scale = float(scaling) if scaling is not None else d ** -0.5
     if blocks is not None:
-        need = N.size_query("ma_paged_blocks_workspace_bytes", b, h, hq, t, d, query_block)
+        if blocks.shape[3] == 0:
+            blocks = torch.full((b, h, runs, 1), -1, device=query.device, dtype=torch.int32)
+        need = N.size_query("ma_paged_blocks_workspace_bytes", b, h, hq, t, d, blocks.shape[3], block_tokens, query_block)
     else:
         need = N.size_query("ma_paged_workspace_bytes", b, h, hq, t, d)
     if need < 0:
         raise N.KernelUnavailableError(f"{hq // h * t} rows for each of {b * h} KV heads are not built")
-    ws = torch.empty((need,), device=query.device, dtype=torch.uint8)
+    ws = query.new_empty((need,), dtype=torch.uint8) if need else None
     if blocks is not None:
-        if blocks.shape[3] == 0:
-            blocks = torch.full((b, h, runs, 1), -1, device=query.device, dtype=torch.int32)
         _call(prefix.index, "ma_paged_attention_blocks", N.t4(query), b, hq, t, d, prefix._nat, h, N.t4(current_key),
               N.t4(current_value), N.ptr(new_lens), causal_block, scale, N.t4(out), blocks.data_ptr(), blocks.shape[3],
-              block_tokens, query_block, ws.data_ptr(), need)
+              block_tokens, query_block, N.ptr(ws), need)
         return out
     _call(prefix.index, "ma_paged_attention", N.t4(query), b, hq, t, d, prefix._nat, h, N.t4(current_key),
           N.t4(current_value), N.ptr(new_lens), causal_block, scale, N.t4(out), ws.data_ptr(), need)

@@ -39,8 +39,7 @@ def _t4(dtype=N.MA_BF16, ptr=4096):
     (E, dict(run=-1)), (E, dict(hq=5)), (E, dict(t=0)), (E, dict(causal=-1)), (E, dict(kc=_t4(ptr=None))),
     (E, dict(out=_t4(N.MA_F16))), (U, dict(d=96)), (E, dict(p=dict(pool=None))), (E, dict(q=_t4(ptr=None))),
     # (a head's rows, segments and items that the kernels do not count)
-    (E, dict(t=1 << 28)), (U, dict(b=1 << 13, h=32, hq=32, t=64, run=1)),
-    (U, dict(count=1 << 20, b=1024, hq=8, t=4, p=dict(width=1 << 24))),
+    (E, dict(t=1 << 28)), (U, dict(b=1 << 13, h=32, hq=32, t=64, run=1)), (E, dict(b=1 << 20, h=32, hq=32, t=64, run=1)),
     (N.MA_EWORKSPACE, dict(ws=None)), (N.MA_EWORKSPACE, dict(ws=4100)), (N.MA_EWORKSPACE, dict(bytes=256))])
 def test_bad_lists_are_refused(lib, rc, change):
     a = dict(q=_t4(), b=2, hq=4, t=2, d=64, p={}, h=2, kc=_t4(), vc=_t4(), causal=0, out=_t4(), blocks=4096, count=4, per=64,
@@ -52,8 +51,10 @@ def test_bad_lists_are_refused(lib, rc, change):
 
 
 def test_workspace_sizes(lib):
-    whole, runs = lib.ma_paged_workspace_bytes, lib.ma_paged_blocks_workspace_bytes
+    runs = lib.ma_paged_blocks_workspace_bytes
     for t in (1, 5, 40):
-        assert runs(2, 4, 28, t, 128, 0) == runs(2, 4, 28, t, 128, t) == runs(2, 4, 28, t, 128, 99) == whole(2, 4, 28, t, 128)
-    assert runs(2, 4, 28, 512, 128, 1) > 0 and runs(2, 4, 28, 512, 128, -1) == -1
-    assert runs(1 << 16, 1 << 10, 1 << 10, 64, 128, 1) == -1
+        assert runs(2, 4, 28, t, 128, 64, 32, 0) == runs(2, 4, 28, t, 128, 64, 32, t) == runs(2, 4, 28, t, 128, 64, 32, 99) > 0
+    assert runs(2, 4, 28, 512, 128, 8, 32, 1) == 0             # a workgroup a segment: nothing to join
+    for bad in ((2, 4, 28, 512, 128, 8, 32, -1), (2, 4, 28, 512, 128, 0, 32, 1), (2, 4, 28, 512, 128, 8, 33, 1),
+                (2, 4, 28, 512, 128, 8, 0, 1), (1 << 16, 1 << 10, 1 << 10, 64, 128, 8, 32, 1), (2, 3, 4, 1, 64, 8, 32, 0)):
+        assert runs(*bad) == -1
