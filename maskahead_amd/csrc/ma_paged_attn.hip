@@ -63,7 +63,7 @@ struct AttnArgs {
     // a run (R = G run), and RG = runs * RGR.
     const int32_t *blocks;    // [B, H, runs, count]
     int count, m, run, RGR;   // entries of a list, groups of a block
-    int parts;                // workgroups of a segment
+    int parts, wide;          // workgroups of a segment; they have 8 waves (few rows)
 };
 
 // values that every lane holds alike, as scalars
@@ -834,13 +834,13 @@ __device__ __forceinline__ void each_odd(const AttnArgs &a, const Items &it, int
             }
     }
 }
-// ... added to a tile's sums, of a wave's items d0, d0 + WAVES, ...
-template <int D, bool BF16>
+// ... added to a tile's sums, of a wave's items d0, d0 + NW, ...
+template <int D, bool BF16, int NW>
 __device__ __forceinline__ void add_odd(const AttnArgs &a, const Items &it, int b, int h, int d0, int d1, int keys, int hh,
                                         Tile<D> &t) {
     constexpr int NC = D / 16;
 #pragma unroll 1
-    for (int i = d0; i < d1; i += WAVES) {
+    for (int i = d0; i < d1; i += NW) {
         const Rows r = rows_of(a, it, b, h, i - it.ng);
         const int end = r.tail ? 0 : min(r.j0 + PG_GROUP, r.cnt);
 #pragma unroll 1
@@ -883,15 +883,15 @@ struct FewShared {
     ScanShared scan;
 };
 
-template <int D, int NT, bool BF16, bool MASK, bool SEL>
-__global__ __launch_bounds__(256, 2) void paged_few_kernel(AttnArgs a) {
+template <int D, int NT, bool BF16, bool MASK, bool SEL, int NW>
+__global__ __launch_bounds__(64 * NW, 2) void paged_few_kernel(AttnArgs a) {
     constexpr int CB = D / 32, NC = D / 16;
     __shared__ FewShared<D, NT> sh;
     const int tid = threadIdx.x, lane = tid & 63, wave = uniform(tid >> 6), n16 = lane & 15, hh = lane >> 4;
     Stretch st;
     Part pt;
     int pos;
-    for (bool more = first_part<256, SEL>(a, sh.scan, WAVES, st, pt, pos); more; more = another_part<SEL>(a, st, pt, pos)) {
+    for (bool more = first_part<64 * NW, SEL>(a, sh.scan, NW, st, pt, pos); more; more = another_part<SEL>(a, st, pt, pos)) {
         const Items it = st.it;
         const int b = st.b, h = pt.h, row0 = pt.rg * NT * 16, t0 = pt.t0;
         uint4 q[NT][CB];
@@ -903,7 +903,7 @@ __global__ __launch_bounds__(256, 2) void paged_few_kernel(AttnArgs a) {
         for (int nt = 0; nt < NT; ++nt) load_q<D, SEL>(a, b, h, t0, row0 + nt * 16 + (hidden(lane) & 15), it.n, hh, q[nt]);
         const int last = min(pt.i1, it.ng);
         int i = pt.i0 + wave, k = 0;
-        Records recs = find_records<D, WAVES, SEL>(a, it, b, h, pt.run, i, last, lane);
+        Records recs = find_records<D, NW, SEL>(a, it, b, h, pt.run, i, last, lane);
         RawK<D> rk;
         RawV<D> rv;
         bool dead = false;
@@ -920,9 +920,9 @@ __global__ __launch_bounds__(256, 2) void paged_few_kernel(AttnArgs a) {
             clear(t[nt]);
         }
         float lo = P_FIRST;
-        for (; i < last; i += WAVES) {
+        for (; i < last; i += NW) {
             if (++k == 64) {
-                recs = find_records<D, WAVES, SEL>(a, it, b, h, pt.run, i + WAVES, last, lane);
+                recs = find_records<D, NW, SEL>(a, it, b, h, pt.run, i + NW, last, lane);
                 k = 0;
             }
             // (behind the last one the pool's first record is loaded: no branch around the loads)
@@ -1019,7 +1019,7 @@ __global__ __launch_bounds__(256, 2) void paged_few_kernel(AttnArgs a) {
         // the tail and the block's own keys
         bool odd = false;
         const int rows_at = i;
-        for (; i < pt.i1; i += WAVES) {
+        for (; i < pt.i1; i += NW) {
             const Rows r = rows_of(a, it, b, h, i - it.ng);
             if (r.cnt == 0) continue;
             const int l = hidden(lane), lh = l >> 4;
@@ -1069,13 +1069,47 @@ __global__ __launch_bounds__(256, 2) void paged_few_kernel(AttnArgs a) {
         }
         if (odd) {
 #pragma unroll
-            for (int nt = 0; nt < NT; ++nt) add_odd<D, BF16>(a, it, b, h, rows_at, pt.i1, keys_seen(a, it, t0 + (row0 + nt * 16 + n16) % positions<SEL>(a)), hh, t[nt]);
+            for (int nt = 0; nt < NT; ++nt) add_odd<D, BF16, NW>(a, it, b, h, rows_at, pt.i1, keys_seen(a, it, t0 + (row0 + nt * 16 + n16) % positions<SEL>(a)), hh, t[nt]);
         }
         // the waves' parts joined; whole segments written out, cut ones left as a partial
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
             settle(t[nt]);
+            if constexpr (NW > WAVES) {       // the upper half's into the lower half's first
+                __syncthreads();
+                if (wave >= WAVES) {
+                    if (hh == 0) {
+                        sh.m[wave - WAVES][n16] = t[nt].m;
+                        sh.l[wave - WAVES][n16] = t[nt].l[0];
+                    }
+#pragma unroll
+                    for (int r = 0; r < 4; ++r)
+#pragma unroll
+                        for (int ct = 0; ct < NC; ct += 4)
+                            *(f32x4_t *)&sh.o[wave - WAVES][n16 * FewShared<D, NT>::OS + NC * (4 * hh + r) + ct] =
+                                f32x4_t{t[nt].acc[ct][r], t[nt].acc[ct + 1][r], t[nt].acc[ct + 2][r], t[nt].acc[ct + 3][r]};
+                }
+                __syncthreads();
+                if (wave < WAVES) {
+                    const float m = fmaxf(t[nt].m, sh.m[wave][n16]);
+                    const float f = __builtin_amdgcn_exp2f(t[nt].m - m), g = __builtin_amdgcn_exp2f(sh.m[wave][n16] - m);
+                    t[nt].l[0] = t[nt].l[0] * f + sh.l[wave][n16] * g;
+                    t[nt].m = m;
+#pragma unroll
+                    for (int r = 0; r < 4; ++r)
+#pragma unroll
+                        for (int ct = 0; ct < NC; ct += 4) {
+                            const f32x4_t v = *(const f32x4_t *)&sh.o[wave][n16 * FewShared<D, NT>::OS + NC * (4 * hh + r) + ct];
+#pragma unroll
+                            for (int z = 0; z < 4; ++z) t[nt].acc[ct + z][r] = t[nt].acc[ct + z][r] * f + v[z] * g;
+                        }
+                }
+            }
             __syncthreads();
+            if (NW > WAVES && wave >= WAVES) {
+                __syncthreads();
+                continue;
+            }
             if (hh == 0) {
                 sh.m[wave][n16] = t[nt].m;
                 sh.l[wave][n16] = t[nt].l[0];
@@ -1661,10 +1695,19 @@ int launch_many(const AttnArgs &a, hipStream_t st) {
     return MA_OK;
 }
 
+// few rows over selected blocks, 8 waves a workgroup
+template <int D, bool BF16, bool MASK>
+int launch_wide(const AttnArgs &a, const Shape &s, hipStream_t st) {
+    if (s.nt == 1) paged_few_kernel<D, 1, BF16, MASK, true, 2 * WAVES><<<grid_of<true>(a), 512, 0, st>>>(a);
+    else paged_few_kernel<D, 2, BF16, MASK, true, 2 * WAVES><<<grid_of<true>(a), 512, 0, st>>>(a);
+    return MA_OK;
+}
+
 template <int D, bool BF16, bool MASK, bool SEL>
 int launch_attn(const AttnArgs &a, const Shape &s, hipStream_t st) {
-    if (s.nt == 1) paged_few_kernel<D, 1, BF16, MASK, SEL><<<grid_of<SEL>(a), 256, 0, st>>>(a);
-    else if (s.nt == 2) paged_few_kernel<D, 2, BF16, MASK, SEL><<<grid_of<SEL>(a), 256, 0, st>>>(a);
+    if (SEL && s.nt && a.wide) return launch_wide<D, BF16, MASK>(a, s, st);
+    if (s.nt == 1) paged_few_kernel<D, 1, BF16, MASK, SEL, WAVES><<<grid_of<SEL>(a), 256, 0, st>>>(a);
+    else if (s.nt == 2) paged_few_kernel<D, 2, BF16, MASK, SEL, WAVES><<<grid_of<SEL>(a), 256, 0, st>>>(a);
     else if (s.rw == 2) return launch_many<D, 2, BF16, MASK, SEL>(a, st);
     else if (s.rw == 4) return launch_many<D, 4, BF16, MASK, SEL>(a, st);
     else return launch_many<D, 8, BF16, MASK, SEL>(a, st);
@@ -1688,7 +1731,7 @@ int launch(const AttnArgs &a, const Shape &s, hipStream_t st) {
 // all runs, segments, workgroups of a segment.
 struct Plan {
     Shape s;
-    int run, parts;
+    int run, parts, wide;
     int64_t runs, RG, segments;
     Layout l;
 };
@@ -1706,10 +1749,15 @@ static bool plan_of(int B, int H, int Hq, int T, int D, int query_block, int cou
     if (p.RG * H > INT32_MAX || p.RG * H * B > INT32_MAX) return false;
     p.segments = p.RG * H * B;
     p.parts = 1;
+    p.wide = 0;
     if (count) {
         const int64_t items = min((int64_t)count * m, (int64_t)INT32_MAX) + p.s.rows0 + ((1 + (T + PG_GROUP - 1) / PG_GROUP) << p.s.dense);
         const int share = p.s.nt ? FEW_SHARE : MANY_SHARE;
         p.parts = (int)max(min(p.s.W / p.segments, (items + share - 1) / share), (int64_t)1);
+        if (p.s.nt && p.parts == 2) {         // (as many waves, and nothing to join)
+            p.parts = 1;
+            p.wide = 1;
+        }
         if (p.segments * p.parts > INT32_MAX - 8) return false;
     }
     p.l = layout_of(p.s, count ? 0 : p.segments, !count ? 2LL * p.s.W : p.parts > 1 ? p.segments * p.parts : 0, D);
@@ -1768,7 +1816,7 @@ static int paged_attention(const char *who, const ma_tensor4 &q, int B, int Hq, 
                      (long long)RG, s.nt ? 23 : 24);
         return MA_EUNSUPPORTED;
     }
-    if (m && plan.segments * plan.parts * (s.nt ? 256 : 512) > UINT32_MAX - 8 * 512) {
+    if (m && plan.segments * plan.parts * 512 > UINT32_MAX - 8 * 512) {
         ma_set_error("%s: %lld segments are not built (2^32 threads)", who, (long long)plan.segments);
         return MA_EUNSUPPORTED;
     }
@@ -1805,6 +1853,7 @@ static int paged_attention(const char *who, const ma_tensor4 &q, int B, int Hq, 
         a.run = plan.run;
         a.RGR = s.RG;
         a.parts = plan.parts;
+        a.wide = plan.wide;
         if (D == 128) return p->dtype == MA_BF16 ? launch<128, true, true>(a, s, st) : launch<128, false, true>(a, s, st);
         return p->dtype == MA_BF16 ? launch<64, true, true>(a, s, st) : launch<64, false, true>(a, s, st);
     }

@@ -297,3 +297,47 @@ def test_blocks_longer_than_requests(gpu, per):
     assert torch.equal(out, paged_attention(q.to(gpu), r.cache.prefixes[0], blocks=lists[..., :1].contiguous(), block_tokens=per))
     full = paged_attention(q.to(gpu), r.cache.prefixes[0])
     assert ((out.double() - full.double()).abs() <= 2 * torch.finfo(BF).eps * full.double().abs() + 2.0 ** -9).all()
+
+
+@pytest.mark.parametrize("d,h,g,t,dtype,causal", [(128, 2, 7, 1, BF, 0), (64, 2, 7, 3, F16, 1), (64, 4, 4, 8, BF, 2), (128, 4, 3, 6, F16, 0)])
+@pytest.mark.parametrize("count,dead", [(3, False), (14, True)])
+def test_a_workgroup_for_each_request(gpu, d, h, g, t, dtype, causal, count, dead):
+    """About as many heads of requests as the card has CUs: the widest workgroups, and nothing to join."""
+    b = 200 // h
+    lens = [(97 * i) % 640 for i in range(b)]
+    new = [(i * 5) % (t + 1) for i in range(b)]
+    r = Requests(gpu, lens, h=h, d=d, dtype=dtype, page=32, room=0)
+    q = torch.randn((b, h * g, t, d), generator=r.gen).to(dtype)
+    ck, cv = r.block(new, t)
+    if causal:
+        for i, n in enumerate(new):
+            if n > 1:
+                cv[i, :, n - 1, 5::9] = float("inf") if i % 2 else float("nan")     # (the last position's alone see it)
+    lists = _lists(r.gen, lens, h, 1, count, 32, holes=dead)
+    mask = (torch.rand((b, h, 600), generator=r.gen) < 0.6).to(torch.uint8) if dead else None
+    before = torch.randn((b, h * g, t, d), generator=r.gen).to(dtype)
+    out = paged_attention(q.to(gpu), r.cache.prefix(0, mask=mask.to(gpu) if dead else None), ck.to(gpu), cv.to(gpu),
+                          out=before.to(gpu), new_lens=r.i32(new), causal_block=causal, blocks=lists.to(gpu))
+    if causal:
+        for i, n in enumerate(new):
+            # rows that see the last key: those of its causal block
+            if n > 1:
+                last = (lens[i] + n - 1) // causal
+                rows = [x for x in range(n) if (lens[i] + x) // causal >= last]
+                assert not torch.isfinite(out[i, :, rows][..., 5::9]).any()
+                keep = torch.ones(d, dtype=torch.bool)
+                keep[5::9] = False
+                assert torch.isfinite(out[i, :, :n][..., keep.to(gpu)]).all()
+                early = [x for x in range(n) if x not in rows]
+                assert torch.isfinite(out[i, :, early]).all()
+                cv[i, :, n - 1, 5::9] = 0.0
+                out[i, :, rows] = torch.where(keep.to(gpu), out[i, :, rows], 0.0)
+        again = paged_attention(q.to(gpu), r.cache.prefix(0, mask=mask.to(gpu) if dead else None), ck.to(gpu), cv.to(gpu),
+                                out=before.to(gpu), new_lens=r.i32(new), causal_block=causal, blocks=lists.to(gpu))
+        for i, n in enumerate(new):
+            last = (lens[i] + n - 1) // causal
+            for x in range(n):
+                if n == 1 or (lens[i] + x) // causal < last:
+                    assert torch.equal(again[i, :, x], out[i, :, x])
+        out = again
+    _check(r, q, ck, cv, out, lists, new, per=32, run=0, causal=causal, mask=mask, before=before)
