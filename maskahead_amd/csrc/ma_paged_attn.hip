@@ -683,7 +683,6 @@ __device__ __forceinline__ Part part_of(const AttnArgs &a, const Stretch &st, in
     const int i0 = rel - p.hr * st.it.items, i1 = min(st.it.items, i0 + (st.e - pos));
     p.h = a.RG == 1 ? p.hr : (int)((unsigned)p.hr / (unsigned)a.RG);
     p.rg = p.hr - p.h * a.RG;
-    p.run = p.t0 = 0;
     p.next = pos + i1 - i0;
     p.first = i0 == 0;
     p.whole = i0 == 0 && i1 == st.it.items;
@@ -709,13 +708,13 @@ __device__ __forceinline__ void next_part(const AttnArgs &a, Stretch &st, const 
 
 // Over selected blocks every segment holds about as many items as its list, so no line is cut: a segment
 // has a.parts workgroups of equal shares, known from the workgroup's number and its request's length.
-// False: a run behind the new tokens.
-__device__ __forceinline__ bool own_part(const AttnArgs &a, int unit, Stretch &st, Part &p) {
+// (A stretch of one place, or of none where the run lies behind the new tokens.)
+__device__ __forceinline__ Stretch own_part(const AttnArgs &a, int unit, Part &p) {
+    Stretch st{};
     // (workgroups of one XCD next to one another: runs of a head list the same pages)
     const unsigned w = (unsigned)(blockIdx.x % 8) * (gridDim.x / 8) + blockIdx.x / 8;
     const unsigned seg = w / (unsigned)a.parts, part = w - seg * a.parts;
-    if (seg >= (unsigned)a.B * a.HR) return false;
-    st = Stretch{};
+    if (seg >= (unsigned)a.B * a.HR) return st;
     st.b = (int)(seg / (unsigned)a.HR);
     p.hr = (int)(seg - (unsigned)st.b * a.HR);
     p.h = (int)((unsigned)p.hr / (unsigned)a.RG);
@@ -724,7 +723,7 @@ __device__ __forceinline__ bool own_part(const AttnArgs &a, int unit, Stretch &s
     p.rg -= p.run * a.RGR;
     p.t0 = p.run * a.run;
     const int n = a.new_lens ? min(max(a.new_lens[st.b], 0), a.T) : a.T, len = min(max(a.p.lengths[st.b], 0), a.max_len);
-    if (p.t0 >= n) return false;
+    if (p.t0 >= n) return st;
     Items it{};
     it.n = n;
     it.len = len;
@@ -735,28 +734,9 @@ __device__ __forceinline__ bool own_part(const AttnArgs &a, int unit, Stretch &s
     p.i0 = work_before(a, st.it, 0, min((int)part * share, st.it.items));
     p.i1 = work_before(a, st.it, 0, min((int)(part + 1) * share, st.it.items));
     p.slot = (int)w;
-    return true;
+    st.e = 1;
+    return st;
 }
-// The parts of a workgroup, one after the other: of its stretch, or its own alone
-template <int THREADS, bool SEL>
-__device__ __forceinline__ bool first_part(const AttnArgs &a, ScanShared &sh, int unit, Stretch &st, Part &p, int &pos) {
-    if constexpr (SEL) return own_part(a, unit, st, p);
-    st = find_stretch<THREADS>(a, sh, unit);
-    pos = st.s;
-    if (pos >= st.e) return false;
-    p = part_of(a, st, pos);
-    return true;
-}
-template <bool SEL>
-__device__ __forceinline__ bool another_part(const AttnArgs &a, Stretch &st, Part &p, int &pos) {
-    if (SEL) return false;
-    note_segment(a, st, p, pos);
-    next_part(a, st, p, pos);
-    if (pos >= st.e) return false;
-    p = part_of(a, st, pos);
-    return true;
-}
-
 // The records of a wave's next 64 packed items, one a lane: items first, first + EVERY, ... below
 // last of one (request, head).  Looked up at once, so that no item waits for its table entry
 // (a load in the loop also waits for every load before it).  Records are 16-byte aligned: bit 0
@@ -888,12 +868,13 @@ __global__ __launch_bounds__(64 * NW, 2) void paged_few_kernel(AttnArgs a) {
     constexpr int CB = D / 32, NC = D / 16;
     __shared__ FewShared<D, NT> sh;
     const int tid = threadIdx.x, lane = tid & 63, wave = uniform(tid >> 6), n16 = lane & 15, hh = lane >> 4;
-    Stretch st;
-    Part pt;
-    int pos;
-    for (bool more = first_part<64 * NW, SEL>(a, sh.scan, NW, st, pt, pos); more; more = another_part<SEL>(a, st, pt, pos)) {
+    Part own;
+    Stretch st = SEL ? own_part(a, NW, own) : find_stretch<64 * NW>(a, sh.scan, NW);
+    int pos = st.s;
+    while (pos < st.e) {
         const Items it = st.it;
-        const int b = st.b, h = pt.h, row0 = pt.rg * NT * 16, t0 = pt.t0;
+        const Part pt = SEL ? own : part_of(a, st, pos);
+        const int b = st.b, h = pt.h, row0 = pt.rg * NT * 16, t0 = SEL ? pt.t0 : 0;
         uint4 q[NT][CB];
         float c[NT];
         Tile<D> t[NT];
@@ -903,7 +884,7 @@ __global__ __launch_bounds__(64 * NW, 2) void paged_few_kernel(AttnArgs a) {
         for (int nt = 0; nt < NT; ++nt) load_q<D, SEL>(a, b, h, t0, row0 + nt * 16 + (hidden(lane) & 15), it.n, hh, q[nt]);
         const int last = min(pt.i1, it.ng);
         int i = pt.i0 + wave, k = 0;
-        Records recs = find_records<D, NW, SEL>(a, it, b, h, pt.run, i, last, lane);
+        Records recs = find_records<D, NW, SEL>(a, it, b, h, SEL ? pt.run : 0, i, last, lane);
         RawK<D> rk;
         RawV<D> rv;
         bool dead = false;
@@ -922,7 +903,7 @@ __global__ __launch_bounds__(64 * NW, 2) void paged_few_kernel(AttnArgs a) {
         float lo = P_FIRST;
         for (; i < last; i += NW) {
             if (++k == 64) {
-                recs = find_records<D, NW, SEL>(a, it, b, h, pt.run, i + NW, last, lane);
+                recs = find_records<D, NW, SEL>(a, it, b, h, SEL ? pt.run : 0, i + NW, last, lane);
                 k = 0;
             }
             // (behind the last one the pool's first record is loaded: no branch around the loads)
@@ -1160,6 +1141,9 @@ __global__ __launch_bounds__(64 * NW, 2) void paged_few_kernel(AttnArgs a) {
                 }
             }
         }
+        if (SEL) break;
+        note_segment(a, st, pt, pos);
+        next_part(a, st, pt, pos);
     }
 }
 
@@ -1212,12 +1196,13 @@ __global__ __launch_bounds__(512, 2) void paged_many_kernel(AttnArgs a) {
     const int rw = wave % RW, tw = wave / RW;
     const int si = wave >> 1;              // the item of a step that this wave unpacks (STEP and more: none)
     const bool sv = wave & 1;              // its values (else its keys)
-    Stretch st;
-    Part pt;
-    int pos;
-    for (bool more = first_part<512, SEL>(a, sh.scan, STEP, st, pt, pos); more; more = another_part<SEL>(a, st, pt, pos)) {
+    Part own;
+    Stretch st = SEL ? own_part(a, STEP, own) : find_stretch<512>(a, sh.scan, STEP);
+    int pos = st.s;
+    while (pos < st.e) {
         const Items it = st.it;
-        const int b = st.b, h = pt.h, row0 = pt.rg * (2 * RW * 16) + rw * 32, t0 = pt.t0;
+        const Part pt = SEL ? own : part_of(a, st, pos);
+        const int b = st.b, h = pt.h, row0 = pt.rg * (2 * RW * 16) + rw * 32, t0 = SEL ? pt.t0 : 0;
         const bool busy = row0 < a.R;      // this wave has rows
         uint4 q[2][CB];
         float c[2];
@@ -1242,7 +1227,7 @@ __global__ __launch_bounds__(512, 2) void paged_many_kernel(AttnArgs a) {
         // the words of step x's item of this wave (behind the last one: of the pool's first record)
         auto fetch = [&](int x) {
             if (si >= STEP) return;
-            if (x % 64 == 0) recs = find_records<D, STEP, SEL>(a, it, b, h, pt.run, pt.i0 + x * STEP + si, last, lane);
+            if (x % 64 == 0) recs = find_records<D, STEP, SEL>(a, it, b, h, SEL ? pt.run : 0, pt.i0 + x * STEP + si, last, lane);
             if (SEL && MASK) group = __builtin_amdgcn_readlane(recs.group, x % 64);
             const rec_t rec = record_at(recs, x % 64, dead);
             load_either(raw, rec, lane, sv, poff);
@@ -1525,6 +1510,9 @@ __global__ __launch_bounds__(512, 2) void paged_many_kernel(AttnArgs a) {
                 }
             }
         }
+        if (SEL) break;
+        note_segment(a, st, pt, pos);
+        next_part(a, st, pt, pos);
     }
 }
 
@@ -1539,11 +1527,11 @@ __global__ __launch_bounds__(512, 2) void paged_many_kernel(AttnArgs a) {
 // MB in 8.9 us).  Waves of few rows: one token of 2 long requests, some 30 partials a segment, 66.1
 // us with 8, 67.3 with 4, 66.1 with 16; of 64 requests 52.8, 52.3, 53.7.  Of many: 32 tokens of 8
 // requests 50.9 us with 4, 51.2 with 2, 51.9 with 8.
-constexpr int merge_waves(bool tiles) { return tiles ? 4 : 8; }
+constexpr int merge_waves(bool tiles, bool sel) { return tiles ? (sel ? 1 : 4) : 8; }
 
 template <int D, bool BF16, bool TILES, bool SEL>
-__global__ __launch_bounds__(64 * merge_waves(TILES)) void paged_merge_kernel(AttnArgs a, int rows) {
-    constexpr int NC = D / 16, GR = merge_waves(TILES);
+__global__ __launch_bounds__(64 * merge_waves(TILES, SEL)) void paged_merge_kernel(AttnArgs a, int rows) {
+    constexpr int NC = D / 16, GR = merge_waves(TILES, SEL);
     __shared__ float sm[GR][64], sl[GR][64];
     __shared__ f32x4_t so[GR][NC / 4][64];
     const int b = blockIdx.x / a.HR, hr = blockIdx.x - b * a.HR;
@@ -1720,8 +1708,8 @@ int launch(const AttnArgs &a, const Shape &s, hipStream_t st) {
     if (SEL && a.parts == 1) return ma_check_launch("ma_paged_attention_blocks");      // (nothing to join)
     // (a row group of few rows has fewer than its slots hold)
     const int rows = min(s.rows, a.R);
-    if (s.nt) paged_merge_kernel<D, BF16, false, SEL><<<dim3(a.B * a.H * a.RG, (rows + 3) / 4), 64 * merge_waves(false), 0, st>>>(a, s.rows);
-    else paged_merge_kernel<D, BF16, true, SEL><<<dim3(a.B * a.H * a.RG, (rows + 15) / 16 * 4), 64 * merge_waves(true), 0, st>>>(a, s.rows);
+    if (s.nt) paged_merge_kernel<D, BF16, false, SEL><<<dim3(a.B * a.H * a.RG, (rows + 3) / 4), 64 * merge_waves(false, SEL), 0, st>>>(a, s.rows);
+    else paged_merge_kernel<D, BF16, true, SEL><<<dim3(a.B * a.H * a.RG, (rows + 15) / 16 * 4), 64 * merge_waves(true, SEL), 0, st>>>(a, s.rows);
     return ma_check_launch(SEL ? "ma_paged_attention_blocks" : "ma_paged_attention");
 }
 
@@ -1737,6 +1725,7 @@ struct Plan {
 };
 // Items that a workgroup's share holds at least.
 constexpr int FEW_SHARE = 8, MANY_SHARE = 16;
+constexpr int HALF_ROWS_ITEMS = 48;
 
 // false: not built
 static bool plan_of(int B, int H, int Hq, int T, int D, int query_block, int count, int64_t m, Plan &p) {
@@ -1745,6 +1734,12 @@ static bool plan_of(int B, int H, int Hq, int T, int D, int query_block, int cou
     p.runs = (T + p.run - 1) / p.run;
     if ((int64_t)(Hq / H) * p.run > INT32_MAX / 16) return false;
     p.s = shape_of(Hq / H * p.run);
+    if (count && count * m <= HALF_ROWS_ITEMS && p.s.rw == 8 && p.s.RG * p.runs <= p.s.W / 2 / ((int64_t)B * H)) {
+        // half as many rows a workgroup where its segment would be cut in two: nothing, or half, to join
+        p.s.rw = 4;
+        p.s.rows = p.s.rw * 32;
+        p.s.RG = (Hq / H * p.run + p.s.rows - 1) / p.s.rows;
+    }
     p.RG = p.s.RG * p.runs;
     if (p.RG * H > INT32_MAX || p.RG * H * B > INT32_MAX) return false;
     p.segments = p.RG * H * B;
@@ -1811,7 +1806,7 @@ static int paged_attention(const char *who, const ma_tensor4 &q, int B, int Hq, 
         return MA_EUNSUPPORTED;
     }
     // the merge: a workgroup a segment (and rows), threads of one dimension below 2^32
-    if (plan.segments * 64 * merge_waves(s.nt == 0) > UINT32_MAX) {
+    if (plan.segments * 64 * merge_waves(s.nt == 0, false) > UINT32_MAX) {
         ma_set_error("%s: %d requests, %d heads and %lld row groups of each are not built (2^%d segments)", who, B, H,
                      (long long)RG, s.nt ? 23 : 24);
         return MA_EUNSUPPORTED;
