@@ -603,9 +603,10 @@ extern "C" int ma_select_blocks(ma_tensor4 q, int B, int Hq, int T, int D, const
     a.last = keep_last;
     const int span = 16 * groups_of(a.G * run) * SEL_WAVES;
     const int64_t rows = (int64_t)B * H * runs, units = rows * ((a.ngcap + span - 1) / span);
-    if (units > INT32_MAX / 2) {
-        ma_set_error("%s: %lld selections over %lld tokens are not built (2^30 times %d groups)", who, (long long)rows,
-                     (long long)tokens, span);
+    // (threads of a launch's one dimension: below 2^32)
+    if (units > INT32_MAX / 2 || rows > UINT32_MAX / 1024) {
+        ma_set_error("%s: %lld selections over %lld tokens are not built (2^22, and 2^30 times %d groups)", who,
+                     (long long)rows, (long long)tokens, span);
         return MA_EUNSUPPORTED;
     }
     a.units = (int)units;

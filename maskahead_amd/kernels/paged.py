@@ -266,6 +266,8 @@ def _check_rows(name: str, t: torch.Tensor, prefix: PagedPrefix, out: torch.Tens
         return torch.empty_like(t)        # (half the time of one by shape)
     if _check_block(f"out_{name}", out, prefix, shape[1]) != shape:
         raise ValueError(f"out_{name} must be {tuple(shape)}")
+    if any(st == 0 and n > 1 for st, n in zip(out.stride(), shape)):
+        raise ValueError(f"out_{name} holds rows that share their memory")
     return out
 
 

@@ -238,6 +238,8 @@ def test_refused_shapes(gpu):
                  lambda: rotate_block(p, q, rotary=table, out_key=k),
                  lambda: rotate_block(p, q, k, rotary=table, out_query=q[:, :2]),
                  lambda: rotate_block(p, q.half(), k, rotary=table),
+                 lambda: rotate_block(p, q, out_query=q[:, :1].expand(2, 4, 3, 128), rotary=table),
+                 lambda: append_pages(p, k, k, news, slots, rotary=table, query=q, out_query=q[:1].expand(2, 4, 3, 128)),
                  lambda: append_pages(p, k, k, news, slots, query=q),
                  lambda: append_pages(p, k, k, news, slots, rotary=table, query=q[:, :, :1]),
                  lambda: append_pages(p, k, k, news, slots, rotary=table, out_query=q),

@@ -150,7 +150,7 @@ def test_pages_that_are_none_and_dead_tokens(gpu):
         _check(pool, table, lens, [2] * 3, q, 2, got, count=11, first=1, last=1, mask=mask)
 
 
-@pytest.mark.parametrize("groups", [1023, 4096, 5000, 17000])
+@pytest.mark.parametrize("groups", [1023, 4096, 5000, 17000, 33000])
 def test_long_requests(gpu, groups):
     """Every way in which a selection keeps its keys."""
     lens = [32 * groups + 3, 32]

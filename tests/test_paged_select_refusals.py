@@ -39,7 +39,7 @@ def _t4(dtype=N.MA_BF16, ptr=4096):
     (E, dict(per=-32)), (E, dict(count=0)), (E, dict(first=-1)), (E, dict(last=-1)), (E, dict(first=3, last=2)),
     (E, dict(first=2147483647, last=2147483647)), (E, dict(q=_t4(ptr=None))), (E, dict(blocks=None)),
     (E, dict(q=_t4(N.MA_F16))), (U, dict(d=96)), (E, dict(p=dict(pool=4104))), (E, dict(p=dict(table=None))),
-    (E, dict(b=0)), (U, dict(p=dict(dtype=N.MA_F32))), (U, dict(b=1 << 20, t=4096, run=1)), (U, dict(t=1 << 28)),
+    (E, dict(b=0)), (U, dict(p=dict(dtype=N.MA_F32))), (U, dict(b=1 << 20, t=4096, run=1)), (U, dict(b=1 << 12, t=512, run=1)), (U, dict(t=1 << 28)),
     (N.MA_EWORKSPACE, dict(ws=None)), (N.MA_EWORKSPACE, dict(ws=4100)), (N.MA_EWORKSPACE, dict(bytes=255))])
 def test_bad_selections_are_refused(lib, rc, change):
     a = dict(q=_t4(), b=2, hq=4, t=2, d=64, p={}, h=2, run=0, per=64, count=4, first=1, last=1, blocks=4096, ws=4096,
