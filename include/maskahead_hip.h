@@ -417,13 +417,13 @@ typedef struct ma_rotary {
 /* q [B, Hq, T, D] and k [B, Hk, T, D] (Hk 0: none) rotated into q_out and k_out, which may be q and k
  * themselves (but must not overlap them otherwise): token t of request b at position lengths[b] + t (or
  * r->first's).  All share one dtype of bf16 and f16; D 64 or 128.  One launch.  MA_EUNSUPPORTED: B >
- * 65535, or more than 65535 groups of 4 heads. */
+ * 65535, or more than 65535 pairs of heads. */
 int ma_rotate_block(ma_tensor4 q, int Hq, ma_tensor4 q_out, ma_tensor4 k, int Hk, ma_tensor4 k_out, int B, int T, int D,
                     const int32_t *lengths, const ma_rotary *r, void *stream);
 /* ma_page_append whose keys are rotated on the way (codes, scales, zeros and tail rows are those of
  * ma_rotate_block's keys, bit for bit), and in the same launch all T rows of q [B, Hq, T, D] (Hq 0:
  * none) rotated into q_out as ma_rotate_block does.  k is not written.  MA_EUNSUPPORTED also: H and the
- * groups of 4 query heads are more than 65535. */
+ * pairs of query heads are more than 65535. */
 int ma_page_append_rotary(const ma_pages *p, ma_tensor4 k, ma_tensor4 v, int B, int H, int T, int D,
                           const int32_t *new_lens, const int64_t *slots, const ma_rotary *r, ma_tensor4 q, int Hq,
                           ma_tensor4 q_out, void *stream);

@@ -9,6 +9,9 @@
 // written out; one cut between workgroups leaves f32 partials (row maximum, sum, unnormalised
 // output), which paged_merge_kernel joins in a fixed order: the same call gives the same bits.
 //
+// Over selected blocks of a request's tokens the lists say what is read, about as much for every segment:
+// no line is cut there, a segment has a fixed number of workgroups (own_part).
+//
 // Two kernels walk the line.  Up to 32 rows (single tokens, short blocks) are bound by the
 // cache's bytes: there every wave unpacks records into its own registers.  More rows are bound
 // by the matrix cores: there a record is unpacked once, into LDS, for up to 256 rows.
@@ -1526,7 +1529,8 @@ __global__ __launch_bounds__(512, 2) void paged_many_kernel(AttnArgs a) {
 // bound: latency (desc, then partials), many rows: their bytes (8 requests' 224 rows of 4 heads, 33
 // MB in 8.9 us).  Waves of few rows: one token of 2 long requests, some 30 partials a segment, 66.1
 // us with 8, 67.3 with 4, 66.1 with 16; of 64 requests 52.8, 52.3, 53.7.  Of many: 32 tokens of 8
-// requests 50.9 us with 4, 51.2 with 2, 51.9 with 8.
+// requests 50.9 us with 4, 51.2 with 2, 51.9 with 8.  Of many over selected blocks, two partials mostly:
+// the merge of 128 segments 10.3 us with 4, 8.5 with 2, 7.4 with 1.
 constexpr int merge_waves(bool tiles, bool sel) { return tiles ? (sel ? 1 : 4) : 8; }
 
 template <int D, bool BF16, bool TILES, bool SEL>
@@ -1723,7 +1727,15 @@ struct Plan {
     int64_t runs, RG, segments;
     Layout l;
 };
-// Items that a workgroup's share holds at least.
+// Selected blocks: a segment has as many workgroups as keep the card busy, but each has FEW_SHARE (many
+// rows: MANY_SHARE) items at least: 4 096 tokens of 16 segments 14.3 us with 4, 13.5 with 8, 13.3 with 16, 15.4
+// with 32; 8 tokens' rows over 32 groups of 24 segments 12.1, 12.8, 15.6, 18.7.  Where a segment of few rows
+// would have two, it has one of 8 waves: as many loads under way, and no merge (one token of 64 requests,
+// 64 groups of each head, 26.8 -> 22.7 us: 75 MB, 3.3 TB/s, of which 7 us are the launch and the chain of
+// loads: length, list, table, record).  8 waves also where it would have more: 13.5 -> 14.2 and 12.8 -> 15.7.
+// Many rows, where it would have two or more and lists of up to HALF_ROWS_ITEMS groups: row groups of 8
+// tiles for 16, which unpack every group twice and join half as much: 512 positions in runs of 32 (224
+// rows), 8 groups each, 50 -> 42 us; 64 groups 86 -> 87; 128 groups 100 -> 111.
 constexpr int FEW_SHARE = 8, MANY_SHARE = 16;
 constexpr int HALF_ROWS_ITEMS = 48;
 

@@ -206,6 +206,13 @@ __global__ __launch_bounds__(PLAN_THREADS) void page_plan_kernel(PlanArgs a) {
 // (2^-13).  f16 quotients come as near as 2^-23 and are divided.  8 ragged prompts of up to 8 192
 // tokens (8 heads, D 128): 266 MB in 55 to 69 us, 3.9 to 4.8 TB/s (53 without any arithmetic);
 // one token of 64 requests 4.3 us.
+//
+// With a rotary table (ROT) the keys waves turn the new rows before they look for minima, and further
+// workgroups turn the block's queries.  All 128 channels of halves, the usual form, ask for the
+// group's 32 table rows before the keys (table_rows): 39 424 tokens of 7 prompts (8 heads, D 128), append
+// and read-back, 137 us, where without a table they take 127 and with table rows asked for as they are
+// needed 153; of what is left 5 us are registers (4 waves a SIMD, not 6) and 5 arithmetic and lane moves.
+// One token of 64 requests, their 28 query heads turned too: 6.2 us.
 struct AppendArgs {
     PagesDev p;
     const uint16_t *k, *v;
@@ -376,7 +383,7 @@ __device__ __forceinline__ void turn_rows(const RotaryDev &r, int pos, int t0, i
 template <int D, int DT, bool ROT>
 __global__ __launch_bounds__(256) void page_append_kernel(AppendArgs a) {
     constexpr int NC = D / 16, CL = D / 4, SL = 64 / CL, TPL = PG_GROUP / SL;   // CL lanes a row, SL slices of the tokens
-    if (ROT && (int)blockIdx.y >= a.H) {      // 64 rows of 4 query heads
+    if (ROT && (int)blockIdx.y >= a.H) {      // 64 rows of 2 query heads
         constexpr int U = D / 16;
         const int first = a.rot.first[blockIdx.z];
         for (int t = 64 * blockIdx.x + threadIdx.x / U, y = 0; y < U / 4; ++y, t += 256 / U)
@@ -576,7 +583,7 @@ tail_rows:
 }
 
 // ------------------------------------------------------------------ rotation alone
-// A thread: 16 channels of one token of 4 heads (rotary_heads); blockIdx.y: 4 heads of q, then of k.
+// A thread: 16 channels of one token of 2 heads (rotary_heads); blockIdx.y: 2 heads of q, then of k.
 struct RotateArgs {
     RotaryDev r;
     RotaryRows q, k;
@@ -875,13 +882,12 @@ extern "C" int ma_rotate_block(ma_tensor4 q, int Hq, ma_tensor4 q_out, ma_tensor
         return MA_EUNSUPPORTED;
     }
     const RotateArgs a{rotary_dev(r, lengths), rotary_rows(q, q_out, Hq), rotary_rows(k, k_out, Hk), T, (int)qg};
-    const int wg = threads <= 64 ? 64 : 256;
-    const dim3 grid((unsigned)((threads + wg - 1) / wg), (unsigned)(qg + kg), B);
+    const dim3 grid((unsigned)((threads + 255) / 256), (unsigned)(qg + kg), B);
     hipStream_t st = (hipStream_t)stream;
-    if (D == 128 && q.dtype == MA_BF16) rotate_kernel<128, MA_BF16><<<grid, wg, 0, st>>>(a);
-    else if (D == 128) rotate_kernel<128, MA_F16><<<grid, wg, 0, st>>>(a);
-    else if (q.dtype == MA_BF16) rotate_kernel<64, MA_BF16><<<grid, wg, 0, st>>>(a);
-    else rotate_kernel<64, MA_F16><<<grid, wg, 0, st>>>(a);
+    if (D == 128 && q.dtype == MA_BF16) rotate_kernel<128, MA_BF16><<<grid, 256, 0, st>>>(a);
+    else if (D == 128) rotate_kernel<128, MA_F16><<<grid, 256, 0, st>>>(a);
+    else if (q.dtype == MA_BF16) rotate_kernel<64, MA_BF16><<<grid, 256, 0, st>>>(a);
+    else rotate_kernel<64, MA_F16><<<grid, 256, 0, st>>>(a);
     return ma_check_launch(who);
 }
 

@@ -89,10 +89,14 @@ __device__ __forceinline__ void rotary_unit(uint4 &a, uint4 &b, const float (&c)
     b = uint4{bw[0], bw[1], bw[2], bw[3]};
 }
 
-// Rows of up to 4 heads of one request at their positions: a thread takes 16 channels (8 pairs,
-// or 16 that are not turned) of one token, so that it reads its cosines and sines once for
-// the heads.  in and out may be the same rows.
-constexpr int ROTARY_HEADS = 4;
+// Rows of up to 2 heads of one request at their positions: a thread takes 16 channels (8 pairs,
+// or 16 that are not turned) of one token, and reads its cosines and sines once for both.  in and out
+// may be the same rows.
+//
+// bound: the bytes, 4 D a row and 4 dim a position.  4 096 tokens of 4 requests (32 query and 8 KV heads,
+// D 128): 344 MB in 62.6 us, 5.5 TB/s (one head a thread 66.3, four 63.8, eight 67.3); a token of 64
+// requests (28 and 4 heads) 4.2 us, which is a launch and two loads in a row (4.1, 4.6, 6.3).
+constexpr int ROTARY_HEADS = 2;
 struct RotaryRows {
     const uint16_t *in;
     uint16_t *out;

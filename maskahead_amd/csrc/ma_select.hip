@@ -54,7 +54,7 @@ __device__ __forceinline__ void unpack8(uint4 w, float (&x)[8]) {
 }
 
 typedef __attribute__((ext_vector_type(4))) int i32x4_t;
-// 16 codes x scale, rounded half to even, as digits: the sum with 1.5 2^23 + 128 leaves code + 128 in
+// Codes, rounded half to even, and their digits (2.25 instructions a value): the sum with 1.5 2^23 + 128 leaves code + 128 in
 // the lowest 16 bits, whose upper byte is hi, and whose lower is lo + 128.
 __device__ __forceinline__ uint32_t code_bits(float x, float scale) {
     return __float_as_uint(__builtin_fmaf(x, scale, 12583040.0f));
@@ -148,6 +148,15 @@ __device__ __forceinline__ Unit find_unit(const SelectArgs &a, int u, int span, 
 // ------------------------------------------------------------------ scores of groups
 // A workgroup: 64 GW groups of one (request, head) and the rows of one run; a wave holds the digits of
 // its 16 GW groups' parameters and passes all rows by them, whose digits lie in LDS, 64 rows at a time.
+//
+// bound: few rows: latency (lengths, table and rows, parameters: three loads in a row) and 4 D bytes a
+// group and head.  One token of 64 requests of 700 to 16 384 tokens (28 query and 4 KV heads, D 128): 20 MB
+// in 10.0 us; of 2 requests of 90 000 to 131 072 (32 and 8 heads): 29 MB in 10.7.  A workgroup for every unit
+// that a table row can name, which need not look for its request, was slower where most rows are shorter
+// (the first with its top 16.3 -> 19.7).  Many rows: no one unit, 224 rows of 16 runs over 2 x 350 to 512
+// groups 24.5 us, of which products 5, the running maximum 3 and the rows' digits 4.6; 16 groups a
+// wave 28, and few rows the same with 32 (half as many waves to wait for the loads).  Digits of f16 and their
+// products, which take twice the time and registers: 12.3, 13.4 and 44.5 us.
 struct RowScale {
     double by, add;      // a row's power of two and 0; no row: 0 and -inf; one that is not finite: 0 and inf
 };
@@ -337,6 +346,10 @@ __device__ __forceinline__ void wave_offsets(uint32_t v, int wave, uint32_t &bef
 // PER > 0: a thread keeps its keys, at most PER, of at most THREADS * PER blocks; 0: they are read again in
 // every turn.  Scores are read a wave's width at a time and handed over in LDS (dynamic, THREADS * PER keys)
 // to the threads that hold PER neighbours; the first are asked for before the request's length is known.
+//
+// bound: latency (loads, then five barriers).  256 rows of up to 512 blocks 5.5 us, 16 of up to 2 048 (of two
+// groups) 8.0, of which some 3 are the launch.  256 threads hold up to 1 024 blocks (1 024 threads: 6.5 us where
+// they take 5.9), 1 024 threads more (256: 14.3 us where they take 8.9).
 template <int THREADS, int PER>
 __global__ __launch_bounds__(THREADS) void select_top_kernel(SelectArgs a) {
     using Shared = TopShared<THREADS>;
