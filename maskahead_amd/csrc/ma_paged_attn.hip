@@ -669,6 +669,8 @@ __device__ __forceinline__ Stretch find_stretch(const AttnArgs &a, ScanShared &s
 struct Part {
     int h, rg, hr, i0, i1;   // its items of work [i0, i1); rg: the row group of the head's (SEL: of the run's)
     int run, t0;             // SEL: the run and its first position; else 0
+    int entry;               // ... its list's entry of the lane's number, and
+    uint16_t touched[4];     // what asked for its 16-bit rows early
     int next;                // where the stretch goes on
     bool first, whole;       // the segment begins here; all of it lies here
     int slot;                // of its partial, where it is not whole: the first or the last of the stretch
@@ -712,6 +714,7 @@ __device__ __forceinline__ void next_part(const AttnArgs &a, Stretch &st, const 
 // Over selected blocks every segment holds about as many items as its list, so no line is cut: a segment
 // has a.parts workgroups of equal shares, known from the workgroup's number and its request's length.
 // (A stretch of one place, or of none where the run lies behind the new tokens.)
+template <int D, bool TOUCH>
 __device__ __forceinline__ Stretch own_part(const AttnArgs &a, int unit, Part &p) {
     Stretch st{};
     // (workgroups of one XCD next to one another: runs of a head list the same pages)
@@ -725,6 +728,23 @@ __device__ __forceinline__ Stretch own_part(const AttnArgs &a, int unit, Part &p
     p.run = (int)((unsigned)p.rg / (unsigned)a.RGR);
     p.rg -= p.run * a.RGR;
     p.t0 = p.run * a.run;
+    // What needs no length is asked for with it: the list (64 entries, one a lane) and, by one wave of the
+    // workgroup that will read them, a word of every line of the tail's and the block's first rows, which
+    // come from memory otherwise when nothing is left to do meanwhile.
+    const int lane = threadIdx.x & 63;
+    p.entry = a.blocks[(((int64_t)st.b * a.H + p.h) * (a.RG / a.RGR) + p.run) * a.count + min(lane, a.count - 1)];
+    p.touched[0] = p.touched[1] = p.touched[2] = p.touched[3] = 0;
+    if (TOUCH && part == (unsigned)a.parts - 1 && threadIdx.x < 64) {
+        const int j = lane >> 1, c = (lane & 1) * (D / 2);
+        const int64_t tail = (int64_t)st.b * a.p.s_tb + (int64_t)p.h * a.p.s_th + j * a.p.s_tt + c;
+        p.touched[0] = a.p.kt[tail];
+        p.touched[1] = a.p.vt[tail];
+        if (a.kc.ptr) {
+            const int64_t t = min(j, a.T - 1);
+            p.touched[2] = ((const uint16_t *)a.kc.ptr)[(int64_t)st.b * a.kc.s[0] + (int64_t)p.h * a.kc.s[1] + t * a.kc.s[2] + c];
+            p.touched[3] = ((const uint16_t *)a.vc.ptr)[(int64_t)st.b * a.vc.s[0] + (int64_t)p.h * a.vc.s[1] + t * a.vc.s[2] + c];
+        }
+    }
     const int n = a.new_lens ? min(max(a.new_lens[st.b], 0), a.T) : a.T, len = min(max(a.p.lengths[st.b], 0), a.max_len);
     if (p.t0 >= n) return st;
     Items it{};
@@ -750,17 +770,18 @@ struct Records {
     int group;
 };
 template <int D, int EVERY, bool SEL>
-__device__ __forceinline__ Records find_records(const AttnArgs &a, const Items &it, int b, int h, int run, int first, int last,
-                                                int lane) {
+__device__ __forceinline__ Records find_records(const AttnArgs &a, const Items &it, int b, int h, int run, int entry,
+                                                int first, int last, int lane) {
     const int per = a.p.page_tokens / PG_GROUP;
     int i = first + EVERY * lane;
     uint64_t r = (uint64_t)a.p.pool | 1u;
     bool there = i < last;
-    if (SEL && there) {
+    if (SEL) {
         const int e = (int)((unsigned)i / (unsigned)a.m), ng = it.len / PG_GROUP;
-        const int block = a.blocks[(((int64_t)b * a.H + h) * (a.RG / a.RGR) + run) * a.count + e];
+        int block = __shfl(entry, min(e, 63));
+        if (there && e >= 64) block = a.blocks[(((int64_t)b * a.H + h) * (a.RG / a.RGR) + run) * a.count + e];
         // (a block behind the request's last is none: its first group's number is not computed)
-        there = block >= 0 && block <= (ng - 1) / a.m;
+        there = there && block >= 0 && block <= (ng - 1) / a.m;
         i = there ? block * a.m + (i - e * a.m) : 0;
         there = there && i < ng;
     }
@@ -872,7 +893,7 @@ __global__ __launch_bounds__(64 * NW, 2) void paged_few_kernel(AttnArgs a) {
     __shared__ FewShared<D, NT> sh;
     const int tid = threadIdx.x, lane = tid & 63, wave = uniform(tid >> 6), n16 = lane & 15, hh = lane >> 4;
     Part own;
-    Stretch st = SEL ? own_part(a, NW, own) : find_stretch<64 * NW>(a, sh.scan, NW);
+    Stretch st = SEL ? own_part<D, true>(a, NW, own) : find_stretch<64 * NW>(a, sh.scan, NW);
     int pos = st.s;
     while (pos < st.e) {
         const Items it = st.it;
@@ -887,7 +908,7 @@ __global__ __launch_bounds__(64 * NW, 2) void paged_few_kernel(AttnArgs a) {
         for (int nt = 0; nt < NT; ++nt) load_q<D, SEL>(a, b, h, t0, row0 + nt * 16 + (hidden(lane) & 15), it.n, hh, q[nt]);
         const int last = min(pt.i1, it.ng);
         int i = pt.i0 + wave, k = 0;
-        Records recs = find_records<D, NW, SEL>(a, it, b, h, SEL ? pt.run : 0, i, last, lane);
+        Records recs = find_records<D, NW, SEL>(a, it, b, h, SEL ? pt.run : 0, SEL ? own.entry : 0, i, last, lane);
         RawK<D> rk;
         RawV<D> rv;
         bool dead = false;
@@ -906,7 +927,7 @@ __global__ __launch_bounds__(64 * NW, 2) void paged_few_kernel(AttnArgs a) {
         float lo = P_FIRST;
         for (; i < last; i += NW) {
             if (++k == 64) {
-                recs = find_records<D, NW, SEL>(a, it, b, h, SEL ? pt.run : 0, i + NW, last, lane);
+                recs = find_records<D, NW, SEL>(a, it, b, h, SEL ? pt.run : 0, SEL ? own.entry : 0, i + NW, last, lane);
                 k = 0;
             }
             // (behind the last one the pool's first record is loaded: no branch around the loads)
@@ -1001,6 +1022,7 @@ __global__ __launch_bounds__(64 * NW, 2) void paged_few_kernel(AttnArgs a) {
                 for (int ct = 0; ct < NC; ++ct) t[nt].acc[ct] += t[nt].z;
         }
         // the tail and the block's own keys
+        if (SEL) asm volatile("" ::"v"(own.touched[0]), "v"(own.touched[1]), "v"(own.touched[2]), "v"(own.touched[3]));
         bool odd = false;
         const int rows_at = i;
         for (; i < pt.i1; i += NW) {
@@ -1200,7 +1222,7 @@ __global__ __launch_bounds__(512, 2) void paged_many_kernel(AttnArgs a) {
     const int si = wave >> 1;              // the item of a step that this wave unpacks (STEP and more: none)
     const bool sv = wave & 1;              // its values (else its keys)
     Part own;
-    Stretch st = SEL ? own_part(a, STEP, own) : find_stretch<512>(a, sh.scan, STEP);
+    Stretch st = SEL ? own_part<D, false>(a, STEP, own) : find_stretch<512>(a, sh.scan, STEP);
     int pos = st.s;
     while (pos < st.e) {
         const Items it = st.it;
@@ -1230,7 +1252,7 @@ __global__ __launch_bounds__(512, 2) void paged_many_kernel(AttnArgs a) {
         // the words of step x's item of this wave (behind the last one: of the pool's first record)
         auto fetch = [&](int x) {
             if (si >= STEP) return;
-            if (x % 64 == 0) recs = find_records<D, STEP, SEL>(a, it, b, h, SEL ? pt.run : 0, pt.i0 + x * STEP + si, last, lane);
+            if (x % 64 == 0) recs = find_records<D, STEP, SEL>(a, it, b, h, SEL ? pt.run : 0, SEL ? own.entry : 0, pt.i0 + x * STEP + si, last, lane);
             if (SEL && MASK) group = __builtin_amdgcn_readlane(recs.group, x % 64);
             const rec_t rec = record_at(recs, x % 64, dead);
             load_either(raw, rec, lane, sv, poff);
