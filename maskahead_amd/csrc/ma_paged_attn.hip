@@ -81,21 +81,20 @@ __device__ __forceinline__ int uniform(int x) { return __builtin_amdgcn_readfirs
 // START 1, 8, 12, 16, 20: one token of 64 ragged requests 58, 52.4, 52.8, 52.4, 54.1 us, of 2 long
 // ones 66.8 to 67.3; of many rows 9 % slower with 1, 4 to 16 within 2 % of one another.
 constexpr int START = 8;
-//
-// Over selected blocks the packed items are the groups of the list's entries, those that a request
-// has no block for left out; an entry that names none, and groups behind the request's last, are
-// items that nothing is seen of.
 struct Items {
     int n, len, ng, rem, items;      // ng: packed items
 };
-// (seen: the block's keys that any row of a segment sees)
+// Over selected blocks (SEL) the packed items are the groups of as many of the list's entries as the
+// request has blocks; an entry that names none, and groups behind the request's last, are items that
+// nothing is seen of.  seen: the block's keys that any row of the segment sees.
 template <bool SEL>
 __device__ __forceinline__ Items items_from(const AttnArgs &a, int n, int len, int seen = 0) {
     Items r;
     r.n = n;
     r.len = len;
     r.ng = len / PG_GROUP;
-    if (SEL) r.ng = (int)min((unsigned)a.count, ((unsigned)r.ng + (unsigned)a.m - 1) / (unsigned)a.m) * min(a.m, r.ng);
+    if (SEL)         // (of a block longer than the request, the request's)
+        r.ng = (int)min((unsigned)a.count, ((unsigned)r.ng + (unsigned)a.m - 1) / (unsigned)a.m) * min(a.m, r.ng);
     r.rem = len % PG_GROUP;
     const int cur = a.kc.ptr ? ((SEL ? seen : n) + PG_GROUP - 1) / PG_GROUP : 0;
     const int rows = (r.rem ? 1 : 0) + cur;
@@ -760,6 +759,7 @@ __device__ __forceinline__ Stretch own_part(const AttnArgs &a, int unit, Part &p
     st.e = 1;
     return st;
 }
+
 // The records of a wave's next 64 packed items, one a lane: items first, first + EVERY, ... below
 // last of one (request, head).  Looked up at once, so that no item waits for its table entry
 // (a load in the loop also waits for every load before it).  Records are 16-byte aligned: bit 0

@@ -9,7 +9,8 @@ from .ops import (
     quantize_values_into,
     selector_topk,
 )
-from .paged import PagedPrefix, append_pages, dequantize_pages, paged_attention, plan_pages
+from .paged import (PagedPrefix, append_pages, dequantize_pages, paged_attention, plan_pages, rotary_table,
+                    rotate_block, select_blocks)
 from .select import prefix_scores_topk, topk_ascending
 from .splitk import Prefix, dequantize_prefix, prefix_scores, splitk_attention
 from .step0 import Step0Buffers, step0_select
@@ -30,6 +31,9 @@ __all__ = [
     "prefix_scores_topk",
     "quantize_key_groups_into",
     "quantize_values_into",
+    "rotary_table",
+    "rotate_block",
+    "select_blocks",
     "selector_topk",
     "splitk_attention",
     "Step0Buffers",

@@ -4,6 +4,14 @@
     out = paged_attention(q, prefix, k, v, new_lens=new_lens)          # per layer
     append_pages(prefix, k, v, new_lens, slots)                        # per layer
 
+``rotate_block`` (and ``append_pages`` on the way) turns queries and keys at their requests'
+positions, ``select_blocks`` lists the blocks of stored tokens that a run of queries should read, and
+``paged_attention(blocks=...)`` reads those alone:
+
+    q, k = rotate_block(prefix, q, k, rotary=table)                    # rotary_table, made once
+    blocks = select_blocks(q, prefix, 64, new_lens=new_lens)
+    out = paged_attention(q, prefix, k, v, new_lens=new_lens, blocks=blocks)
+
 The reference's cache holds one scalar length for all its batch rows (cache.py:94-96), and
 ``splitk_attention`` follows it; here every request has its own, read by the kernels, so a
 step of a ragged batch needs no padding, no host copy of a length and one launch per layer
