@@ -17,8 +17,6 @@ using namespace ma;
 
 namespace {
 
-constexpr int SEL_WAVES = 4, SEL_TILES = 4;             // row tiles in LDS at once: one a wave
-constexpr int SEL_FEW_ROWS = 32;
 constexpr float LEAST = -3.4028234663852886e38f;
 
 struct SelectArgs {
@@ -54,33 +52,37 @@ __device__ __forceinline__ void unpack8(uint4 w, float (&x)[8]) {
 }
 
 typedef __attribute__((ext_vector_type(4))) int i32x4_t;
-// Codes, rounded half to even, and their digits (2.25 instructions a value): the sum with 1.5 2^23 + 128 leaves code + 128 in
-// the lowest 16 bits, whose upper byte is hi, and whose lower is lo + 128.
-__device__ __forceinline__ uint32_t code_bits(float x, float scale) {
-    return __float_as_uint(__builtin_fmaf(x, scale, 12583040.0f));
+// Codes, rounded half to even, and their digits (2.25 instructions a value): the sum with 1.5 2^23 + 128
+// leaves code + 128 in the lowest 16 bits, whose upper byte is hi, and whose lower is lo + 128.  Two codes
+// + 128 in a word:
+__device__ __forceinline__ uint32_t code_pair(float x, float y, float scale) {
+    const uint32_t a = __float_as_uint(__builtin_fmaf(x, scale, 12583040.0f));
+    const uint32_t b = __float_as_uint(__builtin_fmaf(y, scale, 12583040.0f));
+    return __builtin_amdgcn_perm(b, a, 0x05040100u);
 }
-// (four codes into byte i of the digits)
-__device__ __forceinline__ void put_digits(uint32_t a, uint32_t b, uint32_t c, uint32_t d, int i, i32x4_t &hi, i32x4_t &lo) {
-    const uint32_t x = __builtin_amdgcn_perm(b, a, 0x05010400u), y = __builtin_amdgcn_perm(d, c, 0x05010400u);
-    lo[i] = (int)(__builtin_amdgcn_perm(y, x, 0x05040100u) ^ 0x80808080u);
-    hi[i] = (int)__builtin_amdgcn_perm(y, x, 0x07060302u);
+// ... into word i of the digits; ... and 0 for a negative code
+__device__ __forceinline__ void put_digits(uint32_t x, uint32_t y, int i, i32x4_t &hi, i32x4_t &lo) {
+    lo[i] = (int)(__builtin_amdgcn_perm(y, x, 0x06040200u) ^ 0x80808080u);
+    hi[i] = (int)__builtin_amdgcn_perm(y, x, 0x07050301u);
 }
-// 16 channels of a row (RELU: 0 where they are negative)
-template <int DT>
-__device__ __forceinline__ void row_digits(const uint4 (&w)[2], float scale, bool relu, i32x4_t &hi, i32x4_t &lo) {
+typedef __attribute__((ext_vector_type(2))) int16_t s16x2_t;
+__device__ __forceinline__ uint32_t positive(uint32_t x) {
+    return __builtin_bit_cast(uint32_t, __builtin_elementwise_max(__builtin_bit_cast(s16x2_t, x), (s16x2_t){128, 128}));
+}
+// 16 channels: f(i, pairs of channels 4 i .. 4 i + 3)
+template <int DT, class F>
+__device__ __forceinline__ void each_pair(const uint4 (&w)[2], float scale, F f) {
 #pragma unroll
     for (int y = 0; y < 2; ++y) {
         float v[8];
         unpack8<DT>(w[y], v);
-        if (relu) {
-#pragma unroll
-            for (int i = 0; i < 8; ++i) v[i] = fmaxf(v[i], 0.0f);
-        }
 #pragma unroll
         for (int i = 0; i < 2; ++i)
-            put_digits(code_bits(v[4 * i], scale), code_bits(v[4 * i + 1], scale), code_bits(v[4 * i + 2], scale),
-                       code_bits(v[4 * i + 3], scale), 2 * y + i, hi, lo);
+            f(2 * y + i, code_pair(v[4 * i], v[4 * i + 1], scale), code_pair(v[4 * i + 2], v[4 * i + 3], scale));
     }
+}
+__device__ __forceinline__ void group_digits(const uint4 (&w)[2], float scale, i32x4_t &hi, i32x4_t &lo) {
+    each_pair<MA_F16>(w, scale, [&](int i, uint32_t x, uint32_t y) { put_digits(x, y, i, hi, lo); });
 }
 __device__ __forceinline__ i32x4_t mfma_i8(i32x4_t a, i32x4_t b, i32x4_t c) {
     return __builtin_amdgcn_mfma_i32_16x16x64_i8(a, b, c, 0, 0, 0);
@@ -146,78 +148,69 @@ __device__ __forceinline__ Unit find_unit(const SelectArgs &a, int u, int span, 
 }
 
 // ------------------------------------------------------------------ scores of groups
-// A workgroup: 64 GW groups of one (request, head) and the rows of one run; a wave holds the digits of
-// its 16 GW groups' parameters and passes all rows by them, whose digits lie in LDS, 64 rows at a time.
+// A workgroup of NW waves: 16 NW groups of one (request, head) and the rows of one run; a wave holds the
+// digits of its 16 groups' parameters and passes all rows by them, whose digits lie in LDS, a tile of 16
+// rows from every wave at a time.
 //
 // bound: few rows: latency (lengths, table and rows, parameters: three loads in a row) and 4 D bytes a
 // group and head.  One token of 64 requests of 700 to 16 384 tokens (28 query and 4 KV heads, D 128): 20 MB
-// in 10.0 us; of 2 requests of 90 000 to 131 072 (32 and 8 heads): 29 MB in 10.7.  A workgroup for every unit
+// in 9.7 us; of 2 requests of 90 000 to 131 072 (32 and 8 heads): 29 MB in 10.5.  A workgroup for every unit
 // that a table row can name, which need not look for its request, was slower where most rows are shorter
-// (the first with its top 16.3 -> 19.7).  Many rows: no one unit, 224 rows of 16 runs over 2 x 350 to 512
-// groups 24.5 us, of which products 5, the running maximum 3 and the rows' digits 4.6; 16 groups a
-// wave 28, and few rows the same with 32 (half as many waves to wait for the loads).  Digits of f16 and their
-// products, which take twice the time and registers: 12.3, 13.4 and 44.5 us.
+// (the first with its top 16.3 -> 19.7).  Many rows: the instructions around the products.  224 rows of 16
+// runs over 350 and 512 groups: 22.1 us, of which the matrix cores 5 and the other instructions 10 (1 700 a
+// wave: the running maximum 340, digits of rows 350 and of parameters 250), at 14 waves a CU; waves of 32
+// groups 24.9.  Digits of f16 and their products, which take twice the time and registers: 12.3, 13.4 and
+// 44.5 us.
 struct RowScale {
     double by, add;      // a row's power of two and 0; no row: 0 and -inf; one that is not finite: 0 and inf
 };
-template <int D, int DT, int GW>
-__global__ __launch_bounds__(64 * SEL_WAVES, GW == 1 ? 4 : 2) void select_score_kernel(SelectArgs a) {
-    constexpr int KB = D / 64, SPAN = 16 * GW * SEL_WAVES;
-    __shared__ i32x4_t dig[SEL_TILES][4][KB][64];         // hi, lo, and those of the positive codes
-    __shared__ RowScale scales[SEL_TILES][16];
+template <int D, int DT, int NW>
+__global__ __launch_bounds__(64 * NW, 4) void select_score_kernel(SelectArgs a) {
+    constexpr int KB = D / 64, SPAN = 16 * NW;
+    __shared__ i32x4_t dig[NW][4][KB][64];         // hi, lo, and those of the positive codes
+    __shared__ RowScale scales[NW][16];
     const int tid = threadIdx.x, lane = tid & 63, wave = uniform(tid >> 6), n16 = lane & 15, hh = lane >> 4;
     const int R = a.G * a.run, tiles = (R + 15) / 16, per = a.p.page_tokens / PG_GROUP;
     for (int u = blockIdx.x; u < a.units; u += gridDim.x) {
         const Unit x = find_unit(a, u, SPAN, lane);
         if (x.b < 0) return;         // (all waves alike)
         const int b = x.b, h = x.h, n = x.n, ng = x.len / PG_GROUP;
-        // the wave's groups
-        const int g0 = x.span * SPAN + 16 * GW * wave + n16;
-        int gi[GW], page[GW];
-#pragma unroll
-        for (int y = 0; y < GW; ++y) {
-            const int g = min(g0 + 16 * y, ng - 1), pg = g / per;
-            gi[y] = g - pg * per;
-            page[y] = a.p.table[(int64_t)b * a.p.s_table + pg];
-        }
+        // the lane's group (behind the last: the last, which is not stored again)
+        const int g = x.span * SPAN + 16 * wave + n16, gc = min(g, ng - 1), pg = gc / per;
+        const int page = a.p.table[(int64_t)b * a.p.s_table + pg];
         // the rows of tile t (this wave's), or of the only one
         uint4 w[KB][2];
+        int pos_of_row = 0;
         auto load_rows = [&](int t) {
-            const int rc = min(16 * t + n16, R - 1), qh = rc / a.run, pos = x.run * a.run + rc - qh * a.run;
+            const int rc = min(16 * t + n16, R - 1), qh = rc / a.run;
+            pos_of_row = x.run * a.run + rc - qh * a.run;
             const uint16_t *src = (const uint16_t *)a.q.ptr + (int64_t)b * a.q.s[0] + (int64_t)(h * a.G + qh) * a.q.s[1] +
-                                  (int64_t)min(pos, a.T - 1) * a.q.s[2] + 16 * hh;
+                                  (int64_t)min(pos_of_row, a.T - 1) * a.q.s[2] + 16 * hh;
 #pragma unroll
             for (int kb = 0; kb < KB; ++kb)
 #pragma unroll
                 for (int y = 0; y < 2; ++y) w[kb][y] = pg_load16(src + 64 * kb + 8 * y);
         };
         load_rows(tiles == 1 ? 0 : wave);       // (behind the last tile: the last row)
-        bool live[GW];
-        uint4 sw[GW][KB][2], zw[GW][KB][2];
+        const uint8_t *rec = pg_record(a.p, page, gc - pg * per, h, 40 * D);
+        bool live = rec != nullptr;
+        if (!rec) rec = a.p.pool;
+        uint4 sw[KB][2], zw[KB][2];
 #pragma unroll
-        for (int y = 0; y < GW; ++y) {
-            const uint8_t *rec = pg_record(a.p, page[y], gi[y], h, 40 * D);
-            live[y] = rec != nullptr;
-            if (!rec) rec = a.p.pool;
+        for (int kb = 0; kb < KB; ++kb)
 #pragma unroll
-            for (int kb = 0; kb < KB; ++kb)
-#pragma unroll
-                for (int z = 0; z < 2; ++z) {
-                    sw[y][kb][z] = *(const uint4 *)(rec + 32 * D + 2 * (64 * kb + 16 * hh + 8 * z));
-                    zw[y][kb][z] = *(const uint4 *)(rec + 34 * D + 2 * (64 * kb + 16 * hh + 8 * z));
-                }
-        }
-        if (a.p.mask) {
-#pragma unroll
-            for (int y = 0; y < GW; ++y) {
-                const bool any = pg_mask_bits(a.p, b, h, min(g0 + 16 * y, ng - 1) * PG_GROUP + 8 * hh) != 0;
-                live[y] = live[y] && max_rows(any ? 1.f : 0.f) != 0.f;
+            for (int z = 0; z < 2; ++z) {
+                sw[kb][z] = *(const uint4 *)(rec + 32 * D + 2 * (64 * kb + 16 * hh + 8 * z));
+                zw[kb][z] = *(const uint4 *)(rec + 34 * D + 2 * (64 * kb + 16 * hh + 8 * z));
             }
+        if (a.p.mask) {
+            const bool any = pg_mask_bits(a.p, b, h, gc * PG_GROUP + 8 * hh) != 0;
+            live = live && max_rows(any ? 1.f : 0.f) != 0.f;
         }
-        // the rows' digits into LDS: a tile a wave, or 64 channels of the only one, as they are or the positive ones
+        // the rows' digits into LDS: a tile a wave, or 64 channels of the only one
         auto put_rows = [&](int t0) {
             const int t = tiles == 1 ? 0 : wave;
-            if (t0 + t >= tiles || (tiles == 1 && wave >= 2 * KB)) return;
+            if (t0 + t >= tiles || (tiles == 1 && wave >= KB)) return;
             u16x2_t most{};
 #pragma unroll
             for (int kb = 0; kb < KB; ++kb) most_of(w[kb][0], most), most_of(w[kb][1], most);
@@ -226,92 +219,73 @@ __global__ __launch_bounds__(64 * SEL_WAVES, GW == 1 ? 4 : 2) void select_score_
             const int e = max((int)(__float_as_uint(mx) >> 23) - 127, -100);
             const float scale = odd ? 0.f : pow2(13 - e);
 #pragma unroll
-            for (int kb = 0; kb < KB; ++kb)
-#pragma unroll
-                for (int relu = 0; relu < 2; ++relu) {
-                    if (tiles == 1 && kb + KB * relu != wave) continue;
-                    i32x4_t hi, lo;
-                    row_digits<DT>(w[kb], scale, relu, hi, lo);
-                    dig[t][2 * relu][kb][lane] = hi;
-                    dig[t][2 * relu + 1][kb][lane] = lo;
-                }
-            const int row = 16 * (t0 + t) + n16, pos = x.run * a.run + row % a.run;
-            const bool none = row >= R || pos >= n;
+            for (int kb = 0; kb < KB; ++kb) {
+                if (tiles == 1 && kb != wave) continue;
+                i32x4_t hi, lo, rh, rl;
+                each_pair<DT>(w[kb], scale, [&](int i, uint32_t v0, uint32_t v1) {
+                    put_digits(v0, v1, i, hi, lo);
+                    put_digits(positive(v0), positive(v1), i, rh, rl);
+                });
+                dig[t][0][kb][lane] = hi;
+                dig[t][1][kb][lane] = lo;
+                dig[t][2][kb][lane] = rh;
+                dig[t][3][kb][lane] = rl;
+            }
+            const bool none = 16 * (t0 + t) + n16 >= R || pos_of_row >= n;
             if (hh == 0) scales[t][n16] = RowScale{none || odd ? 0.0 : (double)pow2(e), none ? -INFINITY : odd ? INFINITY : 0.0};
         };
         __syncthreads();         // the unit's before is read
         put_rows(0);
-        i32x4_t zh[GW][KB], zl[GW][KB], sh[GW][KB], sl[GW][KB];
-        int f[GW];
-        bool odd[GW];
+        u16x2_t ms{}, mz{};
 #pragma unroll
-        for (int y = 0; y < GW; ++y) {
-            u16x2_t ms{}, mz{};
+        for (int kb = 0; kb < KB; ++kb)
 #pragma unroll
-            for (int kb = 0; kb < KB; ++kb)
+            for (int z = 0; z < 2; ++z) most_of(sw[kb][z], ms), most_of(zw[kb][z], mz);
+        const float top = fmaxf(15.0f * most_float<MA_F16>(ms), most_float<MA_F16>(mz));
+        const bool odd = top == INFINITY;
+        const int f = max((int)(__float_as_uint(top) >> 23) - 127, -24);
+        const float scale = odd ? 0.f : pow2(13 - f);
+        i32x4_t zh[KB], zl[KB], sh[KB], sl[KB];
 #pragma unroll
-                for (int z = 0; z < 2; ++z) most_of(sw[y][kb][z], ms), most_of(zw[y][kb][z], mz);
-            const float top = fmaxf(15.0f * most_float<MA_F16>(ms), most_float<MA_F16>(mz));
-            odd[y] = top == INFINITY;
-            f[y] = max((int)(__float_as_uint(top) >> 23) - 127, -24);
-            const float scale = odd[y] ? 0.f : pow2(13 - f[y]);
-#pragma unroll
-            for (int kb = 0; kb < KB; ++kb) {
-                row_digits<MA_F16>(zw[y][kb], scale, false, zh[y][kb], zl[y][kb]);
-                row_digits<MA_F16>(sw[y][kb], 15.0f * scale, false, sh[y][kb], sl[y][kb]);
-            }
+        for (int kb = 0; kb < KB; ++kb) {
+            group_digits(zw[kb], scale, zh[kb], zl[kb]);
+            group_digits(sw[kb], 15.0f * scale, sh[kb], sl[kb]);
         }
-        // (the rows' largest exact score, before the group's power of two)
-        double best[GW];
-#pragma unroll
-        for (int y = 0; y < GW; ++y) best[y] = -INFINITY;
-        for (int t0 = 0; t0 < tiles; t0 += SEL_TILES) {
+        double best = -INFINITY;         // the rows' largest exact score, before the group's power of two
+        for (int t0 = 0; t0 < tiles; t0 += NW) {
             if (t0) {
                 __syncthreads();          // the rows before are read
                 put_rows(t0);
             }
             __syncthreads();
-            if (t0 + SEL_TILES < tiles) load_rows(t0 + SEL_TILES + wave);
-            for (int t = 0; t < min(SEL_TILES, tiles - t0); ++t) {
-                i32x4_t c2[GW], c1[GW], c0[GW];
-#pragma unroll
-                for (int y = 0; y < GW; ++y) c2[y] = c1[y] = c0[y] = i32x4_t{};
+            if (t0 + NW < tiles) load_rows(t0 + NW + wave);
+            for (int t = 0; t < min(NW, tiles - t0); ++t) {
+                i32x4_t c2{}, c1{}, c0{};
 #pragma unroll
                 for (int kb = 0; kb < KB; ++kb) {
                     const i32x4_t qh = dig[t][0][kb][lane], ql = dig[t][1][kb][lane];
                     const i32x4_t rh = dig[t][2][kb][lane], rl = dig[t][3][kb][lane];
-#pragma unroll
-                    for (int y = 0; y < GW; ++y) {
-                        c1[y] = mfma_i8(qh, zl[y][kb], c1[y]);
-                        c2[y] = mfma_i8(qh, zh[y][kb], c2[y]);
-                        c0[y] = mfma_i8(ql, zl[y][kb], c0[y]);
-                        c1[y] = mfma_i8(ql, zh[y][kb], c1[y]);
-                        c2[y] = mfma_i8(rh, sh[y][kb], c2[y]);
-                        c1[y] = mfma_i8(rh, sl[y][kb], c1[y]);
-                        c0[y] = mfma_i8(rl, sl[y][kb], c0[y]);
-                        c1[y] = mfma_i8(rl, sh[y][kb], c1[y]);
-                    }
+                    c1 = mfma_i8(qh, zl[kb], c1);
+                    c2 = mfma_i8(qh, zh[kb], c2);
+                    c0 = mfma_i8(ql, zl[kb], c0);
+                    c1 = mfma_i8(ql, zh[kb], c1);
+                    c2 = mfma_i8(rh, sh[kb], c2);
+                    c1 = mfma_i8(rh, sl[kb], c1);
+                    c0 = mfma_i8(rl, sl[kb], c0);
+                    c1 = mfma_i8(rl, sh[kb], c1);
                 }
                 // lane (n, h): rows 4 h + r by group n (256 c1 + c0 is below 2^31)
 #pragma unroll
                 for (int r = 0; r < 4; ++r) {
                     const RowScale e = scales[t][4 * hh + r];
-#pragma unroll
-                    for (int y = 0; y < GW; ++y) {
-                        const double s = __builtin_fma((double)c2[y][r], 65536.0, (double)(c1[y][r] * 256 + c0[y][r]));
-                        best[y] = __builtin_fmax(best[y], __builtin_fma(s, e.by, e.add));
-                    }
+                    const double s = __builtin_fma((double)c2[r], 65536.0, (double)(c1[r] * 256 + c0[r]));
+                    best = __builtin_fmax(best, __builtin_fma(s, e.by, e.add));
                 }
             }
         }
-#pragma unroll
-        for (int y = 0; y < GW; ++y) {
-            float v = best[y] == -INFINITY ? -INFINITY : fmaxf((float)__builtin_ldexp(best[y], f[y] - 26), LEAST);
-            v = max_rows(odd[y] && v > -INFINITY ? INFINITY : v);
-            const int g = g0 + 16 * y;
-            if (hh == 0 && g < ng)
-                a.group[(((int64_t)b * a.H + h) * a.runs + x.run) * a.ngcap + g] = live[y] ? v : -INFINITY;
-        }
+        float v = best == -INFINITY ? -INFINITY : fmaxf((float)__builtin_ldexp(best, f - 26), LEAST);
+        v = max_rows(odd && v > -INFINITY ? INFINITY : v);
+        if (hh == 0 && g < ng) a.group[(((int64_t)b * a.H + h) * a.runs + x.run) * a.ngcap + g] = live ? v : -INFINITY;
     }
 }
 
@@ -535,12 +509,18 @@ __global__ __launch_bounds__(THREADS) void select_top_kernel(SelectArgs a) {
 
 int64_t align256(int64_t x) { return (x + 255) / 256 * 256; }
 
-// groups of a wave: 16 of few rows, whose time is that of the loads, 32 of many
-int groups_of(int rows) { return rows <= SEL_FEW_ROWS ? 1 : 2; }
+// Waves of a workgroup: 8 share the rows' digits among twice the groups, which pays where those take several
+// turns of 4 tiles and the workgroups keep every SIMD busy; else 4, which wait for less.  With their tops:
+// 512 positions of 2 requests in runs of 32 (224 rows) 28.4 us with 8, 31.8 with 4; 32 tokens of 32 requests
+// 20.6 and 22.2, of 64 29.9 and 28.6, of 16 19.3 and 17.4, of 8 18.9 and 17.1; 8 tokens (56 rows) of 64
+// requests 19.2 and 17.8; one token of 64 17.3 and 15.3.
+int waves_of(int rows, int64_t selections, int64_t groups) {
+    return rows > 64 && selections * ((groups + 127) / 128) >= 2LL * ma_num_cus() ? 8 : 4;
+}
 template <int D, int DT>
-void launch_score(const SelectArgs &a, unsigned grid, hipStream_t st) {
-    if (groups_of(a.G * a.run) == 1) select_score_kernel<D, DT, 1><<<grid, 64 * SEL_WAVES, 0, st>>>(a);
-    else select_score_kernel<D, DT, 2><<<grid, 64 * SEL_WAVES, 0, st>>>(a);
+void launch_score(const SelectArgs &a, int waves, unsigned grid, hipStream_t st) {
+    if (waves == 4) select_score_kernel<D, DT, 4><<<grid, 256, 0, st>>>(a);
+    else select_score_kernel<D, DT, 8><<<grid, 512, 0, st>>>(a);
 }
 template <int THREADS, int PER>
 int launch_top(const SelectArgs &a, unsigned rows, hipStream_t st) {
@@ -614,8 +594,9 @@ extern "C" int ma_select_blocks(ma_tensor4 q, int B, int Hq, int T, int D, const
     a.count = count;
     a.first = keep_first;
     a.last = keep_last;
-    const int span = 16 * groups_of(a.G * run) * SEL_WAVES;
-    const int64_t rows = (int64_t)B * H * runs, units = rows * ((a.ngcap + span - 1) / span);
+    const int64_t rows = (int64_t)B * H * runs;
+    const int waves = waves_of(a.G * run, rows, a.ngcap), span = 16 * waves;
+    const int64_t units = rows * ((a.ngcap + span - 1) / span);
     // (threads of a launch's one dimension: below 2^32)
     if (units > INT32_MAX / 2 || rows > UINT32_MAX / 1024) {
         ma_set_error("%s: %lld selections over %lld tokens are not built (2^22, and 2^30 times %d groups)", who,
@@ -625,8 +606,8 @@ extern "C" int ma_select_blocks(ma_tensor4 q, int B, int Hq, int T, int D, const
     a.units = (int)units;
     const unsigned grid = (unsigned)min(units, (int64_t)ma_num_cus() * 4);
     hipStream_t st = (hipStream_t)stream;
-    if (D == 128) p->dtype == MA_BF16 ? launch_score<128, MA_BF16>(a, grid, st) : launch_score<128, MA_F16>(a, grid, st);
-    else p->dtype == MA_BF16 ? launch_score<64, MA_BF16>(a, grid, st) : launch_score<64, MA_F16>(a, grid, st);
+    if (D == 128) p->dtype == MA_BF16 ? launch_score<128, MA_BF16>(a, waves, grid, st) : launch_score<128, MA_F16>(a, waves, grid, st);
+    else p->dtype == MA_BF16 ? launch_score<64, MA_BF16>(a, waves, grid, st) : launch_score<64, MA_F16>(a, waves, grid, st);
     if (int rc = ma_check_launch(who)) return rc;
     int rc;
     if (a.nbcap <= 1024) rc = launch_top<256, 4>(a, (unsigned)rows, st);

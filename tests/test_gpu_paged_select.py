@@ -225,3 +225,28 @@ def test_nothing_to_select_from_and_refusals(gpu):
         select_blocks(q.half(), p, 2)
     with pytest.raises(ValueError):
         select_blocks(q[:1], p, 2)
+
+
+def test_many_runs_of_many_rows(gpu):
+    """Workgroups that share their rows' digits among 128 groups."""
+    lens, h, t, run = [2100, 900, 4300, 32], 4, 200, 17
+    pool, table, prefix = _store(gpu, lens, h=h, page=64, seed=12, width=300)
+    new = [200, 45, 170, 0]
+    q = torch.randn((4, h * 4, t, 64), generator=torch.Generator().manual_seed(3)).to(BF)
+    got = select_blocks(q.to(gpu), prefix(), 7, new_lens=torch.tensor(new, dtype=torch.int32, device=gpu), query_block=run,
+                        keep_first=1, return_scores=True)
+    # (of 48 selections a request some are checked against whole numbers, all against a call of their own)
+    blocks, scores = (x.cpu() for x in got)
+    for b, kv, r in ((0, 0, 0), (0, 3, 11), (1, 2, 2), (2, 1, 9), (1, 0, 5)):
+        rows = q[b, kv * 4:kv * 4 + 4, r * run:min((r + 1) * run, new[b])].flatten(0, 1)
+        s = group_scores(pool, table[b].tolist(), lens[b] // 32, kv, rows) if len(rows) else []
+        took, block = select_rule(s, 1, 7, 1, 0)
+        assert blocks[b, kv, r].tolist() == took + [-1] * (7 - len(took))
+        assert torch.equal(scores[b, kv, r, :len(block)], torch.tensor(block, dtype=torch.float64).float())
+    for r in range(12):
+        one = torch.tensor([min(max(n - r * run, 0), run) for n in new], dtype=torch.int32, device=gpu)
+        part = torch.zeros((4, h * 4, run, 64), dtype=BF)
+        x = q[:, :, r * run:(r + 1) * run]
+        part[:, :, :x.shape[2]] = x
+        alone = select_blocks(part.to(gpu), prefix(), 7, new_lens=one, keep_first=1, return_scores=True)
+        assert torch.equal(alone[0][:, :, 0].cpu(), blocks[:, :, r]) and torch.equal(alone[1][:, :, 0].cpu(), scores[:, :, r])
