@@ -397,7 +397,7 @@ int ma_page_plan_append(const int32_t *lengths, const int32_t *new_lens, int B, 
  * and ma_quantize_values' arithmetic into the record that slots (ma_page_plan's) names, and
  * the rest becomes the tail.  Requests without new tokens, and those whose slots are -1, are
  * left as they are.  k, v share p->dtype.  One launch.  MA_EUNSUPPORTED (here and in
- * ma_page_dequant): B or H > 65535. */
+ * ma_page_dequant): B or H > 65535; here also T of 2^30. */
 int ma_page_append(const ma_pages *p, ma_tensor4 k, ma_tensor4 v, int B, int H, int T, int D,
                    const int32_t *new_lens, const int64_t *slots, void *stream);
 /* The rotation of rows at their positions (no counterpart in the reference, whose models rotate
@@ -417,7 +417,7 @@ typedef struct ma_rotary {
 /* q [B, Hq, T, D] and k [B, Hk, T, D] (Hk 0: none) rotated into q_out and k_out, which may be q and k
  * themselves (but must not overlap them otherwise): token t of request b at position lengths[b] + t (or
  * r->first's).  All share one dtype of bf16 and f16; D 64 or 128.  One launch.  MA_EUNSUPPORTED: B >
- * 65535, or more than 65535 pairs of heads. */
+ * 65535, more than 65535 pairs of heads, or T D of 2^36. */
 int ma_rotate_block(ma_tensor4 q, int Hq, ma_tensor4 q_out, ma_tensor4 k, int Hk, ma_tensor4 k_out, int B, int T, int D,
                     const int32_t *lengths, const ma_rotary *r, void *stream);
 /* ma_page_append whose keys are rotated on the way (codes, scales, zeros and tail rows are those of

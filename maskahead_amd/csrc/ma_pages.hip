@@ -877,8 +877,9 @@ extern "C" int ma_rotate_block(ma_tensor4 q, int Hq, ma_tensor4 q_out, ma_tensor
     }
     const int64_t qg = ((int64_t)Hq + ROTARY_HEADS - 1) / ROTARY_HEADS, kg = ((int64_t)Hk + ROTARY_HEADS - 1) / ROTARY_HEADS;
     const int64_t threads = (int64_t)T * (D / 16);
-    if (B > 65535 || qg + kg > 65535) {
-        ma_set_error("%s: more than 65535 requests or groups of %d heads are not built", who, ROTARY_HEADS);
+    if (B > 65535 || qg + kg > 65535 || threads > UINT32_MAX - 255) {       // (threads of one dimension: below 2^32)
+        ma_set_error("%s: more than 65535 requests or groups of %d heads, or 2^32 threads for %d tokens, are not built", who,
+                     ROTARY_HEADS, T);
         return MA_EUNSUPPORTED;
     }
     const RotateArgs a{rotary_dev(r, lengths), rotary_rows(q, q_out, Hq), rotary_rows(k, k_out, Hk), T, (int)qg};
@@ -916,8 +917,8 @@ static int page_append(const char *who, const ma_pages *p, const ma_tensor4 &k, 
     }
     const int64_t units = ((int64_t)T + PG_GROUP - 1) / PG_GROUP;
     const int64_t heads = H + ((int64_t)Hq + ROTARY_HEADS - 1) / ROTARY_HEADS;
-    if (B > 65535 || heads > 65535) {
-        ma_set_error("%s: more than 65535 requests or heads are not built", who);
+    if (B > 65535 || heads > 65535 || (units + 1) / 2 * 256 > UINT32_MAX) {
+        ma_set_error("%s: more than 65535 requests or heads, or 2^30 new tokens, are not built", who);
         return MA_EUNSUPPORTED;
     }
     AppendArgs a{pages_dev(p), (const uint16_t *)k.ptr, (const uint16_t *)v.ptr, k.s[0], k.s[1], k.s[2], v.s[0],

@@ -321,7 +321,8 @@ def append_pages(prefix: PagedPrefix, key: torch.Tensor, value: torch.Tensor, ne
     rotary (a ``rotary_table``): the keys are rotated at their positions on the way; what is stored
     is what ``rotate_block`` and an append of its result would store, bit for bit, and key is not
     written.  interleaved, positions: as there.  With query [B, Hq, T, D] the same launch rotates all
-    its rows, and they are returned (in out_query, if given, which may be query)."""
+    its rows, and they are returned (in out_query, if given, which may be query and overlaps nothing
+    else that the call reads)."""
     shape = _check_block("key", key, prefix, prefix.heads)
     if _check_block("value", value, prefix, prefix.heads) != shape:
         raise ValueError("key and value shapes differ")

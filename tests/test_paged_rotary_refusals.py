@@ -61,7 +61,7 @@ def test_no_table_is_refused(lib):
     (E, dict(q=_t4(ptr=None))), (E, dict(qo=_t4(ptr=None))), (E, dict(k=_t4(ptr=None))), (E, dict(ko=_t4(ptr=None))),
     (E, dict(hq=0)), (E, dict(hk=-1)), (E, dict(b=0)), (E, dict(t=0)), (U, dict(d=96)), (E, dict(lengths=None)),
     (U, dict(q=_t4(N.MA_F32))), (E, dict(qo=_t4(N.MA_F16))), (E, dict(k=_t4(N.MA_F16))), (E, dict(ko=_t4(N.MA_F32))),
-    (U, dict(b=65536)), (U, dict(hq=4 * 65535)), (U, dict(hk=4 * 65535))])
+    (U, dict(b=65536)), (U, dict(hq=4 * 65535)), (U, dict(hk=4 * 65535)), (U, dict(t=1 << 30))])
 def test_bad_rows_are_refused(lib, rc, change):
     a = dict(q=_t4(), hq=4, qo=_t4(), k=_t4(), hk=2, ko=_t4(), b=2, t=1, d=64, lengths=4096)
     a.update(change)
@@ -72,7 +72,7 @@ def test_bad_rows_are_refused(lib, rc, change):
 @pytest.mark.parametrize("rc,change", [
     (E, dict(k=_t4(ptr=None))), (E, dict(q=_t4(ptr=None))), (E, dict(qo=_t4(ptr=None))), (E, dict(hq=-1)),
     (E, dict(t=0)), (E, dict(q=_t4(N.MA_F16))), (E, dict(qo=_t4(N.MA_F16))), (E, dict(v=_t4(N.MA_F16))),
-    (U, dict(d=96)), (U, dict(b=65536)), (U, dict(hq=4 * 65535)), (E, dict(p=dict(pool=4104))), (E, dict(p=dict(lengths=None)))])
+    (U, dict(d=96)), (U, dict(b=65536)), (U, dict(hq=4 * 65535)), (U, dict(t=(1 << 30) + 64)), (E, dict(p=dict(pool=4104))), (E, dict(p=dict(lengths=None)))])
 def test_bad_appends_are_refused(lib, rc, change):
     a = dict(k=_t4(), v=_t4(), q=_t4(), hq=4, qo=_t4(), b=2, t=1, d=64, p={})
     a.update(change)
