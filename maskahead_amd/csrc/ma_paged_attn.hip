@@ -1755,7 +1755,7 @@ struct Plan {
 // would have two, it has one of 8 waves: as many loads under way, and no merge (one token of 64 requests,
 // 64 groups of each head, 26.8 -> 22.7 us: 75 MB, 3.3 TB/s, of which 7 us are the launch and the chain of
 // loads: length, list, table, record).  8 waves also where it would have more: 13.5 -> 14.2 and 12.8 -> 15.7.
-// 12 waves (155 registers, none spilled): 22.2 -> 24.0.
+// 12 waves (155 registers, none spilled): 22.2 -> 24.0; 8 that ask two records ahead (211 registers): 23.8.
 // Many rows, where it would have two or more and lists of up to HALF_ROWS_ITEMS groups: row groups of 8
 // tiles for 16, which unpack every group twice and join half as much: 512 positions in runs of 32 (224
 // rows), 8 groups each, 50 -> 42 us; 64 groups 86 -> 87; 128 groups 100 -> 111.
