@@ -341,3 +341,41 @@ def test_a_workgroup_for_each_request(gpu, d, h, g, t, dtype, causal, count, dea
                     assert torch.equal(again[i, :, x], out[i, :, x])
         out = again
     _check(r, q, ck, cv, out, lists, new, per=32, run=0, causal=causal, mask=mask, before=before)
+
+
+@pytest.mark.parametrize("d,g,t,run,causal,dtype", [(128, 1, 9, 4, 3, BF), (64, 4, 7, 0, 2, F16), (128, 7, 70, 32, 32, BF),
+                                                    (64, 7, 70, 33, 16, F16), (128, 7, 40, 0, 8, BF)])
+def test_what_is_not_seen_may_hold_anything(gpu, d, g, t, run, causal, dtype):
+    """Blocks that no list names and the block's keys behind a row's causal block: no number there changes a bit."""
+    lens, h = [700, 96, 33], 2
+    r = Requests(gpu, lens, h=h, d=d, dtype=dtype, page=32)
+    q = torch.randn((3, h * g, t, d), generator=r.gen).to(dtype).to(gpu)
+    ck, cv = (x.to(gpu) for x in r.block([t] * 3, t))
+    runs = -(-t // (run or t))
+    lists = torch.tensor([0, 2, -1], dtype=torch.int32, device=gpu).expand(3, h, runs, 3).contiguous()
+    prefix = r.cache.prefixes[0]
+
+    def call():
+        return paged_attention(q, prefix, ck, cv, blocks=lists, query_block=run, causal_block=causal)
+
+    want = call()
+    assert want.isfinite().all()
+    pages = r.cache.block_table
+    for b, x in enumerate(lens):
+        for i in range(x // 32):
+            if i not in (0, 2):
+                r.cache.pool[0, int(pages[b, i])] = 255
+    assert torch.equal(call(), want)
+    ck[:, :, -1], cv[:, :, -1, 3] = ck[:, :, -1] * 0 + float("nan"), float("inf")
+    out = call()
+    for b, x in enumerate(lens):
+        at = (x + torch.arange(t)) // causal
+        last = (at == at[-1]).to(gpu)
+        assert torch.equal(out[b, :, ~last], want[b, :, ~last]) and out[b, :, last].isnan().all()
+    ck[:, :, -1] = 0
+    out = call()
+    for b, x in enumerate(lens):
+        at = (x + torch.arange(t)) // causal
+        last = (at == at[-1]).to(gpu)
+        assert torch.equal(out[b, :, ~last], want[b, :, ~last])
+        assert not out[b, :, last][..., 3].isfinite().any() and out[b, :, last][..., 4:].isfinite().all()
