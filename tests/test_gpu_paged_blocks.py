@@ -5,6 +5,7 @@ import pytest
 import torch
 
 from maskahead_amd.kernels.paged import paged_attention, rotary_table, select_blocks
+from maskahead_amd.paged import PagedKVCache
 
 from _paged import Requests, attend64, check_attention, group_scores, rotated, select_rule
 
@@ -379,3 +380,35 @@ def test_what_is_not_seen_may_hold_anything(gpu, d, g, t, run, causal, dtype):
         last = (at == at[-1]).to(gpu)
         assert torch.equal(out[b, :, ~last], want[b, :, ~last])
         assert not out[b, :, last][..., 3].isfinite().any() and out[b, :, last][..., 4:].isfinite().all()
+
+
+def test_pages_beyond_32_bit_offsets(gpu):
+    """Rotated appends, selections and reads of pages at byte offsets past 2^31 and 2^32: as of a small pool."""
+    d, h, page = 128, 1, 128
+    rec = 40 * d * page // 32
+    total = (1 << 32) // rec + 40
+    far = [total - 1, (1 << 31) // rec + 1, total - 9, 5, (1 << 32) // rec, 0, (1 << 31) // rec - 1, 9]
+    gen = torch.Generator().manual_seed(1)
+    k, v = (torch.randn((2, h, 500, d), generator=gen).to(BF).to(gpu) for _ in range(2))
+    new = torch.tensor([500, 400], dtype=torch.int32, device=gpu)
+    table = rotary_table(600, d, device=gpu)
+    got = []
+    for pages in (total, 8):
+        c = PagedKVCache(num_layers=1, batch_size=2, num_kv_heads=h, head_dim=d, num_pages=pages, max_tokens=1024,
+                         page_tokens=page, device=gpu)
+        if pages == total:
+            c.free_ring[:8] = torch.tensor(far, dtype=torch.int32, device=gpu)
+        c.begin_append(new, 500)
+        c.stage_layer(0, k, v, rotary=table)
+        c.commit_append()
+        c.check()
+        x = list(c.dequantize_layer(0, 500))
+        for t in (1, 40):
+            q = torch.randn((2, 4, t, d), generator=torch.Generator().manual_seed(t)).to(BF).to(gpu)
+            rq, _ = c.rotate(q, rotary=table)
+            lists = c.select(0, rq, 4)
+            x += [rq, lists, c.attend(0, rq, blocks=lists)]
+        got.append(x)
+        if pages == total:
+            assert c.block_table[0, :4].tolist() == far[:4]
+    assert all(torch.equal(x, y) for x, y in zip(*got))
