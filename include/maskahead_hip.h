@@ -480,7 +480,7 @@ int ma_paged_attention_blocks(ma_tensor4 q, int B, int Hq, int T, int D, const m
  * page_tokens / block_tokens).  workspace: ma_select_workspace_bytes(B, H, runs, width * page_tokens)
  * bytes, 256-byte aligned, written before it is read; calls that may run at once need one each (blocks of
  * 32 tokens with scores need none).  Two launches.  MA_EUNSUPPORTED: 2^22 selections, 2^27 rows of a
- * selection, or 2^30 times 64 groups in all (as many as the table's rows can name). */
+ * selection, T and query_block together 2^31, or 2^30 times 64 groups in all (as many as the table's rows can name). */
 int64_t ma_select_workspace_bytes(int B, int H, int runs, int64_t tokens);
 int ma_select_blocks(ma_tensor4 q, int B, int Hq, int T, int D, const ma_pages *p, int H, const int32_t *new_lens,
                      int query_block, int block_tokens, int count, int keep_first, int keep_last, int32_t *blocks,

@@ -1766,8 +1766,9 @@ constexpr int HALF_ROWS_ITEMS = 48;
 static bool plan_of(int B, int H, int Hq, int T, int D, int query_block, int count, int64_t m, Plan &p) {
     if (B <= 0 || H <= 0 || Hq <= 0 || Hq % H || T <= 0 || (D != 64 && D != 128) || query_block < 0) return false;
     p.run = query_block == 0 || query_block > T ? T : query_block;
+    // (a run's rows, and the position behind the last run or 32 keys, have 32 bits)
+    if ((int64_t)(Hq / H) * p.run > INT32_MAX / 16 || (int64_t)T + max(p.run, PG_GROUP) > INT32_MAX) return false;
     p.runs = (T + p.run - 1) / p.run;
-    if ((int64_t)(Hq / H) * p.run > INT32_MAX / 16) return false;
     p.s = shape_of(Hq / H * p.run);
     if (count && count * m <= HALF_ROWS_ITEMS && p.s.rw == 8 && p.s.RG * p.runs <= p.s.W / 2 / ((int64_t)B * H)) {
         // half as many rows a workgroup where its segment would be cut in two: nothing, or half, to join

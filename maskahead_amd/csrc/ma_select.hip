@@ -562,7 +562,12 @@ extern "C" int ma_select_blocks(ma_tensor4 q, int B, int Hq, int T, int D, const
         ma_set_error("%s: queries and tails must share one dtype", who);
         return MA_EINVAL;
     }
-    const int run = query_block == 0 || query_block > T ? T : query_block, runs = (T + run - 1) / run;
+    const int run = query_block == 0 || query_block > T ? T : query_block;
+    if ((int64_t)T + run > INT32_MAX) {         // (the position behind the last run has 32 bits)
+        ma_set_error("%s: %d positions in runs of %d are not built (2^31 together)", who, T, run);
+        return MA_EUNSUPPORTED;
+    }
+    const int runs = (T + run - 1) / run;
     const int64_t tokens = (int64_t)p->width * p->page_tokens, need = ma_select_workspace_bytes(B, H, runs, tokens);
     if (need < 0 || (int64_t)(Hq / H) * run > INT32_MAX / 16) {
         ma_set_error("%s: %d rows of %d heads, or 2^31 selections, are not built", who, run, Hq / H);
