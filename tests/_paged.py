@@ -241,3 +241,29 @@ def select_rule(scores, m, count, first, last):
     must = [i for i in there if i < first or i >= nb - last]
     rest = sorted((i for i in there if i not in must), key=lambda i: (-block[i], i))
     return sorted(must + rest[:count - len(must)]), block
+
+
+def group_scores_of(pool, row, ng, h, q):
+    """group_scores of finite rows and parameters, all groups at once (whole numbers in 64 bits): [ng] float32."""
+    import numpy as np
+
+    _, _, per, rec = pool.shape
+    d = rec // 40
+    at = torch.as_tensor(row, dtype=torch.int64)[torch.arange(ng) // per]
+    par = pool[at, h, torch.arange(ng) % per, 32 * d:36 * d].contiguous().view(torch.float16).numpy().astype(np.float64)
+    s, z = 15 * par[:, :d], par[:, d:]
+
+    def whole(x, top, least):
+        m, e = np.frexp(top)                     # top = m 2^e, m of [1/2, 1)
+        e = np.maximum(np.where(m == 0, least, e - 1), least)
+        return np.rint(np.ldexp(x, (13 - e)[:, None])).astype(np.int64), e
+
+    rows = q.to(torch.float64).numpy()
+    qc, e = whole(rows, np.abs(rows).max(1), -100)
+    top = np.maximum(np.abs(s).max(1), np.abs(z).max(1))
+    zc, f = whole(z, top, -24)
+    sc, _ = whole(s, top, -24)
+    best = np.full(ng, -np.inf)
+    for c, x in zip(qc, e):                      # (a row at a time: sums below 2^53, so exact in float64 too)
+        best = np.maximum(best, np.ldexp((zc @ c + sc @ np.maximum(c, 0)).astype(np.float64), x + f - 26))
+    return torch.from_numpy(best).float()
