@@ -68,21 +68,27 @@ class PagedKVCache:
         self.lengths = torch.zeros((batch_size,), device=dev, dtype=torch.int32)
         self.free_ring = torch.arange(num_pages, device=dev, dtype=torch.int32)
         self.ring_state = torch.tensor([0, num_pages, 0, 0], device=dev, dtype=torch.int32)
-        self.prefixes = [self.prefix(i) for i in range(num_layers)]
         self._ends = torch.zeros_like(self.lengths)     # lengths of the append in progress
-        self._after = [self.prefix(i, staged=True) for i in range(num_layers)]
+        self.prefixes = [self._describe(i, None, False) for i in range(num_layers)]
+        self._after = [self._describe(i, None, True) for i in range(num_layers)]
         self._plan: tuple | None = None     # (new_lens, slots, ends, staged layers) of an append in progress
 
     def _check_layer(self, layer: int) -> None:
         if not 0 <= layer < self.num_layers:
             raise IndexError(layer)
 
-    def prefix(self, layer: int, *, mask: torch.Tensor | None = None, staged: bool = False) -> PagedPrefix:
-        """The kernels' descriptor of one layer, with an optional mask of dead entries; staged: as
-        it is once the append in progress has staged it, new tokens included."""
-        self._check_layer(layer)
+    def _describe(self, layer: int, mask: torch.Tensor | None, staged: bool) -> PagedPrefix:
         return PagedPrefix(self.pool[layer], self.k_tail[layer], self.v_tail[layer], self.block_table,
                            self._ends if staged else self.lengths, mask=mask)
+
+    def prefix(self, layer: int, *, mask: torch.Tensor | None = None, staged: bool = False) -> PagedPrefix:
+        """The kernels' descriptor of one layer, with an optional mask of dead entries; staged: as the
+        append in progress has staged it, new tokens included (RuntimeError where it has not; it describes
+        that append until the commit)."""
+        self._check_layer(layer)
+        if staged:
+            self._check_readable(layer, True)
+        return self._describe(layer, mask, staged)
 
     def _check_readable(self, layer: int, staged: bool = False) -> None:
         """A staged layer's tail holds the new tokens while lengths are still the old ones."""
@@ -96,7 +102,7 @@ class PagedKVCache:
     def _readable(self, layer: int, mask: torch.Tensor | None, staged: bool) -> PagedPrefix:
         self._check_readable(layer, staged)
         if mask is not None:
-            return self.prefix(layer, mask=mask, staged=staged)
+            return self._describe(layer, mask, staged)
         return (self._after if staged else self.prefixes)[layer]
 
     @property
