@@ -381,7 +381,7 @@ typedef struct ma_pages {
  * new_lens[b].  lengths is not written: the caller takes ends when the tokens are stored.
  * A plan that cannot be met changes nothing (slots -1, ends = lengths) and adds to status:
  * 1 the ring runs out, 2 a request outgrows its table row, 4 new_lens[b] > T, 8 a negative
- * length.  status is never cleared here.  One launch; plans of one ring are ordered by the
+ * length (32: ma_rotary's).  status is never cleared here.  One launch; plans of one ring are ordered by the
  * caller (one stream).  MA_EINVAL: ends overlaps lengths or new_lens, table rows overlap;
  * MA_EUNSUPPORTED: 2^31 tokens of a request, 2^29 pages. */
 int ma_page_plan(const int32_t *lengths, const int32_t *new_lens, int B, int T, int page_tokens, int32_t *table,
@@ -407,12 +407,16 @@ int ma_page_append(const ma_pages *p, ma_tensor4 k, ma_tensor4 v, int B, int H, 
  *   table  [rows, dim] f32, cosines then sines of a position's dim/2 angles; row stride s_row, rows
  *          16-byte aligned, dim a multiple of 16
  *   first  [B] i32, the position of every request's new token 0, or NULL: the lengths
+ *   status i32 or NULL: 32 is or'ed into it where a position of a real new token lies outside the table
+ *   count  [B] i32, the real new tokens of every request, or NULL: all T (an append has its own new_lens)
  * Positions outside the table take its nearest row. */
 typedef struct ma_rotary {
     const float *table;
     const int32_t *first;
     int64_t s_row;
     int32_t rows, dim, interleaved, reserved;
+    int32_t *status;
+    const int32_t *count;
 } ma_rotary;
 /* q [B, Hq, T, D] and k [B, Hk, T, D] (Hk 0: none) rotated into q_out and k_out, which may be q and k
  * themselves (but must not overlap them otherwise): token t of request b at position lengths[b] + t (or

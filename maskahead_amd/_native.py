@@ -61,7 +61,7 @@ class MaPages(ctypes.Structure):
 class MaRotary(ctypes.Structure):
     _fields_ = [("table", ctypes.c_void_p), ("first", ctypes.c_void_p), ("s_row", ctypes.c_int64),
                 ("rows", ctypes.c_int32), ("dim", ctypes.c_int32), ("interleaved", ctypes.c_int32),
-                ("reserved", ctypes.c_int32)]
+                ("reserved", ctypes.c_int32), ("status", ctypes.c_void_p), ("count", ctypes.c_void_p)]
 
 
 _P = ctypes.c_void_p

@@ -573,6 +573,7 @@ tail_rows:
         const RotaryRows x{fresh + (int64_t)j0 * st, tail + (int64_t)first * a.p.s_tt, 0, 0, st, 0, 0, a.p.s_tt, 1};
         const int pos = (int)min((int64_t)a.rot.first[b] + j0, (int64_t)INT32_MAX);
         for (int i = lane; i < cnt * U; i += 64) rotary_heads<D, DT>(a.rot, x, pos, 0, 0, i / U, i % U);
+        if (h == 0 && lane == 0) rotary_note(a.rot, a.rot.first[b], n);
         return;
     }
     constexpr int CH = D / 8;           // 16-byte chunks of a row
@@ -598,6 +599,8 @@ __global__ __launch_bounds__(256) void rotate_kernel(RotateArgs a) {
     const bool key = g >= a.qgroups;
     rotary_heads<D, DT>(a.r, key ? a.k : a.q, a.r.first[b], b, (key ? g - a.qgroups : g) * ROTARY_HEADS, (int)t,
                         threadIdx.x % U);
+    if (a.r.status && (blockIdx.x | blockIdx.y | threadIdx.x) == 0)
+        rotary_note(a.r, a.r.first[b], a.r.count ? min(a.r.count[b], a.T) : a.T);
 }
 
 // ------------------------------------------------------------------ read-back

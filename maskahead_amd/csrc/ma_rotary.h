@@ -18,10 +18,19 @@ struct RotaryDev {
     int64_t s_row;
     int rows, dim;
     bool next;                 // channels 2 i and 2 i + 1 are a pair (else i and i + dim / 2)
+    int32_t *status;           // (or NULL: nobody asks)
+    const int32_t *count;
 };
 
 inline RotaryDev rotary_dev(const ma_rotary *r, const int32_t *lengths) {
-    return RotaryDev{r->table, r->first ? r->first : lengths, r->s_row, r->rows, r->dim, r->interleaved != 0};
+    return RotaryDev{r->table, r->first ? r->first : lengths, r->s_row, r->rows, r->dim, r->interleaved != 0,
+                     r->status, r->count};
+}
+
+// of n new tokens from position first on, is one outside the table?  (One thread a request, behind its rows.)
+constexpr int ROTARY_OUTSIDE = 32;
+__device__ __forceinline__ void rotary_note(const RotaryDev &r, int first, int n) {
+    if (r.status && n > 0 && (first < 0 || (int64_t)first + n > r.rows)) atomicOr(r.status, ROTARY_OUTSIDE);
 }
 
 // the table's row of request b's token t (positions beyond the table: its last row)

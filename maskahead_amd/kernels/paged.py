@@ -205,13 +205,19 @@ _PLAN_ERRORS = ((1, "the free pages run out"), (2, "a request outgrows its block
                 (16, "a negative number of new tokens"))
 
 
+_OUTSIDE = 32     # of the status: a new token's position that a rotary table does not hold
+
+
 def check_plan(ring_state: torch.Tensor) -> None:
-    """Raise RuntimeError for what plans since the last check could not meet (waits for them,
-    and clears the status)."""
+    """Raise RuntimeError for what plans since the last check could not meet, and for new tokens
+    that were rotated outside of their table (waits for them, and clears the status)."""
     status = int(ring_state[3].item())
     if status:
         ring_state[3].zero_()
-        raise RuntimeError("page plan refused: " + ", ".join(text for bit, text in _PLAN_ERRORS if status & bit))
+        what = ["page plan refused: " + ", ".join(text for bit, text in _PLAN_ERRORS if status & bit)] if status & ~_OUTSIDE else []
+        if status & _OUTSIDE:
+            what.append("new tokens at positions outside the rotary table were turned by its nearest row")
+        raise RuntimeError("; ".join(what))
 
 
 def _check_block(name: str, t: torch.Tensor, prefix: PagedPrefix, heads: int | None = None) -> torch.Size:
@@ -247,11 +253,13 @@ def rotary_table(positions: int, head_dim: int, *, base: float = 10000.0, rotary
     return torch.cat((angle.cos(), angle.sin()), 1).float()
 
 
-_ROTARY_PACK = struct.Struct("=QQqiiii").pack
+_ROTARY_PACK = struct.Struct("=QQqiiiiQQ").pack
 
 
-def _rotary(prefix: PagedPrefix, table: torch.Tensor, interleaved: bool, positions: torch.Tensor | None) -> N.MaRotary:
-    """The kernels' descriptor of a rotary table (positions None: the prefix's lengths)."""
+def _rotary(prefix: PagedPrefix, table: torch.Tensor, interleaved: bool, positions: torch.Tensor | None,
+            ring_state: torch.Tensor | None, new_lens: torch.Tensor | None = None) -> N.MaRotary:
+    """The kernels' descriptor of a rotary table (positions None: the prefix's lengths; ring_state: whose
+    status is told of positions outside the table)."""
     s = table.shape
     if len(s) != 2 or table.dtype is not torch.float32 or not s[0] or not 0 < s[1] <= prefix.head_dim or s[1] % 16 or \
             table.stride(1) != 1:
@@ -262,9 +270,16 @@ def _rotary(prefix: PagedPrefix, table: torch.Tensor, interleaved: bool, positio
         raise ValueError(f"rotary is on {table.device}, expected {prefix.device}")
     if positions is not None:
         _i32(positions, "positions", (prefix.batch,), prefix.index)
+    status = count = 0
+    if ring_state is not None:
+        _i32(ring_state, "ring_state", (4,), prefix.index)
+        status = ring_state.data_ptr() + 12
+        if new_lens is not None:
+            _i32(new_lens, "new_lens", (prefix.batch,), prefix.index)
+            count = new_lens.data_ptr()
     return N.MaRotary.from_buffer_copy(_ROTARY_PACK(
         table.data_ptr(), 0 if positions is None else positions.data_ptr(), table.stride(0) if s[0] > 1 else s[1],
-        _c_int("rotary's positions", s[0]), s[1], bool(interleaved), 0))
+        _c_int("rotary's positions", s[0]), s[1], bool(interleaved), 0, status, count))
 
 
 def _check_rows(name: str, t: torch.Tensor, prefix: PagedPrefix, out: torch.Tensor | None) -> torch.Tensor:
@@ -281,15 +296,17 @@ def _check_rows(name: str, t: torch.Tensor, prefix: PagedPrefix, out: torch.Tens
 
 def rotate_block(prefix: PagedPrefix, query: torch.Tensor, key: torch.Tensor | None = None, *, rotary: torch.Tensor,
                  interleaved: bool = False, positions: torch.Tensor | None = None,
-                 out_query: torch.Tensor | None = None, out_key: torch.Tensor | None = None):
+                 out_query: torch.Tensor | None = None, out_key: torch.Tensor | None = None,
+                 new_lens: torch.Tensor | None = None, ring_state: torch.Tensor | None = None):
     """query [B, Hq, T, D] and key [B, Hk, T, D] (or None) rotated at their positions: position t of
     request b is prefix.lengths[b] + t (positions int32 [B]: positions[b] + t).  Returns (query, key).
 
     rotary is a ``rotary_table``; channels i and i + rotary_dim / 2 are a pair (interleaved: 2 i
     and 2 i + 1), channels from rotary_dim on stay as they are.  x' = x cos - y sin, y' = y cos + x
     sin, each operation rounded to f32, the result once to its type.  Positions outside the table
-    take its nearest row.  All T rows are rotated.  out_query may be query, out_key key; otherwise
-    they must not overlap them."""
+    take its nearest row; with ring_state (``plan_pages``) such a position of a real new token (t <
+    new_lens[b]; None: T) is noted in its status, for ``check_plan``.  All T rows are rotated.  out_query may
+    be query, out_key key; otherwise they must not overlap them."""
     out_query = _check_rows("query", query, prefix, out_query)
     if key is None and out_key is not None:
         raise ValueError("out_key without a key")
@@ -297,11 +314,12 @@ def rotate_block(prefix: PagedPrefix, query: torch.Tensor, key: torch.Tensor | N
         out_key = _check_rows("key", key, prefix, out_key)
         if key.shape[2] != query.shape[2]:
             raise ValueError(f"key must hold {query.shape[2]} positions like the queries")
-    rot = _rotary(prefix, rotary, interleaved, positions)
+    rot = _rotary(prefix, rotary, interleaved, positions, ring_state, new_lens)
     b, hq, t, d = query.shape
     hk = 0 if key is None else key.shape[1]
     if hq == 0 and hk:      # (the kernel wants rows in its first place)
-        rotate_block(prefix, key, None, rotary=rotary, interleaved=interleaved, positions=positions, out_query=out_key)
+        rotate_block(prefix, key, None, rotary=rotary, interleaved=interleaved, positions=positions, out_query=out_key,
+                     new_lens=new_lens, ring_state=ring_state)
     elif b and t and hq:
         _call(prefix.index, "ma_rotate_block", N.t4(query), hq, N.t4(out_query), N.t4(key if hk else None), hk,
               N.t4(out_key if hk else None), b, t, d, prefix.lengths.data_ptr(), rot)
@@ -311,7 +329,7 @@ def rotate_block(prefix: PagedPrefix, query: torch.Tensor, key: torch.Tensor | N
 def append_pages(prefix: PagedPrefix, key: torch.Tensor, value: torch.Tensor, new_lens: torch.Tensor,
                  slots: torch.Tensor, *, rotary: torch.Tensor | None = None, interleaved: bool = False,
                  positions: torch.Tensor | None = None, query: torch.Tensor | None = None,
-                 out_query: torch.Tensor | None = None) -> torch.Tensor | None:
+                 out_query: torch.Tensor | None = None, ring_state: torch.Tensor | None = None) -> torch.Tensor | None:
     """Store new_lens[b] (0 .. T) tokens of key, value [B, Hkv, T, D] behind request b's
     prefix.lengths[b] tokens: every 32-token group that they complete is quantized into the
     page that ``slots`` (``plan_pages``) names, the rest stays in the tail at 16 bits.
@@ -320,7 +338,7 @@ def append_pages(prefix: PagedPrefix, key: torch.Tensor, value: torch.Tensor, ne
 
     rotary (a ``rotary_table``): the keys are rotated at their positions on the way; what is stored
     is what ``rotate_block`` and an append of its result would store, bit for bit, and key is not
-    written.  interleaved, positions: as there.  With query [B, Hq, T, D] the same launch rotates all
+    written.  interleaved, positions, ring_state: as there.  With query [B, Hq, T, D] the same launch rotates all
     its rows, and they are returned (in out_query, if given, which may be query and overlaps nothing
     else that the call reads)."""
     shape = _check_block("key", key, prefix, prefix.heads)
@@ -339,7 +357,7 @@ def append_pages(prefix: PagedPrefix, key: torch.Tensor, value: torch.Tensor, ne
             _call(prefix.index, "ma_page_append", prefix._nat, N.t4(key), N.t4(value), b, h, t, d, new_lens.data_ptr(),
                   slots.data_ptr())
         return None
-    rot, hq = _rotary(prefix, rotary, interleaved, positions), 0
+    rot, hq = _rotary(prefix, rotary, interleaved, positions, ring_state), 0
     if query is not None:
         out_query = _check_rows("query", query, prefix, out_query)
         hq = query.shape[1]

@@ -126,15 +126,18 @@ class PagedKVCache:
 
     def rotate(self, query: torch.Tensor, key: torch.Tensor | None = None, *, rotary: torch.Tensor,
                interleaved: bool = False, positions: torch.Tensor | None = None):
-        """``rotate_block`` of a block behind the stored tokens: (query, key), for ``attend``."""
-        return rotate_block(self.prefixes[0], query, key, rotary=rotary, interleaved=interleaved, positions=positions)
+        """``rotate_block`` of a block behind the stored tokens: (query, key), for ``attend``.  During an
+        append ``check`` reports new tokens behind the table (their positions taken from the lengths)."""
+        told = {} if positions is not None or self._plan is None else dict(ring_state=self.ring_state, new_lens=self._plan[0])
+        return rotate_block(self.prefixes[0], query, key, rotary=rotary, interleaved=interleaved, positions=positions, **told)
 
     def stage_layer(self, layer: int, key: torch.Tensor, value: torch.Tensor, *, rotary: torch.Tensor | None = None,
                     interleaved: bool = False, positions: torch.Tensor | None = None,
                     query: torch.Tensor | None = None) -> torch.Tensor | None:
         """Write one layer's new tokens, key and value [B, Hkv, T, D] (rows behind a request's
         new_lens are not stored).  Before the commit the layer is read with staged=True alone.
-        rotary: the keys are rotated on the way, and query, which is returned (``append_pages``)."""
+        rotary: the keys are rotated on the way, and query, which is returned (``append_pages``); ``check``
+        reports new tokens behind the table, as in ``rotate``."""
         if self._plan is None:
             raise RuntimeError("begin_append must be called before stage_layer")
         new_lens, slots, _, staged = self._plan
@@ -142,7 +145,7 @@ class PagedKVCache:
             raise RuntimeError(f"layer {layer} was staged twice")
         self._check_layer(layer)
         query = append_pages(self.prefixes[layer], key, value, new_lens, slots, rotary=rotary, interleaved=interleaved,
-                             positions=positions, query=query)
+                             positions=positions, query=query, ring_state=self.ring_state if positions is None else None)
         staged.add(layer)
         return query
 
@@ -179,7 +182,8 @@ class PagedKVCache:
         self.lengths.copy_(ends)
 
     def check(self) -> None:
-        """Raise RuntimeError for a plan that could not be met since the last check (waits)."""
+        """Raise RuntimeError for a plan that could not be met since the last check, and for new tokens
+        that were rotated behind the end of their table (waits)."""
         check_plan(self.ring_state)
 
     # -- reading --------------------------------------------------------------------------

@@ -3,9 +3,13 @@
 import pytest
 import torch
 
+from maskahead_amd.kernels.paged import rotary_table
+
 from _paged import Requests
 
 pytestmark = pytest.mark.gpu
+
+BF = torch.bfloat16
 
 
 def test_a_staged_descriptor_needs_a_staged_layer(gpu):
@@ -33,3 +37,77 @@ def test_a_staged_descriptor_needs_a_staged_layer(gpu):
         with pytest.raises(IndexError):
             c.prefix(layer, staged=True)
     assert c.prefix(0).lengths.tolist() == [0, 64]
+
+
+@pytest.mark.parametrize("t,new,rows,behind", [(3, [3, 0], 42, True), (3, [3, 0], 43, False), (3, [2, 0], 42, False),
+                                               (1, [1, 0], 40, True), (70, [70, 3], 110, False), (70, [70, 3], 109, True),
+                                               (70, [2, 60], 64, True)])
+@pytest.mark.parametrize("way", ["staged", "rotated"])
+def test_positions_behind_the_table_are_reported(gpu, t, new, rows, behind, way):
+    """A new token whose position the rotary table does not hold takes its last row: check() says so."""
+    lens = [40, 100 if new[1] == 0 else 5]       # (an idle request may lie behind the table)
+    r = Requests(gpu, lens, h=2, d=64, page=32, room=128)
+    c = r.cache
+    table = rotary_table(rows, 64, device=gpu)
+    k, v = (torch.nan_to_num(x).to(gpu) for x in r.block(new, t))
+    q = torch.zeros((2, 4, t, 64), dtype=BF, device=gpu)
+    first = c.lengths.clone()
+    c.rotate(q, k, rotary=table)                 # (no append in progress: whose rows count is not known)
+    c.check()
+    c.begin_append(r.i32(new), t)
+    c.rotate(q, k, rotary=table, positions=first)        # (the caller's own positions are the caller's)
+    c.check()
+    if way == "rotated":
+        _, k = c.rotate(q, k, rotary=table)
+        c.stage_layer(0, k, v)
+    else:
+        c.stage_layer(0, k, v, rotary=table, query=q)
+    c.commit_append()
+    if behind:
+        with pytest.raises(RuntimeError, match="rotary table"):
+            c.check()
+    c.check()                                    # (reported once)
+
+
+def test_a_captured_step_reports_too(gpu):
+    r = Requests(gpu, [30], h=1, d=64, page=32, room=32)
+    c = r.cache
+    table = rotary_table(33, 64, device=gpu)
+    k, v = (x.to(gpu) for x in r.block([1], 1))
+    q = torch.zeros((1, 2, 1, 64), dtype=BF, device=gpu)
+    news = r.i32([1])
+
+    def step():
+        c.begin_append(news, 1)
+        c.stage_layer(0, k, v, rotary=table, query=q)
+        c.commit_append()
+
+    step()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        step()
+    for i in range(4):                           # positions 31, 32, 33, 34 of a table of 33
+        graph.replay()
+        torch.cuda.synchronize()
+        if i < 2:
+            c.check()
+        else:
+            with pytest.raises(RuntimeError, match="rotary table"):
+                c.check()
+    assert c.lengths.tolist() == [35]
+
+
+def test_a_plan_and_a_position_are_both_named(gpu):
+    r = Requests(gpu, [40], h=1, d=64, page=32, room=30)
+    c = r.cache
+    table = rotary_table(41, 64, device=gpu)
+    k, v = (x.to(gpu) for x in r.block([2], 2))
+    c.begin_append(r.i32([2]), 2)
+    c.stage_layer(0, k, v, rotary=table)
+    c.commit_append()
+    c.begin_append(r.i32([200]), 2)
+    c.stage_layer(0, k, v)
+    c.commit_append()
+    with pytest.raises(RuntimeError, match="page plan refused.*more new tokens.*rotary table"):
+        c.check()
+    c.check()
