@@ -282,6 +282,25 @@ def _rotary(prefix: PagedPrefix, table: torch.Tensor, interleaved: bool, positio
         _c_int("rotary's positions", s[0]), s[1], bool(interleaved), 0, status, count))
 
 
+def _rows_overlap(t: torch.Tensor) -> bool:
+    """Two rows of [B, H, T, D] (channels contiguous) have bytes in common."""
+    if t.is_contiguous():
+        return False
+    end = t.shape[3]
+    dims = sorted((st, n) for st, n in zip(t.stride(), t.shape[:3]) if n > 1)
+    for st, n in dims:
+        if st < end:
+            break
+        end += st * (n - 1)
+    else:
+        return False         # (every step is longer than what the shorter ones span)
+    starts = torch.zeros(1, dtype=torch.int64)
+    for st, n in dims:       # (rows between rows: rare)
+        starts = (starts[:, None] + st * torch.arange(n)).flatten()
+    starts = starts.sort().values
+    return bool((starts[1:] - starts[:-1] < t.shape[3]).any())
+
+
 def _check_rows(name: str, t: torch.Tensor, prefix: PagedPrefix, out: torch.Tensor | None) -> torch.Tensor:
     """The output of rotated rows t [B, H, T, D]: `out`, or a new tensor."""
     shape = _check_block(name, t, prefix)
@@ -289,7 +308,7 @@ def _check_rows(name: str, t: torch.Tensor, prefix: PagedPrefix, out: torch.Tens
         return torch.empty_like(t)        # (half the time of one by shape)
     if _check_block(f"out_{name}", out, prefix, shape[1]) != shape:
         raise ValueError(f"out_{name} must be {tuple(shape)}")
-    if any(st == 0 and n > 1 for st, n in zip(out.stride(), shape)):
+    if _rows_overlap(out):
         raise ValueError(f"out_{name} holds rows that share their memory")
     return out
 
