@@ -461,7 +461,8 @@ int ma_paged_attention(ma_tensor4 q, int B, int Hq, int T, int D, const ma_pages
  * last block are none; one listed twice weighs twice.  No more than the first ceil(whole groups /
  * block) entries are looked at.  workspace: ma_paged_blocks_workspace_bytes() bytes, which may be 0 (it is
  * not looked at then).  One or two launches.  MA_EUNSUPPORTED: 2^23 segments (requests x heads x runs x row
- * groups) or more, 2^29 groups of a list. */
+ * groups) or more.  MA_EINVAL also for what has no workspace (-1 bytes): 2^31 segments, 2^27 rows of a KV
+ * head's run, T and query_block 2^31 together. */
 int64_t ma_paged_blocks_workspace_bytes(int B, int H, int Hq, int T, int D, int count, int block_tokens, int query_block);
 int ma_paged_attention_blocks(ma_tensor4 q, int B, int Hq, int T, int D, const ma_pages *p, int H, ma_tensor4 kc,
                               ma_tensor4 vc, const int32_t *new_lens, int causal_block, float scale, ma_tensor4 out,

@@ -1832,11 +1832,11 @@ static int paged_attention(const char *who, const ma_tensor4 &q, int B, int Hq, 
     const Shape &s = plan.s;
     const Layout &l = plan.l;
     const int64_t RG = plan.RG;
-    // the line: every request as long as its table row, with room for what the stretches round up; or one segment
-    int64_t groups = (int64_t)p->width * p->page_tokens / PG_GROUP;
-    if (m) groups = min((int64_t)count, (groups + m - 1) / m) * min((int64_t)m, groups);
+    // the line: every request as long as its table row, with room for what the stretches round up.  (Lists lie
+    // on none: a segment holds at most 2^27 groups of its list, twice a table row's, beside its 16-bit rows.)
+    const int64_t groups = (int64_t)p->width * p->page_tokens / PG_GROUP;
     const int64_t most = START + s.rows0 + groups + ((1 + (T + PG_GROUP - 1) / PG_GROUP) << s.dense);
-    if (groups > INT32_MAX / 4 || (m ? most + 64LL * plan.parts : most * plan.segments + 64LL * s.W) > INT32_MAX) {
+    if (!m && most * plan.segments + 64LL * s.W > INT32_MAX) {
         ma_set_error("%s: %d requests of up to %lld tokens and %lld row groups of each head are not built (2^31 items)", who,
                      B, (long long)p->width * p->page_tokens, (long long)RG);
         return MA_EUNSUPPORTED;

@@ -72,3 +72,16 @@ def test_outputs_whose_rows_share_memory(shape, strides, shared):
             P._check_rows("query", rows, prefix, out)
     else:
         assert P._check_rows("query", rows, prefix, out) is out
+
+
+@pytest.mark.parametrize("kw,rc", [
+    (dict(b=1 << 13, h=32, t=64, run=1), N.MA_EUNSUPPORTED), (dict(b=1 << 18, h=32, t=1, run=0), N.MA_EUNSUPPORTED),
+    (dict(b=1 << 25, h=32, t=2, run=1), N.MA_EINVAL), (dict(b=1 << 26, h=32, t=1, run=0), N.MA_EINVAL),
+    (dict(b=1, h=1, t=1 << 27, run=0), N.MA_EINVAL)])
+def test_segments_that_are_not_built(lib, kw, rc):
+    """2^23 segments or more are unsupported; what has no workspace is an invalid argument."""
+    b, h, t, run = kw["b"], kw["h"], kw["t"], kw["run"]
+    need = lib.ma_paged_blocks_workspace_bytes(b, h, h, t, 64, 8, 32, run)
+    assert (need == -1) == (rc == N.MA_EINVAL)
+    assert lib.ma_paged_attention_blocks(_t4(), b, h, t, 64, _pages(), h, _t4(), _t4(), None, 0, 1.0, _t4(), 4096, 8, 32, run,
+                                         4096, 1 << 50, None) == rc
