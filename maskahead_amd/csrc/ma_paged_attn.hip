@@ -1758,9 +1758,10 @@ struct Plan {
 // 12 waves (155 registers, none spilled): 22.2 -> 24.0; 8 that ask two records ahead (211 registers): 23.8.
 // Many rows, where it would have two or more and lists of up to HALF_ROWS_ITEMS groups: row groups of 8
 // tiles for 16, which unpack every group twice and join half as much: 512 positions in runs of 32 (224
-// rows), 8 groups each, 50 -> 42 us; 64 groups 86 -> 87; 128 groups 100 -> 111.
+// rows) of 8, 16, 24 groups 47.5 -> 43.8, 51.5 -> 48.8, 56.5 -> 55.1 us; of 32, 40, 48, 64, 128 groups
+// 59.0 -> 61.5, 67 -> 68, 72.6 -> 72.8, 81 -> 84, 116 -> 125.
 constexpr int FEW_SHARE = 8, MANY_SHARE = 16;
-constexpr int HALF_ROWS_ITEMS = 48;
+constexpr int HALF_ROWS_ITEMS = 24;
 
 // false: not built
 static bool plan_of(int B, int H, int Hq, int T, int D, int query_block, int count, int64_t m, Plan &p) {
