@@ -103,7 +103,7 @@ __device__ __forceinline__ void rotary_unit(uint4 &a, uint4 &b, const float (&c)
 // may be the same rows.
 //
 // bound: the bytes, 4 D a row and 4 dim a position.  4 096 tokens of 4 requests (32 query and 8 KV heads,
-// D 128): 344 MB in 62.6 us, 5.5 TB/s (one head a thread 66.3, four 63.8, eight 67.3); a token of 64
+// D 128): 344 MB in 62.6 us, 5.5 TB/s, where a copy of as many bytes reaches 5.3 (one head a thread 66.3, four 63.8, eight 67.3); a token of 64
 // requests (28 and 4 heads) 4.2 us, which is a launch and two loads in a row (4.1, 4.6, 6.3).
 constexpr int ROTARY_HEADS = 2;
 struct RotaryRows {

@@ -157,7 +157,7 @@ __device__ __forceinline__ Unit find_unit(const SelectArgs &a, int u, int span, 
 // in 9.7 us; of 2 requests of 90 000 to 131 072 (32 and 8 heads): 29 MB in 10.5.  A workgroup for every unit
 // that a table row can name, which need not look for its request, was slower where most rows are shorter
 // (the first with its top 16.3 -> 19.7).  Many rows: the instructions around the products.  224 rows of 16
-// runs over 350 and 512 groups: 22.1 us, of which the matrix cores 5 and the other instructions 10 (1 700 a
+// runs over 350 and 512 groups: 22.1 us, of which the matrix cores 5 and the other instructions 10 (1 640 a
 // wave: the running maximum 340, digits of rows 350 and of parameters 250), at 14 waves a CU; waves of 32
 // groups 24.9.  Digits of f16 and their products, which take twice the time and registers: 12.3, 13.4 and
 // 44.5 us.
