@@ -370,8 +370,8 @@ def append_pages(prefix: PagedPrefix, key: torch.Tensor, value: torch.Tensor, ne
     if slots.get_device() != prefix.index:
         raise ValueError(f"slots is on {slots.device}, expected {prefix.device}")
     if rotary is None:
-        if query is not None or out_query is not None or positions is not None:
-            raise ValueError("query, out_query and positions need a rotary table")
+        if query is not None or out_query is not None or positions is not None or ring_state is not None:
+            raise ValueError("query, out_query, positions and ring_state need a rotary table")
         if b and t:
             _call(prefix.index, "ma_page_append", prefix._nat, N.t4(key), N.t4(value), b, h, t, d, new_lens.data_ptr(),
                   slots.data_ptr())

@@ -144,8 +144,9 @@ class PagedKVCache:
         if layer in staged:
             raise RuntimeError(f"layer {layer} was staged twice")
         self._check_layer(layer)
+        told = self.ring_state if rotary is not None and positions is None else None
         query = append_pages(self.prefixes[layer], key, value, new_lens, slots, rotary=rotary, interleaved=interleaved,
-                             positions=positions, query=query, ring_state=self.ring_state if positions is None else None)
+                             positions=positions, query=query, ring_state=told)
         staged.add(layer)
         return query
 

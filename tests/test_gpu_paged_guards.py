@@ -3,7 +3,8 @@
 import pytest
 import torch
 
-from maskahead_amd.kernels.paged import rotary_table
+from maskahead_amd._native import KernelUnavailableError
+from maskahead_amd.kernels.paged import append_pages, rotary_table, rotate_block
 
 from _paged import Requests
 
@@ -111,3 +112,48 @@ def test_a_plan_and_a_position_are_both_named(gpu):
     with pytest.raises(RuntimeError, match="page plan refused.*more new tokens.*rotary table"):
         c.check()
     c.check()
+
+
+def test_a_status_of_the_callers_own(gpu):
+    """rotate_block and append_pages with a ring_state: positions of the caller's, below the table too."""
+    r = Requests(gpu, [40, 3], h=2, d=128, page=32, room=32)
+    p, table = r.cache.prefixes[0], rotary_table(20, 128, device=gpu)
+    q = torch.zeros((2, 4, 3, 128), dtype=BF, device=gpu)
+    k = torch.zeros((2, 2, 3, 128), dtype=BF, device=gpu)
+    slots = torch.tensor([[0, 1, 2], [-1, -1, -1]], device=gpu)      # (request 1 stores nothing)
+    state = r.i32([0, 0, 0, 0])
+
+    def status(call, *first, new=(3, 3)):
+        state.fill_(5)
+        call(r.i32(list(first)), r.i32(list(new)))
+        assert state[:3].tolist() == [5] * 3
+        return int(state[3])
+
+    def turn(first, new):
+        rotate_block(p, q, k, rotary=table, positions=first, new_lens=new, ring_state=state)
+
+    def keys_alone(first, new):
+        rotate_block(p, q[:, :0], k, rotary=table, positions=first, new_lens=new, ring_state=state)
+
+    def all_rows(first, new):
+        rotate_block(p, q, rotary=table, positions=first, ring_state=state)
+
+    def append(first, new):
+        append_pages(p, k, k, new, slots, rotary=table, positions=first, query=q, ring_state=state)
+
+    for call in (turn, keys_alone, all_rows, append):
+        assert status(call, 17, 0) == 5
+        for first in (18, -1, 20, 2 ** 31 - 1, -2 ** 31):
+            assert status(call, first, 0) == 37
+            assert status(call, 0, first) == (5 if call is append else 37)
+        assert status(call, 18, 0, new=(2, 0)) == (37 if call is all_rows else 5)
+        assert status(call, 99, 0, new=(0, 3)) == (37 if call is all_rows else 5)
+        assert status(call, 99, 0, new=(-1, 3)) == (37 if call is all_rows else 5)
+        assert status(call, 17, 0, new=(90, 0)) == 5
+    for bad in (state.long(), state[:3], state.cpu()):
+        with pytest.raises((ValueError, KernelUnavailableError)):
+            rotate_block(p, q, rotary=table, ring_state=bad)
+    with pytest.raises(ValueError):
+        rotate_block(p, q, rotary=table, ring_state=state, new_lens=r.i32([1]))
+    with pytest.raises(ValueError):
+        append_pages(p, k, k, r.i32([1, 1]), slots, ring_state=state)
